@@ -7,6 +7,20 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, _HERE)
 sys.path.insert(0, os.path.dirname(_HERE))
 
+_PLUGIN = os.path.join(os.path.dirname(_HERE), "llm_amd", "lib", "libggml-mi355.so")
+_REF_HEADER = "/root/reference/ggml/include/ggml.h"
+
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: test needs a real MI355X (run with -m gpu on the GPU box)")
+
+
+def pytest_collection_modifyitems(items):
+    """The plugin includes the reference's headers and its tests run the reference's own tools: where neither the plugin nor the
+    reference's sources exist there is nothing to build them from, and those tests are skipped (the kernel library's run everywhere)."""
+    if os.path.exists(_PLUGIN) or os.path.exists(_REF_HEADER):
+        return
+    skip = pytest.mark.skip(reason="libggml-mi355.so cannot be built here: the reference's headers are absent")
+    for it in items:
+        if it.module.__name__ in ("test_backend_plugin_gpu", "test_stock_tools_gpu") or it.name == "test_plugin_exports_the_loader_symbols":
+            it.add_marker(skip)
