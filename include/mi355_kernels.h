@@ -65,7 +65,8 @@ enum mi355_error {
 MI355_API int         mi355_abi_version(void);          /* == MI355_ABI_VERSION of the header the library was built from;
                                                          * the plugin and the Python binding refuse a library that differs */
 MI355_API int64_t     mi355_args_sizeof(int which);     /* sizeof of 0 mi355_mmvq_args, 1 qkv_rope, 2 glu_matvec, 3 moe_down,
-                                                         * 4 fattn_args, 5 mi355_tensor, 6 qkv_finish_args, 7 decode_layer_args; -1 otherwise */
+                                                         * 4 fattn_args, 5 mi355_tensor, 6 qkv_finish_args, 7 decode_layer_args,
+                                                         * 8 qk_norm_rope_args; -1 otherwise */
 MI355_API const char *mi355_error_string(int err);      /* MI355_E_* or hipGetErrorString */
 MI355_API int64_t     mi355_blck_size(int type);        /* elements per block, 0 if unknown */
 MI355_API int64_t     mi355_type_size(int type);        /* bytes per block, 0 if unknown */
@@ -730,6 +731,46 @@ MI355_API int     mi355_flash_attn_ext_bf16(const mi355_fattn_args *args, void *
  * call failed (mi355_error_string handles all three). */
 MI355_API int64_t mi355_flash_attn_ext_noalloc_max_bytes(void);
 MI355_API int     mi355_flash_attn_ext_noalloc(const mi355_fattn_args *args, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * A KV cache of bounded size.  NO COUNTERPART IN THE REFERENCE, which stores every token in a row of its own: here each (sequence, KV
+ * head) keeps the slots that attention uses.  mi355_qk_norm_rope stores new tokens into given slots, mi355_flash_attn_ext_mass (decode
+ * steps) and mi355_attn_mass (prompts) accumulate the attention weight each slot draws, mi355_kv_evict picks the slots to keep and, for a
+ * prompt, gathers them.  Per-slot tables beside K and V, [ne3][n_head_kv][slots] with byte strides nb2 (head) and nb3 (sequence): the
+ * position a slot holds (int32) and its accumulated weight, its "mass" (f32).  Keys are stored rotated, so a slot's place says nothing.
+ *
+ * Attention input of models that normalise queries and keys per head, in one launch: q_out = rope(rms_norm(q) * q_norm), K cache row =
+ * rope(rms_norm(k) * k_norm), V cache row = v.  Replaces the node run RMS_NORM MUL ROPE (q and k) and the stores of K and V (SET_ROWS / CPY):
+ * eight launches of ggml-cuda (norm.cu, binbcast.cu, rope.cu, set-rows.cu).
+ *   q f32 [head_dim, n_head, n, ne3], k f32 [head_dim, n_head_kv, n, ne3], v f32 [dv, n_head_kv, n, ne3] (v and v_out may be NULL: no V):
+ *   byte strides nb1 (token), nb2 (head), nb3 (sequence), 16-byte aligned; q_out likewise (it may be q itself)
+ *   k_out, v_out: caches of type_kv f32 | f16 | bf16 (16-byte aligned) | q8_0 | q4_0 (2-byte aligned, whole 32-blocks, else MI355_E_SHAPE),
+ *   byte strides nb1 (row), nb2 (head), nb3 (sequence), n_rows rows per head
+ *   rows: int32 cache row of each (token, head, sequence), strides nb1 / nb2 / nb3 (0: shared); NULL: token i goes to row i.  A row outside
+ *   [0, n_rows) is not stored (q_out is written all the same).  Rows of one call must be distinct per head and sequence.
+ *   q_norm, k_norm f32 [head_dim]; NULL: no weight.  pos int32 [n, ne3], freq_factors f32 [n_dims / 2] or NULL, rope parameters as in
+ *   mi355_rope_f32, modes NORMAL and NEOX; n_dims 0: no rotation.  Angles are computed in 64 bits: at far positions they are nearer to the
+ *   formula than mi355_rope_f32's, which follows the reference's 32-bit products.
+ *   slot_pos, slot_mass (optional): the rows' entries are set to the token's position and to 0.
+ * head_dim and dv multiples of 8 up to 256, n_dims a multiple of 8, else MI355_E_UNSUPPORTED; at most 2^24 tokens a call. */
+typedef struct mi355_qk_norm_rope_args {
+    const float *q; int64_t q_nb1, q_nb2, q_nb3;
+    const float *k; int64_t k_nb1, k_nb2, k_nb3;
+    const float *v; int64_t v_nb1, v_nb2, v_nb3;
+    const float *q_norm, *k_norm;
+    float *q_out; int64_t qo_nb1, qo_nb2, qo_nb3;
+    void *k_out; int64_t ko_nb1, ko_nb2, ko_nb3;
+    void *v_out; int64_t vo_nb1, vo_nb2, vo_nb3;
+    const int32_t *rows; int64_t rows_nb1, rows_nb2, rows_nb3;
+    const int32_t *pos; int64_t pos_nb1, pos_nb3;
+    const float *freq_factors;
+    int32_t *slot_pos; int64_t sp_nb2, sp_nb3;
+    float *slot_mass; int64_t sm_nb2, sm_nb3;
+    int64_t head_dim, dv, n_head, n_head_kv, n, ne3, n_rows;   /* dv 0: head_dim */
+    int32_t type_kv, n_dims, mode, n_ctx_orig;
+    float eps, freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow;
+} mi355_qk_norm_rope_args;
+MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stream);
 
 #ifdef __cplusplus
 }

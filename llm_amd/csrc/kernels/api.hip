@@ -16,6 +16,7 @@ int64_t mi355_args_sizeof(int which) {
         case 5: return (int64_t)sizeof(mi355_tensor);
         case 6: return (int64_t)sizeof(mi355_qkv_finish_args);
         case 7: return (int64_t)sizeof(mi355_decode_layer_args);
+        case 8: return (int64_t)sizeof(mi355_qk_norm_rope_args);
     }
     return -1;
 }

@@ -514,3 +514,81 @@ def set_rows(src, ids, dst, type_dst):
         td.nb[0] = B.TYPE_SIZE[type_dst]
     K.check(K.lib.mi355_set_rows(ts, ti, td, _stream()), "mi355_set_rows")
     return dst
+
+
+_KV_DTYPE = {B.F32: torch.float32, B.F16: torch.float16, B.BF16: torch.bfloat16, B.Q8_0: torch.uint8, B.Q4_0: torch.uint8}
+
+
+def _kv_rows(t, type_kv, name):
+    """checks a cache tensor [seqs, kv heads, slots, row]: f32 / f16 / bf16 values, or uint8 bytes of q8_0 / q4_0 blocks"""
+    if type_kv not in _KV_DTYPE:
+        raise ValueError(f"{name}: caches are f32, f16, bf16, q8_0 or q4_0, not type {type_kv}")
+    if t.dim() != 4 or t.dtype != _KV_DTYPE[type_kv] or (t.shape[3] > 1 and t.stride(3) != 1):
+        raise ValueError(f"{name}: expected [seqs, kv heads, slots, row] of {_KV_DTYPE[type_kv]} with contiguous rows")
+    return t.shape[3] if t.dtype != torch.uint8 else t.shape[3] // B.TYPE_SIZE[type_kv] * 32
+
+
+def _here(*ts):
+    """every tensor lies on the current device, whose current stream the launch goes to"""
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise ValueError(f"tensor on {t.device}, the current device is cuda:{dev}")
+
+
+def qk_norm_rope(q, k, v, q_norm, k_norm, eps, pos, k_cache, v_cache, type_kv, rows=None, slot_pos=None, slot_mass=None, n_dims=None, mode=2,
+                 n_ctx_orig=8192, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0,
+                 freq_factors=None, q_out=None):
+    """Per-head RMS norm x weight and rotation of q and k, k and v into their cache rows (mi355_qk_norm_rope).  q [seqs, tokens, heads, d],
+    k [seqs, tokens, kv heads, d], v [.., dv] (or None, with v_cache None) f32, strides free (contiguous rows); q_norm / k_norm f32 [d] or
+    None; pos int32 [seqs, tokens]; caches [seqs, kv heads, slots, row] of type_kv; rows int32 [seqs, kv heads, tokens] (None: token i goes
+    to slot i); slot_pos int32, slot_mass f32 [seqs, kv heads, slots] or None -> q rotated, f32 [seqs, heads, tokens, d] (q_out's strides)."""
+    _here(q, k, v, q_norm, k_norm, pos, k_cache, v_cache, rows, slot_pos, slot_mass, freq_factors, q_out)
+    S, n, H, d = q.shape
+    hk, dv = k.shape[2], 0
+    if q.dtype != torch.float32 or k.dtype != torch.float32 or tuple(k.shape) != (S, n, hk, d) or q.stride(3) != 1 or k.stride(3) != 1:
+        raise ValueError("q and k: f32 [seqs, tokens, heads, d] with contiguous rows")
+    if (v is None) != (v_cache is None):
+        raise ValueError("v and v_cache come together")
+    slots = k_cache.shape[2]
+    if _kv_rows(k_cache, type_kv, "k_cache") != d or tuple(k_cache.shape[:2]) != (S, hk):
+        raise ValueError("k_cache does not fit k")
+    if v is not None:
+        dv = v.shape[3]
+        if v.dtype != torch.float32 or tuple(v.shape[:3]) != (S, n, hk) or v.stride(3) != 1:
+            raise ValueError("v: f32 [seqs, tokens, kv heads, dv] with contiguous rows")
+        if _kv_rows(v_cache, type_kv, "v_cache") != dv or tuple(v_cache.shape[:3]) != (S, hk, slots):
+            raise ValueError("v_cache does not fit v and k_cache")
+    if pos.dtype != torch.int32 or tuple(pos.shape) != (S, n) or (rows is not None and (rows.dtype != torch.int32 or tuple(rows.shape) != (S, hk, n))):
+        raise ValueError("pos: int32 [seqs, tokens], rows: int32 [seqs, kv heads, tokens]")
+    for t, dt in ((slot_pos, torch.int32), (slot_mass, torch.float32)):
+        if t is not None and (t.dtype != dt or tuple(t.shape) != (S, hk, slots) or (slots > 1 and t.stride(2) != 1)):
+            raise ValueError("slot_pos int32 / slot_mass f32: [seqs, kv heads, slots], slots contiguous")
+    n_dims = d if n_dims is None else n_dims
+    for t, m in ((q_norm, d), (k_norm, d), (freq_factors, n_dims // 2)):
+        if t is not None and (t.dtype != torch.float32 or t.numel() < m or not t.is_contiguous()):
+            raise ValueError("q_norm, k_norm: f32 [d]; freq_factors: f32 [n_dims / 2]")
+    if q_out is None:
+        q_out = torch.empty((S, H, n, d), dtype=torch.float32, device=q.device)
+    elif q_out.dtype != torch.float32 or tuple(q_out.shape) != (S, H, n, d) or q_out.stride(3) != 1:
+        raise ValueError("q_out: f32 [seqs, heads, tokens, d] with contiguous rows")
+    if q.numel() == 0:
+        return q_out
+    a, ptr = K.QkNormRopeArgs(), lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    st = lambda t, *i: [t.stride(j) * t.element_size() for j in i] if t is not None else [0] * len(i)  # noqa: E731
+    a.q, (a.q_nb1, a.q_nb2, a.q_nb3) = q.data_ptr(), st(q, 1, 2, 0)
+    a.k, (a.k_nb1, a.k_nb2, a.k_nb3) = k.data_ptr(), st(k, 1, 2, 0)
+    a.v, (a.v_nb1, a.v_nb2, a.v_nb3) = ptr(v), st(v, 1, 2, 0)
+    a.q_norm, a.k_norm, a.freq_factors = ptr(q_norm), ptr(k_norm), ptr(freq_factors)
+    a.q_out, (a.qo_nb1, a.qo_nb2, a.qo_nb3) = q_out.data_ptr(), st(q_out, 2, 1, 0)
+    a.k_out, (a.ko_nb1, a.ko_nb2, a.ko_nb3) = k_cache.data_ptr(), st(k_cache, 2, 1, 0)
+    a.v_out, (a.vo_nb1, a.vo_nb2, a.vo_nb3) = ptr(v_cache), st(v_cache, 2, 1, 0)
+    a.rows, (a.rows_nb1, a.rows_nb2, a.rows_nb3) = ptr(rows), st(rows, 2, 1, 0)
+    a.pos, (a.pos_nb1, a.pos_nb3) = pos.data_ptr(), st(pos, 1, 0)
+    a.slot_pos, (a.sp_nb2, a.sp_nb3) = ptr(slot_pos), st(slot_pos, 1, 0)
+    a.slot_mass, (a.sm_nb2, a.sm_nb3) = ptr(slot_mass), st(slot_mass, 1, 0)
+    a.head_dim, a.dv, a.n_head, a.n_head_kv, a.n, a.ne3, a.n_rows = d, dv, H, hk, n, S, slots
+    a.type_kv, a.n_dims, a.mode, a.n_ctx_orig, a.eps = type_kv, n_dims, mode, n_ctx_orig, eps
+    a.freq_base, a.freq_scale, a.ext_factor, a.attn_factor, a.beta_fast, a.beta_slow = freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow
+    K.check(K.lib.mi355_qk_norm_rope(a, _stream()), "mi355_qk_norm_rope")
+    return q_out

@@ -1,0 +1,48 @@
+"""Refusals of the bounded KV cache's entry points: every argument check answers before anything is launched, so no GPU is needed.
+Pointers here are only ever compared with NULL and tested for alignment."""
+import pytest
+
+import llm_amd.blocks as B
+import llm_amd.kernels as K
+
+E_TYPE, E_SHAPE, E_ALIGN, E_NULL, E_WORKSPACE, E_UNSUPPORTED = -1, -2, -3, -4, -5, -6
+P = 1 << 20        # a well-aligned address that is never followed
+
+
+def store_args(**kw):
+    a = K.QkNormRopeArgs()
+    for f in ("q", "k", "v", "q_norm", "k_norm", "q_out", "k_out", "v_out", "rows", "pos", "slot_pos", "slot_mass"):
+        setattr(a, f, P)
+    for f in ("q", "k", "v", "qo", "ko", "vo"):
+        for i, nb in enumerate((4096, 512, 1 << 16)):
+            setattr(a, f"{f}_nb{i + 1}", nb)
+    a.head_dim, a.dv, a.n_head, a.n_head_kv, a.n, a.ne3, a.n_rows = 128, 0, 8, 2, 1, 1, 16
+    a.type_kv, a.n_dims, a.mode, a.n_ctx_orig = B.F16, 128, 2, 4096
+    a.eps, a.freq_base, a.freq_scale, a.attn_factor, a.beta_fast, a.beta_slow = 1e-6, 1e4, 1.0, 1.0, 32.0, 1.0
+    for f, v in kw.items():
+        setattr(a, f, v)
+    return a
+
+
+@pytest.mark.parametrize("code, kw", [
+    (E_NULL, dict(q=None)), (E_NULL, dict(k=None)), (E_NULL, dict(q_out=None)), (E_NULL, dict(k_out=None)), (E_NULL, dict(pos=None)),
+    (E_NULL, dict(v=None)), (E_NULL, dict(v_out=None)),
+    (E_UNSUPPORTED, dict(head_dim=0)), (E_UNSUPPORTED, dict(head_dim=100)), (E_UNSUPPORTED, dict(head_dim=264)), (E_UNSUPPORTED, dict(dv=12)),
+    (E_UNSUPPORTED, dict(dv=512)), (E_UNSUPPORTED, dict(mode=8)), (E_UNSUPPORTED, dict(n_dims=20)),
+    (E_SHAPE, dict(n_dims=136)), (E_SHAPE, dict(n_dims=-8)), (E_SHAPE, dict(n=-1)), (E_SHAPE, dict(ne3=-1)), (E_SHAPE, dict(n_head=0)),
+    (E_SHAPE, dict(n_head_kv=0)), (E_SHAPE, dict(n_rows=-1)), (E_SHAPE, dict(n=1 << 25)), (E_SHAPE, dict(n=1 << 20, ne3=1 << 20)),
+    (E_SHAPE, dict(freq_base=0.0)), (E_SHAPE, dict(freq_base=float("nan"))), (E_SHAPE, dict(freq_scale=0.0)), (E_SHAPE, dict(ext_factor=1.0, n_ctx_orig=0)),
+    (E_SHAPE, dict(type_kv=B.Q8_0, head_dim=80, n_dims=80)), (E_SHAPE, dict(type_kv=B.Q4_0, dv=72)),
+    (E_TYPE, dict(type_kv=B.Q4_K)), (E_TYPE, dict(type_kv=B.I32)),
+    (E_ALIGN, dict(q=P + 4)), (E_ALIGN, dict(k_nb2=520)), (E_ALIGN, dict(q_out=P + 8)), (E_ALIGN, dict(q_norm=P + 4)), (E_ALIGN, dict(k_out=P + 2)),
+    (E_ALIGN, dict(vo_nb1=264)), (E_ALIGN, dict(type_kv=B.Q8_0, k_out=P + 1)), (E_ALIGN, dict(pos=P + 2)), (E_ALIGN, dict(rows_nb2=6)),
+    (E_ALIGN, dict(slot_mass=P + 1)),
+])
+def test_qk_norm_rope_refuses(code, kw):
+    assert K.lib.mi355_qk_norm_rope(store_args(**kw), None) == code
+
+
+def test_qk_norm_rope_of_nothing_launches_nothing():
+    assert K.lib.mi355_qk_norm_rope(None, None) == E_NULL
+    assert K.lib.mi355_qk_norm_rope(store_args(n=0), None) == 0
+    assert K.lib.mi355_qk_norm_rope(store_args(ne3=0), None) == 0

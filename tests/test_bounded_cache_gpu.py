@@ -1,0 +1,265 @@
+"""The bounded KV cache on the GPU against its formulas in 64 bits (on the CPU): the normalised and rotated store, the attention with the
+weight every slot draws, the eviction, and the three run one after the other as a decode loop does."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import llm_amd.blocks as B
+import llm_amd.kernels as K
+import llm_amd.ops as ops
+
+pytestmark = pytest.mark.gpu
+
+U32, U16, UBF = 2.0 ** -24, 2.0 ** -11, 2.0 ** -8          # half a step relative to the value: f32, f16, bf16
+DTYPE = {B.F32: torch.float32, B.F16: torch.float16, B.BF16: torch.bfloat16}
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def values(rows, t):
+    """f64 values of cache rows (CPU tensor)"""
+    if t in DTYPE:
+        return rows.double()
+    b = rows.reshape(*rows.shape[:-1], -1, B.TYPE_SIZE[t])
+    d = b[..., :2].contiguous().view(torch.float16).double()
+    q = b[..., 2:].contiguous()
+    q = q.view(torch.int8).double() if t == B.Q8_0 else torch.cat([q & 15, q >> 4], -1).double() - 8
+    return (d * q).reshape(*rows.shape[:-1], -1)
+
+
+def cache(shape, t, g, scale=1.0):
+    """random cache rows of type t (CPU)"""
+    if t in DTYPE:
+        return (torch.randn(shape, generator=g) * scale).to(DTYPE[t])
+    n = math.prod(shape[:-1])
+    return torch.from_numpy(B.random_blocks(t, n, shape[-1], seed=int(torch.randint(0, 1 << 30, (1,), generator=g)),
+                                            scale=scale * (0.02 if t == B.Q8_0 else 0.3))).reshape(*shape[:-1], -1)
+
+
+# ---- qk_norm_rope --------------------------------------------------------------------------------------------------------------------
+
+def store_oracle(x, w, eps, pos, n_dims, mode, base=10000.0, ff=None, freq_scale=1.0, ext=0.0, attn=1.0, n_ctx=8192, fast=32.0, slow=1.0):
+    """-> (values, per value a bound of its f32 error) of rope(rms_norm(x) * w), x [S, n, H, d] -> [S, H, n, d]"""
+    x = x.double()
+    d = x.shape[-1]
+    y = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * (w.double() if w is not None else 1.0)
+    # the sum of squares: at most d / 64 + 8 additions deep in any of the kernels' trees (16 lanes x 8 values); root, quotient, two products
+    err = y.abs() * (24 * U32)
+    if n_dims:
+        i = torch.arange(n_dims // 2, dtype=torch.float64)
+        f = base ** (-2.0 * i / n_dims) / (ff.double() if ff is not None else 1.0)
+        if ext != 0.0:
+            dim = lambda rot: n_dims * math.log(n_ctx / (rot * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+            lo, hi = max(0, math.floor(dim(fast))), min(n_dims - 1, math.ceil(dim(slow)))
+            mix = (1 - torch.clamp((i - lo) / max(0.001, hi - lo), 0, 1)) * ext
+            f = f * (freq_scale * (1 - mix) + mix)
+            attn *= 1 + 0.1 * math.log(1 / freq_scale)
+        else:
+            f = f * freq_scale
+        t = pos.double()[:, :, None, None] * f
+        r, keep = y[..., :n_dims], y[..., n_dims:]
+        a, b = (r[..., 0::2], r[..., 1::2]) if mode == 0 else (r[..., : n_dims // 2], r[..., n_dims // 2:])
+        c, s = torch.cos(t) * attn, torch.sin(t) * attn
+        u, v = a * c - b * s, a * s + b * c
+        # the norm's 24, the angle rounded to f32 revolutions (2 pi 2^-26 of a turn), sincos (4 steps of 2^-24), products and sum (3)
+        e = torch.hypot(a, b) * (36 * U32 * max(1.0, abs(attn)))
+        # f32 parameters of YaRN (the ramp's ends, freq_scale): relative 2^-23 of the angle
+        if ext != 0.0 or freq_scale != 1.0:
+            e = e + torch.hypot(a, b) * (t.abs() * 2.0 ** -22 + 2.0 ** -22)
+        if mode == 0:
+            y, err = torch.cat([torch.stack([u, v], -1).flatten(-2), keep], -1), torch.cat([torch.stack([e, e], -1).flatten(-2), err[..., n_dims:]], -1)
+        else:
+            y, err = torch.cat([u, v, keep], -1), torch.cat([e, e, err[..., n_dims:]], -1)
+    return y.transpose(1, 2), err.transpose(1, 2)
+
+
+def store_case(S, n, H, HK, d, dv, slots, t, seed, layout="dense"):
+    g = gen(seed)
+    mk = lambda h, m: torch.randn((S, n, h, m), generator=g) * 3  # noqa: E731
+    q, k, v = mk(H, d), mk(HK, d), mk(HK, dv)
+    dev = dict(q=q.cuda(), k=k.cuda(), v=v.cuda())
+    if layout == "packed":                       # one row of q, k and v heads per token, as a fused projection leaves it
+        both = torch.cat([x.reshape(S, n, -1) for x in (q, k, v)], -1).cuda()
+        off = 0
+        for name, h, m in (("q", H, d), ("k", HK, d), ("v", HK, dv)):
+            dev[name] = both[..., off:off + h * m].unflatten(-1, (h, m))
+            off += h * m
+    qw, kw = 1 + 0.3 * torch.randn(d, generator=g), 1 + 0.3 * torch.randn(d, generator=g)
+    rows = torch.stack([torch.randperm(slots, generator=g)[:n] for _ in range(S * HK)]).reshape(S, HK, n).to(torch.int32)
+    kc, vc = cache((S, HK, slots, d), t, g), cache((S, HK, slots, dv), t, g)
+    pos = torch.randint(0, 200000, (S, n), generator=g).to(torch.int32)
+    return q, k, v, dev, qw, kw, rows, kc, vc, pos
+
+
+def check_rows(got, before, rows, want, err, t):
+    """stored rows hold the values (rounded once), every other row its bytes of before"""
+    S, HK, slots = before.shape[:3]
+    at = (torch.arange(S)[:, None, None], torch.arange(HK)[None, :, None], rows.long())
+    touched = torch.zeros((S, HK, slots), dtype=torch.bool)
+    touched[at] = True
+    assert torch.equal(got[~touched].view(torch.uint8) if got.dtype != torch.uint8 else got[~touched],
+                       before[~touched].view(torch.uint8) if before.dtype != torch.uint8 else before[~touched])
+    u = {B.F32: 0.0, B.F16: U16, B.BF16: UBF}[t]
+    x = got[at].double()
+    # once rounded; below the normal range of f16 half a step is 2^-25
+    assert ((x - want).abs() <= err + u * (want.abs() + err) + (2.0 ** -25 if t == B.F16 else 0.0)).all()
+
+
+STORE = [
+    # S, n, H, HK, d, dv, slots, type, n_dims, mode, layout
+    (1, 1, 32, 8, 128, 128, 64, B.F16, 128, 2, "dense"),
+    (1, 1, 32, 8, 128, 128, 64, B.F16, 128, 0, "packed"),
+    (3, 1, 64, 8, 128, 128, 9, B.BF16, 128, 2, "dense"),
+    (1, 37, 8, 2, 64, 64, 50, B.F32, 64, 2, "packed"),
+    (2, 5, 5, 5, 80, 80, 7, B.F16, 40, 2, "dense"),
+    (1, 130, 4, 1, 96, 64, 131, B.BF16, 48, 0, "dense"),
+    (1, 7, 3, 1, 256, 256, 7, B.F16, 256, 2, "packed"),
+    (2, 3, 2, 1, 256, 128, 4, B.F32, 64, 0, "dense"),
+    (1, 2, 1, 1, 8, 8, 3, B.F16, 8, 2, "dense"),
+    (1, 9, 6, 3, 72, 40, 11, B.F16, 72, 0, "dense"),
+    (1, 4, 4, 2, 128, 128, 5, B.F16, 0, 2, "dense"),
+    (1, 600, 16, 2, 128, 128, 600, B.F16, 128, 2, "dense"),
+]
+
+
+@pytest.mark.parametrize("S,n,H,HK,d,dv,slots,t,n_dims,mode,layout", STORE)
+def test_store_against_the_formula(S, n, H, HK, d, dv, slots, t, n_dims, mode, layout):
+    q, k, v, dev, qw, kw, rows, kc, vc, pos = store_case(S, n, H, HK, d, dv, slots, t, 17 + n + d, layout)
+    kg, vg = kc.cuda(), vc.cuda()
+    sp, sm = torch.full((S, HK, slots), 7, dtype=torch.int32, device="cuda"), torch.full((S, HK, slots), 3.0, device="cuda")
+    qo = ops.qk_norm_rope(dev["q"], dev["k"], dev["v"], qw.cuda(), kw.cuda(), 1e-6, pos.cuda(), kg, vg, t, rows=rows.cuda(), slot_pos=sp, slot_mass=sm,
+                          n_dims=n_dims, mode=mode, freq_base=500000.0)
+    want, err = store_oracle(q, qw, 1e-6, pos, n_dims, mode, base=500000.0)
+    assert ((qo.cpu().double() - want).abs() <= err).all()
+    check_rows(kg.cpu(), kc, rows, *store_oracle(k, kw, 1e-6, pos, n_dims, mode, base=500000.0), t)
+    check_rows(vg.cpu(), vc, rows, v.double().transpose(1, 2), torch.zeros(()), t)
+    at = (torch.arange(S)[:, None, None], torch.arange(HK)[None, :, None], rows.long())
+    wp, wm = torch.full((S, HK, slots), 7, dtype=torch.int32), torch.full((S, HK, slots), 3.0)
+    wp[at], wm[at] = pos[:, None, :].expand(S, HK, n), 0.0
+    assert torch.equal(sp.cpu(), wp) and torch.equal(sm.cpu(), wm)
+
+
+@pytest.mark.parametrize("t", [B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("d,dv,n_dims,mode", [(128, 128, 128, 2), (64, 96, 64, 0), (96, 32, 40, 2), (256, 256, 64, 2), (32, 32, 8, 0)])
+def test_store_into_blocks_quantizes_the_rotated_rows(t, d, dv, n_dims, mode):
+    """the f32 rows of the same call, quantized by SET_ROWS: the same bytes"""
+    S, n, H, HK, slots = 2, 11, 4, 2, 12
+    q, k, v, dev, qw, kw, rows, kc, vc, pos = store_case(S, n, H, HK, d, dv, slots, t, d + n_dims)
+    v[0, 0, 0, :32] = 0.0
+    dev["v"] = v.cuda()
+    kg, vg = kc.cuda(), vc.cuda()
+    args = (dev["q"], dev["k"], dev["v"], qw.cuda(), kw.cuda(), 1e-6, pos.cuda())
+    qo = ops.qk_norm_rope(*args, kg, vg, t, rows=rows.cuda(), n_dims=n_dims, mode=mode)
+    kf, vf = torch.zeros((S, HK, slots, d), device="cuda"), torch.zeros((S, HK, slots, dv), device="cuda")
+    qf = ops.qk_norm_rope(*args, kf, vf, B.F32, rows=rows.cuda(), n_dims=n_dims, mode=mode)
+    assert torch.equal(qo, qf)
+    for got, src, before in ((kg, kf, kc), (vg, vf, vc)):
+        all_rows = torch.arange(slots, dtype=torch.int64, device="cuda")
+        blocks = torch.zeros_like(got)
+        for s in range(S):
+            for h in range(HK):
+                ops.set_rows(src[s, h].contiguous(), all_rows, blocks[s, h], t)
+        at = (torch.arange(S)[:, None, None], torch.arange(HK)[None, :, None], rows.long())
+        want = before.clone()
+        want[at] = blocks.cpu()[at]
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("mode", [0, 2])
+def test_store_with_yarn_and_frequency_factors(mode):
+    q, k, v, dev, qw, kw, rows, kc, vc, pos = store_case(1, 6, 4, 2, 128, 128, 8, B.F32, 5)
+    pos = torch.tensor([[0, 1, 77, 4096, 30000, 131071]], dtype=torch.int32)
+    ff = 1 + torch.rand(64, generator=gen(3)) * 7
+    kw_ = dict(n_dims=128, mode=mode, freq_base=1e6, freq_scale=0.25, ext_factor=1.0, attn_factor=0.9, n_ctx_orig=32768)
+    kg, vg = kc.cuda(), vc.cuda()
+    qo = ops.qk_norm_rope(dev["q"], dev["k"], dev["v"], qw.cuda(), None, 1e-5, pos.cuda(), kg, vg, B.F32, rows=rows.cuda(), freq_factors=ff.cuda(), **kw_)
+    o = dict(base=1e6, ff=ff, freq_scale=0.25, ext=1.0, attn=0.9, n_ctx=32768)
+    want, err = store_oracle(q, qw, 1e-5, pos, 128, mode, **o)
+    assert ((qo.cpu().double() - want).abs() <= err).all()
+    check_rows(kg.cpu(), kc, rows, *store_oracle(k, None, 1e-5, pos, 128, mode, **o), B.F32)
+
+
+def test_store_skips_rows_outside_the_cache_and_q_may_stay_in_place():
+    S, n, H, HK, d, slots = 1, 5, 4, 2, 128, 6
+    q, k, v, dev, qw, kw, _, kc, vc, pos = store_case(S, n, H, HK, d, d, slots, B.F16, 11)
+    rows = torch.tensor([[[-1, 0, 6, 5, 2 ** 31 - 1], [3, -2 ** 31, 1, 100, 2]]], dtype=torch.int32)
+    sp, sm = torch.full((S, HK, slots), 7, dtype=torch.int32, device="cuda"), torch.full((S, HK, slots), 3.0, device="cuda")
+    kg, vg = kc.cuda(), vc.cuda()
+    want, err = store_oracle(q, qw, 1e-6, pos, d, 2)
+    qo = ops.qk_norm_rope(dev["q"], dev["k"], dev["v"], qw.cuda(), kw.cuda(), 1e-6, pos.cuda(), kg, vg, B.F16, rows=rows.cuda(), slot_pos=sp, slot_mass=sm,
+                          q_out=dev["q"].transpose(1, 2))
+    assert qo.data_ptr() == dev["q"].data_ptr() and ((qo.cpu().double() - want).abs() <= err).all()
+    wk, e = store_oracle(k, kw, 1e-6, pos, d, 2)
+    for h in range(HK):
+        for i in range(n):
+            r = int(rows[0, h, i])
+            if 0 <= r < slots:
+                assert ((kg[0, h, r].cpu().double() - wk[0, h, i]).abs() <= e[0, h, i] + U16 * (wk[0, h, i].abs() + e[0, h, i]) + 2.0 ** -25).all()
+                assert torch.equal(vg[0, h, r].cpu(), v[0, i, h].half()) and int(sp[0, h, r]) == int(pos[0, i]) and float(sm[0, h, r]) == 0.0
+        for r in set(range(slots)) - set(rows[0, h].tolist()):
+            assert torch.equal(kg[0, h, r].cpu(), kc[0, h, r]) and torch.equal(vg[0, h, r].cpu(), vc[0, h, r])
+            assert int(sp[0, h, r]) == 7 and float(sm[0, h, r]) == 3.0
+
+
+def test_store_without_v_without_rows_of_nothing_and_of_zeros():
+    q, k, _, dev, qw, kw, _, kc, _, pos = store_case(1, 3, 2, 1, 64, 64, 3, B.F16, 12)
+    q[0, 1] = 0.0                                 # a row of zeros normalises to zeros
+    kg = kc.cuda()
+    qo = ops.qk_norm_rope(q.cuda(), dev["k"], None, qw.cuda(), kw.cuda(), 1e-6, pos.cuda(), kg, None, B.F16)
+    want, err = store_oracle(q, qw, 1e-6, pos, 64, 2)
+    assert ((qo.cpu().double() - want).abs() <= err).all() and (qo[0, :, 1] == 0).all()
+    check_rows(kg.cpu(), kc, torch.arange(3)[None, None], *store_oracle(k, kw, 1e-6, pos, 64, 2), B.F16)
+    none = torch.zeros((1, 0, 2, 64), device="cuda")
+    out = ops.qk_norm_rope(none, none[:, :, :1], None, None, None, 1e-6, pos.cuda()[:, :0], kg, None, B.F16)
+    assert out.shape == (1, 2, 0, 64)
+
+
+def test_store_on_another_stream_and_captured():
+    """launched on the current stream whatever it is; a captured launch reads new rows and positions at every replay"""
+    S, n, H, HK, d, slots = 2, 1, 8, 2, 128, 16
+    q, k, v, dev, qw, kw, rows, kc, vc, pos = store_case(S, n, H, HK, d, d, slots, B.F16, 13)
+    qg, kg, vg, rg, pg, qwg, kwg = dev["q"], kc.cuda(), vc.cuda(), rows.cuda(), pos.cuda(), qw.cuda(), kw.cuda()
+    qo = torch.empty((S, H, n, d), device="cuda")
+    run = lambda: ops.qk_norm_rope(qg, dev["k"], dev["v"], qwg, kwg, 1e-6, pg, kg, vg, B.F16, rows=rg, q_out=qo)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    g = gen(4)
+    for _ in range(4):
+        rows = torch.stack([torch.randperm(slots, generator=g)[:n] for _ in range(S * HK)]).reshape(S, HK, n).to(torch.int32)
+        pos = torch.randint(0, 100000, (S, n), generator=g).to(torch.int32)
+        before = kg.cpu()
+        rg.copy_(rows); pg.copy_(pos); qo.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, err = store_oracle(q, qw, 1e-6, pos, d, 2)
+        assert ((qo.cpu().double() - want).abs() <= err).all()
+        check_rows(kg.cpu(), before, rows, *store_oracle(k, kw, 1e-6, pos, d, 2), B.F16)
+
+
+def test_store_wrapper_refuses_what_does_not_fit():
+    q, k, v, dev, qw, kw, rows, kc, vc, pos = store_case(1, 2, 4, 2, 64, 64, 4, B.F16, 14)
+    a = [dev["q"], dev["k"], dev["v"], qw.cuda(), kw.cuda(), 1e-6, pos.cuda(), kc.cuda(), vc.cuda(), B.F16]
+    for i, bad in ((0, dev["q"].half()), (1, dev["k"][:, :1]), (2, None), (6, pos.cuda().long()), (7, kc.cuda().bfloat16()), (7, kc.cuda()[..., :32]),
+                   (8, vc.cuda()[:, :, :3]), (3, qw), (9, B.Q4_K)):
+        b = list(a)
+        b[i] = bad
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope(*b)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope(*a, rows=rows.cuda().long())
+    with pytest.raises(K.Mi355Error):
+        ops.qk_norm_rope(*a, mode=1)
+    with pytest.raises(K.Mi355Error):
+        ops.qk_norm_rope(dev["q"][..., 4:36], dev["k"][..., 4:36], None, None, None, 1e-6, pos.cuda(), kc.cuda()[..., 4:36], None, B.F16)   # 8-byte aligned cache
