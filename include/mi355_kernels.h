@@ -66,7 +66,7 @@ MI355_API int         mi355_abi_version(void);          /* == MI355_ABI_VERSION 
                                                          * the plugin and the Python binding refuse a library that differs */
 MI355_API int64_t     mi355_args_sizeof(int which);     /* sizeof of 0 mi355_mmvq_args, 1 qkv_rope, 2 glu_matvec, 3 moe_down,
                                                          * 4 fattn_args, 5 mi355_tensor, 6 qkv_finish_args, 7 decode_layer_args,
-                                                         * 8 qk_norm_rope_args; -1 otherwise */
+                                                         * 8 qk_norm_rope_args, 9 kv_evict_args; -1 otherwise */
 MI355_API const char *mi355_error_string(int err);      /* MI355_E_* or hipGetErrorString */
 MI355_API int64_t     mi355_blck_size(int type);        /* elements per block, 0 if unknown */
 MI355_API int64_t     mi355_type_size(int type);        /* bytes per block, 0 if unknown */
@@ -771,6 +771,34 @@ typedef struct mi355_qk_norm_rope_args {
     float eps, freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow;
 } mi355_qk_norm_rope_args;
 MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stream);
+
+/* The slots of a bounded cache that stay, per (sequence, KV head): of the first n_used[i3] slots the n_keep with the largest mass, where a slot
+ * whose position is below n_sink or at least n_past[i3] - n_recent counts as +inf; ties go to the lower slot, NaN counts as -inf.
+ *   mass f32, slot_pos int32 [n_kv, n_head_kv, ne3] (strides nb2 / nb3); n_used int32 [ne3] (NULL: n_kv; clamped to [0, n_kv]); n_past int32
+ *   [ne3]: tokens the sequence has seen.  All read on the device: a captured call follows them.
+ *   kept int32 [n_keep, n_head_kv, ne3]: the kept slots, ascending, -1 behind the last where n_used < n_keep
+ *   evicted int32 [n_evict, n_head_kv, ne3] or NULL: the first n_evict of the other slots in use, ascending, -1 behind the last -- what the next
+ *   mi355_qk_norm_rope takes as rows.
+ *   k, v / k_out, v_out (optional): the kept rows, gathered into other memory in kept's order (type_kv, rows of d and dv values, strides nb1
+ *   (slot) / nb2 / nb3; 2-byte aligned, faster at 16); rows behind the last kept one stay as they were.  mass_out, pos_out [n_keep, ..] (optional): the
+ *   tables of the gathered rows, 0 and -1 behind the last.
+ * n_sink + n_recent <= n_keep, n_keep >= 1, else MI355_E_SHAPE. */
+typedef struct mi355_kv_evict_args {
+    const float *mass; int64_t mass_nb2, mass_nb3;
+    const int32_t *slot_pos; int64_t pos_nb2, pos_nb3;
+    const int32_t *n_used, *n_past;
+    int32_t *kept; int64_t kept_nb2, kept_nb3;
+    int32_t *evicted; int64_t ev_nb2, ev_nb3;
+    const void *k; int64_t k_nb1, k_nb2, k_nb3;
+    const void *v; int64_t v_nb1, v_nb2, v_nb3;
+    void *k_out; int64_t ko_nb1, ko_nb2, ko_nb3;
+    void *v_out; int64_t vo_nb1, vo_nb2, vo_nb3;
+    float *mass_out; int64_t mo_nb2, mo_nb3;
+    int32_t *pos_out; int64_t po_nb2, po_nb3;
+    int64_t n_kv, n_keep, n_evict, n_head_kv, ne3, d, dv;      /* dv 0: d */
+    int32_t type_kv, n_sink, n_recent;
+} mi355_kv_evict_args;
+MI355_API int mi355_kv_evict(const mi355_kv_evict_args *args, void *stream);
 
 #ifdef __cplusplus
 }

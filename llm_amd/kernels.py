@@ -28,7 +28,7 @@ EXPORTS = [
     "mi355_dequantize_row", "mi355_mul_mat_vec_q", "mi355_mul_mat_q", "mi355_mul_mat_skinny", "mi355_mul_mat_skinny_slice", "mi355_quantize_act_q8k", "mi355_mul_mat_skinny_k", "mi355_mul_mat_skinny_k_slice", "mi355_mul_mat_skinny_k_group", "mi355_mul_mat_qk", "mi355_mul_mat_id_skinny_workspace_bytes", "mi355_mul_mat_id_skinny", "mi355_mul_mat_id_skinny_pair", "mi355_argsort_f32", "mi355_moe_router_f32", "mi355_sum_rows_f32", "mi355_mul_mat_f32", "mi355_mul_mat_dq", "mi355_mul_mat_dq_slice", "mi355_kv_store_q8_0", "mi355_mul_mat_dq_slice_ws", "mi355_glu_mul_mat_dq", "mi355_mul_mat_dq_parts_bytes", "mi355_mul_mat_dq_parts", "mi355_mul_mat_dq_parts_pair", "mi355_qkv_finish", "mi355_mul_mat_dq_workspace_bytes", "mi355_act_bf16", "mi355_mul_mat_id_dq_workspace_bytes", "mi355_mul_mat_id_dq", "mi355_mul_mat_workspace_bytes", "mi355_mul_mat",
     "mi355_decode_layer_sync_bytes", "mi355_decode_layer", "mi355_stream_read", "mi355_map_f32", "mi355_norm_f32",
     "mi355_mul_mat_id_tables_bytes", "mi355_mul_mat_id_skinny_ex", "mi355_moe_router_norm_f32", "mi355_kv_store_q", "mi355_moe_combine2_f32",
-    "mi355_qk_norm_rope",
+    "mi355_qk_norm_rope", "mi355_kv_evict",
 ]
 
 
@@ -155,6 +155,19 @@ class QkNormRopeArgs(C.Structure):
     ]
 
 
+class KvEvictArgs(C.Structure):
+    """mi355_kv_evict_args (include/mi355_kernels.h)"""
+    _fields_ = [
+        ("mass", _vp), ("mass_nb2", _i64), ("mass_nb3", _i64), ("slot_pos", _vp), ("pos_nb2", _i64), ("pos_nb3", _i64), ("n_used", _vp), ("n_past", _vp),
+        ("kept", _vp), ("kept_nb2", _i64), ("kept_nb3", _i64), ("evicted", _vp), ("ev_nb2", _i64), ("ev_nb3", _i64),
+        ("k", _vp), ("k_nb1", _i64), ("k_nb2", _i64), ("k_nb3", _i64), ("v", _vp), ("v_nb1", _i64), ("v_nb2", _i64), ("v_nb3", _i64),
+        ("k_out", _vp), ("ko_nb1", _i64), ("ko_nb2", _i64), ("ko_nb3", _i64), ("v_out", _vp), ("vo_nb1", _i64), ("vo_nb2", _i64), ("vo_nb3", _i64),
+        ("mass_out", _vp), ("mo_nb2", _i64), ("mo_nb3", _i64), ("pos_out", _vp), ("po_nb2", _i64), ("po_nb3", _i64),
+        ("n_kv", _i64), ("n_keep", _i64), ("n_evict", _i64), ("n_head_kv", _i64), ("ne3", _i64), ("d", _i64), ("dv", _i64),
+        ("type_kv", _i32), ("n_sink", _i32), ("n_recent", _i32),
+    ]
+
+
 TAIL_NONE, TAIL_QKV, TAIL_ROWS = 0, 1, 2
 
 lib.mi355_abi_version.restype = C.c_int
@@ -249,6 +262,7 @@ lib.mi355_decode_layer_sync_bytes.restype = _i64
 lib.mi355_decode_layer_sync_bytes.argtypes = []
 lib.mi355_decode_layer.argtypes = [C.POINTER(DecodeLayerArgs), _vp, _vp]
 lib.mi355_qk_norm_rope.argtypes = [C.POINTER(QkNormRopeArgs), _vp]
+lib.mi355_kv_evict.argtypes = [C.POINTER(KvEvictArgs), _vp]
 
 
 lib.mi355_timing_enable.argtypes = [C.c_int]
@@ -289,7 +303,8 @@ def check(code, where):
 
 
 # the hand-kept ctypes mirrors must have the C structs' sizes (a stale library or binding would read struct tails as garbage)
-for _which, _cls in enumerate((MmvqArgs, QkvRopeArgs, GluMatvecArgs, MoeDownArgs, FattnArgs, Tensor, QkvFinishArgs, DecodeLayerArgs, QkNormRopeArgs)):
+for _which, _cls in enumerate((MmvqArgs, QkvRopeArgs, GluMatvecArgs, MoeDownArgs, FattnArgs, Tensor, QkvFinishArgs, DecodeLayerArgs, QkNormRopeArgs,
+                              KvEvictArgs)):
     if lib.mi355_args_sizeof(_which) != C.sizeof(_cls):
         raise ImportError(f"{_cls.__name__}: ctypes mirror is {C.sizeof(_cls)} bytes, the library's struct {lib.mi355_args_sizeof(_which)}")
 

@@ -592,3 +592,53 @@ def qk_norm_rope(q, k, v, q_norm, k_norm, eps, pos, k_cache, v_cache, type_kv, r
     a.freq_base, a.freq_scale, a.ext_factor, a.attn_factor, a.beta_fast, a.beta_slow = freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow
     K.check(K.lib.mi355_qk_norm_rope(a, _stream()), "mi355_qk_norm_rope")
     return q_out
+
+
+def kv_evict(mass, slot_pos, n_past, n_keep, n_sink=0, n_recent=0, n_used=None, n_evict=None, k=None, v=None, type_kv=B.F16, d=None, k_out=None, v_out=None):
+    """The slots to keep (mi355_kv_evict): mass f32, slot_pos int32 [seqs, kv heads, slots] (slots contiguous), n_past / n_used int32 [seqs]
+    -> (kept int32 [seqs, kv heads, n_keep], evicted int32 [.., n_evict]); n_evict None: slots - n_keep.  With caches k, v [seqs, kv heads,
+    slots, row] of type_kv their kept rows are gathered too, into k_out, v_out [seqs, kv heads, n_keep, row] (None: new)
+    -> (kept, evicted, mass of the kept, positions of the kept), or (.., k_out, v_out) where those were None."""
+    _here(mass, slot_pos, n_past, n_used, k, v, k_out, v_out)
+    S, hk, slots = mass.shape
+    if mass.dtype != torch.float32 or slot_pos.dtype != torch.int32 or slot_pos.shape != mass.shape or (slots > 1 and (mass.stride(2) != 1 or slot_pos.stride(2) != 1)):
+        raise ValueError("mass f32, slot_pos int32: [seqs, kv heads, slots], slots contiguous")
+    for t in (n_past, n_used):
+        if t is not None and (t.dtype != torch.int32 or t.numel() != S or not t.is_contiguous()):
+            raise ValueError("n_past, n_used: int32 [seqs]")
+    if (k is None) != (v is None) or (k_out is None) != (v_out is None) or (k is None and k_out is not None):
+        raise ValueError("k and v, and k_out and v_out, come together")
+    n_evict = max(0, slots - n_keep) if n_evict is None else n_evict
+    a, new = K.KvEvictArgs(), k is not None and k_out is None
+    lists = torch.empty((S, hk, max(n_keep, 0) + max(n_evict, 0)), dtype=torch.int32, device=mass.device)
+    kept, evicted = lists[..., :n_keep], lists[..., n_keep:]
+    st = lambda t, *i: [t.stride(j) * t.element_size() for j in i]  # noqa: E731
+    a.mass, (a.mass_nb2, a.mass_nb3) = mass.data_ptr(), st(mass, 1, 0)
+    a.slot_pos, (a.pos_nb2, a.pos_nb3) = slot_pos.data_ptr(), st(slot_pos, 1, 0)
+    a.n_used, a.n_past = n_used.data_ptr() if n_used is not None else None, n_past.data_ptr()
+    a.kept, (a.kept_nb2, a.kept_nb3) = kept.data_ptr(), st(kept, 1, 0)
+    a.evicted, (a.ev_nb2, a.ev_nb3) = evicted.data_ptr() if n_evict > 0 else None, st(evicted, 1, 0)
+    a.n_kv, a.n_keep, a.n_evict, a.n_head_kv, a.ne3 = slots, n_keep, n_evict, hk, S
+    a.type_kv, a.n_sink, a.n_recent = type_kv, n_sink, n_recent
+    if k is not None:
+        dk, dv = _kv_rows(k, type_kv, "k"), _kv_rows(v, type_kv, "v")
+        if tuple(k.shape[:3]) != (S, hk, slots) or tuple(v.shape[:3]) != (S, hk, slots) or (d is not None and d != dk):
+            raise ValueError("k, v: [seqs, kv heads, slots, row] beside mass")
+        if new:
+            k_out, v_out = (torch.zeros((S, hk, n_keep, t.shape[3]), dtype=t.dtype, device=t.device) for t in (k, v))
+        for t, o in ((k, k_out), (v, v_out)):
+            if o.dtype != t.dtype or tuple(o.shape) != (S, hk, n_keep, t.shape[3]) or (o.shape[3] > 1 and o.stride(3) != 1):
+                raise ValueError("k_out, v_out: [seqs, kv heads, n_keep, row] of the caches' type")
+        mass_out = torch.empty((S, hk, n_keep), dtype=torch.float32, device=mass.device)
+        pos_out = torch.empty((S, hk, n_keep), dtype=torch.int32, device=mass.device)
+        a.k, (a.k_nb1, a.k_nb2, a.k_nb3) = k.data_ptr(), st(k, 2, 1, 0)
+        a.v, (a.v_nb1, a.v_nb2, a.v_nb3) = v.data_ptr(), st(v, 2, 1, 0)
+        a.k_out, (a.ko_nb1, a.ko_nb2, a.ko_nb3) = k_out.data_ptr(), st(k_out, 2, 1, 0)
+        a.v_out, (a.vo_nb1, a.vo_nb2, a.vo_nb3) = v_out.data_ptr(), st(v_out, 2, 1, 0)
+        a.mass_out, (a.mo_nb2, a.mo_nb3) = mass_out.data_ptr(), st(mass_out, 1, 0)
+        a.pos_out, (a.po_nb2, a.po_nb3) = pos_out.data_ptr(), st(pos_out, 1, 0)
+        a.d, a.dv = dk, dv
+    K.check(K.lib.mi355_kv_evict(a, _stream()), "mi355_kv_evict")
+    if k is None:
+        return kept, evicted
+    return (kept, evicted, mass_out, pos_out) + ((k_out, v_out) if new else ())

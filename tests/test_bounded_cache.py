@@ -46,3 +46,37 @@ def test_qk_norm_rope_of_nothing_launches_nothing():
     assert K.lib.mi355_qk_norm_rope(None, None) == E_NULL
     assert K.lib.mi355_qk_norm_rope(store_args(n=0), None) == 0
     assert K.lib.mi355_qk_norm_rope(store_args(ne3=0), None) == 0
+
+
+def evict_args(**kw):
+    a = K.KvEvictArgs()
+    for i, f in enumerate(("mass", "slot_pos", "n_past", "kept", "evicted", "k", "v", "k_out", "v_out", "mass_out", "pos_out")):
+        setattr(a, f, P * (i + 1))
+    for f in ("mass", "pos", "kept", "ev", "k", "v", "ko", "vo", "mo", "po"):
+        setattr(a, f + "_nb2", 4096)
+        setattr(a, f + "_nb3", 1 << 16)
+        if f in ("k", "v", "ko", "vo"):
+            setattr(a, f + "_nb1", 256)
+    a.n_kv, a.n_keep, a.n_evict, a.n_head_kv, a.ne3, a.d, a.dv, a.type_kv = 100, 50, 50, 2, 1, 128, 0, B.F16
+    for f, v in kw.items():
+        setattr(a, f, v)
+    return a
+
+
+@pytest.mark.parametrize("code, kw", [
+    (E_NULL, dict(mass=None)), (E_NULL, dict(slot_pos=None)), (E_NULL, dict(n_past=None)), (E_NULL, dict(kept=None)), (E_NULL, dict(k=None)),
+    (E_NULL, dict(v_out=None)),
+    (E_SHAPE, dict(n_kv=-1)), (E_SHAPE, dict(n_kv=1 << 32)), (E_SHAPE, dict(n_keep=0)), (E_SHAPE, dict(n_evict=-1)), (E_SHAPE, dict(n_sink=-1)),
+    (E_SHAPE, dict(n_sink=26, n_recent=25)), (E_SHAPE, dict(n_recent=51)), (E_SHAPE, dict(n_sink=2 ** 31 - 1, n_recent=2 ** 31 - 1)),
+    (E_SHAPE, dict(n_head_kv=0)), (E_SHAPE, dict(ne3=-1)), (E_SHAPE, dict(ne3=65536)), (E_SHAPE, dict(d=0)), (E_SHAPE, dict(type_kv=B.Q8_0, d=40)),
+    (E_SHAPE, dict(type_kv=B.Q4_0, dv=8)), (E_TYPE, dict(type_kv=B.Q4_K)), (E_TYPE, dict(type_kv=99)),
+    (E_ALIGN, dict(mass=P + 2)), (E_ALIGN, dict(kept_nb2=6)), (E_ALIGN, dict(k_out=P + 1)), (E_ALIGN, dict(v_nb1=257)),
+    (E_UNSUPPORTED, dict(k_out=6 * P)), (E_UNSUPPORTED, dict(v_out=7 * P)), (E_UNSUPPORTED, dict(mass_out=P)), (E_UNSUPPORTED, dict(pos_out=2 * P)),
+])
+def test_kv_evict_refuses(code, kw):
+    assert K.lib.mi355_kv_evict(evict_args(**kw), None) == code
+
+
+def test_kv_evict_of_no_sequences_launches_nothing():
+    assert K.lib.mi355_kv_evict(None, None) == E_NULL
+    assert K.lib.mi355_kv_evict(evict_args(ne3=0), None) == 0

@@ -263,3 +263,128 @@ def test_store_wrapper_refuses_what_does_not_fit():
         ops.qk_norm_rope(*a, mode=1)
     with pytest.raises(K.Mi355Error):
         ops.qk_norm_rope(dev["q"][..., 4:36], dev["k"][..., 4:36], None, None, None, 1e-6, pos.cuda(), kc.cuda()[..., 4:36], None, B.F16)   # 8-byte aligned cache
+
+
+# ---- kv_evict ------------------------------------------------------------------------------------------------------------------------
+
+def evict_oracle(mass, pos, past, used, n_keep, n_evict, sink, recent):
+    """numpy: (kept, evicted) by a stable sort of the keys"""
+    S, HK, n = mass.shape
+    kept, evicted = np.full((S, HK, n_keep), -1, np.int32), np.full((S, HK, n_evict), -1, np.int32)
+    for s in range(S):
+        u = min(max(int(used[s]), 0), n)
+        for h in range(HK):
+            key = mass[s, h, :u].astype(np.float64)
+            key = np.where(np.isnan(key), -np.inf, key)
+            p = pos[s, h, :u].astype(np.int64)
+            key = np.where((p < sink) | (p >= int(past[s]) - recent), np.inf, key)
+            order = np.lexsort((np.arange(u), -key))
+            k, e = np.sort(order[:n_keep]), np.sort(order[n_keep:])[:n_evict]
+            kept[s, h, :len(k)], evicted[s, h, :len(e)] = k, e
+    return kept, evicted
+
+
+def evict_case(S, HK, n, seed, kind="spread"):
+    r = np.random.default_rng(seed)
+    mass = (r.random((S, HK, n)) ** 6 * 20).astype(np.float32)
+    if kind == "ties":
+        mass = r.integers(0, 3, (S, HK, n)).astype(np.float32)
+        mass[r.random(mass.shape) < 0.2] = -0.0
+    elif kind == "equal":
+        mass[:] = 0.25
+    elif kind == "odd":                  # infinities, NaNs, negative and subnormal values, neighbours in the last bit
+        pool = np.array([np.inf, -np.inf, np.nan, -np.nan, 0.0, -0.0, 1e-45, -1e-45, 1.0, np.nextafter(np.float32(1), np.float32(2)), -1.0, 3e38, -3e38], np.float32)
+        mass = pool[r.integers(0, len(pool), (S, HK, n))]
+    pos = np.stack([r.permutation(2 * n + 3)[:n] for _ in range(S * HK)]).reshape(S, HK, n).astype(np.int32)
+    return mass, pos
+
+
+EVICT = [
+    # S, HK, n_kv, n_keep, sink, recent, used, kind
+    (1, 1, 1, 1, 0, 0, None, "spread"), (1, 2, 2, 1, 0, 0, None, "spread"), (2, 3, 65, 64, 4, 16, None, "spread"), (1, 8, 2049, 2048, 4, 512, None, "spread"),
+    (3, 2, 1000, 100, 4, 25, [1000, 100, 99], "ties"), (4, 1, 777, 300, 0, 0, [0, 1, 301, 5000], "equal"), (2, 2, 500, 123, 0, 0, [-7, 500], "odd"),
+    (1, 2, 4097, 17, 17, 0, None, "ties"), (1, 2, 5000, 4999, 0, 4999, None, "odd"), (1, 1, 100, 200, 10, 10, None, "spread"),
+    (2, 4, 32768, 4096, 4, 1024, [32768, 20001], "spread"), (1, 2, 70001, 9000, 4, 100, None, "ties"), (1, 1, 140000, 100000, 4, 100, None, "odd"),
+]
+
+
+@pytest.mark.parametrize("S,HK,n,n_keep,sink,recent,used,kind", EVICT)
+def test_evict_picks_the_heaviest(S, HK, n, n_keep, sink, recent, used, kind):
+    mass, pos = evict_case(S, HK, n, n + n_keep, kind)
+    past = np.full(S, 2 * n + 3, np.int32)
+    u = np.array(used if used is not None else [n] * S, np.int32)
+    for n_evict in {max(0, n - n_keep), min(1, n - n_keep) if n > n_keep else 0}:
+        kept, evicted = ops.kv_evict(torch.from_numpy(mass).cuda(), torch.from_numpy(pos).cuda(), torch.from_numpy(past).cuda(), n_keep, sink, recent,
+                                     n_used=torch.from_numpy(u).cuda() if used is not None else None, n_evict=n_evict)
+        wk, we = evict_oracle(mass, pos, past, u, n_keep, n_evict, sink, recent)
+        assert np.array_equal(kept.cpu().numpy(), wk) and np.array_equal(evicted.cpu().numpy(), we)
+
+
+@pytest.mark.parametrize("t,d,dv", [(B.F16, 128, 128), (B.Q8_0, 128, 96), (B.Q4_0, 64, 64), (B.BF16, 72, 40), (B.F32, 256, 256), (B.F16, 1, 3)])
+def test_evict_gathers_rows_as_they_are(t, d, dv):
+    """rows byte for byte, tables beside them; rows behind the last kept one, and memory around the views, stay as they were"""
+    S, HK, n, n_keep = 2, 3, 300, 90
+    mass, pos = evict_case(S, HK, n, d + dv)
+    past, u = np.full(S, 2 * n + 3, np.int32), np.array([n, 60], np.int32)
+    rb = lambda m: B.row_size(t, m)  # noqa: E731
+    g = gen(9)
+    raw = [torch.randint(0, 256, (S, n, HK, rb(m) + 32), generator=g).to(torch.uint8).cuda() for m in (d, dv)]             # slot-major storage, padded rows
+    out = [torch.full((S, HK, n_keep + 2, rb(m) + 16), 77, dtype=torch.uint8, device="cuda") for m in (d, dv)]
+    view = lambda x, m: x[..., 16:16 + rb(m)] if t in (B.Q8_0, B.Q4_0) else x[..., 16:16 + rb(m)].view(DTYPE[t])  # noqa: E731
+    src = [view(x, m).transpose(1, 2) for x, m in zip(raw, (d, dv))]
+    dst = [(x[..., :rb(m)] if t in (B.Q8_0, B.Q4_0) else x[..., :rb(m)].view(DTYPE[t]))[:, :, :n_keep] for x, m in zip(out, (d, dv))]
+    kept, evicted, mo, po = ops.kv_evict(torch.from_numpy(mass).cuda(), torch.from_numpy(pos).cuda(), torch.from_numpy(past).cuda(), n_keep, 4, 20,
+                                         n_used=torch.from_numpy(u).cuda(), k=src[0], v=src[1], type_kv=t, k_out=dst[0], v_out=dst[1])
+    wk, _ = evict_oracle(mass, pos, past, u, n_keep, 0, 4, 20)
+    assert np.array_equal(kept.cpu().numpy(), wk)
+    wm, wp = np.zeros((S, HK, n_keep), np.float32), np.full((S, HK, n_keep), -1, np.int32)
+    want = [torch.full_like(x.cpu(), 77) for x in out]
+    for s in range(S):
+        for h in range(HK):
+            k = wk[s, h][wk[s, h] >= 0]
+            wm[s, h, :len(k)], wp[s, h, :len(k)] = mass[s, h, k], pos[s, h, k]
+            for w, x, m in zip(want, raw, (d, dv)):
+                w[s, h, :len(k), :rb(m)] = x[s, :, h, 16:16 + rb(m)].cpu()[torch.from_numpy(k).long()]
+    assert np.array_equal(mo.cpu().numpy(), wm) and np.array_equal(po.cpu().numpy(), wp)
+    for w, x in zip(want, out):
+        assert torch.equal(x.cpu(), w)
+
+
+def test_evict_new_outputs_captured_and_refusals():
+    S, HK, n, n_keep = 2, 2, 600, 128
+    mass, pos = evict_case(S, HK, n, 1)
+    past = torch.tensor([2 * n + 3] * S, dtype=torch.int32).cuda()
+    m, p = torch.from_numpy(mass).cuda(), torch.from_numpy(pos).cuda()
+    k, v = (torch.randn((S, HK, n, 64), generator=gen(s)).half().cuda() for s in (1, 2))
+    used = torch.tensor([n, n], dtype=torch.int32).cuda()
+    run = lambda: ops.kv_evict(m, p, past, n_keep, 4, 32, n_used=used, k=k, v=v)  # noqa: E731
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept, evicted, mo, po, ko, vo = run()
+    for seed, u in ((2, [600, 600]), (3, [600, 50]), (4, [0, 599]), (5, [600, 128])):
+        mass, pos = evict_case(S, HK, n, seed)
+        m.copy_(torch.from_numpy(mass)); p.copy_(torch.from_numpy(pos)); used.copy_(torch.tensor(u, dtype=torch.int32))
+        ko.zero_(); vo.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        wk, we = evict_oracle(mass, pos, past.cpu().numpy(), u, n_keep, n - n_keep, 4, 32)
+        assert np.array_equal(kept.cpu().numpy(), wk) and np.array_equal(evicted.cpu().numpy(), we)
+        for x, y in ((k, ko), (v, vo)):
+            for s in range(S):
+                for h in range(HK):
+                    i = torch.from_numpy(wk[s, h][wk[s, h] >= 0]).long()
+                    assert torch.equal(y[s, h, :len(i)].cpu(), x[s, h].cpu()[i]) and (y[s, h, len(i):] == 0).all()
+    with pytest.raises(K.Mi355Error):
+        ops.kv_evict(m, p, past, 0)
+    with pytest.raises(K.Mi355Error):
+        ops.kv_evict(m, p, past, 10, 6, 5)
+    with pytest.raises(K.Mi355Error):
+        ops.kv_evict(m, p, past, n, k=k, v=v, k_out=k, v_out=v)
+    for bad in (dict(k=k), dict(k=k, v=v.float()), dict(k=k, v=v, k_out=ko), dict(k=k, v=v[:, :, :5]), dict(n_used=used.long())):
+        with pytest.raises(ValueError):
+            ops.kv_evict(m, p, past, n_keep, **bad)
+    with pytest.raises(ValueError):
+        ops.kv_evict(m.double(), p, past, n_keep)
+    kept, evicted = ops.kv_evict(m[:, :, :0], p[:, :, :0], past, 3)
+    assert (kept == -1).all() and evicted.shape == (S, HK, 0)
