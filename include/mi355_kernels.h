@@ -66,7 +66,7 @@ MI355_API int         mi355_abi_version(void);          /* == MI355_ABI_VERSION 
                                                          * the plugin and the Python binding refuse a library that differs */
 MI355_API int64_t     mi355_args_sizeof(int which);     /* sizeof of 0 mi355_mmvq_args, 1 qkv_rope, 2 glu_matvec, 3 moe_down,
                                                          * 4 fattn_args, 5 mi355_tensor, 6 qkv_finish_args, 7 decode_layer_args,
-                                                         * 8 qk_norm_rope_args, 9 kv_evict_args; -1 otherwise */
+                                                         * 8 qk_norm_rope_args, 9 kv_evict_args, 10 attn_mass_args; -1 otherwise */
 MI355_API const char *mi355_error_string(int err);      /* MI355_E_* or hipGetErrorString */
 MI355_API int64_t     mi355_blck_size(int type);        /* elements per block, 0 if unknown */
 MI355_API int64_t     mi355_type_size(int type);        /* bytes per block, 0 if unknown */
@@ -771,6 +771,26 @@ typedef struct mi355_qk_norm_rope_args {
     float eps, freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow;
 } mi355_qk_norm_rope_args;
 MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stream);
+
+/* FLASH_ATTN_EXT of a decode step (at most MI355_MASS_MAX_Q queries per sequence) that also accumulates the attention weight every slot draws:
+ *   mass_out[j] = decay * mass_in[j] + sum over the queries and the heads that share the KV head of softmax(...)[j]
+ * args as for mi355_flash_attn_ext (K and V of one type).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be
+ * mass_out itself; NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate (the query is not rounded to the cache's type, the
+ * weights are not rounded before they meet V).  A slot hidden by the mask takes no part whatever its row holds; a query that sees no slot gives
+ * a row of zeros and no weight.  workspace: *_workspace_bytes, 16-byte aligned, no initial contents, not shared by calls that can overlap. */
+#define MI355_MASS_MAX_Q 8
+typedef struct mi355_attn_mass_args {
+    const float *mass_in; int64_t in_nb2, in_nb3;
+    float *mass_out; int64_t out_nb2, out_nb3;
+    float decay;
+} mi355_attn_mass_args;
+MI355_API int64_t mi355_flash_attn_ext_mass_workspace_bytes(const mi355_fattn_args *args);
+MI355_API int     mi355_flash_attn_ext_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace,
+                                            int64_t workspace_bytes, void *stream);
+/* The weights alone, for any number of queries (a prompt, or the last ones of it): v, dst and dv of args are not used. */
+MI355_API int64_t mi355_attn_mass_workspace_bytes(const mi355_fattn_args *args);
+MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace, int64_t workspace_bytes,
+                                  void *stream);
 
 /* The slots of a bounded cache that stay, per (sequence, KV head): of the first n_used[i3] slots the n_keep with the largest mass, where a slot
  * whose position is below n_sink or at least n_past[i3] - n_recent counts as +inf; ties go to the lower slot, NaN counts as -inf.

@@ -18,6 +18,7 @@ int64_t mi355_args_sizeof(int which) {
         case 7: return (int64_t)sizeof(mi355_decode_layer_args);
         case 8: return (int64_t)sizeof(mi355_qk_norm_rope_args);
         case 9: return (int64_t)sizeof(mi355_kv_evict_args);
+        case 10: return (int64_t)sizeof(mi355_attn_mass_args);
     }
     return -1;
 }

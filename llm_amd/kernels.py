@@ -28,7 +28,8 @@ EXPORTS = [
     "mi355_dequantize_row", "mi355_mul_mat_vec_q", "mi355_mul_mat_q", "mi355_mul_mat_skinny", "mi355_mul_mat_skinny_slice", "mi355_quantize_act_q8k", "mi355_mul_mat_skinny_k", "mi355_mul_mat_skinny_k_slice", "mi355_mul_mat_skinny_k_group", "mi355_mul_mat_qk", "mi355_mul_mat_id_skinny_workspace_bytes", "mi355_mul_mat_id_skinny", "mi355_mul_mat_id_skinny_pair", "mi355_argsort_f32", "mi355_moe_router_f32", "mi355_sum_rows_f32", "mi355_mul_mat_f32", "mi355_mul_mat_dq", "mi355_mul_mat_dq_slice", "mi355_kv_store_q8_0", "mi355_mul_mat_dq_slice_ws", "mi355_glu_mul_mat_dq", "mi355_mul_mat_dq_parts_bytes", "mi355_mul_mat_dq_parts", "mi355_mul_mat_dq_parts_pair", "mi355_qkv_finish", "mi355_mul_mat_dq_workspace_bytes", "mi355_act_bf16", "mi355_mul_mat_id_dq_workspace_bytes", "mi355_mul_mat_id_dq", "mi355_mul_mat_workspace_bytes", "mi355_mul_mat",
     "mi355_decode_layer_sync_bytes", "mi355_decode_layer", "mi355_stream_read", "mi355_map_f32", "mi355_norm_f32",
     "mi355_mul_mat_id_tables_bytes", "mi355_mul_mat_id_skinny_ex", "mi355_moe_router_norm_f32", "mi355_kv_store_q", "mi355_moe_combine2_f32",
-    "mi355_qk_norm_rope", "mi355_kv_evict",
+    "mi355_qk_norm_rope", "mi355_kv_evict", "mi355_flash_attn_ext_mass_workspace_bytes", "mi355_flash_attn_ext_mass", "mi355_attn_mass_workspace_bytes",
+    "mi355_attn_mass",
 ]
 
 
@@ -168,7 +169,13 @@ class KvEvictArgs(C.Structure):
     ]
 
 
+class AttnMassArgs(C.Structure):
+    """mi355_attn_mass_args (include/mi355_kernels.h)"""
+    _fields_ = [("mass_in", _vp), ("in_nb2", _i64), ("in_nb3", _i64), ("mass_out", _vp), ("out_nb2", _i64), ("out_nb3", _i64), ("decay", C.c_float)]
+
+
 TAIL_NONE, TAIL_QKV, TAIL_ROWS = 0, 1, 2
+MASS_MAX_Q = 8           # MI355_MASS_MAX_Q
 
 lib.mi355_abi_version.restype = C.c_int
 lib.mi355_args_sizeof.restype = _i64
@@ -263,6 +270,10 @@ lib.mi355_decode_layer_sync_bytes.argtypes = []
 lib.mi355_decode_layer.argtypes = [C.POINTER(DecodeLayerArgs), _vp, _vp]
 lib.mi355_qk_norm_rope.argtypes = [C.POINTER(QkNormRopeArgs), _vp]
 lib.mi355_kv_evict.argtypes = [C.POINTER(KvEvictArgs), _vp]
+for _n in ("mi355_flash_attn_ext_mass", "mi355_attn_mass"):
+    getattr(lib, _n).argtypes = [C.POINTER(FattnArgs), C.POINTER(AttnMassArgs), _vp, _i64, _vp]
+    getattr(lib, _n + "_workspace_bytes").argtypes = [C.POINTER(FattnArgs)]
+    getattr(lib, _n + "_workspace_bytes").restype = _i64
 
 
 lib.mi355_timing_enable.argtypes = [C.c_int]
@@ -304,7 +315,7 @@ def check(code, where):
 
 # the hand-kept ctypes mirrors must have the C structs' sizes (a stale library or binding would read struct tails as garbage)
 for _which, _cls in enumerate((MmvqArgs, QkvRopeArgs, GluMatvecArgs, MoeDownArgs, FattnArgs, Tensor, QkvFinishArgs, DecodeLayerArgs, QkNormRopeArgs,
-                              KvEvictArgs)):
+                              KvEvictArgs, AttnMassArgs)):
     if lib.mi355_args_sizeof(_which) != C.sizeof(_cls):
         raise ImportError(f"{_cls.__name__}: ctypes mirror is {C.sizeof(_cls)} bytes, the library's struct {lib.mi355_args_sizeof(_which)}")
 

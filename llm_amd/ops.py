@@ -642,3 +642,67 @@ def kv_evict(mass, slot_pos, n_past, n_keep, n_sink=0, n_recent=0, n_used=None, 
     if k is None:
         return kept, evicted
     return (kept, evicted, mass_out, pos_out) + ((k_out, v_out) if new else ())
+
+
+def _mass_args(q, k, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap):
+    """checks and arguments that flash_attn_ext_mass and attn_mass share -> (FattnArgs without V and dst, AttnMassArgs, mass_out)"""
+    _here(q, k, mask, mass, mass_out)
+    S, H, n, d = q.shape
+    if q.dtype != torch.float32 or q.stride(3) != 1:
+        raise ValueError("q: f32 [seqs, heads, tokens, d] with contiguous rows")
+    if _kv_rows(k, type_kv, "k") != d or k.shape[0] != S:
+        raise ValueError("k: [seqs, kv heads, slots, row] with rows of d values")
+    hk, slots = k.shape[1], k.shape[2]
+    a, w = K.FattnArgs(), K.AttnMassArgs()
+    a.q, a.q_nb1, a.q_nb2, a.q_nb3 = q.data_ptr(), q.stride(2) * 4, q.stride(1) * 4, q.stride(0) * 4
+    es = k.element_size()
+    a.k, a.type_k, a.k_nb1, a.k_nb2, a.k_nb3 = k.data_ptr(), type_kv, k.stride(2) * es, k.stride(1) * es, k.stride(0) * es
+    if mask is not None:
+        if mask.dim() == 2:
+            mask = mask[None, None]
+        elif mask.dim() == 3:
+            mask = mask[:, None]
+        if mask.element_size() != 2 or mask.dim() != 4 or mask.shape[2] < n or mask.shape[3] != slots or (slots > 1 and mask.stride(3) != 1):
+            raise ValueError("mask: f16 (or its bits) [seqs | 1, heads | 1, >= tokens, slots], the two first may be left out")
+        a.mask, a.m_nb1, a.m_nb2, a.m_nb3 = mask.data_ptr(), mask.stride(2) * 2, mask.stride(1) * 2, mask.stride(0) * 2
+        a.m_ne2, a.m_ne3 = mask.shape[1], mask.shape[0]
+    a.d, a.n_q, a.n_kv, a.n_head, a.n_head_kv, a.ne3 = d, n, slots, H, hk, S
+    a.scale, a.max_bias, a.logit_softcap = scale, max_bias, logit_softcap
+    if mass_out is None:
+        mass_out = torch.empty((S, hk, slots), dtype=torch.float32, device=q.device)
+    for t in (mass, mass_out):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (S, hk, slots) or (slots > 1 and t.stride(2) != 1)):
+            raise ValueError("mass, mass_out: f32 [seqs, kv heads, slots], slots contiguous")
+    if mass is not None:
+        w.mass_in, w.in_nb2, w.in_nb3 = mass.data_ptr(), mass.stride(1) * 4, mass.stride(0) * 4
+    w.mass_out, w.out_nb2, w.out_nb3, w.decay = mass_out.data_ptr(), mass_out.stride(1) * 4, mass_out.stride(0) * 4, decay
+    return a, w, mass_out
+
+
+def flash_attn_ext_mass(q, k, v, mask, type_kv, scale, mass=None, decay=1.0, mass_out=None, max_bias=0.0, logit_softcap=0.0):
+    """A decode step's attention and the weight every slot draws (mi355_flash_attn_ext_mass).  q f32 [seqs, heads, tokens <= 8, d], k, v
+    [seqs, kv heads, slots, row] of type_kv, mask f16 [seqs | 1, heads | 1, >= tokens, slots] (or [seqs | 1, tokens, slots], [tokens, slots],
+    None); mass f32 [seqs, kv heads, slots] or None; mass_out may be mass -> (f32 [seqs, tokens, heads, dv], mass_out = decay mass + weights)."""
+    a, w, mass_out = _mass_args(q, k, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
+    _here(v)
+    dv = _kv_rows(v, type_kv, "v")
+    if tuple(v.shape[:3]) != tuple(k.shape[:3]):
+        raise ValueError("v: [seqs, kv heads, slots, row] beside k")
+    S, H, n, _ = q.shape
+    dst = torch.empty((S, n, H, dv), dtype=torch.float32, device=q.device)
+    es = v.element_size()
+    a.v, a.type_v, a.v_nb1, a.v_nb2, a.v_nb3 = v.data_ptr(), type_kv, v.stride(2) * es, v.stride(1) * es, v.stride(0) * es
+    a.dst, a.d_nb1, a.d_nb2, a.d_nb3, a.dv = dst.data_ptr(), dv * 4, H * dv * 4, n * H * dv * 4, dv
+    need = K.lib.mi355_flash_attn_ext_mass_workspace_bytes(a)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    K.check(K.lib.mi355_flash_attn_ext_mass(a, w, ws.data_ptr(), need, _stream()), "mi355_flash_attn_ext_mass")
+    return dst, mass_out
+
+
+def attn_mass(q, k, mask, type_kv, scale, mass=None, decay=1.0, mass_out=None, max_bias=0.0, logit_softcap=0.0):
+    """The weight every slot draws from any number of queries (mi355_attn_mass); arguments as flash_attn_ext_mass, without V -> mass_out."""
+    a, w, mass_out = _mass_args(q, k, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
+    need = K.lib.mi355_attn_mass_workspace_bytes(a)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+    K.check(K.lib.mi355_attn_mass(a, w, ws.data_ptr(), need, _stream()), "mi355_attn_mass")
+    return mass_out

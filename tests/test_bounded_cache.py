@@ -80,3 +80,59 @@ def test_kv_evict_refuses(code, kw):
 def test_kv_evict_of_no_sequences_launches_nothing():
     assert K.lib.mi355_kv_evict(None, None) == E_NULL
     assert K.lib.mi355_kv_evict(evict_args(ne3=0), None) == 0
+
+
+def attn_args(**kw):
+    a, w = K.FattnArgs(), K.AttnMassArgs()
+    for f in ("q", "k", "v", "mask", "dst"):
+        setattr(a, f, P)
+    for f in ("q", "k", "v", "m", "d"):
+        for i, nb in enumerate((512, 4096, 1 << 16)):
+            setattr(a, f"{f}_nb{i + 1}", nb)
+    a.type_k = a.type_v = B.F16
+    a.d, a.n_q, a.n_kv, a.n_head, a.n_head_kv, a.ne3, a.dv, a.m_ne2, a.m_ne3, a.scale = 128, 1, 64, 8, 2, 1, 0, 1, 1, 0.1
+    w.mass_in = w.mass_out = P
+    w.in_nb2 = w.out_nb2 = 256
+    w.in_nb3 = w.out_nb3 = 1024
+    w.decay = 1.0
+    for f, v in kw.items():
+        setattr(w if f in ("mass_in", "mass_out", "in_nb2", "out_nb3", "decay") else a, f, v)
+    return a, w
+
+
+BOTH = [
+    (E_NULL, dict(q=None)), (E_NULL, dict(k=None)), (E_NULL, dict(mass_out=None)),
+    (E_UNSUPPORTED, dict(d=0)), (E_UNSUPPORTED, dict(d=100)), (E_UNSUPPORTED, dict(d=512)),
+    (E_TYPE, dict(type_k=B.F32, type_v=B.F32)), (E_TYPE, dict(type_k=B.Q4_K, type_v=B.Q4_K)),
+    (E_SHAPE, dict(type_k=B.Q8_0, type_v=B.Q8_0, d=80)), (E_SHAPE, dict(n_head=0)), (E_SHAPE, dict(n_head_kv=3)), (E_SHAPE, dict(n_head_kv=0)),
+    (E_SHAPE, dict(n_q=0)), (E_SHAPE, dict(n_q=65536)), (E_SHAPE, dict(n_kv=-1)), (E_SHAPE, dict(n_kv=1 << 31)), (E_SHAPE, dict(ne3=0)),
+    (E_SHAPE, dict(m_ne2=0)), (E_SHAPE, dict(m_ne3=0)), (E_SHAPE, dict(n_head=65536, n_head_kv=1)),
+    (E_ALIGN, dict(q=P + 4)), (E_ALIGN, dict(q_nb1=520)), (E_ALIGN, dict(k=P + 8)), (E_ALIGN, dict(k_nb1=264)), (E_ALIGN, dict(mask=P + 1)),
+    (E_ALIGN, dict(m_nb1=511)), (E_ALIGN, dict(mass_in=P + 2)), (E_ALIGN, dict(out_nb3=1022)), (E_ALIGN, dict(type_k=B.Q4_0, type_v=B.Q4_0, k_nb2=4097)),
+]
+
+
+@pytest.mark.parametrize("code, kw", BOTH + [
+    (E_NULL, dict(v=None)), (E_NULL, dict(dst=None)), (E_UNSUPPORTED, dict(dv=136)), (E_UNSUPPORTED, dict(dv=12)), (E_TYPE, dict(type_v=B.BF16)),
+    (E_SHAPE, dict(type_k=B.Q8_0, type_v=B.Q8_0, dv=40)), (E_UNSUPPORTED, dict(n_q=9)), (E_ALIGN, dict(v_nb3=8)), (E_ALIGN, dict(dst=P + 4)),
+])
+def test_flash_attn_ext_mass_refuses(code, kw):
+    assert K.lib.mi355_flash_attn_ext_mass(*attn_args(**kw), P, 1 << 40, None) == code
+
+
+@pytest.mark.parametrize("code, kw", BOTH)
+def test_attn_mass_refuses(code, kw):
+    assert K.lib.mi355_attn_mass(*attn_args(**{k: v for k, v in kw.items()}), P, 1 << 40, None) == code
+
+
+def test_attention_mass_workspaces():
+    for fn, size in ((K.lib.mi355_flash_attn_ext_mass, K.lib.mi355_flash_attn_ext_mass_workspace_bytes), (K.lib.mi355_attn_mass, K.lib.mi355_attn_mass_workspace_bytes)):
+        assert fn(None, None, P, 1 << 40, None) == E_NULL and size(None) == -1
+        for kw in (dict(), dict(n_q=7, n_kv=5000, ne3=3), dict(n_kv=100000, n_head=64, n_head_kv=8)):
+            a, w = attn_args(**kw)
+            need = size(a)
+            assert need >= 0
+            if need > 0:
+                assert fn(a, w, P, need - 1, None) == E_WORKSPACE and fn(a, w, None, 0, None) == E_WORKSPACE
+                assert fn(a, w, P + 4, need, None) == E_ALIGN
+    assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=-1)[0]) == -1

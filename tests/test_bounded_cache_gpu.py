@@ -388,3 +388,254 @@ def test_evict_new_outputs_captured_and_refusals():
         ops.kv_evict(m.double(), p, past, n_keep)
     kept, evicted = ops.kv_evict(m[:, :, :0], p[:, :, :0], past, 3)
     assert (kept == -1).all() and evicted.shape == (S, HK, 0)
+
+
+# ---- attention with the weight every slot draws ----------------------------------------------------------------------------------------
+
+def attn_oracle(q, k, v, mask, scale, mass, decay, max_bias=0.0, softcap=0.0):
+    """f64 on the CPU: (dst [S, n, H, dv] | None, its bound, mass, its bound).  q [S, H, n, d], k / v f64 values, mask f16 [1 | S, 1 | H, >= n, slots]"""
+    S, H, n, d = q.shape
+    HK, slots = k.shape[1], k.shape[2]
+    G = H // HK
+    kk = k.repeat_interleave(G, 1)
+    hidden = torch.zeros((1, 1, 1, slots), dtype=torch.bool) if mask is None else mask[:, :, :n].double() == float("-inf")
+    m = torch.zeros((1, 1, 1, slots), dtype=torch.float64) if mask is None else torch.where(hidden, 0.0, mask[:, :, :n].double())
+    if max_bias > 0:
+        p2 = 1 << int(math.floor(math.log2(H)))
+        m0, m1 = 2.0 ** (-max_bias / p2), 2.0 ** (-max_bias / 2 / p2)
+        sl = torch.tensor([m0 ** (h + 1) if h < p2 else m1 ** (2 * (h - p2) + 1) for h in range(H)], dtype=torch.float64)
+        m = m * sl[None, :, None, None]
+    qd = q.double()
+    ok = (~hidden).expand(S, H, n, slots)
+    # slots that no query sees may hold anything
+    seen = ok.any(1).any(1)[:, None, :, None] if mask is not None else None
+    clean = lambda x: x if seen is None else torch.where(seen, x, torch.zeros((), dtype=torch.float64))  # noqa: E731
+    kk = clean(kk)
+    dot, mag = qd @ kk.transpose(2, 3), qd.abs() @ kk.abs().transpose(2, 3)
+    s = softcap * torch.tanh(dot * scale / softcap) if softcap else dot * scale
+    s = s + m
+    # a logit: products and sum of d terms in any order, scale, mask; tanh to 8 steps
+    es = (d + 10) * U32 * abs(scale) * mag + 6 * U32 * (s.abs() + m.abs()) + (8 * U32 * abs(softcap))
+    es = torch.where(ok, es, torch.zeros((), dtype=torch.float64)).amax(-1, keepdim=True)
+    s = torch.where(ok, s, torch.full((), float("-inf"), dtype=torch.float64))
+    top = s.amax(-1, keepdim=True)
+    p = torch.where(ok, torch.exp(s - torch.where(top.isinf(), torch.zeros_like(top), top)), torch.zeros((), dtype=torch.float64))
+    tot = p.sum(-1, keepdim=True)
+    p = torch.where(tot > 0, p / tot, torch.zeros((), dtype=torch.float64))
+    # p: its logit and those of the sum, exp and its argument (|s - top| in steps of 2^-24), the sum of the slots in any order
+    span = torch.where(ok, (s - top).abs(), torch.zeros((), dtype=torch.float64))
+    span = torch.where(p > 1e-12, span, torch.zeros_like(span)).amax(-1, keepdim=True)
+    rel = 2 * es + (10 + slots + 4 * span) * U32
+    w = (p * (1 + 0 * rel)).reshape(S, HK, G * n, slots)
+    wm = w.sum(2) + (decay * mass.double() if mass is not None and decay != 0 else 0.0)
+    em = (p * rel).reshape(S, HK, G * n, slots).sum(2) + (G * n + 4) * U32 * wm.abs() + G * n * 2.0 ** -126
+    if v is None:
+        return None, None, wm, em
+    vv = clean(v.repeat_interleave(G, 1))
+    o = (p @ vv).transpose(1, 2)
+    eo = (((p * rel) @ vv.abs()) + (slots + 4) * U32 * (p @ vv.abs())).transpose(1, 2) + 2.0 ** -126
+    return o, eo, wm, em
+
+
+def check_attn(q, kc, vc, t, mask, scale, mass, decay, near=True, **kw):
+    """through both entry points (vc None: attn_mass alone)"""
+    dev = lambda x: x.cuda() if x is not None else None  # noqa: E731
+    k64, v64 = values(kc, t), values(vc, t) if vc is not None else None
+    wd, ed, wm, em = attn_oracle(q, k64, v64, mask[None, None] if mask is not None and mask.dim() == 2 else mask, scale, mass, decay, **kw)
+    o = dict(max_bias=kw.get("max_bias", 0.0), logit_softcap=kw.get("softcap", 0.0))
+    got = ops.attn_mass(dev(q), dev(kc), dev(mask), t, scale, mass=dev(mass), decay=decay, **o).cpu().double()
+    assert ((got - wm).abs() <= em).all(), float(((got - wm).abs() / em).max())
+    if vc is not None:
+        d1, m1 = ops.flash_attn_ext_mass(dev(q), dev(kc), dev(vc), dev(mask), t, scale, mass=dev(mass), decay=decay, **o)
+        d1, m1 = d1.cpu().double(), m1.cpu().double()
+        assert ((m1 - wm).abs() <= em).all(), float(((m1 - wm).abs() / em).max())
+        assert ((d1 - wd).abs() <= ed).all(), float(((d1 - wd).abs() / ed).max())
+        if near and wd.norm() > 0:       # roundings of random inputs do not add up: far below the bounds above, which hold for any input
+            assert (d1 - wd).norm() <= 1e-5 * wd.norm()
+    if near and wm.norm() > 0:
+        assert (got - wm).norm() <= 1e-5 * wm.norm()
+
+
+def attn_case(S, H, HK, n, slots, d, dv, t, seed, qscale=1.5):
+    g = gen(seed)
+    return (torch.randn((S, H, n, d), generator=g) * qscale, cache((S, HK, slots, d), t, g), cache((S, HK, slots, dv), t, g) if dv else None,
+            torch.rand((S, HK, slots), generator=g) * 2)
+
+
+def causal(S, n, slots, lens=None, pad=0):
+    lens = lens or [slots] * S
+    j, i = torch.arange(slots), torch.arange(n + pad)
+    m = torch.stack([torch.where(j[None] < torch.clamp(torch.tensor(L) - (n - 1 - i[:, None]), min=0), 0.0, float("-inf")) for L in lens])
+    return m.half()[:, None]
+
+
+ATTN = [
+    # S, H, HK, n, slots, d, dv, type
+    (1, 32, 8, 1, 512, 128, 128, B.F16), (1, 8, 8, 1, 1, 64, 64, B.F16), (1, 8, 2, 1, 2, 128, 128, B.Q8_0), (2, 4, 1, 2, 63, 64, 64, B.BF16),
+    (1, 16, 2, 3, 65, 128, 128, B.Q4_0), (3, 6, 2, 1, 257, 96, 64, B.F16), (1, 12, 1, 8, 130, 128, 128, B.F16), (2, 5, 5, 4, 300, 80, 80, B.F16),
+    (1, 8, 1, 5, 1000, 256, 256, B.F16), (1, 8, 1, 5, 1000, 256, 128, B.BF16), (1, 32, 8, 8, 777, 128, 128, B.Q8_0), (1, 64, 8, 1, 4099, 128, 128, B.F16),
+    (2, 32, 8, 1, 3000, 128, 128, B.Q4_0), (1, 2, 1, 1, 40, 8, 8, B.F16), (1, 32, 1, 8, 200, 64, 64, B.Q8_0), (1, 3, 1, 7, 129, 72, 40, B.BF16),
+    (4, 8, 4, 1, 1500, 32, 32, B.Q4_0), (1, 40, 8, 6, 520, 112, 112, B.F16), (1, 64, 1, 1, 333, 192, 128, B.F16), (9, 4, 2, 1, 31, 160, 96, B.Q8_0),
+]
+
+
+@pytest.mark.parametrize("S,H,HK,n,slots,d,dv,t", ATTN)
+def test_attention_mass_of_a_step(S, H, HK, n, slots, d, dv, t):
+    q, k, v, mass = attn_case(S, H, HK, n, slots, d, dv, t, slots + d)
+    lens = [max(n, slots - i * slots // (2 * S)) for i in range(S)]
+    check_attn(q, k, v, t, causal(S, n, slots, [min(L, slots) for L in lens], pad=3), 1 / math.sqrt(d), mass, 0.9)
+
+
+@pytest.mark.parametrize("S,H,HK,n,slots,d,t", [
+    (1, 8, 2, 17, 33, 64, B.F16), (1, 32, 8, 64, 1000, 128, B.F16), (2, 4, 1, 33, 300, 128, B.Q8_0), (1, 6, 2, 100, 100, 96, B.BF16), (1, 4, 4, 257, 257, 64, B.Q4_0),
+    (1, 5, 1, 70, 515, 256, B.F16), (1, 2, 2, 9, 2049, 80, B.F16), (3, 8, 8, 12, 140, 128, B.BF16), (1, 64, 8, 10, 130, 128, B.Q4_0), (1, 4, 2, 300, 900, 128, B.F16),
+    (1, 8, 1, 520, 520, 128, B.BF16), (1, 1, 1, 1, 5000, 128, B.Q8_0), (1, 3, 1, 130, 65, 8, B.F16),
+])
+def test_attention_mass_of_a_prompt(S, H, HK, n, slots, d, t):
+    q, k, _, mass = attn_case(S, H, HK, n, slots, d, 0, t, slots + n)
+    check_attn(q, k, None, t, causal(S, n, slots), 1 / math.sqrt(d), mass, 1.0)
+    check_attn(q, k, None, t, None, 1 / math.sqrt(d), None, 1.0)
+
+
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_attention_mass_masks(t, n):
+    """queries that see nothing, masks per head, biases, the lowest value in every place; hidden rows of NaN and infinities"""
+    S, H, HK, slots, d = 2, 8, 2, 200, 128
+    q, k, v, mass = attn_case(S, H, HK, n, slots, d, d if n <= 8 else 0, t, n)
+    g = gen(n)
+    mask = torch.where(torch.rand((S, H, n, slots), generator=g) < 0.3, float("-inf"), 0.0) + torch.randn((S, H, n, slots), generator=g)
+    mask[0, 1, 0], mask[1, :, n - 1], mask[0, 5, :, 7] = float("-inf"), float("-inf"), float("-inf")
+    mask[..., 100:140] = float("-inf")                        # hidden from everyone
+    mask[0, 3, 0, 1:] = float("-inf")                         # one slot left
+    mask = mask.half()
+    for bad in ((k, v) if v is not None else (k,)):
+        if t in DTYPE:
+            bad[:, :, 100:120], bad[:, :, 120:130], bad[:, :, 130:140] = float("nan"), float("inf"), float("-inf")
+        else:
+            bad[:, :, 100:140] = 255                           # a scale of NaN
+    check_attn(q, k, v, t, mask, 1 / math.sqrt(d), mass, 0.5)
+    check_attn(q, k, v, t, mask, 1 / math.sqrt(d), mass, 0.5, max_bias=8.0)
+    low = torch.full((1, 1, n, slots), -65504.0).half()
+    low[..., 100:140] = float("-inf")
+    check_attn(q, k, v, t, low, 1 / math.sqrt(d), mass, 0.5, near=False)
+    low[..., 50] = 0.0                                        # one slot beside the lowest values: it draws everything
+    check_attn(q, k, v, t, low, 1 / math.sqrt(d), mass, 0.5, near=False)
+
+
+@pytest.mark.parametrize("t", [B.F16, B.Q8_0])
+def test_attention_mass_hidden_from_one_head_only(t):
+    """a row of NaN that one head sees spoils that head's result and no other's"""
+    H, HK, slots, d, n = 4, 2, 70, 64, 2
+    q, k, v, mass = attn_case(1, H, HK, n, slots, d, d, t, 3)
+    mask = torch.zeros((1, H, n, slots)).half()
+    mask[0, [0, 2, 3], :, 9] = float("-inf")
+    for x in (k, v):
+        if t in DTYPE:
+            x[:, :, 9] = float("nan")
+        else:
+            x[:, :, 9] = 255
+    dst, _ = ops.flash_attn_ext_mass(q.cuda(), k.cuda(), v.cuda(), mask.cuda(), t, 0.125)
+    assert torch.isnan(dst[0, :, 1]).all() and torch.isfinite(dst[0, :, [0, 2, 3]]).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 50])
+def test_attention_mass_softcap_bias_and_sharp_logits(n):
+    S, H, HK, slots, d = 1, 6, 2, 333, 128
+    q, k, v, mass = attn_case(S, H, HK, n, slots, d, d if n <= 8 else 0, B.F16, 40 + n)
+    check_attn(q, k, v, B.F16, causal(S, n, slots), 0.088, mass, 1.0, softcap=30.0)
+    check_attn(q * 20, k, v, B.F16, causal(S, n, slots), 0.088, mass, 1.0, near=False)                 # almost all weight on single slots
+    check_attn(q * 1e-3, k, v, B.F16, None, 0.088, mass, 1.0)                                        # almost equal weights
+    big = q.clone()
+    big[..., 0] *= 1e6                                                                               # beyond the range of f16
+    check_attn(big, k, v, B.F16, causal(S, n, slots), 1e-6, mass, 1.0, near=False)
+
+
+def test_attention_mass_strided_caches_in_place_and_unread():
+    """slot-major caches (every head's rows of a slot side by side), q as [seq, token, head, d], mass_out on mass, decay 0 over NaN"""
+    S, H, HK, n, slots, d = 2, 8, 2, 2, 150, 128
+    for t in (B.F16, B.Q8_0, B.Q4_0):
+        g = gen(t)
+        q = torch.randn((S, n, H, d), generator=g)
+        k, v = (cache((S, slots, HK, d), t, g) for _ in range(2))
+        mass = torch.rand((S, HK, slots + 5), generator=g)
+        mask = causal(S, n, slots)
+        kg, vg, qg, mg = k.cuda().transpose(1, 2), v.cuda().transpose(1, 2), q.cuda().transpose(1, 2), mass.cuda()
+        wd, ed, wm, em = attn_oracle(q.transpose(1, 2), values(k.transpose(1, 2), t), values(v.transpose(1, 2), t), mask, 0.1, mass[..., :slots], 0.75)
+        dst, out = ops.flash_attn_ext_mass(qg, kg, vg, mask.cuda(), t, 0.1, mass=mg[..., :slots], decay=0.75, mass_out=mg[..., :slots])
+        assert out.data_ptr() == mg.data_ptr() and ((dst.cpu().double() - wd).abs() <= ed).all() and ((mg[..., :slots].cpu().double() - wm).abs() <= em).all()
+        assert torch.equal(mg[..., slots:].cpu(), mass[..., slots:])
+        _, _, wm, em = attn_oracle(q.transpose(1, 2), values(k.transpose(1, 2), t), None, mask, 0.1, None, 0.0)
+        nan = torch.full((S, HK, slots), float("nan"), device="cuda")
+        for got in (ops.flash_attn_ext_mass(qg, kg, vg, mask.cuda(), t, 0.1, mass=nan, decay=0.0)[1], ops.attn_mass(qg, kg, mask.cuda(), t, 0.1, mass=nan, decay=0.0)):
+            assert ((got.cpu().double() - wm).abs() <= em).all()
+
+
+@pytest.mark.parametrize("n", [1, 24])
+def test_attention_mass_offsets_past_32_bits(n):
+    """slots 100 MiB apart: the last rows lie beyond 4 GiB"""
+    H, HK, slots, d, step = 4, 1, 48, 128, 100 << 20
+    q, k, v, mass = attn_case(1, H, HK, n, slots, d, d, B.F16, 77)
+    raw = torch.empty(step * slots, dtype=torch.uint8, device="cuda")
+    far = lambda off: raw.view(torch.float16).as_strided((1, HK, slots, d), (0, 0, step // 2, 1), off)  # noqa: E731
+    kg, vg = far(0), far(4096)
+    kg.copy_(k), vg.copy_(v)
+    mask = causal(1, n, slots)
+    wd, ed, wm, em = attn_oracle(q, values(k, B.F16), values(v, B.F16), mask, 0.1, mass, 1.0)
+    assert ((ops.attn_mass(q.cuda(), kg, mask.cuda(), B.F16, 0.1, mass=mass.cuda()).cpu().double() - wm).abs() <= em).all()
+    if n <= 8:
+        dst, out = ops.flash_attn_ext_mass(q.cuda(), kg, vg, mask.cuda(), B.F16, 0.1, mass=mass.cuda())
+        assert ((dst.cpu().double() - wd).abs() <= ed).all() and ((out.cpu().double() - wm).abs() <= em).all()
+
+
+def test_attention_mass_two_streams_captured_and_nothing_cached():
+    """two captured graphs with workspaces of their own, replayed on two streams at once, inputs changed between the replays; an empty cache"""
+    S, H, HK, slots, d = 1, 32, 8, 3000, 128
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    state = []
+    for i, n in enumerate((1, 30)):
+        q, k, v, mass = attn_case(S, H, HK, n, slots, d, d, B.F16, i)
+        dev = [x.cuda() for x in (q, k, v, mass, causal(S, n, slots))]
+        out = torch.empty((S, HK, slots), device="cuda")
+        def run(dev=dev, n=n, out=out):
+            q, k, v, mass, mask = dev
+            if n <= 8:
+                return ops.flash_attn_ext_mass(q, k, v, mask, B.F16, 0.09, mass=mass, mass_out=out)
+            return ops.attn_mass(q, k, mask, B.F16, 0.09, mass=mass, mass_out=out)
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = run()
+        state.append((graph, dev, res, run, out))
+    for rep in range(4):
+        for graph, dev, *_ in state:
+            dev[0].copy_(torch.randn(dev[0].shape, generator=gen(50 + rep)))
+            dev[3].copy_(torch.rand(dev[3].shape, generator=gen(60 + rep)))
+        torch.cuda.synchronize()
+        for side, (graph, *_) in zip(sides, state):
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, dev, res, run, out in state:
+            got = [x.clone() for x in (res if isinstance(res, tuple) else (res,))]
+            want = run()
+            for x, y in zip(got, want if isinstance(want, tuple) else (want,)):
+                assert torch.equal(x, y)          # no atomics: the same bits every time
+    q = torch.randn((1, 4, 1, 64), device="cuda")
+    none = torch.zeros((1, 2, 0, 64), dtype=torch.float16, device="cuda")
+    dst, mass = ops.flash_attn_ext_mass(q, none, none, None, B.F16, 0.1)
+    assert (dst == 0).all() and mass.shape == (1, 2, 0)
+
+
+def test_attention_mass_wrapper_refuses_what_does_not_fit():
+    q, k, v, mass = (x.cuda() for x in attn_case(1, 4, 2, 1, 10, 64, 64, B.F16, 1))
+    ok = dict(q=q, k=k, v=v, mask=None, type_kv=B.F16, scale=0.1)
+    for bad in (dict(q=q.half()), dict(k=k.float()), dict(k=k[..., :32]), dict(v=v[:, :, :5]), dict(mask=torch.zeros((1, 5), device="cuda").half()),
+                dict(mask=torch.zeros((1, 10), device="cuda")), dict(mass=mass.double()), dict(mass_out=mass[:, :, :3]), dict(type_kv=B.Q8_0), dict(k=k.cpu())):
+        with pytest.raises(ValueError):
+            ops.flash_attn_ext_mass(**{**ok, **bad})
+    with pytest.raises(K.Mi355Error):
+        ops.flash_attn_ext_mass(q.expand(1, 4, 9, 64).contiguous(), k, v, None, B.F16, 0.1)
+    with pytest.raises(K.Mi355Error):
+        ops.flash_attn_ext_mass(q[:, :3], k, v, None, B.F16, 0.1)
