@@ -20,8 +20,10 @@ struct MArgs {
     int n_q, n_kv, n_head, n_head_kv, d, dv;
     float scale, max_bias, logit_softcap, m0, m1, decay;
     uint32_t n_head_log2;
-    float * logits;     // [ne3][n_head][n_q][n_kv] (with dst), else NULL
-    float * stats;      // [ne3][n_head][n_q][2]: m, 1 / l (0: sees nothing)
+    int nsplit, lpitch;
+    float * logits;     // steps: [ne3][n_head_kv][rows][lpitch], log2 domain
+    float * stats;      // steps: [ne3][n_head_kv][nsplit][rows][2]: maximum (log2 domain) and sum; prompts: [ne3][n_head][n_q][2]: m, 1 / l
+    float * part;       // steps: [ne3][n_head_kv][nsplit][rows][D]
 };
 
 constexpr int MT = 256;
@@ -50,7 +52,533 @@ template <int TYPE> static __device__ __forceinline__ float logit(const MArgs & 
     return t + mv;
 }
 
-// one workgroup per (query, head, sequence): statistics, and with dst the attention row
+// ---- decode steps (at most 8 queries): one pass over K and V on the matrix cores --------------------------------------------------------
+//
+// Bound by the cache's bytes: at GQA 4..8 the rows that meet a K or V row fill one 16-row matrix tile, so the arithmetic is small change.
+// A wave owns 32 slots at a time, nothing is shared between waves until the end:
+//   S^T[slot][row] = K Q^T      v_mfma_f32_16x16x32: K rows come from memory straight into the A operand (lane = slot, 16 bytes each)
+//   O^T[f][row]   += V^T P^T    P^T is the S^T accumulator as it lies; V goes through LDS and is read transposed (ds_read_b64_tr_b16)
+// A "row" is a (query, head of the KV head) pair.  f32 results from 16-bit operands: q and P are split into two f16 (three bf16) parts whose
+// products are added in the accumulator, 22 (24) bits; cache values are exact in 16 bits (blocks: their integers, scales applied in f32 --
+// K's to the partial products of each 32-block, V's to P).  Logits are kept (log2 domain) for the pass that forms the weights.
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int TYPE> struct Fmt {       // 16-bit format of the operands and the parts an f32 is split into
+    static constexpr bool bf = TYPE == MI355_TYPE_BF16, quant = TYPE == MI355_TYPE_Q8_0 || TYPE == MI355_TYPE_Q4_0;
+    static constexpr int parts = bf ? 3 : 2;
+    static constexpr int block = TYPE == MI355_TYPE_Q8_0 ? 34 : 18;
+};
+template <bool BF> static __device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    else              return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+// x[8] -> parts of 8 16-bit values each, part 0 the largest.  f16: rounded, then the rest rounded; bf16: upper halves, cut off
+template <bool BF, int P> static __device__ __forceinline__ void split8(const float * x, v4i * out) {
+    if constexpr (BF) {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = x[i];
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t u0 = __float_as_uint(r[2 * i]), u1 = __float_as_uint(r[2 * i + 1]);
+                out[p][i] = (int)__builtin_amdgcn_perm(u1, u0, 0x07060302u);
+                r[2 * i] -= __uint_as_float(u0 & 0xffff0000u);
+                r[2 * i + 1] -= __uint_as_float(u1 & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            // one rounding of hi for both of its uses: left to itself the compiler folds the product behind x into the operand's conversion
+            // (one rounding) but not into lo's (two), and near a tie lo then belongs to the other neighbour
+            int bits = __builtin_bit_cast(int, h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
+            asm("" : "+v"(bits));
+            const h2 hi = __builtin_bit_cast(h2, bits);
+            const h2 lo = {(_Float16)(x[2 * i] - (float)hi[0]), (_Float16)(x[2 * i + 1] - (float)hi[1])};
+            out[0][i] = bits;
+            out[1][i] = __builtin_bit_cast(int, lo);
+        }
+    }
+}
+
+// 8 consecutive features (chunk j) of a cache row on their way to an operand: the bytes, then 16-bit values (blocks: the integers)
+template <int TYPE> struct Chunk {
+    v4i raw;
+    __device__ __forceinline__ void load(const char * row, int j) { raw = *(const v4i *)(row + j * 16); }
+    __device__ __forceinline__ v4i operand(int) const { return raw; }
+    __device__ __forceinline__ float scale() const { return 1.0f; }
+};
+static __device__ __forceinline__ v4i bytes_f16(uint32_t w0, uint32_t w1, float bias) {      // 8 bytes -> f16 of (byte - bias); 0x6400 | b is 1024 + b
+    const _Float16 c = (_Float16)(1024.0f + bias);
+    const h2 cc = {c, c};
+    v4i r;
+    r[0] = __builtin_bit_cast(int, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u)) - cc);
+    r[1] = __builtin_bit_cast(int, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u)) - cc);
+    r[2] = __builtin_bit_cast(int, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u)) - cc);
+    r[3] = __builtin_bit_cast(int, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)) - cc);
+    return r;
+}
+template <> struct Chunk<MI355_TYPE_Q8_0> {
+    uint32_t w0, w1; uint16_t d;
+    __device__ __forceinline__ void load(const char * row, int j) {
+        const char * b = row + (j >> 2) * 34;
+        d = *(const uint16_t *)b;
+        __builtin_memcpy(&w0, b + 2 + (j & 3) * 8, 4); __builtin_memcpy(&w1, b + 6 + (j & 3) * 8, 4);
+    }
+    __device__ __forceinline__ v4i operand(int) const { return bytes_f16(w0 ^ 0x80808080u, w1 ^ 0x80808080u, 128.0f); }
+    __device__ __forceinline__ float scale() const { return h2f(d); }
+};
+template <> struct Chunk<MI355_TYPE_Q4_0> {
+    uint32_t w0, w1; uint16_t d;
+    __device__ __forceinline__ void load(const char * row, int j) {
+        const char * b = row + (j >> 2) * 18;
+        d = *(const uint16_t *)b;
+        __builtin_memcpy(&w0, b + 2 + (j & 1) * 8, 4); __builtin_memcpy(&w1, b + 6 + (j & 1) * 8, 4);
+    }
+    __device__ __forceinline__ v4i operand(int j) const {
+        const int sh = (j & 2) * 2;
+        return bytes_f16((w0 >> sh) & 0x0f0f0f0fu, (w1 >> sh) & 0x0f0f0f0fu, 8.0f);
+    }
+    __device__ __forceinline__ float scale() const { return h2f(d); }
+};
+// non-finite 16-bit values of a chunk -> 0; true if there was one
+template <bool BF> static __device__ __forceinline__ bool sanitize(v4i & x) {
+    bool bad = false;
+    constexpr uint32_t e = BF ? 0x7f80u : 0x7c00u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t u = (uint32_t)x[i];
+        if ((u & e) == e) { u &= 0xffff0000u; bad = true; }
+        if ((u & (e << 16)) == (e << 16)) { u &= 0xffffu; bad = true; }
+        x[i] = (int)u;
+    }
+    return bad;
+}
+
+static __device__ __forceinline__ float max_groups(float v) {       // over the four 16-lane groups, lanes of equal place
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+static __device__ __forceinline__ float sum_groups(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+template <int TYPE, int D, int NW, bool HASV>
+__global__ void __launch_bounds__(NW * 64)
+mass_step_kernel(const MArgs a) {
+    typedef Fmt<TYPE> F;
+    constexpr int KS = D / 32, FT = D / 16, P = F::parts;
+    constexpr int VP = D * 2 + 32;                              // V tile row pitch (bytes)
+    constexpr int OP = D + 4;                                   // merge row pitch (floats)
+    constexpr int VB = HASV ? (32 * VP > 16 * OP * 4 ? 32 * VP : 16 * OP * 4) : 16;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[NW][VB];
+    __shared__ __attribute__((aligned(16))) float kd[F::quant ? NW : 1][F::quant ? 32 : 1][KS], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 : 1][KS];
+    __shared__ float wm[NW][16], wl[NW][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int lr = lane & 15, g = lane >> 4;
+    const int ratio = a.n_head / a.n_head_kv, R = ratio * a.n_q;
+    const int hk = blockIdx.y % a.n_head_kv, r0 = blockIdx.y / a.n_head_kv * 16, i3 = blockIdx.z, split = blockIdx.x;
+    const int r = r0 + lr < R ? r0 + lr : R - 1;                // this lane's row (the lanes past the last one repeat it)
+    const int iq = r / ratio, h = hk * ratio + r % ratio;
+    const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
+    const char * vb = HASV ? a.v + hk * a.v_nb2 + i3 * a.v_nb3 : nullptr;
+    const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
+    const bool m8 = mrow && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
+    const float slope = m_slope(a, h) * LOG2E;
+    const bool capped = a.logit_softcap != 0.0f;
+
+    const int ntiles = (a.n_kv + 31) / 32, per = (ntiles + a.nsplit - 1) / a.nsplit;
+    const int t0 = split * per, t1 = t0 + per < ntiles ? t0 + per : ntiles;
+
+    Chunk<TYPE> kc[2][KS], vc[HASV ? D / 16 : 1];
+    auto load_k = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int j = 32 * t + 16 * u + lr;
+            const char * row = kb + (int64_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) kc[u][ks].load(row, (4 * ks + g) * 8 < a.d ? 4 * ks + g : 0);
+        }
+    };
+    auto load_v = [&](int t) {
+        if constexpr (HASV) {
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {                  // 64 chunks of 8 features at a time
+                const int c = 64 * i + lane, j = 32 * t + c / (D / 8), cc = c % (D / 8);
+                vc[i].load(vb + (int64_t)(j < a.n_kv ? j : a.n_kv - 1) * a.v_nb1, cc * 8 < a.dv ? cc : 0);
+            }
+        }
+    };
+    int t = t0 + wave;
+    if (t < t1) { load_k(t); load_v(t); }
+
+    // q: scale and log2(e) on it, for f16 the row's largest value brought to [2^14, 2^15) by a power of two that the
+    // logits get back (its small values then stay clear of the subnormal range)
+    v4i qf[KS][P];
+    float qe = 1.0f;
+    {
+        const float * qp = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
+        const float qs = capped ? a.scale / a.logit_softcap : a.scale * LOG2E;
+        float x[KS][8], amax = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int f = 32 * ks + 8 * g;
+            v4f x0 = {0.0f, 0.0f, 0.0f, 0.0f}, x1 = x0;
+            if (f < a.d) { x0 = *(const v4f *)(qp + f); x1 = *(const v4f *)(qp + f + 4); }
+#pragma unroll
+            for (int i = 0; i < 4; i++) { x[ks][i] = x0[i] * qs; x[ks][4 + i] = x1[i] * qs; }
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[ks][i]));
+        }
+        if (!F::bf) {
+            amax = max_groups(amax);
+            const int e = amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+            qe = ldexpf(1.0f, e);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[ks][i] = ldexpf(x[ks][i], -e);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) split8<F::bf, P>(x[ks], qf[ks]);
+    }
+
+    float m = -INFINITY, l = 0.0f;              // of this lane's row; l over this lane's slots only
+    v4f o[HASV ? FT : 1];
+#pragma unroll
+    for (int i = 0; i < (HASV ? FT : 1); i++) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float * lg = a.logits + (((int64_t)i3 * a.n_head_kv + hk) * R + r) * a.lpitch;
+
+    for (; t < t1; t += NW) {
+        // mask of slots 32 t + 16 u + 4 g + i
+        float mv[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int j = 32 * t + 16 * u + 4 * g;
+            if (m8 && j + 4 <= a.n_kv) {
+                const u2 w = *(const u2 *)(mrow + 2 * j);
+                mv[u][0] = h2f((uint16_t)w.x); mv[u][1] = h2f((uint16_t)(w.x >> 16)); mv[u][2] = h2f((uint16_t)w.y); mv[u][3] = h2f((uint16_t)(w.y >> 16));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) mv[u][i] = j + i >= a.n_kv ? -INFINITY : mrow ? h2f(((const uint16_t *)mrow)[j + i]) : 0.0f;
+            }
+        }
+        if constexpr (F::quant) {               // scales of the 32 slots where every lane can read them
+            if (g < KS) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) if (ks % 4 == g) kd[wave][16 * u + lr][ks] = kc[u][ks].scale();
+            }
+            if constexpr (HASV) {
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) {
+                    const int c = 64 * i + lane, cc = c % (D / 8);
+                    if ((cc & 3) == 0) vd[wave][c / (D / 8)][cc >> 2] = vc[i].scale();
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        // ---- S^T
+        float s[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
+            float dk[4][KS];
+            if constexpr (F::quant)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) dk[i][ks] = kd[wave][16 * u + 4 * g + i][ks];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                v4f b = F::quant ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : c;
+                const v4i kop = kc[u][ks].operand(g);
+#pragma unroll
+                for (int p = P - 1; p >= 0; p--) b = mfma16<F::bf>(kop, qf[ks][p], b);
+                if constexpr (F::quant) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) c[i] = __builtin_fmaf(b[i], dk[i][ks], c[i]);
+                } else c = b;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x = c[i] * qe;
+                if (capped) x = a.logit_softcap * LOG2E * tanhf(x);
+                s[u][i] = mv[u][i] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[u][i], slope, x);
+            }
+        }
+        if (t + NW < t1) load_k(t + NW);        // in flight during the rest of this tile
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int j = 32 * t + 16 * u + 4 * g;
+            if (r0 + lr < R) {
+                if (j + 4 <= a.lpitch) *(v4f *)(lg + j) = v4f{s[u][0], s[u][1], s[u][2], s[u][3]};
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[u][i]);
+        }
+        mx = max_groups(mx);
+        const float ms = mx == -INFINITY ? 0.0f : mx;
+        const float corr = __builtin_amdgcn_exp2f(m - ms);      // m = -inf: 0
+        float p[8];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[4 * u + i] = __builtin_amdgcn_exp2f(s[u][i] - ms);
+        l *= corr;
+#pragma unroll
+        for (int i = 0; i < 8; i++) l += p[i];
+        m = mx;
+        if constexpr (HASV) {
+            if (__any(corr != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < FT; i++) o[i] = o[i] * corr;
+            }
+            // ---- V tile into LDS.  A slot that some row does not see must not reach that row through 0 * NaN: its non-finite values are
+            // taken out here and added below to the rows that do see it
+            bool some = false;
+#pragma unroll
+            for (int i = 0; i < 8; i++) some |= s[i >> 2][i & 3] == -INFINITY;
+            uint64_t bad = 0;                                   // rows of the tile with values taken out
+            const bool hidden = !F::quant && __any(some);
+            uint32_t unseen = 0;                                // bit j: slot 32 t + j is hidden from some row
+            if (hidden) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint64_t b = __ballot(s[u][i] == -INFINITY);
+#pragma unroll
+                        for (int gg = 0; gg < 4; gg++) if ((b >> (16 * gg)) & 0xffff) unseen |= 1u << (16 * u + 4 * gg + i);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const int c = 64 * i + lane, row = c / (D / 8), cc = c % (D / 8);
+                v4i x = vc[i].operand(cc & 3);
+                if (cc * 8 >= a.dv) x = v4i{0, 0, 0, 0};
+                if (hidden) {
+                    bool taken = false;
+                    if (unseen >> row & 1) taken = sanitize<F::bf>(x);
+                    const uint64_t b = __ballot(taken);
+                    constexpr int rows = 512 / D;               // slots per 64 chunks
+#pragma unroll
+                    for (int q = 0; q < rows; q++) if (b & (rows == 1 ? ~0ull : ((1ull << (D / 8 % 64)) - 1) << (q * (D / 8)))) bad |= 1ull << (i * rows + q);
+                }
+                *(v4i *)(lds[wave] + row * VP + cc * 16) = x;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (t + NW < t1) load_v(t + NW);
+            // ---- O^T
+            const uint8_t * vt = lds[wave] + (4 * g + (lr >> 2)) * VP + 8 * (lr & 3);
+            v4i pf[P];
+            float back = 1.0f;
+#pragma unroll
+            for (int f = 0; f < FT; f++) {
+                if constexpr (F::quant) {
+                    if (f % 2 == 0) {                           // a new 32-block: P times the slots' scales, their largest brought to [1, 2)
+                        float x[8], dm = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float dd = vd[wave][(i & 4) * 4 + 4 * g + (i & 3)][f / 2];
+                            x[i] = s[i >> 2][i & 3] == -INFINITY ? 0.0f : dd;
+                            dm = fmaxf(dm, fabsf(x[i]));
+                        }
+                        dm = max_groups(dm);
+                        const int e = dm > 0.0f && dm < INFINITY ? __builtin_amdgcn_frexp_expf(dm) - 1 : 0;
+                        back = ldexpf(1.0f, e - 14);
+                        const float fwd = ldexpf(1.0f, 14 - e);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[i] = x[i] * fwd * p[i];
+                        split8<false, 2>(x, pf);
+                    }
+                } else if (f == 0) {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = F::bf ? p[i] : p[i] * 16384.0f;      // f16: clear of the subnormal range
+                    split8<F::bf, P>(x, pf);
+                }
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(vt + 32 * f));
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(vt + 32 * f + 16 * VP));
+                v4i vop;
+                __builtin_memcpy(&vop, &lo, 8);
+                __builtin_memcpy((char *)&vop + 8, &hi, 8);
+                if constexpr (F::quant) {
+                    v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int q = P - 1; q >= 0; q--) c = mfma16<false>(vop, pf[q], c);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[f][i] = __builtin_fmaf(c[i], back, o[f][i]);
+                } else {
+#pragma unroll
+                    for (int q = P - 1; q >= 0; q--) o[f] = mfma16<F::bf>(vop, pf[q], o[f]);
+                }
+            }
+            if (!F::quant && bad) {                             // non-finite values of slots that only some rows see
+                for (int row = 0; row < 32; row++) {
+                    if (!(bad >> row & 1)) continue;
+                    const int from = ((row & 15) >> 2) * 16 + lr, i = (row >> 4) * 4 + (row & 3);
+                    float pr = 0.0f, sr = -INFINITY;
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        const float a0 = __shfl(p[q], from, 64), a1 = __shfl(s[q >> 2][q & 3], from, 64);
+                        if (q == i) { pr = a0; sr = a1; }
+                    }
+                    const int j = 32 * t + row;
+                    if (j >= a.n_kv) continue;
+                    const char * vr = vb + (int64_t)j * a.v_nb1;
+#pragma unroll
+                    for (int f = 0; f < FT; f++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int e = 16 * f + 4 * g + q;
+                            if (e >= a.dv) continue;
+                            const float x = kv_value<TYPE>(vr, e);
+                            if (sr != -INFINITY && !(fabsf(x) < INFINITY)) o[f][q] += pr * x;
+                        }
+                }
+            }
+        }
+    }
+    // ---- the waves' states meet in LDS
+    l = sum_groups(l);
+    if (g == 0) { wm[wave][lr] = m; wl[wave][lr] = l; }
+    if constexpr (HASV) {
+        float * ob = (float *)lds[wave] + lr * OP + 4 * g;
+#pragma unroll
+        for (int f = 0; f < FT; f++) *(v4f *)(ob + 16 * f) = F::bf || F::quant ? o[f] : o[f] * (1.0f / 16384.0f);
+    }
+    __syncthreads();
+    const int rows = R - r0 < 16 ? R - r0 : 16;
+    const int64_t slot = (((int64_t)i3 * a.n_head_kv + hk) * a.nsplit + split) * R + r0;
+    if (HASV) {
+        for (int idx = tid; idx < rows * (D / 4); idx += NW * 64) {
+            const int rr = idx / (D / 4), f4 = idx % (D / 4);
+            if (4 * f4 >= a.dv) continue;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][rr]);
+            const float ms = M == -INFINITY ? 0.0f : M;
+            v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float c = __builtin_amdgcn_exp2f(wm[w][rr] - ms);
+                L = __builtin_fmaf(wl[w][rr], c, L);
+                O = O + *(const v4f *)((const float *)lds[w] + rr * OP + 4 * f4) * c;
+            }
+            *(v4f *)(a.part + (slot + rr) * D + 4 * f4) = O;
+        }
+    }
+    if (tid < rows) {
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][tid]);
+        const float ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < NW; w++) L = __builtin_fmaf(wl[w][tid], __builtin_amdgcn_exp2f(wm[w][tid] - ms), L);
+        a.stats[(slot + tid) * 2] = M; a.stats[(slot + tid) * 2 + 1] = L;
+    }
+}
+
+// The slices' statistics meet: workgroups 0 .. mass_wgs - 1 form the weights of 256 slots each from the logits, the others a row of dst each
+template <int D>
+__global__ void __launch_bounds__(256)
+mass_finish_kernel(const MArgs a, int mass_wgs) {
+    __shared__ float sm[64], sl[64];
+    const int tid = threadIdx.x, hk = blockIdx.y, i3 = blockIdx.z;
+    const int ratio = a.n_head / a.n_head_kv, R = ratio * a.n_q;
+    const int64_t base = ((int64_t)i3 * a.n_head_kv + hk) * a.nsplit * R;
+    const float * st = a.stats + base * 2;
+    if ((int)blockIdx.x < mass_wgs) {
+        const int j = blockIdx.x * 256 + tid;
+        const float * lg = a.logits + ((int64_t)i3 * a.n_head_kv + hk) * R * a.lpitch;
+        float t = 0.0f;
+        for (int r0 = 0; r0 < R; r0 += 64) {                    // 64 rows' statistics at a time, four lanes a row
+            __syncthreads();
+            const int r = r0 + (tid >> 2), q = tid & 3;
+            float M = -INFINITY, L = 0.0f;
+            if (r < R) for (int s = q; s < a.nsplit; s += 4) {
+                const float ms = st[((int64_t)s * R + r) * 2], ls = st[((int64_t)s * R + r) * 2 + 1];
+                const float mn = fmaxf(M, ms), mz = mn == -INFINITY ? 0.0f : mn;
+                L = L * __builtin_amdgcn_exp2f(M - mz) + ls * __builtin_amdgcn_exp2f(ms - mz);
+                M = mn;
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                const float mo = __shfl_xor(M, o, 64), lo = __shfl_xor(L, o, 64);
+                const float mn = fmaxf(M, mo), mz = mn == -INFINITY ? 0.0f : mn;
+                L = L * __builtin_amdgcn_exp2f(M - mz) + lo * __builtin_amdgcn_exp2f(mo - mz);
+                M = mn;
+            }
+            if (q == 0) { sm[tid >> 2] = M == -INFINITY ? 0.0f : M; sl[tid >> 2] = L == 0.0f ? 0.0f : 1.0f / L; }
+            __syncthreads();
+            if (j < a.n_kv)
+                for (int rr = 0; rr < 64 && r0 + rr < R; rr++) {
+                    const float s = lg[(int64_t)(r0 + rr) * a.lpitch + j];
+                    t += s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - sm[rr]) * sl[rr];
+                }
+        }
+        if (j >= a.n_kv) return;
+        if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
+        ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
+        return;
+    }
+    const int r = blockIdx.x - mass_wgs, iq = r / ratio, h = hk * ratio + r % ratio;
+    float M = -INFINITY, L = 0.0f, O = 0.0f;
+    for (int s = 0; s < a.nsplit; s++) M = fmaxf(M, st[((int64_t)s * R + r) * 2]);
+    const float ms = M == -INFINITY ? 0.0f : M;
+    if (tid >= a.dv) return;
+    for (int s = 0; s < a.nsplit; s++) {
+        const float c = __builtin_amdgcn_exp2f(st[((int64_t)s * R + r) * 2] - ms);
+        L = __builtin_fmaf(st[((int64_t)s * R + r) * 2 + 1], c, L);
+        O = __builtin_fmaf(a.part[(base + (int64_t)s * R + r) * D + tid], c, O);
+    }
+    ((float *)(a.dst + (int64_t)h * a.d_nb1 + (int64_t)iq * a.d_nb2 + (int64_t)i3 * a.d_nb3))[tid] = L == 0.0f ? 0.0f : O / L;
+}
+
+constexpr int STEP_WAVES = 4;
+
+template <int TYPE, int D, bool HASV> static int step_launch(const MArgs & a, int ne3, hipStream_t s) {
+    const int R = a.n_head / a.n_head_kv * a.n_q;
+    MI355_LAUNCH("fattn_mass_step", (mass_step_kernel<TYPE, D, STEP_WAVES, HASV>), dim3((unsigned)a.nsplit, (unsigned)(a.n_head_kv * ((R + 15) / 16)), (unsigned)ne3),
+                 dim3(STEP_WAVES * 64), 0, s, a);
+    MI355_CHECK_LAUNCH();
+    const int mass_wgs = (a.n_kv + 255) / 256;
+    if (mass_wgs + (HASV ? R : 0) == 0) return MI355_OK;
+    MI355_LAUNCH("fattn_mass_finish", mass_finish_kernel<D>, dim3((unsigned)(mass_wgs + (HASV ? R : 0)), (unsigned)a.n_head_kv, (unsigned)ne3), dim3(256), 0, s, a, mass_wgs);
+    MI355_CHECK_LAUNCH();
+    return MI355_OK;
+}
+template <int TYPE, bool HASV> static int step_dispatch(const MArgs & a, int ne3, hipStream_t s) {
+    if (a.d <= 64) return step_launch<TYPE, 64, HASV>(a, ne3, s);
+    if (a.d <= 128) return step_launch<TYPE, 128, HASV>(a, ne3, s);
+    return step_launch<TYPE, 256, HASV>(a, ne3, s);
+}
+
+static int step_d(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// slices of the KV range: two workgroups per CU in all, none with less than one 32-slot tile per wave
+static int64_t step_splits(const mi355_fattn_args * p) {
+    const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (p->n_kv + 31) / 32, base = p->n_head_kv * ((R + 15) / 16) * p->ne3;
+    int64_t n = 512 / base, most = (tiles + STEP_WAVES - 1) / STEP_WAVES;
+    if (n > most) n = most;
+    if (n > 128) n = 128;
+    return n < 1 ? 1 : n;
+}
+
+// ---- prompts ------------------------------------------------------------------------------------------------------------------------------
+// one workgroup per (query, head, sequence): statistics
 template <int TYPE>
 __global__ void __launch_bounds__(MT)
 mass_rows_kernel(const MArgs a) {
@@ -64,11 +592,9 @@ mass_rows_kernel(const MArgs a) {
     const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
     const float slope = m_slope(a, h);
     const int64_t row = ((int64_t)i3 * a.n_head + h) * a.n_q + iq;
-    float * lg = a.logits ? a.logits + row * a.n_kv : nullptr;
     float m = -INFINITY, l = 0.0f;
     for (int j = tid; j < a.n_kv; j += MT) {
         const float s = logit<TYPE>(a, q, kb + (int64_t)j * a.k_nb1, mrow, slope, j);
-        if (lg) lg[j] = s;
         if (s == -INFINITY) continue;
         const float mn = fmaxf(m, s);
         l = l * expf(m - mn) + expf(s - mn);
@@ -82,18 +608,6 @@ mass_rows_kernel(const MArgs a) {
     const float L = block_sum_n<MT / 64>(m == -INFINITY ? l : l * expf(m - M), sh);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     if (tid == 0) { a.stats[row * 2] = M; a.stats[row * 2 + 1] = inv; }
-    if (!a.dst) return;
-    __syncthreads();
-    float * o = (float *)(a.dst + h * a.d_nb1 + iq * a.d_nb2 + i3 * a.d_nb3);
-    const char * vb = a.v + hk * a.v_nb2 + i3 * a.v_nb3;
-    for (int e = tid; e < a.dv; e += MT) {
-        float t = 0.0f;
-        for (int j = 0; j < a.n_kv; j++) {
-            const float s = lg[j];
-            if (s != -INFINITY) t = __builtin_fmaf(expf(s - M), kv_value<TYPE>(vb + (int64_t)j * a.v_nb1, e), t);
-        }
-        o[e] = t * inv;
-    }
 }
 
 // one thread per slot: its weight over the heads and queries of its KV head
@@ -109,15 +623,11 @@ mass_slots_kernel(const MArgs a) {
         for (int iq = 0; iq < a.n_q; iq++) {
             const int64_t row = ((int64_t)i3 * a.n_head + h) * a.n_q + iq;
             float s = -INFINITY;
-            if (a.logits) {
-                if (j < a.n_kv) s = a.logits[row * a.n_kv + j];
-            } else {
-                __syncthreads();
-                if (tid < a.d) q[tid] = ((const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3))[tid];
-                __syncthreads();
-                const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
-                if (j < a.n_kv) s = logit<TYPE>(a, q, krow, mrow, m_slope(a, h), j);
-            }
+            __syncthreads();
+            if (tid < a.d) q[tid] = ((const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3))[tid];
+            __syncthreads();
+            const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
+            if (j < a.n_kv) s = logit<TYPE>(a, q, krow, mrow, m_slope(a, h), j);
             if (s != -INFINITY) t += expf(s - a.stats[row * 2]) * a.stats[row * 2 + 1];
         }
     if (j >= a.n_kv) return;
@@ -126,18 +636,32 @@ mass_slots_kernel(const MArgs a) {
 }
 
 template <int TYPE> static int mass_launch(const MArgs & a, int ne3, hipStream_t s) {
+    if (a.n_kv == 0) return MI355_OK;
     MI355_LAUNCH("fattn_mass_rows", mass_rows_kernel<TYPE>, dim3((unsigned)a.n_head, (unsigned)a.n_q, (unsigned)ne3), dim3(MT), 0, s, a);
     MI355_CHECK_LAUNCH();
-    if (a.n_kv == 0) return MI355_OK;
     MI355_LAUNCH("fattn_mass", mass_slots_kernel<TYPE>, dim3((unsigned)((a.n_kv + MT - 1) / MT), (unsigned)a.n_head_kv, (unsigned)ne3), dim3(MT), 0, s, a);
     MI355_CHECK_LAUNCH();
     return MI355_OK;
 }
 
-static int64_t mass_workspace(const mi355_fattn_args * p, bool with_dst) {
-    if (!p || p->n_q < 0 || p->n_kv < 0 || p->n_head < 0 || p->ne3 < 0) return -1;
+// steps: [statistics][partial rows of dst][logits]; prompts: statistics
+struct WsParts { int64_t nsplit, lpitch, stats, part, logits; };
+static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     const int64_t rows = p->ne3 * p->n_head * p->n_q;
-    return rows * 8 + (with_dst ? rows * p->n_kv * 4 : 0);
+    WsParts w = {1, 0, rows * 2, 0, 0};
+    if (p->n_q <= MI355_MASS_MAX_Q) {
+        w.nsplit = step_splits(p);
+        w.lpitch = (p->n_kv + 3) / 4 * 4;
+        w.stats = (w.nsplit * rows * 2 + 3) / 4 * 4;
+        w.part = with_dst ? w.nsplit * rows * step_d(p->d) : 0;
+        w.logits = rows * w.lpitch;
+    }
+    return w;
+}
+static int64_t mass_workspace(const mi355_fattn_args * p, bool with_dst) {
+    if (!p || p->n_q < 0 || p->n_kv < 0 || p->n_head < 1 || p->n_head_kv < 1 || p->n_head % p->n_head_kv || p->ne3 < 1 || p->d < 8 || p->d > 256) return -1;
+    const WsParts w = mass_parts(p, with_dst);
+    return (w.stats + w.part + w.logits) * 4;
 }
 
 static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, bool with_dst, void * workspace, int64_t workspace_bytes, void * stream) {
@@ -150,7 +674,7 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     const bool quant = p->type_k == MI355_TYPE_Q8_0 || p->type_k == MI355_TYPE_Q4_0;
     if (quant && (p->d % 32 != 0 || (with_dst && dv % 32 != 0))) return MI355_E_SHAPE;
     if (p->n_head < 1 || p->n_head > 65535 || p->n_head_kv < 1 || p->n_head % p->n_head_kv != 0 || p->n_q < 1 || p->n_q > 65535 || p->n_kv < 0 ||
-        p->n_kv > (1 << 30) || p->ne3 < 1 || p->ne3 > 65535) return MI355_E_SHAPE;
+        p->n_kv > (1 << 30) || p->n_head_kv * ((p->n_head / p->n_head_kv * MI355_MASS_MAX_Q + 15) / 16) > 65535 || p->ne3 < 1 || p->ne3 > 65535) return MI355_E_SHAPE;
     if (with_dst && p->n_q > MI355_MASS_MAX_Q) return MI355_E_UNSUPPORTED;
     if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1)) return MI355_E_SHAPE;
     const int64_t f32s = (int64_t)(uintptr_t)p->q | p->q_nb1 | p->q_nb2 | p->q_nb3 |
@@ -176,9 +700,18 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     a.n_head_log2 = 1u << (uint32_t)floorf(log2f((float)p->n_head));
     a.m0 = powf(2.0f, -(p->max_bias) / a.n_head_log2);
     a.m1 = powf(2.0f, -(p->max_bias / 2.0f) / a.n_head_log2);
+    const WsParts parts = mass_parts(p, with_dst);
+    a.nsplit = (int)parts.nsplit; a.lpitch = (int)parts.lpitch;
     a.stats = (float *)workspace;
-    a.logits = with_dst ? a.stats + p->ne3 * p->n_head * p->n_q * 2 : nullptr;
+    a.part = a.stats + parts.stats;
+    a.logits = a.part + parts.part;
     hipStream_t s = (hipStream_t)stream;
+    if (p->n_q <= MI355_MASS_MAX_Q) switch (p->type_k) {
+        case MI355_TYPE_F16:  return with_dst ? step_dispatch<MI355_TYPE_F16, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_F16, false>(a, (int)p->ne3, s);
+        case MI355_TYPE_BF16: return with_dst ? step_dispatch<MI355_TYPE_BF16, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_BF16, false>(a, (int)p->ne3, s);
+        case MI355_TYPE_Q8_0: return with_dst ? step_dispatch<MI355_TYPE_Q8_0, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_Q8_0, false>(a, (int)p->ne3, s);
+        case MI355_TYPE_Q4_0: return with_dst ? step_dispatch<MI355_TYPE_Q4_0, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_Q4_0, false>(a, (int)p->ne3, s);
+    }
     switch (p->type_k) {
         case MI355_TYPE_F16:  return mass_launch<MI355_TYPE_F16>(a, (int)p->ne3, s);
         case MI355_TYPE_BF16: return mass_launch<MI355_TYPE_BF16>(a, (int)p->ne3, s);

@@ -571,6 +571,27 @@ def test_attention_mass_strided_caches_in_place_and_unread():
             assert ((got.cpu().double() - wm).abs() <= em).all()
 
 
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("n", [1, 8, 20])
+def test_attention_mass_is_as_exact_as_f32(t, n):
+    """the operands are split into 16-bit parts: no further from 64 bits than the same sums in f32 torch, in dst and in the weights"""
+    S, H, HK, slots, d = 1, 16, 4, 2500, 128
+    q, k, v, _ = attn_case(S, H, HK, n, slots, d, d, t, 90 + n)
+    mask = causal(S, n, slots)
+    k64, v64 = values(k, t), values(v, t)
+    wd, _, wm, _ = attn_oracle(q, k64, v64, mask, 0.09, None, 0.0)
+    s = (q @ k64.float().repeat_interleave(4, 1).transpose(2, 3)) * 0.09 + mask.float()
+    p = torch.softmax(s, -1)
+    fd, fm = (p @ v64.float().repeat_interleave(4, 1)).transpose(1, 2), p.reshape(S, HK, 4 * n, slots).sum(2)
+    far = lambda x, y: float((x.cpu().double() - y).norm() / y.norm())  # noqa: E731
+    if n <= 8:
+        dst, mass = ops.flash_attn_ext_mass(q.cuda(), k.cuda(), v.cuda(), mask.cuda(), t, 0.09)
+        assert far(dst, wd) <= 1.5 * far(fd, wd) + 3e-7
+    else:
+        mass = ops.attn_mass(q.cuda(), k.cuda(), mask.cuda(), t, 0.09)
+    assert far(mass, wm) <= 1.5 * far(fm, wm) + 3e-7
+
+
 @pytest.mark.parametrize("n", [1, 24])
 def test_attention_mass_offsets_past_32_bits(n):
     """slots 100 MiB apart: the last rows lie beyond 4 GiB"""
