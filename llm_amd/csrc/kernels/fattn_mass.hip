@@ -11,8 +11,8 @@ namespace {
 
 struct MArgs {
     const char * q; int64_t q_nb1, q_nb2, q_nb3;
-    const char * k; int64_t k_nb1, k_nb2, k_nb3;
-    const char * v; int64_t v_nb1, v_nb2, v_nb3;
+    const char * k; uint32_t k_nb1; int64_t k_nb2, k_nb3;        // (rows at most 2 GiB apart: a row's address is one 32 x 32 + 64 bit multiply-add)
+    const char * v; uint32_t v_nb1; int64_t v_nb2, v_nb3;
     const char * mask; int64_t m_nb1, m_nb2, m_nb3, m_ne2, m_ne3;
     char * dst; int64_t d_nb1, d_nb2, d_nb3;
     const char * mass_in; int64_t in_nb2, in_nb3;
@@ -102,7 +102,7 @@ template <bool BF, int P> static __device__ __forceinline__ void split8(const fl
             int bits = __builtin_bit_cast(int, h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
             asm("" : "+v"(bits));
             const h2 hi = __builtin_bit_cast(h2, bits);
-            const h2 lo = {(_Float16)(x[2 * i] - (float)hi[0]), (_Float16)(x[2 * i + 1] - (float)hi[1])};
+            const h2 lo = {(_Float16)__builtin_fmaf((float)hi[0], -1.0f, x[2 * i]), (_Float16)__builtin_fmaf((float)hi[1], -1.0f, x[2 * i + 1])};
             out[0][i] = bits;
             out[1][i] = __builtin_bit_cast(int, lo);
         }
@@ -112,9 +112,10 @@ template <bool BF, int P> static __device__ __forceinline__ void split8(const fl
 // 8 consecutive features (chunk j) of a cache row on their way to an operand: the bytes, then 16-bit values (blocks: the integers)
 template <int TYPE> struct Chunk {
     v4i raw;
-    __device__ __forceinline__ void load(const char * row, int j) { raw = *(const v4i *)(row + j * 16); }
+    static __device__ __forceinline__ int at(int j) { return j * 16; }       // byte offset of chunk j in a row
+    __device__ __forceinline__ void load(const char * p, int) { raw = *(const v4i *)p; }
     __device__ __forceinline__ v4i operand(int) const { return raw; }
-    __device__ __forceinline__ float scale() const { return 1.0f; }
+    __device__ __forceinline__ uint16_t scale() const { return 0; }
 };
 static __device__ __forceinline__ v4i bytes_f16(uint32_t w0, uint32_t w1, float bias) {      // 8 bytes -> f16 of (byte - bias); 0x6400 | b is 1024 + b
     const _Float16 c = (_Float16)(1024.0f + bias);
@@ -128,26 +129,26 @@ static __device__ __forceinline__ v4i bytes_f16(uint32_t w0, uint32_t w1, float 
 }
 template <> struct Chunk<MI355_TYPE_Q8_0> {
     uint32_t w0, w1; uint16_t d;
-    __device__ __forceinline__ void load(const char * row, int j) {
-        const char * b = row + (j >> 2) * 34;
-        d = *(const uint16_t *)b;
-        __builtin_memcpy(&w0, b + 2 + (j & 3) * 8, 4); __builtin_memcpy(&w1, b + 6 + (j & 3) * 8, 4);
+    static __device__ __forceinline__ int at(int j) { return (j >> 2) * 34 + 2 + (j & 3) * 8; }
+    __device__ __forceinline__ void load(const char * p, int j) {
+        d = *(const uint16_t *)(p - 2 - (j & 3) * 8);
+        __builtin_memcpy(&w0, p, 4); __builtin_memcpy(&w1, p + 4, 4);
     }
     __device__ __forceinline__ v4i operand(int) const { return bytes_f16(w0 ^ 0x80808080u, w1 ^ 0x80808080u, 128.0f); }
-    __device__ __forceinline__ float scale() const { return h2f(d); }
+    __device__ __forceinline__ uint16_t scale() const { return d; }
 };
 template <> struct Chunk<MI355_TYPE_Q4_0> {
     uint32_t w0, w1; uint16_t d;
-    __device__ __forceinline__ void load(const char * row, int j) {
-        const char * b = row + (j >> 2) * 18;
-        d = *(const uint16_t *)b;
-        __builtin_memcpy(&w0, b + 2 + (j & 1) * 8, 4); __builtin_memcpy(&w1, b + 6 + (j & 1) * 8, 4);
+    static __device__ __forceinline__ int at(int j) { return (j >> 2) * 18 + 2 + (j & 1) * 8; }
+    __device__ __forceinline__ void load(const char * p, int j) {
+        d = *(const uint16_t *)(p - 2 - (j & 1) * 8);
+        __builtin_memcpy(&w0, p, 4); __builtin_memcpy(&w1, p + 4, 4);
     }
     __device__ __forceinline__ v4i operand(int j) const {
         const int sh = (j & 2) * 2;
         return bytes_f16((w0 >> sh) & 0x0f0f0f0fu, (w1 >> sh) & 0x0f0f0f0fu, 8.0f);
     }
-    __device__ __forceinline__ float scale() const { return h2f(d); }
+    __device__ __forceinline__ uint16_t scale() const { return d; }
 };
 // non-finite 16-bit values of a chunk -> 0; true if there was one
 template <bool BF> static __device__ __forceinline__ bool sanitize(v4i & x) {
@@ -173,17 +174,19 @@ static __device__ __forceinline__ float sum_groups(float v) {
 }
 
 template <int TYPE, int D, int NW, bool HASV>
-__global__ void __launch_bounds__(NW * 64)
+__global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : D <= 128 ? 2 : 1)
 mass_step_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
     constexpr int KS = D / 32, FT = D / 16, P = F::parts;
+    constexpr int VR = 512 / D, VN = D / 16;                    // V rows per 64 chunks, groups of 64 chunks of a tile
     constexpr int VP = D * 2 + 32;                              // V tile row pitch (bytes)
     constexpr int OP = D + 4;                                   // merge row pitch (floats)
     constexpr int VB = HASV ? (32 * VP > 16 * OP * 4 ? 32 * VP : 16 * OP * 4) : 16;
+    typedef _Float16 hk_t __attribute__((ext_vector_type(KS)));
     __shared__ __attribute__((aligned(16))) uint8_t lds[NW][VB];
-    __shared__ __attribute__((aligned(16))) float kd[F::quant ? NW : 1][F::quant ? 32 : 1][KS], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 : 1][KS];
+    __shared__ __attribute__((aligned(16))) hk_t kd[F::quant ? NW : 1][F::quant ? 32 : 1], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 : 1];
     __shared__ float wm[NW][16], wl[NW][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, g = lane >> 4;
     const int ratio = a.n_head / a.n_head_kv, R = ratio * a.n_q;
     const int hk = blockIdx.y % a.n_head_kv, r0 = blockIdx.y / a.n_head_kv * 16, i3 = blockIdx.z, split = blockIdx.x;
@@ -192,34 +195,61 @@ mass_step_kernel(const MArgs a) {
     const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
     const char * vb = HASV ? a.v + hk * a.v_nb2 + i3 * a.v_nb3 : nullptr;
     const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
-    const bool m8 = mrow && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
-    const float slope = m_slope(a, h) * LOG2E;
+    const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
     const bool capped = a.logit_softcap != 0.0f;
 
     const int ntiles = (a.n_kv + 31) / 32, per = (ntiles + a.nsplit - 1) / a.nsplit;
     const int t0 = split * per, t1 = t0 + per < ntiles ? t0 + per : ntiles;
 
-    Chunk<TYPE> kc[2][KS], vc[HASV ? D / 16 : 1];
+    // chunks past the head size re-read the last one: they meet zeros of q, and features of V that are not stored.  Slots past the end re-read
+    // the last one and are hidden
+    Chunk<TYPE> kc[2][KS], vc[HASV ? VN : 1];
+    const int vcc = lane % (D / 8) < a.dv / 8 ? lane % (D / 8) : a.dv / 8 - 1;
+    const char * vl = vb + Chunk<TYPE>::at(vcc);
+    int kcc[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+        kcc[ks] = F::quant ? Chunk<TYPE>::at(4 * (ks < a.d / 32 ? ks : a.d / 32 - 1) + g) : Chunk<TYPE>::at(4 * ks + g < a.d / 8 ? 4 * ks + g : a.d / 8 - 1);
     auto load_k = [&](int t) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int j = 32 * t + 16 * u + lr;
-            const char * row = kb + (int64_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
+            const char * row = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) kc[u][ks].load(row, (4 * ks + g) * 8 < a.d ? 4 * ks + g : 0);
+            for (int ks = 0; ks < KS; ks++) kc[u][ks].load(row + kcc[ks], g);
         }
     };
     auto load_v = [&](int t) {
         if constexpr (HASV) {
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {                  // 64 chunks of 8 features at a time
-                const int c = 64 * i + lane, j = 32 * t + c / (D / 8), cc = c % (D / 8);
-                vc[i].load(vb + (int64_t)(j < a.n_kv ? j : a.n_kv - 1) * a.v_nb1, cc * 8 < a.dv ? cc : 0);
+            for (int i = 0; i < VN; i++) {
+                const int j = 32 * t + VR * i + lane / (D / 8);
+                vc[i].load(vl + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.v_nb1, vcc);
             }
         }
     };
+    // mask of slots 32 t + 16 u + 4 g + i as it lies, -inf past the last slot
+    auto load_mask = [&](int t, u2 (&w)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int j = 32 * t + 16 * u + 4 * g;
+            if (m8 && j + 4 <= a.n_kv) w[u] = *(const u2 *)(mrow + 2 * (int64_t)j);
+            else {
+                uint32_t x[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = j + i >= a.n_kv ? 0xfc00u : a.mask ? ((const uint16_t *)mrow)[j + i] : 0u;
+                w[u] = u2{x[0] | x[1] << 16, x[2] | x[3] << 16};
+            }
+        }
+    };
+    auto sees = [&](const u2 (&w)[2]) { return __any(!(w[0].x == 0xfc00fc00u && w[0].y == 0xfc00fc00u && w[1].x == 0xfc00fc00u && w[1].y == 0xfc00fc00u)); };
+
+    // a tile hidden from every row costs its mask, which runs one tile ahead of the rows.  The first tile is fetched without asking: one
+    // round trip instead of two at the start
     int t = t0 + wave;
-    if (t < t1) { load_k(t); load_v(t); }
+    u2 mk[2], mkn[2];
+    if (t < t1) { load_k(t); load_v(t); load_mask(t, mk); }
+    if (t + NW < t1) load_mask(t + NW, mkn);
 
     // q: scale and log2(e) on it, for f16 the row's largest value brought to [2^14, 2^15) by a power of two that the
     // logits get back (its small values then stay clear of the subnormal range)
@@ -251,39 +281,45 @@ mass_step_kernel(const MArgs a) {
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) split8<F::bf, P>(x[ks], qf[ks]);
     }
+    const float slope = m_slope(a, h) * LOG2E;
 
     float m = -INFINITY, l = 0.0f;              // of this lane's row; l over this lane's slots only
+    int E = -64;                                // blocks: o holds 2^(14 - E) times its value, E the exponent of the largest scale of V met so far
     v4f o[HASV ? FT : 1];
 #pragma unroll
     for (int i = 0; i < (HASV ? FT : 1); i++) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float * lg = a.logits + (((int64_t)i3 * a.n_head_kv + hk) * R + r) * a.lpitch;
+    const bool mine = r0 + lr < R;
 
-    for (; t < t1; t += NW) {
-        // mask of slots 32 t + 16 u + 4 g + i
+    while (t < t1) {
         float mv[2][4];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int j = 32 * t + 16 * u + 4 * g;
-            if (m8 && j + 4 <= a.n_kv) {
-                const u2 w = *(const u2 *)(mrow + 2 * j);
-                mv[u][0] = h2f((uint16_t)w.x); mv[u][1] = h2f((uint16_t)(w.x >> 16)); mv[u][2] = h2f((uint16_t)w.y); mv[u][3] = h2f((uint16_t)(w.y >> 16));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) mv[u][i] = j + i >= a.n_kv ? -INFINITY : mrow ? h2f(((const uint16_t *)mrow)[j + i]) : 0.0f;
-            }
+            mv[u][0] = h2f((uint16_t)mk[u].x); mv[u][1] = h2f((uint16_t)(mk[u].x >> 16)); mv[u][2] = h2f((uint16_t)mk[u].y); mv[u][3] = h2f((uint16_t)(mk[u].y >> 16));
         }
+        int tn = t + NW;                        // the next tile that a row sees
+        while (tn < t1 && !sees(mkn)) {
+            if (mine) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) if (32 * tn + 16 * u + 4 * g < a.lpitch) *(v4f *)(lg + 32 * tn + 16 * u + 4 * g) = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            }
+            tn += NW;
+            if (tn < t1) load_mask(tn, mkn);
+        }
+        const bool next = tn < t1;
+#pragma unroll
+        for (int u = 0; u < 2; u++) mk[u] = mkn[u];
         if constexpr (F::quant) {               // scales of the 32 slots where every lane can read them
             if (g < KS) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) if (ks % 4 == g) kd[wave][16 * u + lr][ks] = kc[u][ks].scale();
+                    for (int ks = 0; ks < KS; ks++) if (ks % 4 == g) ((uint16_t *)&kd[wave][16 * u + lr])[ks] = kc[u][ks].scale();
             }
             if constexpr (HASV) {
+                if ((lane & 3) == 0) {
 #pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    const int c = 64 * i + lane, cc = c % (D / 8);
-                    if ((cc & 3) == 0) vd[wave][c / (D / 8)][cc >> 2] = vc[i].scale();
+                    for (int i = 0; i < VN; i++) ((uint16_t *)&vd[wave][VR * i + lane / (D / 8)])[lane % (D / 8) / 4] = vc[i].scale();
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -293,12 +329,11 @@ mass_step_kernel(const MArgs a) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
-            float dk[4][KS];
-            if constexpr (F::quant)
+            hk_t dk[4];
+            if constexpr (F::quant) {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++) dk[i][ks] = kd[wave][16 * u + 4 * g + i][ks];
+                for (int i = 0; i < 4; i++) dk[i] = kd[wave][16 * u + 4 * g + i];
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 v4f b = F::quant ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : c;
@@ -307,30 +342,32 @@ mass_step_kernel(const MArgs a) {
                 for (int p = P - 1; p >= 0; p--) b = mfma16<F::bf>(kop, qf[ks][p], b);
                 if constexpr (F::quant) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) c[i] = __builtin_fmaf(b[i], dk[i][ks], c[i]);
+                    for (int i = 0; i < 4; i++) c[i] = __builtin_fmaf(b[i], (float)dk[i][ks], c[i]);
                 } else c = b;
             }
+            if (capped) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float x = c[i] * qe;
-                if (capped) x = a.logit_softcap * LOG2E * tanhf(x);
-                s[u][i] = mv[u][i] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[u][i], slope, x);
+                for (int i = 0; i < 4; i++) c[i] = a.logit_softcap * LOG2E * tanhf(c[i] * qe);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[i] *= qe;
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[u][i] = mv[u][i] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[u][i], slope, c[i]);
         }
-        if (t + NW < t1) load_k(t + NW);        // in flight during the rest of this tile
+        if (next) load_k(tn);                   // in flight during the rest of this tile
+        if (tn + NW < t1) load_mask(tn + NW, mkn);
         float mx = m;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int j = 32 * t + 16 * u + 4 * g;
-            if (r0 + lr < R) {
-                if (j + 4 <= a.lpitch) *(v4f *)(lg + j) = v4f{s[u][0], s[u][1], s[u][2], s[u][3]};
-            }
+            if (mine && j < a.lpitch) *(v4f *)(lg + j) = v4f{s[u][0], s[u][1], s[u][2], s[u][3]};
 #pragma unroll
             for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[u][i]);
         }
         mx = max_groups(mx);
         const float ms = mx == -INFINITY ? 0.0f : mx;
-        const float corr = __builtin_amdgcn_exp2f(m - ms);      // m = -inf: 0
+        float corr = __builtin_amdgcn_exp2f(m - ms);            // m = -inf: 0
         float p[8];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -341,19 +378,40 @@ mass_step_kernel(const MArgs a) {
         for (int i = 0; i < 8; i++) l += p[i];
         m = mx;
         if constexpr (HASV) {
+            bool some = false;
+#pragma unroll
+            for (int i = 0; i < 8; i++) some |= s[i >> 2][i & 3] == -INFINITY;
+            const bool hidden = __any(some);                    // some row does not see some slot of the tile
+            hk_t dd[8];
+            if constexpr (F::quant) {
+                // the scales of V go on P.  A hidden slot's is taken as 0 (it may be NaN)
+                _Float16 dm = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) dd[i] = vd[wave][(i & 4) * 4 + 4 * g + (i & 3)];
+                if (hidden) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) if (s[i >> 2][i & 3] == -INFINITY) dd[i] = (hk_t)(_Float16)0;
+                }
+                hk_t mxd = __builtin_elementwise_abs(dd[0]);
+#pragma unroll
+                for (int i = 1; i < 8; i++) mxd = __builtin_elementwise_max(mxd, __builtin_elementwise_abs(dd[i]));
+#pragma unroll
+                for (int k = 0; k < KS; k++) dm = dm > mxd[k] ? dm : mxd[k];
+                const float dmx = max_groups((float)dm);
+                const int e = dmx > 0.0f && dmx < INFINITY ? __builtin_amdgcn_frexp_expf(dmx) - 1 : -64;
+                const int En = E > e ? E : e;
+                corr = ldexpf(corr, E - En);
+                E = En;
+            }
             if (__any(corr != 1.0f)) {
 #pragma unroll
                 for (int i = 0; i < FT; i++) o[i] = o[i] * corr;
             }
             // ---- V tile into LDS.  A slot that some row does not see must not reach that row through 0 * NaN: its non-finite values are
             // taken out here and added below to the rows that do see it
-            bool some = false;
-#pragma unroll
-            for (int i = 0; i < 8; i++) some |= s[i >> 2][i & 3] == -INFINITY;
-            uint64_t bad = 0;                                   // rows of the tile with values taken out
-            const bool hidden = !F::quant && __any(some);
-            uint32_t unseen = 0;                                // bit j: slot 32 t + j is hidden from some row
-            if (hidden) {
+            uint64_t bad = 0;                                   // slots of the tile with values taken out
+            if constexpr (!F::quant) if (hidden) {
+                uint32_t unseen = 0;                            // bit j: slot 32 t + j is hidden from some row
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -362,68 +420,48 @@ mass_step_kernel(const MArgs a) {
 #pragma unroll
                         for (int gg = 0; gg < 4; gg++) if ((b >> (16 * gg)) & 0xffff) unseen |= 1u << (16 * u + 4 * gg + i);
                     }
-            }
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                const int c = 64 * i + lane, row = c / (D / 8), cc = c % (D / 8);
-                v4i x = vc[i].operand(cc & 3);
-                if (cc * 8 >= a.dv) x = v4i{0, 0, 0, 0};
-                if (hidden) {
+                for (int i = 0; i < VN; i++) {
+                    const int row = VR * i + lane / (D / 8);
                     bool taken = false;
-                    if (unseen >> row & 1) taken = sanitize<F::bf>(x);
+                    if (unseen >> row & 1) taken = sanitize<F::bf>(vc[i].raw);
                     const uint64_t b = __ballot(taken);
-                    constexpr int rows = 512 / D;               // slots per 64 chunks
+                    if (b) {
 #pragma unroll
-                    for (int q = 0; q < rows; q++) if (b & (rows == 1 ? ~0ull : ((1ull << (D / 8 % 64)) - 1) << (q * (D / 8)))) bad |= 1ull << (i * rows + q);
+                        for (int q = 0; q < VR; q++) if (b >> (q * (D / 8)) & ((1ull << (D / 8)) - 1)) bad |= 1ull << (i * VR + q);
+                    }
                 }
-                *(v4i *)(lds[wave] + row * VP + cc * 16) = x;
             }
+#pragma unroll
+            for (int i = 0; i < VN; i++) *(v4i *)(lds[wave] + (VR * i + lane / (D / 8)) * VP + lane % (D / 8) * 16) = vc[i].operand(vcc);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (t + NW < t1) load_v(t + NW);
+            if (next) load_v(tn);
             // ---- O^T
             const uint8_t * vt = lds[wave] + (4 * g + (lr >> 2)) * VP + 8 * (lr & 3);
+            if constexpr (!F::bf) {                             // f16 parts: clear of the subnormal range
+                const float c = F::quant ? ldexpf(1.0f, 14 - E) : 16384.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) p[i] *= c;
+            }
             v4i pf[P];
-            float back = 1.0f;
+            if constexpr (!F::quant) split8<F::bf, P>(p, pf);
 #pragma unroll
             for (int f = 0; f < FT; f++) {
                 if constexpr (F::quant) {
-                    if (f % 2 == 0) {                           // a new 32-block: P times the slots' scales, their largest brought to [1, 2)
-                        float x[8], dm = 0.0f;
+                    if (f % 2 == 0) {                           // a new 32-block
+                        float x[8];
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float dd = vd[wave][(i & 4) * 4 + 4 * g + (i & 3)][f / 2];
-                            x[i] = s[i >> 2][i & 3] == -INFINITY ? 0.0f : dd;
-                            dm = fmaxf(dm, fabsf(x[i]));
-                        }
-                        dm = max_groups(dm);
-                        const int e = dm > 0.0f && dm < INFINITY ? __builtin_amdgcn_frexp_expf(dm) - 1 : 0;
-                        back = ldexpf(1.0f, e - 14);
-                        const float fwd = ldexpf(1.0f, 14 - e);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = x[i] * fwd * p[i];
+                        for (int i = 0; i < 8; i++) x[i] = p[i] * (float)dd[i][f / 2];
                         split8<false, 2>(x, pf);
                     }
-                } else if (f == 0) {
-                    float x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = F::bf ? p[i] : p[i] * 16384.0f;      // f16: clear of the subnormal range
-                    split8<F::bf, P>(x, pf);
                 }
                 const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(vt + 32 * f));
                 const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(vt + 32 * f + 16 * VP));
                 v4i vop;
                 __builtin_memcpy(&vop, &lo, 8);
                 __builtin_memcpy((char *)&vop + 8, &hi, 8);
-                if constexpr (F::quant) {
-                    v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int q = P - 1; q >= 0; q--) c = mfma16<false>(vop, pf[q], c);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) o[f][i] = __builtin_fmaf(c[i], back, o[f][i]);
-                } else {
-#pragma unroll
-                    for (int q = P - 1; q >= 0; q--) o[f] = mfma16<F::bf>(vop, pf[q], o[f]);
-                }
+                for (int q = P - 1; q >= 0; q--) o[f] = mfma16<F::bf>(vop, pf[q], o[f]);
             }
             if (!F::quant && bad) {                             // non-finite values of slots that only some rows see
                 for (int row = 0; row < 32; row++) {
@@ -450,6 +488,7 @@ mass_step_kernel(const MArgs a) {
                 }
             }
         }
+        t = tn;
     }
     // ---- the waves' states meet in LDS
     l = sum_groups(l);
@@ -457,7 +496,7 @@ mass_step_kernel(const MArgs a) {
     if constexpr (HASV) {
         float * ob = (float *)lds[wave] + lr * OP + 4 * g;
 #pragma unroll
-        for (int f = 0; f < FT; f++) *(v4f *)(ob + 16 * f) = F::bf || F::quant ? o[f] : o[f] * (1.0f / 16384.0f);
+        for (int f = 0; f < FT; f++) *(v4f *)(ob + 16 * f) = o[f] * (F::bf ? 1.0f : F::quant ? ldexpf(1.0f, E - 14) : 1.0f / 16384.0f);
     }
     __syncthreads();
     const int rows = R - r0 < 16 ? R - r0 : 16;
@@ -491,60 +530,97 @@ mass_step_kernel(const MArgs a) {
     }
 }
 
-// The slices' statistics meet: workgroups 0 .. mass_wgs - 1 form the weights of 256 slots each from the logits, the others a row of dst each
+// The slices' statistics meet: workgroups 0 .. mass_wgs - 1 form the weights of 256 slots each from the logits, the others a row of dst each.
+// Both start with loads that nothing precedes (a slice's statistics: one load per thread at 64 slices of 4 rows), so the launch is two
+// memory round trips long.
 template <int D>
 __global__ void __launch_bounds__(256)
 mass_finish_kernel(const MArgs a, int mass_wgs) {
-    __shared__ float sm[64], sl[64];
+    __shared__ float sm[256], sl[256];
     const int tid = threadIdx.x, hk = blockIdx.y, i3 = blockIdx.z;
     const int ratio = a.n_head / a.n_head_kv, R = ratio * a.n_q;
     const int64_t base = ((int64_t)i3 * a.n_head_kv + hk) * a.nsplit * R;
-    const float * st = a.stats + base * 2;
+    const v2f * st = (const v2f *)a.stats + base;
     if ((int)blockIdx.x < mass_wgs) {
-        const int j = blockIdx.x * 256 + tid;
-        const float * lg = a.logits + ((int64_t)i3 * a.n_head_kv + hk) * R * a.lpitch;
+        int w = 4;                                              // threads per row: 64 for up to 4 rows .. 4 for 64
+        while (w < 64 && w * 2 * R <= 256) w *= 2;
+        const int rows = 256 / w, j = blockIdx.x * 256 + tid;
+        const float * lg = a.logits + ((int64_t)i3 * a.n_head_kv + hk) * R * a.lpitch + j;
         float t = 0.0f;
-        for (int r0 = 0; r0 < R; r0 += 64) {                    // 64 rows' statistics at a time, four lanes a row
-            __syncthreads();
-            const int r = r0 + (tid >> 2), q = tid & 3;
-            float M = -INFINITY, L = 0.0f;
-            if (r < R) for (int s = q; s < a.nsplit; s += 4) {
-                const float ms = st[((int64_t)s * R + r) * 2], ls = st[((int64_t)s * R + r) * 2 + 1];
-                const float mn = fmaxf(M, ms), mz = mn == -INFINITY ? 0.0f : mn;
-                L = L * __builtin_amdgcn_exp2f(M - mz) + ls * __builtin_amdgcn_exp2f(ms - mz);
-                M = mn;
-            }
+        for (int r0 = 0; r0 < R; r0 += rows) {
+            float s4[4];                                        // the first logits, requested beside the statistics
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
+            for (int i = 0; i < 4; i++) s4[i] = j < a.n_kv && r0 + i < R ? lg[(int64_t)(r0 + i) * a.lpitch] : -INFINITY;
+            const int r = r0 + tid / w;
+            float M = -INFINITY, L = 0.0f;
+            if (r < R) {
+                for (int s = tid % w; s < a.nsplit; s += 4 * w) {
+                    v2f x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = s + i * w < a.nsplit ? st[(int64_t)(s + i * w) * R + r] : v2f{-INFINITY, 0.0f};
+                    const float mn = fmaxf(fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)), M), mz = mn == -INFINITY ? 0.0f : mn;
+                    L *= __builtin_amdgcn_exp2f(M - mz);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) L = __builtin_fmaf(x[i].y, __builtin_amdgcn_exp2f(x[i].x - mz), L);
+                    M = mn;
+                }
+            }
+            for (int o = 1; o < w; o <<= 1) {
                 const float mo = __shfl_xor(M, o, 64), lo = __shfl_xor(L, o, 64);
                 const float mn = fmaxf(M, mo), mz = mn == -INFINITY ? 0.0f : mn;
                 L = L * __builtin_amdgcn_exp2f(M - mz) + lo * __builtin_amdgcn_exp2f(mo - mz);
                 M = mn;
             }
-            if (q == 0) { sm[tid >> 2] = M == -INFINITY ? 0.0f : M; sl[tid >> 2] = L == 0.0f ? 0.0f : 1.0f / L; }
             __syncthreads();
-            if (j < a.n_kv)
-                for (int rr = 0; rr < 64 && r0 + rr < R; rr++) {
-                    const float s = lg[(int64_t)(r0 + rr) * a.lpitch + j];
-                    t += s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - sm[rr]) * sl[rr];
-                }
+            if (tid % w == 0) { sm[tid / w] = M == -INFINITY ? 0.0f : M; sl[tid / w] = L == 0.0f ? 0.0f : 1.0f / L; }
+            __syncthreads();
+            const int n = R - r0 < rows ? R - r0 : rows;
+#pragma unroll
+            for (int i = 0; i < 4; i++) if (i < n && s4[i] != -INFINITY) t = __builtin_fmaf(__builtin_amdgcn_exp2f(s4[i] - sm[i]), sl[i], t);
+            for (int i0 = 4; i0 < n; i0 += 4) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) s4[i] = j < a.n_kv && i0 + i < n ? lg[(int64_t)(r0 + i0 + i) * a.lpitch] : -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (i0 + i < n && s4[i] != -INFINITY) t = __builtin_fmaf(__builtin_amdgcn_exp2f(s4[i] - sm[i0 + i]), sl[i0 + i], t);
+            }
         }
         if (j >= a.n_kv) return;
         if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
         ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
         return;
     }
+    // a row of dst: D / 4 threads per slice of the sum over the splits
+    constexpr int F4 = D / 4, SG = 256 / F4;
+    __shared__ v4f so[SG][F4];
     const int r = blockIdx.x - mass_wgs, iq = r / ratio, h = hk * ratio + r % ratio;
-    float M = -INFINITY, L = 0.0f, O = 0.0f;
-    for (int s = 0; s < a.nsplit; s++) M = fmaxf(M, st[((int64_t)s * R + r) * 2]);
+    const int f4 = tid % F4, sg = tid / F4;
+    const bool in = 4 * f4 < a.dv;
+    float M = -INFINITY;
+    for (int s = tid; s < a.nsplit; s += 256) M = fmaxf(M, st[(int64_t)s * R + r].x);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if ((tid & 63) == 0) sm[tid >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     const float ms = M == -INFINITY ? 0.0f : M;
-    if (tid >= a.dv) return;
-    for (int s = 0; s < a.nsplit; s++) {
-        const float c = __builtin_amdgcn_exp2f(st[((int64_t)s * R + r) * 2] - ms);
-        L = __builtin_fmaf(st[((int64_t)s * R + r) * 2 + 1], c, L);
-        O = __builtin_fmaf(a.part[(base + (int64_t)s * R + r) * D + tid], c, O);
+    float L = 0.0f;
+    v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = sg; s < a.nsplit; s += SG) {
+        const v2f x = st[(int64_t)s * R + r];
+        const v4f y = in ? *(const v4f *)(a.part + (base + (int64_t)s * R + r) * D + 4 * f4) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        const float c = __builtin_amdgcn_exp2f(x.x - ms);
+        L = __builtin_fmaf(x.y, c, L);
+#pragma unroll
+        for (int i = 0; i < 4; i++) O[i] = __builtin_fmaf(y[i], c, O[i]);
     }
-    ((float *)(a.dst + (int64_t)h * a.d_nb1 + (int64_t)iq * a.d_nb2 + (int64_t)i3 * a.d_nb3))[tid] = L == 0.0f ? 0.0f : O / L;
+    so[sg][f4] = O;
+    if (f4 == 0) sl[sg] = L;
+    __syncthreads();
+    if (sg != 0 || !in) return;
+#pragma unroll
+    for (int i = 1; i < SG; i++) { O = O + so[i][f4]; L += sl[i]; }
+    *(v4f *)((float *)(a.dst + (int64_t)h * a.d_nb1 + (int64_t)iq * a.d_nb2 + (int64_t)i3 * a.d_nb3) + 4 * f4) = L == 0.0f ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : O * (1.0f / L);
 }
 
 constexpr int STEP_WAVES = 4;
@@ -677,6 +753,7 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
         p->n_kv > (1 << 30) || p->n_head_kv * ((p->n_head / p->n_head_kv * MI355_MASS_MAX_Q + 15) / 16) > 65535 || p->ne3 < 1 || p->ne3 > 65535) return MI355_E_SHAPE;
     if (with_dst && p->n_q > MI355_MASS_MAX_Q) return MI355_E_UNSUPPORTED;
     if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1)) return MI355_E_SHAPE;
+    if (p->k_nb1 < 0 || p->k_nb1 > 0x7fffffff || (with_dst && (p->v_nb1 < 0 || p->v_nb1 > 0x7fffffff))) return MI355_E_SHAPE;
     const int64_t f32s = (int64_t)(uintptr_t)p->q | p->q_nb1 | p->q_nb2 | p->q_nb3 |
                          (with_dst ? (int64_t)(uintptr_t)p->dst | p->d_nb1 | p->d_nb2 | p->d_nb3 : 0) | (int64_t)(uintptr_t)workspace;
     int64_t cache = (int64_t)(uintptr_t)p->k | p->k_nb1 | p->k_nb2 | p->k_nb3;
@@ -689,8 +766,8 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
 
     MArgs a;
     a.q = (const char *)p->q; a.q_nb1 = p->q_nb1; a.q_nb2 = p->q_nb2; a.q_nb3 = p->q_nb3;
-    a.k = (const char *)p->k; a.k_nb1 = p->k_nb1; a.k_nb2 = p->k_nb2; a.k_nb3 = p->k_nb3;
-    a.v = (const char *)p->v; a.v_nb1 = p->v_nb1; a.v_nb2 = p->v_nb2; a.v_nb3 = p->v_nb3;
+    a.k = (const char *)p->k; a.k_nb1 = (uint32_t)p->k_nb1; a.k_nb2 = p->k_nb2; a.k_nb3 = p->k_nb3;
+    a.v = (const char *)p->v; a.v_nb1 = (uint32_t)p->v_nb1; a.v_nb2 = p->v_nb2; a.v_nb3 = p->v_nb3;
     a.mask = (const char *)p->mask; a.m_nb1 = p->m_nb1; a.m_nb2 = p->m_nb2; a.m_nb3 = p->m_nb3; a.m_ne2 = p->m_ne2; a.m_ne3 = p->m_ne3;
     a.dst = with_dst ? (char *)p->dst : nullptr; a.d_nb1 = p->d_nb1; a.d_nb2 = p->d_nb2; a.d_nb3 = p->d_nb3;
     a.mass_in = w->decay != 0.0f ? (const char *)w->mass_in : nullptr; a.in_nb2 = w->in_nb2; a.in_nb3 = w->in_nb3;
