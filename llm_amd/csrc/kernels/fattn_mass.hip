@@ -113,9 +113,8 @@ template <bool BF, int P> static __device__ __forceinline__ void split8(const fl
 template <int TYPE> struct Chunk {
     v4i raw;
     static __device__ __forceinline__ int at(int j) { return j * 16; }       // byte offset of chunk j in a row
-    __device__ __forceinline__ void load(const char * p, int) { raw = *(const v4i *)p; }
+    __device__ __forceinline__ void load(const char * p) { raw = *(const v4i *)p; }
     __device__ __forceinline__ v4i operand(int) const { return raw; }
-    __device__ __forceinline__ uint16_t scale() const { return 0; }
 };
 static __device__ __forceinline__ v4i bytes_f16(uint32_t w0, uint32_t w1, float bias) {      // 8 bytes -> f16 of (byte - bias); 0x6400 | b is 1024 + b
     const _Float16 c = (_Float16)(1024.0f + bias);
@@ -128,27 +127,19 @@ static __device__ __forceinline__ v4i bytes_f16(uint32_t w0, uint32_t w1, float 
     return r;
 }
 template <> struct Chunk<MI355_TYPE_Q8_0> {
-    uint32_t w0, w1; uint16_t d;
+    uint32_t w0, w1;
     static __device__ __forceinline__ int at(int j) { return (j >> 2) * 34 + 2 + (j & 3) * 8; }
-    __device__ __forceinline__ void load(const char * p, int j) {
-        d = *(const uint16_t *)(p - 2 - (j & 3) * 8);
-        __builtin_memcpy(&w0, p, 4); __builtin_memcpy(&w1, p + 4, 4);
-    }
+    __device__ __forceinline__ void load(const char * p) { __builtin_memcpy(&w0, p, 4); __builtin_memcpy(&w1, p + 4, 4); }
     __device__ __forceinline__ v4i operand(int) const { return bytes_f16(w0 ^ 0x80808080u, w1 ^ 0x80808080u, 128.0f); }
-    __device__ __forceinline__ uint16_t scale() const { return d; }
 };
 template <> struct Chunk<MI355_TYPE_Q4_0> {
-    uint32_t w0, w1; uint16_t d;
+    uint32_t w0, w1;
     static __device__ __forceinline__ int at(int j) { return (j >> 2) * 18 + 2 + (j & 1) * 8; }
-    __device__ __forceinline__ void load(const char * p, int j) {
-        d = *(const uint16_t *)(p - 2 - (j & 1) * 8);
-        __builtin_memcpy(&w0, p, 4); __builtin_memcpy(&w1, p + 4, 4);
-    }
+    __device__ __forceinline__ void load(const char * p) { __builtin_memcpy(&w0, p, 4); __builtin_memcpy(&w1, p + 4, 4); }
     __device__ __forceinline__ v4i operand(int j) const {
         const int sh = (j & 2) * 2;
         return bytes_f16((w0 >> sh) & 0x0f0f0f0fu, (w1 >> sh) & 0x0f0f0f0fu, 8.0f);
     }
-    __device__ __forceinline__ uint16_t scale() const { return d; }
 };
 // non-finite 16-bit values of a chunk -> 0; true if there was one
 template <bool BF> static __device__ __forceinline__ bool sanitize(v4i & x) {
@@ -173,252 +164,313 @@ static __device__ __forceinline__ float sum_groups(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-template <int TYPE, int D, int NW, bool HASV>
-__global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : D <= 128 ? 2 : 1)
+// RT: 16-row tiles of a workgroup.  RP (blocks only): the 16 columns of a tile are RP rows times 16 / RP classes of 32-blocks -- at GQA 4 or 8
+// the columns that would repeat a row each scale P by the blocks of their class, so a lane forms D / 32 / (16 / RP) scaled copies of P and not
+// D / 32; a feature tile takes its result from the columns of its block's class.
+template <int TYPE, int D, int NW, bool HASV, int RT, int RP>
+__global__ void __launch_bounds__(NW * 64, D <= 64 ? (RT == 1 ? 3 : 2) : D <= 128 ? 2 : 1)
 mass_step_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
     constexpr int KS = D / 32, FT = D / 16, P = F::parts;
+    constexpr int NC = 16 / RP, SETS = KS > NC ? KS / NC : 1;   // classes of blocks, scaled copies of P per lane
     constexpr int VR = 512 / D, VN = D / 16;                    // V rows per 64 chunks, groups of 64 chunks of a tile
     constexpr int VP = D * 2 + 32;                              // V tile row pitch (bytes)
     constexpr int OP = D + 4;                                   // merge row pitch (floats)
     constexpr int VB = HASV ? (32 * VP > 16 * OP * 4 ? 32 * VP : 16 * OP * 4) : 16;
+    constexpr int DN = KS / 2;                                  // scales of a tile per lane: 32 rows x KS blocks over 64 lanes
     typedef _Float16 hk_t __attribute__((ext_vector_type(KS)));
     __shared__ __attribute__((aligned(16))) uint8_t lds[NW][VB];
-    __shared__ __attribute__((aligned(16))) hk_t kd[F::quant ? NW : 1][F::quant ? 32 : 1], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 : 1];
-    __shared__ float wm[NW][16], wl[NW][16];
+    __shared__ v4i qs[RT][KS][P][64];
+    __shared__ __attribute__((aligned(16))) uint16_t kd[F::quant ? NW : 1][F::quant ? 32 * KS : 8], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 * KS : 8];
+    __shared__ float wm[NW][16 * RT], wl[NW][16 * RT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, g = lane >> 4;
     const int ratio = a.n_head / a.n_head_kv, R = ratio * a.n_q;
-    const int hk = blockIdx.y % a.n_head_kv, r0 = blockIdx.y / a.n_head_kv * 16, i3 = blockIdx.z, split = blockIdx.x;
-    const int r = r0 + lr < R ? r0 + lr : R - 1;                // this lane's row (the lanes past the last one repeat it)
-    const int iq = r / ratio, h = hk * ratio + r % ratio;
+    const int hk = blockIdx.y % a.n_head_kv, rb = blockIdx.y / a.n_head_kv * 16 * RT, i3 = blockIdx.z, split = blockIdx.x;
     const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
     const char * vb = HASV ? a.v + hk * a.v_nb2 + i3 * a.v_nb3 : nullptr;
-    const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
     const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
     const bool capped = a.logit_softcap != 0.0f;
-
-    const int ntiles = (a.n_kv + 31) / 32, per = (ntiles + a.nsplit - 1) / a.nsplit;
-    const int t0 = split * per, t1 = t0 + per < ntiles ? t0 + per : ntiles;
+    // this lane's rows (columns past the last one repeat it)
+    int r[RT];
+    const char * mrow[RT];
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        r[x] = rb + 16 * x + lr % RP;
+        if (r[x] >= R) r[x] = R - 1;
+        const int iq = r[x] / ratio, h = hk * ratio + r[x] % ratio;
+        mrow[x] = a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3;
+    }
 
     // chunks past the head size re-read the last one: they meet zeros of q, and features of V that are not stored.  Slots past the end re-read
     // the last one and are hidden
+    const int ntiles = (a.n_kv + 31) / 32, TW = a.nsplit * NW;
     Chunk<TYPE> kc[2][KS], vc[HASV ? VN : 1];
+    uint16_t ksc[F::quant ? DN : 1], vsc[F::quant && HASV ? DN : 1];
     const int vcc = lane % (D / 8) < a.dv / 8 ? lane % (D / 8) : a.dv / 8 - 1;
     const char * vl = vb + Chunk<TYPE>::at(vcc);
     int kcc[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++)
         kcc[ks] = F::quant ? Chunk<TYPE>::at(4 * (ks < a.d / 32 ? ks : a.d / 32 - 1) + g) : Chunk<TYPE>::at(4 * ks + g < a.d / 8 ? 4 * ks + g : a.d / 8 - 1);
+    auto slot = [&](int j) { return (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1); };
+    auto load_scales = [&](const char * base, uint32_t nb1, int dim, int t, uint16_t * out) {
+#pragma unroll
+        for (int i = 0; i < DN; i++) {
+            const int n = 64 * i + lane, b = n % KS < dim / 32 ? n % KS : dim / 32 - 1;
+            out[i] = *(const uint16_t *)(base + slot(32 * t + n / KS) * nb1 + b * F::block);
+        }
+    };
     auto load_k = [&](int t) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int j = 32 * t + 16 * u + lr;
-            const char * row = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
+            const char * row = kb + slot(32 * t + 16 * u + lr) * a.k_nb1;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) kc[u][ks].load(row + kcc[ks], g);
+            for (int ks = 0; ks < KS; ks++) kc[u][ks].load(row + kcc[ks]);
         }
+        if constexpr (F::quant) load_scales(kb, a.k_nb1, a.d, t, ksc);
     };
     auto load_v = [&](int t) {
         if constexpr (HASV) {
 #pragma unroll
-            for (int i = 0; i < VN; i++) {
-                const int j = 32 * t + VR * i + lane / (D / 8);
-                vc[i].load(vl + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.v_nb1, vcc);
-            }
+            for (int i = 0; i < VN; i++) vc[i].load(vl + slot(32 * t + VR * i + lane / (D / 8)) * a.v_nb1);
+            if constexpr (F::quant) load_scales(vb, a.v_nb1, a.dv, t, vsc);
         }
     };
     // mask of slots 32 t + 16 u + 4 g + i as it lies, -inf past the last slot
-    auto load_mask = [&](int t, u2 (&w)[2]) {
+    auto load_mask = [&](int t, u2 (&w)[RT][2]) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int j = 32 * t + 16 * u + 4 * g;
-            if (m8 && j + 4 <= a.n_kv) w[u] = *(const u2 *)(mrow + 2 * (int64_t)j);
-            else {
-                uint32_t x[4];
+        for (int x = 0; x < RT; x++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = j + i >= a.n_kv ? 0xfc00u : a.mask ? ((const uint16_t *)mrow)[j + i] : 0u;
-                w[u] = u2{x[0] | x[1] << 16, x[2] | x[3] << 16};
+            for (int u = 0; u < 2; u++) {
+                const int j = 32 * t + 16 * u + 4 * g;
+                if (m8 && j + 4 <= a.n_kv) w[x][u] = *(const u2 *)(mrow[x] + 2 * (int64_t)j);
+                else {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[i] = j + i >= a.n_kv ? 0xfc00u : a.mask ? ((const uint16_t *)mrow[x])[j + i] : 0u;
+                    w[x][u] = u2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+                }
             }
-        }
     };
-    auto sees = [&](const u2 (&w)[2]) { return __any(!(w[0].x == 0xfc00fc00u && w[0].y == 0xfc00fc00u && w[1].x == 0xfc00fc00u && w[1].y == 0xfc00fc00u)); };
+    auto sees = [&](const u2 (&w)[RT][2]) {
+        bool all = true;
+#pragma unroll
+        for (int x = 0; x < RT; x++) all &= w[x][0].x == 0xfc00fc00u && w[x][0].y == 0xfc00fc00u && w[x][1].x == 0xfc00fc00u && w[x][1].y == 0xfc00fc00u;
+        return __any(!all);
+    };
 
-    // a tile hidden from every row costs its mask, which runs one tile ahead of the rows.  The first tile is fetched without asking: one
-    // round trip instead of two at the start
-    int t = t0 + wave;
-    u2 mk[2], mkn[2];
-    if (t < t1) { load_k(t); load_v(t); load_mask(t, mk); }
-    if (t + NW < t1) load_mask(t + NW, mkn);
+    // tiles are dealt to the waves of all slices in turn: sequences shorter than the range keep them all busy.  A tile hidden from every row
+    // costs its mask, which runs one tile ahead of the rows; the first tile is fetched without asking: one round trip instead of two
+    int t = split * NW + wave;
+    u2 mk[RT][2], mkn[RT][2];
+    if (t < ntiles) { load_k(t); load_v(t); load_mask(t, mk); }
+    if (t + TW < ntiles) load_mask(t + TW, mkn);
 
-    // q: scale and log2(e) on it, for f16 the row's largest value brought to [2^14, 2^15) by a power of two that the
-    // logits get back (its small values then stay clear of the subnormal range)
-    v4i qf[KS][P];
-    float qe = 1.0f;
-    {
+    // q for all waves, in LDS as the B operand takes it: a wave splits the 32-feature chunks that fall to it.  Scale and log2(e) go on q; for f16
+    // the row's largest value is brought to [2^14, 2^15) by a power of two that the logits get back (its small values then stay clear of the
+    // subnormal range)
+    constexpr int QN = (KS + NW - 1) / NW;
+    float qe[RT], slope[RT], y[RT][QN][8];
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        const int iq = r[x] / ratio, h = hk * ratio + r[x] % ratio;
+        slope[x] = m_slope(a, h) * LOG2E;
         const float * qp = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
-        const float qs = capped ? a.scale / a.logit_softcap : a.scale * LOG2E;
-        float x[KS][8], amax = 0.0f;
+        const float sc = capped ? a.scale / a.logit_softcap : a.scale * LOG2E;
+        float amax = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int f = 32 * ks + 8 * g;
-            v4f x0 = {0.0f, 0.0f, 0.0f, 0.0f}, x1 = x0;
-            if (f < a.d) { x0 = *(const v4f *)(qp + f); x1 = *(const v4f *)(qp + f + 4); }
+        for (int n = 0; n < QN; n++) {
+            const int f = 32 * (wave + NW * n) + 8 * g;
+            v4f y0 = {0.0f, 0.0f, 0.0f, 0.0f}, y1 = y0;
+            if (f < a.d) { y0 = *(const v4f *)(qp + f) * sc; y1 = *(const v4f *)(qp + f + 4) * sc; }
 #pragma unroll
-            for (int i = 0; i < 4; i++) { x[ks][i] = x0[i] * qs; x[ks][4 + i] = x1[i] * qs; }
-#pragma unroll
-            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[ks][i]));
+            for (int i = 0; i < 4; i++) { y[x][n][i] = y0[i]; y[x][n][4 + i] = y1[i]; amax = fmaxf(amax, fmaxf(fabsf(y0[i]), fabsf(y1[i]))); }
         }
         if (!F::bf) {
             amax = max_groups(amax);
-            const int e = amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
-            qe = ldexpf(1.0f, e);
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[ks][i] = ldexpf(x[ks][i], -e);
+            if (g == 0) wm[wave][16 * x + lr] = amax;
         }
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) split8<F::bf, P>(x[ks], qf[ks]);
     }
-    const float slope = m_slope(a, h) * LOG2E;
-
-    float m = -INFINITY, l = 0.0f;              // of this lane's row; l over this lane's slots only
-    int E = -64;                                // blocks: o holds 2^(14 - E) times its value, E the exponent of the largest scale of V met so far
-    v4f o[HASV ? FT : 1];
+    if (!F::bf) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < (HASV ? FT : 1); i++) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float * lg = a.logits + (((int64_t)i3 * a.n_head_kv + hk) * R + r) * a.lpitch;
-    const bool mine = r0 + lr < R;
-
-    while (t < t1) {
-        float mv[2][4];
+    for (int x = 0; x < RT; x++) {
+        int e = 0;
+        if (!F::bf) {
+            float amax = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            mv[u][0] = h2f((uint16_t)mk[u].x); mv[u][1] = h2f((uint16_t)(mk[u].x >> 16)); mv[u][2] = h2f((uint16_t)mk[u].y); mv[u][3] = h2f((uint16_t)(mk[u].y >> 16));
+            for (int w = 0; w < NW; w++) amax = fmaxf(amax, wm[w][16 * x + lr]);
+            e = amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
         }
-        int tn = t + NW;                        // the next tile that a row sees
-        while (tn < t1 && !sees(mkn)) {
-            if (mine) {
+        qe[x] = ldexpf(1.0f, e);
 #pragma unroll
-                for (int u = 0; u < 2; u++) if (32 * tn + 16 * u + 4 * g < a.lpitch) *(v4f *)(lg + 32 * tn + 16 * u + 4 * g) = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            }
-            tn += NW;
-            if (tn < t1) load_mask(tn, mkn);
+        for (int n = 0; n < QN; n++) {
+            if (wave + NW * n >= KS) continue;
+            v4i w[P];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[x][n][i] = ldexpf(y[x][n][i], -e);
+            split8<F::bf, P>(y[x][n], w);
+#pragma unroll
+            for (int p = 0; p < P; p++) qs[x][wave + NW * n][p][lane] = w[p];
         }
-        const bool next = tn < t1;
+    }
+    __syncthreads();
+
+    float m[RT], l[RT];                         // of this lane's rows; l over this lane's slots only
+    int E[RT];                                  // blocks: o holds 2^(14 - E) times its value, E the exponent of the largest scale of V met so far
+    v4f o[RT][HASV ? FT : 1];
+    float * lg[RT];
 #pragma unroll
-        for (int u = 0; u < 2; u++) mk[u] = mkn[u];
-        if constexpr (F::quant) {               // scales of the 32 slots where every lane can read them
-            if (g < KS) {
+    for (int x = 0; x < RT; x++) {
+        m[x] = -INFINITY; l[x] = 0.0f; E[x] = -64;
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+        for (int i = 0; i < (HASV ? FT : 1); i++) o[x][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        lg[x] = a.logits + (((int64_t)i3 * a.n_head_kv + hk) * R + r[x]) * a.lpitch;
+    }
+    auto mine = [&](int x) { return lr < RP && rb + 16 * x + lr < R; };      // the lane that stores row r[x]
+
+    while (t < ntiles) {
+        u2 mc[RT][2];
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) if (ks % 4 == g) ((uint16_t *)&kd[wave][16 * u + lr])[ks] = kc[u][ks].scale();
-            }
-            if constexpr (HASV) {
-                if ((lane & 3) == 0) {
+        for (int x = 0; x < RT; x++) { mc[x][0] = mk[x][0]; mc[x][1] = mk[x][1]; }
+        int tn = t + TW;                        // the next tile that a row sees
+        while (tn < ntiles && !sees(mkn)) {
 #pragma unroll
-                    for (int i = 0; i < VN; i++) ((uint16_t *)&vd[wave][VR * i + lane / (D / 8)])[lane % (D / 8) / 4] = vc[i].scale();
+            for (int x = 0; x < RT; x++)
+                if (mine(x)) {
+#pragma unroll
+                    for (int u = 0; u < 2; u++) if (32 * tn + 16 * u + 4 * g < a.lpitch) *(v4f *)(lg[x] + 32 * tn + 16 * u + 4 * g) = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 }
+            tn += TW;
+            if (tn < ntiles) load_mask(tn, mkn);
+        }
+        const bool next = tn < ntiles;
+#pragma unroll
+        for (int x = 0; x < RT; x++) { mk[x][0] = mkn[x][0]; mk[x][1] = mkn[x][1]; }
+        if constexpr (F::quant) {               // scales of the 32 slots where every lane can read them
+#pragma unroll
+            for (int i = 0; i < DN; i++) {
+                kd[wave][64 * i + lane] = ksc[i];
+                if constexpr (HASV) vd[wave][64 * i + lane] = vsc[i];
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         // ---- S^T
-        float s[2][4];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
-            hk_t dk[4];
+        v4f c[RT][2];
+        {
+            hk_t dk[2][4];
             if constexpr (F::quant) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) dk[i] = kd[wave][16 * u + 4 * g + i];
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                v4f b = F::quant ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : c;
-                const v4i kop = kc[u][ks].operand(g);
-#pragma unroll
-                for (int p = P - 1; p >= 0; p--) b = mfma16<F::bf>(kop, qf[ks][p], b);
-                if constexpr (F::quant) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) c[i] = __builtin_fmaf(b[i], (float)dk[i][ks], c[i]);
-                } else c = b;
-            }
-            if (capped) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) c[i] = a.logit_softcap * LOG2E * tanhf(c[i] * qe);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) c[i] *= qe;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[u][i] = mv[u][i] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[u][i], slope, c[i]);
-        }
-        if (next) load_k(tn);                   // in flight during the rest of this tile
-        if (tn + NW < t1) load_mask(tn + NW, mkn);
-        float mx = m;
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int j = 32 * t + 16 * u + 4 * g;
-            if (mine && j < a.lpitch) *(v4f *)(lg + j) = v4f{s[u][0], s[u][1], s[u][2], s[u][3]};
-#pragma unroll
-            for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[u][i]);
-        }
-        mx = max_groups(mx);
-        const float ms = mx == -INFINITY ? 0.0f : mx;
-        float corr = __builtin_amdgcn_exp2f(m - ms);            // m = -inf: 0
-        float p[8];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) p[4 * u + i] = __builtin_amdgcn_exp2f(s[u][i] - ms);
-        l *= corr;
-#pragma unroll
-        for (int i = 0; i < 8; i++) l += p[i];
-        m = mx;
-        if constexpr (HASV) {
-            bool some = false;
-#pragma unroll
-            for (int i = 0; i < 8; i++) some |= s[i >> 2][i & 3] == -INFINITY;
-            const bool hidden = __any(some);                    // some row does not see some slot of the tile
-            hk_t dd[8];
-            if constexpr (F::quant) {
-                // the scales of V go on P.  A hidden slot's is taken as 0 (it may be NaN)
-                _Float16 dm = 0;
-#pragma unroll
-                for (int i = 0; i < 8; i++) dd[i] = vd[wave][(i & 4) * 4 + 4 * g + (i & 3)];
-                if (hidden) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) if (s[i >> 2][i & 3] == -INFINITY) dd[i] = (hk_t)(_Float16)0;
-                }
-                hk_t mxd = __builtin_elementwise_abs(dd[0]);
-#pragma unroll
-                for (int i = 1; i < 8; i++) mxd = __builtin_elementwise_max(mxd, __builtin_elementwise_abs(dd[i]));
-#pragma unroll
-                for (int k = 0; k < KS; k++) dm = dm > mxd[k] ? dm : mxd[k];
-                const float dmx = max_groups((float)dm);
-                const int e = dmx > 0.0f && dmx < INFINITY ? __builtin_amdgcn_frexp_expf(dmx) - 1 : -64;
-                const int En = E > e ? E : e;
-                corr = ldexpf(corr, E - En);
-                E = En;
-            }
-            if (__any(corr != 1.0f)) {
-#pragma unroll
-                for (int i = 0; i < FT; i++) o[i] = o[i] * corr;
-            }
-            // ---- V tile into LDS.  A slot that some row does not see must not reach that row through 0 * NaN: its non-finite values are
-            // taken out here and added below to the rows that do see it
-            uint64_t bad = 0;                                   // slots of the tile with values taken out
-            if constexpr (!F::quant) if (hidden) {
-                uint32_t unseen = 0;                            // bit j: slot 32 t + j is hidden from some row
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint64_t b = __ballot(s[u][i] == -INFINITY);
+                    for (int i = 0; i < 4; i++) dk[u][i] = *(const hk_t *)&kd[wave][(16 * u + 4 * g + i) * KS];
+            }
 #pragma unroll
-                        for (int gg = 0; gg < 4; gg++) if ((b >> (16 * gg)) & 0xffff) unseen |= 1u << (16 * u + 4 * gg + i);
+            for (int x = 0; x < RT; x++) c[x][0] = c[x][1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                v4i qv[RT][P];
+#pragma unroll
+                for (int x = 0; x < RT; x++)
+#pragma unroll
+                    for (int p = 0; p < P; p++) qv[x][p] = qs[x][ks][p][lane];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const v4i kop = kc[u][ks].operand(g);
+#pragma unroll
+                    for (int x = 0; x < RT; x++) {
+                        v4f b = F::quant ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : c[x][u];
+#pragma unroll
+                        for (int p = P - 1; p >= 0; p--) b = mfma16<F::bf>(kop, qv[x][p], b);
+                        if constexpr (F::quant) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) c[x][u][i] = __builtin_fmaf(b[i], (float)dk[u][i][ks], c[x][u][i]);
+                        } else c[x][u] = b;
+                    }
+                }
+            }
+        }
+        if (next) load_k(tn);                   // in flight during the rest of this tile
+        if (tn + TW < ntiles) load_mask(tn + TW, mkn);
+        float s[RT][8], p[RT][8], corr[RT];     // slots 32 t + 16 (i >> 2) + 4 g + (i & 3)
+        bool some = false;                      // some row does not see some slot of the tile
+#pragma unroll
+        for (int x = 0; x < RT; x++) {
+            float mx = m[x];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float mv = h2f((uint16_t)(mc[x][i >> 2][(i & 3) >> 1] >> (16 * (i & 1))));
+                float y = c[x][i >> 2][i & 3] * qe[x];
+                if (capped) y = a.logit_softcap * LOG2E * tanhf(y);
+                s[x][i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope[x], y);
+                mx = fmaxf(mx, s[x][i]);
+                some |= s[x][i] == -INFINITY;
+            }
+            if (mine(x)) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int j = 32 * t + 16 * u + 4 * g;
+                    if (j < a.lpitch) *(v4f *)(lg[x] + j) = v4f{s[x][4 * u], s[x][4 * u + 1], s[x][4 * u + 2], s[x][4 * u + 3]};
+                }
+            }
+            mx = max_groups(mx);
+            const float ms = mx == -INFINITY ? 0.0f : mx;
+            corr[x] = __builtin_amdgcn_exp2f(m[x] - ms);        // m = -inf: 0
+            l[x] *= corr[x];
+#pragma unroll
+            for (int i = 0; i < 8; i++) { p[x][i] = __builtin_amdgcn_exp2f(s[x][i] - ms); l[x] += p[x][i]; }
+            m[x] = mx;
+        }
+        if constexpr (HASV) {
+            const bool hidden = __any(some);
+            _Float16 dd[RT][SETS][8];
+            if constexpr (F::quant) {
+                // the scales of V go on P, those of this lane's class of blocks.  A hidden slot's is taken as 0 (it may be NaN)
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    _Float16 dm = 0;
+#pragma unroll
+                    for (int q = 0; q < SETS; q++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const int b = q * NC + lr / RP;
+                            dd[x][q][i] = __builtin_bit_cast(_Float16, vd[wave][(16 * (i >> 2) + 4 * g + (i & 3)) * KS + (b < KS ? b : 0)]);
+                        }
+                    if (hidden) {
+#pragma unroll
+                        for (int q = 0; q < SETS; q++)
+#pragma unroll
+                            for (int i = 0; i < 8; i++) if (s[x][i] == -INFINITY) dd[x][q][i] = 0;
+                    }
+#pragma unroll
+                    for (int q = 0; q < SETS; q++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) dm = __builtin_elementwise_max(dm, __builtin_elementwise_abs(dd[x][q][i]));
+                    const float dmx = max_groups((float)dm);
+                    const int e = dmx > 0.0f && dmx < INFINITY ? __builtin_amdgcn_frexp_expf(dmx) - 1 : -64;
+                    const int En = E[x] > e ? E[x] : e;
+                    corr[x] = ldexpf(corr[x], E[x] - En);
+                    E[x] = En;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < RT; x++)
+                if (__any(corr[x] != 1.0f)) {
+#pragma unroll
+                    for (int i = 0; i < FT; i++) o[x][i] = o[x][i] * corr[x];
+                }
+            // ---- V tile into LDS.  A slot that some row does not see must not reach that row through 0 * NaN: its non-finite values are
+            // taken out here and added below to the rows that do see it
+            uint32_t bad = 0;                                   // slots of the tile with values taken out
+            if constexpr (!F::quant) if (hidden) {
+                uint32_t unseen = 0;                            // bit j: slot 32 t + j is hidden from some row
+#pragma unroll
+                for (int x = 0; x < RT; x++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const uint64_t b = __ballot(s[x][i] == -INFINITY);
+#pragma unroll
+                        for (int gg = 0; gg < 4; gg++) if ((b >> (16 * gg)) & 0xffff) unseen |= 1u << (16 * (i >> 2) + 4 * gg + (i & 3));
                     }
 #pragma unroll
                 for (int i = 0; i < VN; i++) {
@@ -428,7 +480,7 @@ mass_step_kernel(const MArgs a) {
                     const uint64_t b = __ballot(taken);
                     if (b) {
 #pragma unroll
-                        for (int q = 0; q < VR; q++) if (b >> (q * (D / 8)) & ((1ull << (D / 8)) - 1)) bad |= 1ull << (i * VR + q);
+                        for (int q = 0; q < VR; q++) if (b >> (q * (D / 8)) & ((1ull << (D / 8)) - 1)) bad |= 1u << (i * VR + q);
                     }
                 }
             }
@@ -438,21 +490,27 @@ mass_step_kernel(const MArgs a) {
             if (next) load_v(tn);
             // ---- O^T
             const uint8_t * vt = lds[wave] + (4 * g + (lr >> 2)) * VP + 8 * (lr & 3);
-            if constexpr (!F::bf) {                             // f16 parts: clear of the subnormal range
-                const float c = F::quant ? ldexpf(1.0f, 14 - E) : 16384.0f;
+            v4i pf[RT][P];
 #pragma unroll
-                for (int i = 0; i < 8; i++) p[i] *= c;
+            for (int x = 0; x < RT; x++) {
+                if constexpr (!F::bf) {                         // f16 parts: clear of the subnormal range
+                    const float up = F::quant ? ldexpf(1.0f, 14 - E[x]) : 16384.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) p[x][i] *= up;
+                }
+                if constexpr (!F::quant) split8<F::bf, P>(p[x], pf[x]);
             }
-            v4i pf[P];
-            if constexpr (!F::quant) split8<F::bf, P>(p, pf);
 #pragma unroll
             for (int f = 0; f < FT; f++) {
                 if constexpr (F::quant) {
-                    if (f % 2 == 0) {                           // a new 32-block
-                        float x[8];
+                    if (f % (FT / SETS) == 0) {                 // the next scaled copy
 #pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = p[i] * (float)dd[i][f / 2];
-                        split8<false, 2>(x, pf);
+                        for (int x = 0; x < RT; x++) {
+                            float y[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) y[i] = p[x][i] * (float)dd[x][f / (FT / SETS)][i];
+                            split8<false, 2>(y, pf[x]);
+                        }
                     }
                 }
                 const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(vt + 32 * f));
@@ -461,72 +519,80 @@ mass_step_kernel(const MArgs a) {
                 __builtin_memcpy(&vop, &lo, 8);
                 __builtin_memcpy((char *)&vop + 8, &hi, 8);
 #pragma unroll
-                for (int q = P - 1; q >= 0; q--) o[f] = mfma16<F::bf>(vop, pf[q], o[f]);
+                for (int x = 0; x < RT; x++)
+#pragma unroll
+                    for (int q = P - 1; q >= 0; q--) o[x][f] = mfma16<F::bf>(vop, pf[x][q], o[x][f]);
             }
             if (!F::quant && bad) {                             // non-finite values of slots that only some rows see
                 for (int row = 0; row < 32; row++) {
                     if (!(bad >> row & 1)) continue;
-                    const int from = ((row & 15) >> 2) * 16 + lr, i = (row >> 4) * 4 + (row & 3);
-                    float pr = 0.0f, sr = -INFINITY;
-#pragma unroll
-                    for (int q = 0; q < 8; q++) {
-                        const float a0 = __shfl(p[q], from, 64), a1 = __shfl(s[q >> 2][q & 3], from, 64);
-                        if (q == i) { pr = a0; sr = a1; }
-                    }
-                    const int j = 32 * t + row;
+                    const int from = ((row & 15) >> 2) * 16 + lr, i = (row >> 4) * 4 + (row & 3), j = 32 * t + row;
                     if (j >= a.n_kv) continue;
-                    const char * vr = vb + (int64_t)j * a.v_nb1;
+                    const char * vr = vb + (uint64_t)(uint32_t)j * a.v_nb1;
 #pragma unroll
-                    for (int f = 0; f < FT; f++)
+                    for (int x = 0; x < RT; x++) {
+                        float pr = 0.0f, sr = -INFINITY;
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const int e = 16 * f + 4 * g + q;
-                            if (e >= a.dv) continue;
-                            const float x = kv_value<TYPE>(vr, e);
-                            if (sr != -INFINITY && !(fabsf(x) < INFINITY)) o[f][q] += pr * x;
+                        for (int q = 0; q < 8; q++) {
+                            const float a0 = __shfl(p[x][q], from, 64), a1 = __shfl(s[x][q], from, 64);
+                            if (q == i) { pr = a0; sr = a1; }
                         }
+#pragma unroll
+                        for (int f = 0; f < FT; f++)
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const int e = 16 * f + 4 * g + q;
+                                if (e >= a.dv) continue;
+                                const float y = kv_value<TYPE>(vr, e);
+                                if (sr != -INFINITY && !(fabsf(y) < INFINITY)) o[x][f][q] += pr * y;
+                            }
+                    }
                 }
             }
         }
         t = tn;
     }
     // ---- the waves' states meet in LDS
-    l = sum_groups(l);
-    if (g == 0) { wm[wave][lr] = m; wl[wave][lr] = l; }
-    if constexpr (HASV) {
-        float * ob = (float *)lds[wave] + lr * OP + 4 * g;
 #pragma unroll
-        for (int f = 0; f < FT; f++) *(v4f *)(ob + 16 * f) = o[f] * (F::bf ? 1.0f : F::quant ? ldexpf(1.0f, E - 14) : 1.0f / 16384.0f);
+    for (int x = 0; x < RT; x++) {
+        l[x] = sum_groups(l[x]);
+        if (g == 0 && lr < RP) { wm[wave][16 * x + lr] = m[x]; wl[wave][16 * x + lr] = l[x]; }
     }
-    __syncthreads();
-    const int rows = R - r0 < 16 ? R - r0 : 16;
-    const int64_t slot = (((int64_t)i3 * a.n_head_kv + hk) * a.nsplit + split) * R + r0;
-    if (HASV) {
-        for (int idx = tid; idx < rows * (D / 4); idx += NW * 64) {
-            const int rr = idx / (D / 4), f4 = idx % (D / 4);
-            if (4 * f4 >= a.dv) continue;
+    const int64_t base = (((int64_t)i3 * a.n_head_kv + hk) * a.nsplit + split) * R + rb;
+#pragma unroll
+    for (int x = 0; x < RT; x++) {
+        const int rows = R - rb - 16 * x < RP ? R - rb - 16 * x : RP;
+        if constexpr (HASV) {
+            if (x > 0) __syncthreads();                         // the tile before this one has been read
+            float * ob = (float *)lds[wave] + lr % RP * OP + 4 * g;
+            const float back = F::bf ? 1.0f : F::quant ? ldexpf(1.0f, E[x] - 14) : 1.0f / 16384.0f;
+#pragma unroll
+            for (int f = 0; f < FT; f++) if (NC == 1 || f / 2 % NC == lr / RP) *(v4f *)(ob + 16 * f) = o[x][f] * back;
+        }
+        __syncthreads();
+        if constexpr (HASV) {
+            for (int idx = tid; idx < rows * (D / 4); idx += NW * 64) {
+                const int rr = idx / (D / 4), f4 = idx % (D / 4);
+                if (4 * f4 >= a.dv) continue;
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][16 * x + rr]);
+                const float ms = M == -INFINITY ? 0.0f : M;
+                v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < NW; w++) O = O + *(const v4f *)((const float *)lds[w] + rr * OP + 4 * f4) * __builtin_amdgcn_exp2f(wm[w][16 * x + rr] - ms);
+                *(v4f *)(a.part + (base + 16 * x + rr) * D + 4 * f4) = O;
+            }
+        }
+        if (tid < rows) {
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][rr]);
+            for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][16 * x + tid]);
             const float ms = M == -INFINITY ? 0.0f : M;
-            v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float c = __builtin_amdgcn_exp2f(wm[w][rr] - ms);
-                L = __builtin_fmaf(wl[w][rr], c, L);
-                O = O + *(const v4f *)((const float *)lds[w] + rr * OP + 4 * f4) * c;
-            }
-            *(v4f *)(a.part + (slot + rr) * D + 4 * f4) = O;
+            for (int w = 0; w < NW; w++) L = __builtin_fmaf(wl[w][16 * x + tid], __builtin_amdgcn_exp2f(wm[w][16 * x + tid] - ms), L);
+            *(v2f *)(a.stats + (base + 16 * x + tid) * 2) = v2f{M, L};
         }
-    }
-    if (tid < rows) {
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][tid]);
-        const float ms = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-        for (int w = 0; w < NW; w++) L = __builtin_fmaf(wl[w][tid], __builtin_amdgcn_exp2f(wm[w][tid] - ms), L);
-        a.stats[(slot + tid) * 2] = M; a.stats[(slot + tid) * 2 + 1] = L;
     }
 }
 
@@ -625,10 +691,10 @@ mass_finish_kernel(const MArgs a, int mass_wgs) {
 
 constexpr int STEP_WAVES = 4;
 
-template <int TYPE, int D, bool HASV> static int step_launch(const MArgs & a, int ne3, hipStream_t s) {
+template <int TYPE, int D, bool HASV, int RT, int RP> static int step_launch(const MArgs & a, int ne3, hipStream_t s) {
     const int R = a.n_head / a.n_head_kv * a.n_q;
-    MI355_LAUNCH("fattn_mass_step", (mass_step_kernel<TYPE, D, STEP_WAVES, HASV>), dim3((unsigned)a.nsplit, (unsigned)(a.n_head_kv * ((R + 15) / 16)), (unsigned)ne3),
-                 dim3(STEP_WAVES * 64), 0, s, a);
+    MI355_LAUNCH("fattn_mass_step", (mass_step_kernel<TYPE, D, STEP_WAVES, HASV, RT, RP>),
+                 dim3((unsigned)a.nsplit, (unsigned)(a.n_head_kv * ((R + 16 * RT - 1) / (16 * RT))), (unsigned)ne3), dim3(STEP_WAVES * 64), 0, s, a);
     MI355_CHECK_LAUNCH();
     const int mass_wgs = (a.n_kv + 255) / 256;
     if (mass_wgs + (HASV ? R : 0) == 0) return MI355_OK;
@@ -636,17 +702,32 @@ template <int TYPE, int D, bool HASV> static int step_launch(const MArgs & a, in
     MI355_CHECK_LAUNCH();
     return MI355_OK;
 }
-template <int TYPE, bool HASV> static int step_dispatch(const MArgs & a, int ne3, hipStream_t s) {
-    if (a.d <= 64) return step_launch<TYPE, 64, HASV>(a, ne3, s);
-    if (a.d <= 128) return step_launch<TYPE, 128, HASV>(a, ne3, s);
-    return step_launch<TYPE, 256, HASV>(a, ne3, s);
-}
-
+// 16-row tiles per workgroup: one row tile up to 16 rows, then two (a K or V row is then fetched and converted once for 32 rows); D = 256 has no
+// registers for a second one
+static int step_row_tiles(int64_t rows, int64_t d) { return rows > 16 && d <= 128 ? 2 : 1; }
 static int step_d(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-// slices of the KV range: two workgroups per CU in all, none with less than one 32-slot tile per wave
+template <int TYPE, int D, bool HASV> static int step_rows(const MArgs & a, int ne3, hipStream_t s) {
+    const int R = a.n_head / a.n_head_kv * a.n_q;
+    if constexpr (D <= 128) if (step_row_tiles(R, D) == 2) return step_launch<TYPE, D, HASV, 2, 16>(a, ne3, s);
+    if constexpr (Fmt<TYPE>::quant && HASV && D <= 128) {
+        if constexpr (D == 128) if (R <= 4) return step_launch<TYPE, D, HASV, 1, 4>(a, ne3, s);
+        if (R <= 8) return step_launch<TYPE, D, HASV, 1, 8>(a, ne3, s);
+    }
+    return step_launch<TYPE, D, HASV, 1, 16>(a, ne3, s);
+}
+template <int TYPE, bool HASV> static int step_dispatch(const MArgs & a, int ne3, hipStream_t s) {
+    switch (step_d(a.d)) {
+        case 64:  return step_rows<TYPE, 64, HASV>(a, ne3, s);
+        case 128: return step_rows<TYPE, 128, HASV>(a, ne3, s);
+    }
+    return step_rows<TYPE, 256, HASV>(a, ne3, s);
+}
+
+// slices of the KV range: two workgroups per CU in all (what the registers allow), none with less than one 32-slot tile per wave
 static int64_t step_splits(const mi355_fattn_args * p) {
-    const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (p->n_kv + 31) / 32, base = p->n_head_kv * ((R + 15) / 16) * p->ne3;
+    const int64_t R = p->n_head / p->n_head_kv * p->n_q, rows = 16 * step_row_tiles(R, p->d), tiles = (p->n_kv + 31) / 32;
+    const int64_t base = p->n_head_kv * ((R + rows - 1) / rows) * p->ne3;
     int64_t n = 512 / base, most = (tiles + STEP_WAVES - 1) / STEP_WAVES;
     if (n > most) n = most;
     if (n > 128) n = 128;

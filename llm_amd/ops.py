@@ -517,23 +517,28 @@ def set_rows(src, ids, dst, type_dst):
 
 
 _KV_DTYPE = {B.F32: torch.float32, B.F16: torch.float16, B.BF16: torch.bfloat16, B.Q8_0: torch.uint8, B.Q4_0: torch.uint8}
+_KV_BYTES = {B.F32: 4, B.F16: 2, B.BF16: 2, B.Q8_0: 1, B.Q4_0: 1}          # of a cache tensor's element
+_BLOCK = {B.Q8_0: 34, B.Q4_0: 18}
 
 
-def _kv_rows(t, type_kv, name):
-    """checks a cache tensor [seqs, kv heads, slots, row]: f32 / f16 / bf16 values, or uint8 bytes of q8_0 / q4_0 blocks"""
-    if type_kv not in _KV_DTYPE:
-        raise ValueError(f"{name}: caches are f32, f16, bf16, q8_0 or q4_0, not type {type_kv}")
-    if t.dim() != 4 or t.dtype != _KV_DTYPE[type_kv] or (t.shape[3] > 1 and t.stride(3) != 1):
-        raise ValueError(f"{name}: expected [seqs, kv heads, slots, row] of {_KV_DTYPE[type_kv]} with contiguous rows")
-    return t.shape[3] if t.dtype != torch.uint8 else t.shape[3] // B.TYPE_SIZE[type_kv] * 32
+# The entry points of the bounded KV cache are called once per layer and step: their wrappers read every tensor's shape and strides once.
+# A tensor has to lie on the current device, whose current stream the launch goes to.
 
-
-def _here(*ts):
-    """every tensor lies on the current device, whose current stream the launch goes to"""
-    dev = torch.cuda.current_device()
+def _on(dev, *ts):
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensor on {t.device}, the current device is cuda:{dev}")
+
+
+def _cache_rows(t, type_kv, name, S, hk, slots=None):
+    """(slots, values per row, strides) of a cache tensor [seqs, kv heads, slots, row]: f32 / f16 / bf16 values, or uint8 bytes of q8_0 / q4_0
+    blocks, contiguous rows"""
+    s0, s1, s2, s3 = t.shape
+    st = t.stride()
+    if t.dtype is not _KV_DTYPE.get(type_kv) or (s3 > 1 and st[3] != 1) or s0 != S or s1 != hk or (slots is not None and s2 != slots):
+        raise ValueError(f"{name}: expected [{S} seqs, {hk} kv heads, {'slots' if slots is None else slots}, row] of type {B.TYPE_NAMES.get(type_kv, type_kv)} "
+                         f"(f32, f16, bf16, or uint8 bytes of q8_0 / q4_0 blocks), rows contiguous; got {tuple(t.shape)} of {t.dtype}")
+    return s2, (s3 // _BLOCK[type_kv] * 32 if type_kv in _BLOCK else s3), st
 
 
 def qk_norm_rope(q, k, v, q_norm, k_norm, eps, pos, k_cache, v_cache, type_kv, rows=None, slot_pos=None, slot_mass=None, n_dims=None, mode=2,
@@ -543,54 +548,68 @@ def qk_norm_rope(q, k, v, q_norm, k_norm, eps, pos, k_cache, v_cache, type_kv, r
     k [seqs, tokens, kv heads, d], v [.., dv] (or None, with v_cache None) f32, strides free (contiguous rows); q_norm / k_norm f32 [d] or
     None; pos int32 [seqs, tokens]; caches [seqs, kv heads, slots, row] of type_kv; rows int32 [seqs, kv heads, tokens] (None: token i goes
     to slot i); slot_pos int32, slot_mass f32 [seqs, kv heads, slots] or None -> q rotated, f32 [seqs, heads, tokens, d] (q_out's strides)."""
-    _here(q, k, v, q_norm, k_norm, pos, k_cache, v_cache, rows, slot_pos, slot_mass, freq_factors, q_out)
+    f32, i32 = torch.float32, torch.int32
+    dev = torch.cuda.current_device()
+    _on(dev, q, k, v, q_norm, k_norm, pos, k_cache, v_cache, rows, slot_pos, slot_mass, freq_factors, q_out)
     S, n, H, d = q.shape
-    hk, dv = k.shape[2], 0
-    if q.dtype != torch.float32 or k.dtype != torch.float32 or tuple(k.shape) != (S, n, hk, d) or q.stride(3) != 1 or k.stride(3) != 1:
+    kS, kn, hk, kd = k.shape
+    qs, ks = q.stride(), k.stride()
+    if q.dtype is not f32 or k.dtype is not f32 or kS != S or kn != n or kd != d or qs[3] != 1 or ks[3] != 1:
         raise ValueError("q and k: f32 [seqs, tokens, heads, d] with contiguous rows")
     if (v is None) != (v_cache is None):
         raise ValueError("v and v_cache come together")
-    slots = k_cache.shape[2]
-    if _kv_rows(k_cache, type_kv, "k_cache") != d or tuple(k_cache.shape[:2]) != (S, hk):
-        raise ValueError("k_cache does not fit k")
+    slots, kd, kc = _cache_rows(k_cache, type_kv, "k_cache", S, hk)
+    if kd != d:
+        raise ValueError("k_cache: rows of another length than k's")
+    eb = _KV_BYTES[type_kv]
+    dv, vp, vs, vcp, vc = 0, None, (0, 0, 0, 0), None, (0, 0, 0, 0)
     if v is not None:
-        dv = v.shape[3]
-        if v.dtype != torch.float32 or tuple(v.shape[:3]) != (S, n, hk) or v.stride(3) != 1:
+        vS, vn, vh, dv = v.shape
+        vs = v.stride()
+        if v.dtype is not f32 or vS != S or vn != n or vh != hk or vs[3] != 1:
             raise ValueError("v: f32 [seqs, tokens, kv heads, dv] with contiguous rows")
-        if _kv_rows(v_cache, type_kv, "v_cache") != dv or tuple(v_cache.shape[:3]) != (S, hk, slots):
-            raise ValueError("v_cache does not fit v and k_cache")
-    if pos.dtype != torch.int32 or tuple(pos.shape) != (S, n) or (rows is not None and (rows.dtype != torch.int32 or tuple(rows.shape) != (S, hk, n))):
-        raise ValueError("pos: int32 [seqs, tokens], rows: int32 [seqs, kv heads, tokens]")
-    for t, dt in ((slot_pos, torch.int32), (slot_mass, torch.float32)):
-        if t is not None and (t.dtype != dt or tuple(t.shape) != (S, hk, slots) or (slots > 1 and t.stride(2) != 1)):
-            raise ValueError("slot_pos int32 / slot_mass f32: [seqs, kv heads, slots], slots contiguous")
+        _, vd, vc = _cache_rows(v_cache, type_kv, "v_cache", S, hk, slots)
+        if vd != dv:
+            raise ValueError("v_cache: rows of another length than v's")
+        vp, vcp = v.data_ptr(), v_cache.data_ptr()
+    ps = pos.stride()
+    if pos.dtype is not i32 or pos.shape != (S, n):
+        raise ValueError("pos: int32 [seqs, tokens]")
+    rp, rs = None, (0, 0, 0)
+    if rows is not None:
+        if rows.dtype is not i32 or rows.shape != (S, hk, n):
+            raise ValueError("rows: int32 [seqs, kv heads, tokens]")
+        rp, rs = rows.data_ptr(), rows.stride()
+    spp, sps, smp, sms = None, (0, 0, 0), None, (0, 0, 0)
+    if slot_pos is not None:
+        spp, sps = slot_pos.data_ptr(), slot_pos.stride()
+        if slot_pos.dtype is not i32 or slot_pos.shape != (S, hk, slots) or (slots > 1 and sps[2] != 1):
+            raise ValueError("slot_pos: int32 [seqs, kv heads, slots], slots contiguous")
+    if slot_mass is not None:
+        smp, sms = slot_mass.data_ptr(), slot_mass.stride()
+        if slot_mass.dtype is not f32 or slot_mass.shape != (S, hk, slots) or (slots > 1 and sms[2] != 1):
+            raise ValueError("slot_mass: f32 [seqs, kv heads, slots], slots contiguous")
     n_dims = d if n_dims is None else n_dims
     for t, m in ((q_norm, d), (k_norm, d), (freq_factors, n_dims // 2)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() < m or not t.is_contiguous()):
+        if t is not None and (t.dtype is not f32 or t.numel() < m or not t.is_contiguous()):
             raise ValueError("q_norm, k_norm: f32 [d]; freq_factors: f32 [n_dims / 2]")
     if q_out is None:
-        q_out = torch.empty((S, H, n, d), dtype=torch.float32, device=q.device)
-    elif q_out.dtype != torch.float32 or tuple(q_out.shape) != (S, H, n, d) or q_out.stride(3) != 1:
+        q_out = torch.empty((S, H, n, d), dtype=f32, device=q.device)
+    elif q_out.dtype is not f32 or q_out.shape != (S, H, n, d) or q_out.stride(3) != 1:
         raise ValueError("q_out: f32 [seqs, heads, tokens, d] with contiguous rows")
-    if q.numel() == 0:
+    if S == 0 or n == 0:
         return q_out
-    a, ptr = K.QkNormRopeArgs(), lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    st = lambda t, *i: [t.stride(j) * t.element_size() for j in i] if t is not None else [0] * len(i)  # noqa: E731
-    a.q, (a.q_nb1, a.q_nb2, a.q_nb3) = q.data_ptr(), st(q, 1, 2, 0)
-    a.k, (a.k_nb1, a.k_nb2, a.k_nb3) = k.data_ptr(), st(k, 1, 2, 0)
-    a.v, (a.v_nb1, a.v_nb2, a.v_nb3) = ptr(v), st(v, 1, 2, 0)
-    a.q_norm, a.k_norm, a.freq_factors = ptr(q_norm), ptr(k_norm), ptr(freq_factors)
-    a.q_out, (a.qo_nb1, a.qo_nb2, a.qo_nb3) = q_out.data_ptr(), st(q_out, 2, 1, 0)
-    a.k_out, (a.ko_nb1, a.ko_nb2, a.ko_nb3) = k_cache.data_ptr(), st(k_cache, 2, 1, 0)
-    a.v_out, (a.vo_nb1, a.vo_nb2, a.vo_nb3) = ptr(v_cache), st(v_cache, 2, 1, 0)
-    a.rows, (a.rows_nb1, a.rows_nb2, a.rows_nb3) = ptr(rows), st(rows, 2, 1, 0)
-    a.pos, (a.pos_nb1, a.pos_nb3) = pos.data_ptr(), st(pos, 1, 0)
-    a.slot_pos, (a.sp_nb2, a.sp_nb3) = ptr(slot_pos), st(slot_pos, 1, 0)
-    a.slot_mass, (a.sm_nb2, a.sm_nb3) = ptr(slot_mass), st(slot_mass, 1, 0)
-    a.head_dim, a.dv, a.n_head, a.n_head_kv, a.n, a.ne3, a.n_rows = d, dv, H, hk, n, S, slots
-    a.type_kv, a.n_dims, a.mode, a.n_ctx_orig, a.eps = type_kv, n_dims, mode, n_ctx_orig, eps
-    a.freq_base, a.freq_scale, a.ext_factor, a.attn_factor, a.beta_fast, a.beta_slow = freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow
-    K.check(K.lib.mi355_qk_norm_rope(a, _stream()), "mi355_qk_norm_rope")
+    os = q_out.stride()
+    a = K.QkNormRopeArgs(
+        q.data_ptr(), qs[1] * 4, qs[2] * 4, qs[0] * 4, k.data_ptr(), ks[1] * 4, ks[2] * 4, ks[0] * 4, vp, vs[1] * 4, vs[2] * 4, vs[0] * 4,
+        q_norm.data_ptr() if q_norm is not None else None, k_norm.data_ptr() if k_norm is not None else None,
+        q_out.data_ptr(), os[2] * 4, os[1] * 4, os[0] * 4, k_cache.data_ptr(), kc[2] * eb, kc[1] * eb, kc[0] * eb, vcp, vc[2] * eb, vc[1] * eb, vc[0] * eb,
+        rp, rs[2] * 4, rs[1] * 4, rs[0] * 4, pos.data_ptr(), ps[1] * 4, ps[0] * 4, freq_factors.data_ptr() if freq_factors is not None else None,
+        spp, sps[1] * 4, sps[0] * 4, smp, sms[1] * 4, sms[0] * 4, d, dv, H, hk, n, S, slots,
+        type_kv, n_dims, mode, n_ctx_orig, eps, freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow)
+    rc = K.lib.mi355_qk_norm_rope(a, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        raise K.Mi355Error(rc, "mi355_qk_norm_rope")
     return q_out
 
 
@@ -599,110 +618,117 @@ def kv_evict(mass, slot_pos, n_past, n_keep, n_sink=0, n_recent=0, n_used=None, 
     -> (kept int32 [seqs, kv heads, n_keep], evicted int32 [.., n_evict]); n_evict None: slots - n_keep.  With caches k, v [seqs, kv heads,
     slots, row] of type_kv their kept rows are gathered too, into k_out, v_out [seqs, kv heads, n_keep, row] (None: new)
     -> (kept, evicted, mass of the kept, positions of the kept), or (.., k_out, v_out) where those were None."""
-    _here(mass, slot_pos, n_past, n_used, k, v, k_out, v_out)
+    i32 = torch.int32
+    dev = torch.cuda.current_device()
+    _on(dev, mass, slot_pos, n_past, n_used, k, v, k_out, v_out)
     S, hk, slots = mass.shape
-    if mass.dtype != torch.float32 or slot_pos.dtype != torch.int32 or slot_pos.shape != mass.shape or (slots > 1 and (mass.stride(2) != 1 or slot_pos.stride(2) != 1)):
+    ms, ps = mass.stride(), slot_pos.stride()
+    if mass.dtype is not torch.float32 or slot_pos.dtype is not i32 or slot_pos.shape != (S, hk, slots) or (slots > 1 and (ms[2] != 1 or ps[2] != 1)):
         raise ValueError("mass f32, slot_pos int32: [seqs, kv heads, slots], slots contiguous")
     for t in (n_past, n_used):
-        if t is not None and (t.dtype != torch.int32 or t.numel() != S or not t.is_contiguous()):
+        if t is not None and (t.dtype is not i32 or t.shape != (S,) or (S > 1 and t.stride(0) != 1)):
             raise ValueError("n_past, n_used: int32 [seqs]")
     if (k is None) != (v is None) or (k_out is None) != (v_out is None) or (k is None and k_out is not None):
         raise ValueError("k and v, and k_out and v_out, come together")
     n_evict = max(0, slots - n_keep) if n_evict is None else n_evict
-    a, new = K.KvEvictArgs(), k is not None and k_out is None
-    lists = torch.empty((S, hk, max(n_keep, 0) + max(n_evict, 0)), dtype=torch.int32, device=mass.device)
-    kept, evicted = lists[..., :n_keep], lists[..., n_keep:]
-    st = lambda t, *i: [t.stride(j) * t.element_size() for j in i]  # noqa: E731
-    a.mass, (a.mass_nb2, a.mass_nb3) = mass.data_ptr(), st(mass, 1, 0)
-    a.slot_pos, (a.pos_nb2, a.pos_nb3) = slot_pos.data_ptr(), st(slot_pos, 1, 0)
-    a.n_used, a.n_past = n_used.data_ptr() if n_used is not None else None, n_past.data_ptr()
-    a.kept, (a.kept_nb2, a.kept_nb3) = kept.data_ptr(), st(kept, 1, 0)
-    a.evicted, (a.ev_nb2, a.ev_nb3) = evicted.data_ptr() if n_evict > 0 else None, st(evicted, 1, 0)
-    a.n_kv, a.n_keep, a.n_evict, a.n_head_kv, a.ne3 = slots, n_keep, n_evict, hk, S
-    a.type_kv, a.n_sink, a.n_recent = type_kv, n_sink, n_recent
+    keep, ev = max(n_keep, 0), max(n_evict, 0)
+    kept = torch.empty((S, hk, keep), dtype=i32, device=mass.device)
+    evicted = torch.empty((S, hk, ev), dtype=i32, device=mass.device)
+    rows, tables, ret = (None, 0, 0, 0) * 4, (None, 0, 0) * 2, (kept, evicted)
+    dk = dv = 0
     if k is not None:
-        dk, dv = _kv_rows(k, type_kv, "k"), _kv_rows(v, type_kv, "v")
-        if tuple(k.shape[:3]) != (S, hk, slots) or tuple(v.shape[:3]) != (S, hk, slots) or (d is not None and d != dk):
-            raise ValueError("k, v: [seqs, kv heads, slots, row] beside mass")
+        _, dk, ks = _cache_rows(k, type_kv, "k", S, hk, slots)
+        _, dv, vs = _cache_rows(v, type_kv, "v", S, hk, slots)
+        if d is not None and d != dk:
+            raise ValueError(f"k: rows of {dk} values, not {d}")
+        new = k_out is None
         if new:
-            k_out, v_out = (torch.zeros((S, hk, n_keep, t.shape[3]), dtype=t.dtype, device=t.device) for t in (k, v))
-        for t, o in ((k, k_out), (v, v_out)):
-            if o.dtype != t.dtype or tuple(o.shape) != (S, hk, n_keep, t.shape[3]) or (o.shape[3] > 1 and o.stride(3) != 1):
-                raise ValueError("k_out, v_out: [seqs, kv heads, n_keep, row] of the caches' type")
-        mass_out = torch.empty((S, hk, n_keep), dtype=torch.float32, device=mass.device)
-        pos_out = torch.empty((S, hk, n_keep), dtype=torch.int32, device=mass.device)
-        a.k, (a.k_nb1, a.k_nb2, a.k_nb3) = k.data_ptr(), st(k, 2, 1, 0)
-        a.v, (a.v_nb1, a.v_nb2, a.v_nb3) = v.data_ptr(), st(v, 2, 1, 0)
-        a.k_out, (a.ko_nb1, a.ko_nb2, a.ko_nb3) = k_out.data_ptr(), st(k_out, 2, 1, 0)
-        a.v_out, (a.vo_nb1, a.vo_nb2, a.vo_nb3) = v_out.data_ptr(), st(v_out, 2, 1, 0)
-        a.mass_out, (a.mo_nb2, a.mo_nb3) = mass_out.data_ptr(), st(mass_out, 1, 0)
-        a.pos_out, (a.po_nb2, a.po_nb3) = pos_out.data_ptr(), st(pos_out, 1, 0)
-        a.d, a.dv = dk, dv
-    K.check(K.lib.mi355_kv_evict(a, _stream()), "mi355_kv_evict")
-    if k is None:
-        return kept, evicted
-    return (kept, evicted, mass_out, pos_out) + ((k_out, v_out) if new else ())
+            k_out, v_out = (torch.zeros((S, hk, keep, t.shape[3]), dtype=t.dtype, device=t.device) for t in (k, v))
+        _, ko, kos = _cache_rows(k_out, type_kv, "k_out", S, hk, n_keep)
+        _, vo, vos = _cache_rows(v_out, type_kv, "v_out", S, hk, n_keep)
+        if ko != dk or vo != dv:
+            raise ValueError("k_out, v_out: rows of another length than k's, v's")
+        b = _KV_BYTES[type_kv]
+        mass_out = torch.empty((S, hk, keep), dtype=torch.float32, device=mass.device)
+        pos_out = torch.empty((S, hk, keep), dtype=i32, device=mass.device)
+        rows = (k.data_ptr(), ks[2] * b, ks[1] * b, ks[0] * b, v.data_ptr(), vs[2] * b, vs[1] * b, vs[0] * b,
+                k_out.data_ptr(), kos[2] * b, kos[1] * b, kos[0] * b, v_out.data_ptr(), vos[2] * b, vos[1] * b, vos[0] * b)
+        tables = (mass_out.data_ptr(), keep * 4, hk * keep * 4, pos_out.data_ptr(), keep * 4, hk * keep * 4)
+        ret = (kept, evicted, mass_out, pos_out, k_out, v_out) if new else (kept, evicted, mass_out, pos_out)
+    a = K.KvEvictArgs(mass.data_ptr(), ms[1] * 4, ms[0] * 4, slot_pos.data_ptr(), ps[1] * 4, ps[0] * 4,
+                      n_used.data_ptr() if n_used is not None else None, n_past.data_ptr(), kept.data_ptr(), keep * 4, hk * keep * 4,
+                      evicted.data_ptr() if ev else None, ev * 4, hk * ev * 4, *rows, *tables, slots, n_keep, n_evict, hk, S, dk, dv, type_kv, n_sink, n_recent)
+    rc = K.lib.mi355_kv_evict(a, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        raise K.Mi355Error(rc, "mi355_kv_evict")
+    return ret
 
 
-def _mass_args(q, k, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap):
-    """checks and arguments that flash_attn_ext_mass and attn_mass share -> (FattnArgs without V and dst, AttnMassArgs, mass_out)"""
-    _here(q, k, mask, mass, mass_out)
+def _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap):
+    """checks and arguments that flash_attn_ext_mass and attn_mass (v None) share -> (FattnArgs, AttnMassArgs, dst | None, mass_out)"""
+    f32 = torch.float32
+    _on(dev, q, k, v, mask, mass, mass_out)
     S, H, n, d = q.shape
-    if q.dtype != torch.float32 or q.stride(3) != 1:
+    qs = q.stride()
+    if q.dtype is not f32 or qs[3] != 1:
         raise ValueError("q: f32 [seqs, heads, tokens, d] with contiguous rows")
-    if _kv_rows(k, type_kv, "k") != d or k.shape[0] != S:
-        raise ValueError("k: [seqs, kv heads, slots, row] with rows of d values")
-    hk, slots = k.shape[1], k.shape[2]
-    a, w = K.FattnArgs(), K.AttnMassArgs()
-    a.q, a.q_nb1, a.q_nb2, a.q_nb3 = q.data_ptr(), q.stride(2) * 4, q.stride(1) * 4, q.stride(0) * 4
-    es = k.element_size()
-    a.k, a.type_k, a.k_nb1, a.k_nb2, a.k_nb3 = k.data_ptr(), type_kv, k.stride(2) * es, k.stride(1) * es, k.stride(0) * es
+    hk = k.shape[1]
+    slots, kd, ks = _cache_rows(k, type_kv, "k", S, hk)
+    if kd != d:
+        raise ValueError("k: rows of another length than q's")
+    b = _KV_BYTES[type_kv]
+    mp, m1, m2, m3, e2, e3 = None, 0, 0, 0, 0, 0
     if mask is not None:
-        if mask.dim() == 2:
-            mask = mask[None, None]
-        elif mask.dim() == 3:
-            mask = mask[:, None]
-        if mask.element_size() != 2 or mask.dim() != 4 or mask.shape[2] < n or mask.shape[3] != slots or (slots > 1 and mask.stride(3) != 1):
+        sh, st = mask.shape, mask.stride()
+        if len(sh) < 4:                       # the two first dimensions may be left out, or the heads'
+            sh, st = ((1, 1) + sh, (0, 0) + st) if len(sh) == 2 else ((sh[0], 1) + sh[1:], (st[0], 0) + st[1:])
+        e3, e2, m_n, m_s = sh
+        if mask.element_size() != 2 or m_n < n or m_s != slots or (slots > 1 and st[3] != 1):
             raise ValueError("mask: f16 (or its bits) [seqs | 1, heads | 1, >= tokens, slots], the two first may be left out")
-        a.mask, a.m_nb1, a.m_nb2, a.m_nb3 = mask.data_ptr(), mask.stride(2) * 2, mask.stride(1) * 2, mask.stride(0) * 2
-        a.m_ne2, a.m_ne3 = mask.shape[1], mask.shape[0]
-    a.d, a.n_q, a.n_kv, a.n_head, a.n_head_kv, a.ne3 = d, n, slots, H, hk, S
-    a.scale, a.max_bias, a.logit_softcap = scale, max_bias, logit_softcap
+        mp, m1, m2, m3 = mask.data_ptr(), st[2] * 2, st[1] * 2, st[0] * 2
+    dst, vp, v1, v2, v3, dp, dv = None, None, 0, 0, 0, None, 0
+    if v is not None:
+        _, dv, vs = _cache_rows(v, type_kv, "v", S, hk, slots)
+        dst = torch.empty((S, n, H, dv), dtype=f32, device=q.device)
+        vp, v1, v2, v3, dp = v.data_ptr(), vs[2] * b, vs[1] * b, vs[0] * b, dst.data_ptr()
     if mass_out is None:
-        mass_out = torch.empty((S, hk, slots), dtype=torch.float32, device=q.device)
-    for t in (mass, mass_out):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (S, hk, slots) or (slots > 1 and t.stride(2) != 1)):
-            raise ValueError("mass, mass_out: f32 [seqs, kv heads, slots], slots contiguous")
+        mass_out = torch.empty((S, hk, slots), dtype=f32, device=q.device)
+        os = (hk * slots, slots, 1)
+    else:
+        os = mass_out.stride()
+        if mass_out.dtype is not f32 or mass_out.shape != (S, hk, slots) or (slots > 1 and os[2] != 1):
+            raise ValueError("mass_out: f32 [seqs, kv heads, slots], slots contiguous")
+    ip, ns = None, (0, 0, 0)
     if mass is not None:
-        w.mass_in, w.in_nb2, w.in_nb3 = mass.data_ptr(), mass.stride(1) * 4, mass.stride(0) * 4
-    w.mass_out, w.out_nb2, w.out_nb3, w.decay = mass_out.data_ptr(), mass_out.stride(1) * 4, mass_out.stride(0) * 4, decay
-    return a, w, mass_out
+        ip, ns = mass.data_ptr(), mass.stride()
+        if mass.dtype is not f32 or mass.shape != (S, hk, slots) or (slots > 1 and ns[2] != 1):
+            raise ValueError("mass: f32 [seqs, kv heads, slots], slots contiguous")
+    a = K.FattnArgs(q.data_ptr(), qs[2] * 4, qs[1] * 4, qs[0] * 4, k.data_ptr(), type_kv, ks[2] * b, ks[1] * b, ks[0] * b, vp, type_kv, v1, v2, v3,
+                    mp, m1, m2, m3, e2, e3, dp, dv * 4, H * dv * 4, n * H * dv * 4, d, n, slots, H, hk, S, scale, max_bias, logit_softcap, dv)
+    return a, K.AttnMassArgs(ip, ns[1] * 4, ns[0] * 4, mass_out.data_ptr(), os[1] * 4, os[0] * 4, decay), dst, mass_out
 
 
 def flash_attn_ext_mass(q, k, v, mask, type_kv, scale, mass=None, decay=1.0, mass_out=None, max_bias=0.0, logit_softcap=0.0):
     """A decode step's attention and the weight every slot draws (mi355_flash_attn_ext_mass).  q f32 [seqs, heads, tokens <= 8, d], k, v
     [seqs, kv heads, slots, row] of type_kv, mask f16 [seqs | 1, heads | 1, >= tokens, slots] (or [seqs | 1, tokens, slots], [tokens, slots],
     None); mass f32 [seqs, kv heads, slots] or None; mass_out may be mass -> (f32 [seqs, tokens, heads, dv], mass_out = decay mass + weights)."""
-    a, w, mass_out = _mass_args(q, k, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
-    _here(v)
-    dv = _kv_rows(v, type_kv, "v")
-    if tuple(v.shape[:3]) != tuple(k.shape[:3]):
-        raise ValueError("v: [seqs, kv heads, slots, row] beside k")
-    S, H, n, _ = q.shape
-    dst = torch.empty((S, n, H, dv), dtype=torch.float32, device=q.device)
-    es = v.element_size()
-    a.v, a.type_v, a.v_nb1, a.v_nb2, a.v_nb3 = v.data_ptr(), type_kv, v.stride(2) * es, v.stride(1) * es, v.stride(0) * es
-    a.dst, a.d_nb1, a.d_nb2, a.d_nb3, a.dv = dst.data_ptr(), dv * 4, H * dv * 4, n * H * dv * 4, dv
+    dev = torch.cuda.current_device()
+    a, w, dst, mass_out = _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
     need = K.lib.mi355_flash_attn_ext_mass_workspace_bytes(a)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-    K.check(K.lib.mi355_flash_attn_ext_mass(a, w, ws.data_ptr(), need, _stream()), "mi355_flash_attn_ext_mass")
+    rc = K.lib.mi355_flash_attn_ext_mass(a, w, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        raise K.Mi355Error(rc, "mi355_flash_attn_ext_mass")
     return dst, mass_out
 
 
 def attn_mass(q, k, mask, type_kv, scale, mass=None, decay=1.0, mass_out=None, max_bias=0.0, logit_softcap=0.0):
     """The weight every slot draws from any number of queries (mi355_attn_mass); arguments as flash_attn_ext_mass, without V -> mass_out."""
-    a, w, mass_out = _mass_args(q, k, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
+    dev = torch.cuda.current_device()
+    a, w, _, mass_out = _mass_args(dev, q, k, None, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
     need = K.lib.mi355_attn_mass_workspace_bytes(a)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-    K.check(K.lib.mi355_attn_mass(a, w, ws.data_ptr(), need, _stream()), "mi355_attn_mass")
+    rc = K.lib.mi355_attn_mass(a, w, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        raise K.Mi355Error(rc, "mi355_attn_mass")
     return mass_out
