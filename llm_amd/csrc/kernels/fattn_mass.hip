@@ -13,13 +13,14 @@ struct MArgs {
     const char * q; int64_t q_nb1, q_nb2, q_nb3;
     const char * k; uint32_t k_nb1; int64_t k_nb2, k_nb3;        // (rows at most 2 GiB apart: a row's address is one 32 x 32 + 64 bit multiply-add)
     const char * v; uint32_t v_nb1; int64_t v_nb2, v_nb3;
-    const char * mask; int64_t m_nb1, m_nb2, m_nb3, m_ne2, m_ne3;
+    const char * mask; int64_t m_nb1, m_nb2, m_nb3; int m_ne2, m_ne3;
     char * dst; int64_t d_nb1, d_nb2, d_nb3;
     const char * mass_in; int64_t in_nb2, in_nb3;
     char * mass_out; int64_t out_nb2, out_nb3;
     int n_q, n_kv, n_head, n_head_kv, d, dv;
     float scale, max_bias, logit_softcap, m0, m1, decay;
     uint32_t n_head_log2;
+    int ratio; uint32_t by_ratio;   // heads per KV head; ceil(2^32 / ratio), 0 for ratio 1 (r / ratio without a division)
     int nsplit, lpitch;
     float * logits;     // steps: [ne3][n_head_kv][rows][lpitch], log2 domain
     float * stats;      // steps: [ne3][n_head_kv][nsplit][rows][2]: maximum (log2 domain) and sum; prompts: [ne3][n_head][n_q][2]: m, 1 / l
@@ -37,6 +38,11 @@ template <int TYPE> static __device__ __forceinline__ float kv_value(const char 
     return h2f(*(const uint16_t *)b) * (float)(n - 8);
 }
 
+// row r of a KV head = (query, head of the group); r < 2^16
+static __device__ __forceinline__ int m_query(const MArgs & a, int r) { return a.by_ratio ? (int)__umulhi((uint32_t)r, a.by_ratio) : r; }
+static __device__ __forceinline__ const char * m_mask(const MArgs & a, int iq, int h, int i3) {
+    return a.mask + iq * a.m_nb1 + (a.m_ne2 > 1 ? h % a.m_ne2 : 0) * a.m_nb2 + (a.m_ne3 > 1 ? i3 % a.m_ne3 : 0) * a.m_nb3;
+}
 static __device__ __forceinline__ float m_slope(const MArgs & a, uint32_t h) {
     if (!(a.max_bias > 0.0f)) return 1.0f;
     return h < a.n_head_log2 ? powf(a.m0, h + 1) : powf(a.m1, 2 * (h - a.n_head_log2) + 1);
@@ -141,6 +147,17 @@ template <> struct Chunk<MI355_TYPE_Q4_0> {
         return bytes_f16((w0 >> sh) & 0x0f0f0f0fu, (w1 >> sh) & 0x0f0f0f0fu, 8.0f);
     }
 };
+// the same 8 bytes out of raw rows in LDS, whose words are what it reads: a block's integers start 2 bytes past a word in even blocks, on a
+// word in odd ones (34 and 18 are 2 mod 4)
+template <int TYPE> static __device__ __forceinline__ Chunk<TYPE> raw_chunk(const uint8_t * row, int j) {
+    const bool odd = j >> 2 & 1;
+    const uint32_t * q = (const uint32_t *)(row + Chunk<TYPE>::at(j) - (odd ? 4 : 2));
+    const uint32_t x0 = q[0], x1 = q[1], x2 = q[2], pick = odd ? 0x07060504u : 0x05040302u;
+    Chunk<TYPE> c;
+    c.w0 = __builtin_amdgcn_perm(x1, x0, pick);
+    c.w1 = __builtin_amdgcn_perm(x2, x1, pick);
+    return c;
+}
 // non-finite 16-bit values of a chunk -> 0; true if there was one
 template <bool BF> static __device__ __forceinline__ bool sanitize(v4i & x) {
     bool bad = false;
@@ -167,26 +184,33 @@ static __device__ __forceinline__ float sum_groups(float v) {
 // RT: 16-row tiles of a workgroup.  RP (blocks only): the 16 columns of a tile are RP rows times 16 / RP classes of 32-blocks -- at GQA 4 or 8
 // the columns that would repeat a row each scale P by the blocks of their class, so a lane forms D / 32 / (16 / RP) scaled copies of P and not
 // D / 32; a feature tile takes its result from the columns of its block's class.
-template <int TYPE, int D, int NW, bool HASV, int RT, int RP>
+// RAW (blocks only, step_raw): rows come in as consecutive pieces of D / 16 bytes (17 or 9 a row) and are taken apart in LDS.  A lane that loads
+// the 8 bytes of its own chunk reads at every second byte address, which the address unit serves a lane per clock: the 20 loads of a
+// tile then cost a CU's 8 waves 4 us before the first product.
+template <int TYPE, int D, int NW, bool HASV, int RT, int RP, bool RAW>
 __global__ void __launch_bounds__(NW * 64, D <= 64 ? (RT == 1 ? 3 : 2) : D <= 128 ? 2 : 1)
 mass_step_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
+    static_assert(!RAW || F::quant, "raw rows are block rows");
     constexpr int KS = D / 32, FT = D / 16, P = F::parts;
     constexpr int NC = 16 / RP, SETS = KS > NC ? KS / NC : 1;   // classes of blocks, scaled copies of P per lane
     constexpr int VR = 512 / D, VN = D / 16;                    // V rows per 64 chunks, groups of 64 chunks of a tile
     constexpr int VP = D * 2 + 32;                              // V tile row pitch (bytes)
     constexpr int OP = D + 4;                                   // merge row pitch (floats)
-    constexpr int VB = HASV ? (32 * VP > 16 * OP * 4 ? 32 * VP : 16 * OP * 4) : 16;
+    constexpr int VB = HASV ? (32 * VP > 16 * OP * 4 ? 32 * VP : 16 * OP * 4) : F::quant ? 32 * VP : 16;
     constexpr int DN = KS / 2;                                  // scales of a tile per lane: 32 rows x KS blocks over 64 lanes
+    constexpr int PB = D / 16, PR = F::block / 2, PN = (32 * PR + 63) / 64;    // RAW: bytes of a piece, pieces of a row, pieces of a tile per lane
+    typedef uint32_t piece_t __attribute__((ext_vector_type(PB / 4)));
     typedef _Float16 hk_t __attribute__((ext_vector_type(KS)));
     __shared__ __attribute__((aligned(16))) uint8_t lds[NW][VB];
     __shared__ v4i qs[RT][KS][P][64];
+    __shared__ __attribute__((aligned(16))) uint8_t raw[RAW ? NW : 1][RAW ? 32 * PR * PB + 16 : 16];
     __shared__ __attribute__((aligned(16))) uint16_t kd[F::quant ? NW : 1][F::quant ? 32 * KS : 8], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 * KS : 8];
     __shared__ float wm[NW][16 * RT], wl[NW][16 * RT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, g = lane >> 4;
-    const int ratio = a.n_head / a.n_head_kv, R = ratio * a.n_q;
-    const int hk = blockIdx.y % a.n_head_kv, rb = blockIdx.y / a.n_head_kv * 16 * RT, i3 = blockIdx.z, split = blockIdx.x;
+    const int ratio = a.ratio, R = ratio * a.n_q;
+    const int hk = blockIdx.y, rb = blockIdx.x / a.nsplit * 16 * RT, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;
     const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
     const char * vb = HASV ? a.v + hk * a.v_nb2 + i3 * a.v_nb3 : nullptr;
     const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
@@ -198,21 +222,52 @@ mass_step_kernel(const MArgs a) {
     for (int x = 0; x < RT; x++) {
         r[x] = rb + 16 * x + lr % RP;
         if (r[x] >= R) r[x] = R - 1;
-        const int iq = r[x] / ratio, h = hk * ratio + r[x] % ratio;
-        mrow[x] = a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3;
+        const int iq = m_query(a, r[x]), h = hk * ratio + r[x] - iq * ratio;
+        mrow[x] = m_mask(a, iq, h, i3);
     }
 
     // chunks past the head size re-read the last one: they meet zeros of q, and features of V that are not stored.  Slots past the end re-read
     // the last one and are hidden
     const int ntiles = (a.n_kv + 31) / 32, TW = a.nsplit * NW;
-    Chunk<TYPE> kc[2][KS], vc[HASV ? VN : 1];
-    uint16_t ksc[F::quant ? DN : 1], vsc[F::quant && HASV ? DN : 1];
+    Chunk<TYPE> kc[F::quant ? 1 : 2][RAW ? 1 : F::quant ? VN : KS], vc[HASV && !RAW ? VN : 1];
+    uint16_t ksc[F::quant && !RAW ? DN : 1], vsc[F::quant && !RAW && HASV ? DN : 1];
+    piece_t kp[RAW ? PN : 1], vp[RAW && HASV ? PN : 1];
+    uint32_t koff[RAW ? PN : 1], voff[RAW && HASV ? PN : 1];   // of this lane's pieces from a tile's first row
     const int vcc = lane % (D / 8) < a.dv / 8 ? lane % (D / 8) : a.dv / 8 - 1;
     const char * vl = vb + Chunk<TYPE>::at(vcc);
-    int kcc[KS];
+    const int kcc = lane % (D / 8) < a.d / 8 ? lane % (D / 8) : a.d / 8 - 1;
+    const char * kl = kb + Chunk<TYPE>::at(kcc);
+    if constexpr (RAW) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++)
-        kcc[ks] = F::quant ? Chunk<TYPE>::at(4 * (ks < a.d / 32 ? ks : a.d / 32 - 1) + g) : Chunk<TYPE>::at(4 * ks + g < a.d / 8 ? 4 * ks + g : a.d / 8 - 1);
+        for (int i = 0; i < PN; i++) {
+            const uint32_t n = 64 * i + lane < 32 * PR ? 64 * i + lane : 32 * PR - 1, row = n / PR;
+            koff[i] = row * a.k_nb1 + (n - row * PR) * PB;
+            if constexpr (HASV) voff[i] = row * a.v_nb1 + (n - row * PR) * PB;
+        }
+    }
+    auto load_raw = [&](const char * base, uint32_t nb1, const uint32_t * off, int t, piece_t * out) {
+        const char * tile = base + (uint64_t)(32u * (uint32_t)t) * nb1;
+        if (32 * t + 32 <= a.n_kv) {
+#pragma unroll
+            for (int i = 0; i < PN; i++) out[i] = *(const piece_t *)(tile + off[i]);
+        } else {
+            const uint32_t last = a.n_kv - 1 - 32 * t;
+#pragma unroll
+            for (int i = 0; i < PN; i++) {
+                const uint32_t n = 64 * i + lane < 32 * PR ? 64 * i + lane : 32 * PR - 1, row = n / PR;
+                out[i] = *(const piece_t *)(tile + (row < last ? row : last) * nb1 + (n - row * PR) * PB);
+            }
+        }
+    };
+    auto put_raw = [&](const piece_t * in) {
+#pragma unroll
+        for (int i = 0; i < PN; i++) if (64 * i + 64 <= 32 * PR || 64 * i + lane < 32 * PR) *(piece_t *)(raw[wave] + (64 * i + lane) * PB) = in[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    auto raw_scales = [&](uint16_t * out) {
+#pragma unroll
+        for (int i = 0; i < DN; i++) { const int n = 64 * i + lane; out[n] = *(const uint16_t *)(raw[wave] + n / KS * PR * PB + n % KS * F::block); }
+    };
     auto slot = [&](int j) { return (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1); };
     auto load_scales = [&](const char * base, uint32_t nb1, int dim, int t, uint16_t * out) {
 #pragma unroll
@@ -222,16 +277,23 @@ mass_step_kernel(const MArgs a) {
         }
     };
     auto load_k = [&](int t) {
+        if constexpr (RAW) load_raw(kb, a.k_nb1, koff, t, kp);
+        else if constexpr (F::quant) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const char * row = kb + slot(32 * t + 16 * u + lr) * a.k_nb1;
+            for (int i = 0; i < VN; i++) kc[0][i].load(kl + slot(32 * t + VR * i + lane / (D / 8)) * a.k_nb1);
+            load_scales(kb, a.k_nb1, a.d, t, ksc);
+        } else {
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) kc[u][ks].load(row + kcc[ks]);
+            for (int u = 0; u < 2; u++) {
+                const char * row = kb + slot(32 * t + 16 * u + lr) * a.k_nb1;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) kc[u][ks].load(row + Chunk<TYPE>::at(4 * ks + g < a.d / 8 ? 4 * ks + g : a.d / 8 - 1));
+            }
         }
-        if constexpr (F::quant) load_scales(kb, a.k_nb1, a.d, t, ksc);
     };
     auto load_v = [&](int t) {
-        if constexpr (HASV) {
+        if constexpr (HASV && RAW) load_raw(vb, a.v_nb1, voff, t, vp);
+        else if constexpr (HASV) {
 #pragma unroll
             for (int i = 0; i < VN; i++) vc[i].load(vl + slot(32 * t + VR * i + lane / (D / 8)) * a.v_nb1);
             if constexpr (F::quant) load_scales(vb, a.v_nb1, a.dv, t, vsc);
@@ -274,7 +336,7 @@ mass_step_kernel(const MArgs a) {
     float qe[RT], slope[RT], y[RT][QN][8];
 #pragma unroll
     for (int x = 0; x < RT; x++) {
-        const int iq = r[x] / ratio, h = hk * ratio + r[x] % ratio;
+        const int iq = m_query(a, r[x]), h = hk * ratio + r[x] - iq * ratio;
         slope[x] = m_slope(a, h) * LOG2E;
         const float * qp = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
         const float sc = capped ? a.scale / a.logit_softcap : a.scale * LOG2E;
@@ -347,7 +409,10 @@ mass_step_kernel(const MArgs a) {
         const bool next = tn < ntiles;
 #pragma unroll
         for (int x = 0; x < RT; x++) { mk[x][0] = mkn[x][0]; mk[x][1] = mkn[x][1]; }
-        if constexpr (F::quant) {               // scales of the 32 slots where every lane can read them
+        if constexpr (RAW) { put_raw(kp); raw_scales(kd[wave]); __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+        else if constexpr (F::quant) {          // K's integers to rows, the scales of the 32 slots where every lane can read them
+#pragma unroll
+            for (int i = 0; i < VN; i++) *(v4i *)(lds[wave] + (VR * i + lane / (D / 8)) * VP + lane % (D / 8) * 16) = kc[0][i].operand(kcc);
 #pragma unroll
             for (int i = 0; i < DN; i++) {
                 kd[wave][64 * i + lane] = ksc[i];
@@ -376,7 +441,10 @@ mass_step_kernel(const MArgs a) {
                     for (int p = 0; p < P; p++) qv[x][p] = qs[x][ks][p][lane];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const v4i kop = kc[u][ks].operand(g);
+                    v4i kop;
+                    if constexpr (RAW) kop = raw_chunk<TYPE>(raw[wave] + (16 * u + lr) * PR * PB, 4 * ks + g).operand(g);
+                    else if constexpr (F::quant) kop = *(const v4i *)(lds[wave] + (16 * u + lr) * VP + (4 * ks + g) * 16);
+                    else kop = kc[u][ks].operand(g);
 #pragma unroll
                     for (int x = 0; x < RT; x++) {
                         v4f b = F::quant ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : c[x][u];
@@ -424,6 +492,7 @@ mass_step_kernel(const MArgs a) {
         if constexpr (HASV) {
             const bool hidden = __any(some);
             _Float16 dd[RT][SETS][8];
+            if constexpr (RAW) { put_raw(vp); raw_scales(vd[wave]); __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
             if constexpr (F::quant) {
                 // the scales of V go on P, those of this lane's class of blocks.  A hidden slot's is taken as 0 (it may be NaN)
 #pragma unroll
@@ -485,7 +554,12 @@ mass_step_kernel(const MArgs a) {
                 }
             }
 #pragma unroll
-            for (int i = 0; i < VN; i++) *(v4i *)(lds[wave] + (VR * i + lane / (D / 8)) * VP + lane % (D / 8) * 16) = vc[i].operand(vcc);
+            for (int i = 0; i < VN; i++) {
+                v4i x;
+                if constexpr (RAW) x = raw_chunk<TYPE>(raw[wave] + (VR * i + lane / (D / 8)) * PR * PB, vcc).operand(vcc);
+                else x = vc[i].operand(vcc);
+                *(v4i *)(lds[wave] + (VR * i + lane / (D / 8)) * VP + lane % (D / 8) * 16) = x;
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (next) load_v(tn);
             // ---- O^T
@@ -604,7 +678,7 @@ __global__ void __launch_bounds__(256)
 mass_finish_kernel(const MArgs a, int mass_wgs) {
     __shared__ float sm[256], sl[256];
     const int tid = threadIdx.x, hk = blockIdx.y, i3 = blockIdx.z;
-    const int ratio = a.n_head / a.n_head_kv, R = ratio * a.n_q;
+    const int ratio = a.ratio, R = ratio * a.n_q;
     const int64_t base = ((int64_t)i3 * a.n_head_kv + hk) * a.nsplit * R;
     const v2f * st = (const v2f *)a.stats + base;
     if ((int)blockIdx.x < mass_wgs) {
@@ -658,7 +732,7 @@ mass_finish_kernel(const MArgs a, int mass_wgs) {
     // a row of dst: D / 4 threads per slice of the sum over the splits
     constexpr int F4 = D / 4, SG = 256 / F4;
     __shared__ v4f so[SG][F4];
-    const int r = blockIdx.x - mass_wgs, iq = r / ratio, h = hk * ratio + r % ratio;
+    const int r = blockIdx.x - mass_wgs, iq = m_query(a, r), h = hk * ratio + r - iq * ratio;
     const int f4 = tid % F4, sg = tid / F4;
     const bool in = 4 * f4 < a.dv;
     float M = -INFINITY;
@@ -691,10 +765,10 @@ mass_finish_kernel(const MArgs a, int mass_wgs) {
 
 constexpr int STEP_WAVES = 4;
 
-template <int TYPE, int D, bool HASV, int RT, int RP> static int step_launch(const MArgs & a, int ne3, hipStream_t s) {
-    const int R = a.n_head / a.n_head_kv * a.n_q;
-    MI355_LAUNCH("fattn_mass_step", (mass_step_kernel<TYPE, D, STEP_WAVES, HASV, RT, RP>),
-                 dim3((unsigned)a.nsplit, (unsigned)(a.n_head_kv * ((R + 16 * RT - 1) / (16 * RT))), (unsigned)ne3), dim3(STEP_WAVES * 64), 0, s, a);
+template <int TYPE, int D, bool HASV, int RP, bool RAW> static int step_launch(const MArgs & a, int ne3, hipStream_t s) {
+    const int R = a.ratio * a.n_q;
+    MI355_LAUNCH("fattn_mass_step", (mass_step_kernel<TYPE, D, STEP_WAVES, HASV, 1, RP, RAW>),
+                 dim3((unsigned)(a.nsplit * ((R + 15) / 16)), (unsigned)a.n_head_kv, (unsigned)ne3), dim3(STEP_WAVES * 64), 0, s, a);
     MI355_CHECK_LAUNCH();
     const int mass_wgs = (a.n_kv + 255) / 256;
     if (mass_wgs + (HASV ? R : 0) == 0) return MI355_OK;
@@ -702,32 +776,38 @@ template <int TYPE, int D, bool HASV, int RT, int RP> static int step_launch(con
     MI355_CHECK_LAUNCH();
     return MI355_OK;
 }
-// 16-row tiles per workgroup: one row tile up to 16 rows, then two (a K or V row is then fetched and converted once for 32 rows); D = 256 has no
-// registers for a second one
-static int step_row_tiles(int64_t rows, int64_t d) { return rows > 16 && d <= 128 ? 2 : 1; }
 static int step_d(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-template <int TYPE, int D, bool HASV> static int step_rows(const MArgs & a, int ne3, hipStream_t s) {
-    const int R = a.n_head / a.n_head_kv * a.n_q;
-    if constexpr (D <= 128) if (step_row_tiles(R, D) == 2) return step_launch<TYPE, D, HASV, 2, 16>(a, ne3, s);
+// rows of blocks that are whole pieces (see the kernel): full width, pieces aligned, a tile within 32-bit offsets
+template <bool HASV> static bool step_raw(const MArgs & a) {
+    const int D = step_d(a.d);
+    uint64_t low = (uint64_t)(uintptr_t)a.k | a.k_nb1 | (uint64_t)a.k_nb2 | (uint64_t)a.k_nb3;
+    if (HASV) low |= (uint64_t)(uintptr_t)a.v | a.v_nb1 | (uint64_t)a.v_nb2 | (uint64_t)a.v_nb3;
+    return a.d == D && (!HASV || a.dv == D) && (low & (uint64_t)(D / 16 - 1)) == 0 && a.k_nb1 < (1u << 26) && (!HASV || a.v_nb1 < (1u << 26));
+}
+template <int TYPE, int D, bool HASV, bool RAW> static int step_rows(const MArgs & a, int ne3, hipStream_t s) {
+    const int R = a.ratio * a.n_q;
     if constexpr (Fmt<TYPE>::quant && HASV && D <= 128) {
-        if constexpr (D == 128) if (R <= 4) return step_launch<TYPE, D, HASV, 1, 4>(a, ne3, s);
-        if (R <= 8) return step_launch<TYPE, D, HASV, 1, 8>(a, ne3, s);
+        if constexpr (D == 128) if (R <= 4) return step_launch<TYPE, D, HASV, 4, RAW>(a, ne3, s);
+        if (R <= 8) return step_launch<TYPE, D, HASV, 8, RAW>(a, ne3, s);
     }
-    return step_launch<TYPE, D, HASV, 1, 16>(a, ne3, s);
+    return step_launch<TYPE, D, HASV, 16, RAW>(a, ne3, s);
+}
+template <int TYPE, bool HASV, bool RAW> static int step_size(const MArgs & a, int ne3, hipStream_t s) {
+    switch (step_d(a.d)) {
+        case 64:  return step_rows<TYPE, 64, HASV, RAW>(a, ne3, s);
+        case 128: return step_rows<TYPE, 128, HASV, RAW>(a, ne3, s);
+    }
+    return step_rows<TYPE, 256, HASV, RAW>(a, ne3, s);
 }
 template <int TYPE, bool HASV> static int step_dispatch(const MArgs & a, int ne3, hipStream_t s) {
-    switch (step_d(a.d)) {
-        case 64:  return step_rows<TYPE, 64, HASV>(a, ne3, s);
-        case 128: return step_rows<TYPE, 128, HASV>(a, ne3, s);
-    }
-    return step_rows<TYPE, 256, HASV>(a, ne3, s);
+    if constexpr (Fmt<TYPE>::quant) if (step_raw<HASV>(a)) return step_size<TYPE, HASV, true>(a, ne3, s);
+    return step_size<TYPE, HASV, false>(a, ne3, s);
 }
 
 // slices of the KV range: two workgroups per CU in all (what the registers allow), none with less than one 32-slot tile per wave
 static int64_t step_splits(const mi355_fattn_args * p) {
-    const int64_t R = p->n_head / p->n_head_kv * p->n_q, rows = 16 * step_row_tiles(R, p->d), tiles = (p->n_kv + 31) / 32;
-    const int64_t base = p->n_head_kv * ((R + rows - 1) / rows) * p->ne3;
+    const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (p->n_kv + 31) / 32, base = p->n_head_kv * ((R + 15) / 16) * p->ne3;
     int64_t n = 512 / base, most = (tiles + STEP_WAVES - 1) / STEP_WAVES;
     if (n > most) n = most;
     if (n > 128) n = 128;
@@ -746,7 +826,7 @@ mass_rows_kernel(const MArgs a) {
     if (tid < a.d) q[tid] = qr[tid];
     __syncthreads();
     const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
-    const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
+    const char * mrow = a.mask ? m_mask(a, iq, h, i3) : nullptr;
     const float slope = m_slope(a, h);
     const int64_t row = ((int64_t)i3 * a.n_head + h) * a.n_q + iq;
     float m = -INFINITY, l = 0.0f;
@@ -783,7 +863,7 @@ mass_slots_kernel(const MArgs a) {
             __syncthreads();
             if (tid < a.d) q[tid] = ((const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3))[tid];
             __syncthreads();
-            const char * mrow = a.mask ? a.mask + iq * a.m_nb1 + (h % a.m_ne2) * a.m_nb2 + (i3 % a.m_ne3) * a.m_nb3 : nullptr;
+            const char * mrow = a.mask ? m_mask(a, iq, h, i3) : nullptr;
             if (j < a.n_kv) s = logit<TYPE>(a, q, krow, mrow, m_slope(a, h), j);
             if (s != -INFINITY) t += expf(s - a.stats[row * 2]) * a.stats[row * 2 + 1];
         }
@@ -831,9 +911,9 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     const bool quant = p->type_k == MI355_TYPE_Q8_0 || p->type_k == MI355_TYPE_Q4_0;
     if (quant && (p->d % 32 != 0 || (with_dst && dv % 32 != 0))) return MI355_E_SHAPE;
     if (p->n_head < 1 || p->n_head > 65535 || p->n_head_kv < 1 || p->n_head % p->n_head_kv != 0 || p->n_q < 1 || p->n_q > 65535 || p->n_kv < 0 ||
-        p->n_kv > (1 << 30) || p->n_head_kv * ((p->n_head / p->n_head_kv * MI355_MASS_MAX_Q + 15) / 16) > 65535 || p->ne3 < 1 || p->ne3 > 65535) return MI355_E_SHAPE;
+        p->n_kv > (1 << 30) || p->ne3 < 1 || p->ne3 > 65535) return MI355_E_SHAPE;
     if (with_dst && p->n_q > MI355_MASS_MAX_Q) return MI355_E_UNSUPPORTED;
-    if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1)) return MI355_E_SHAPE;
+    if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1 || p->m_ne2 > 0x7fffffff || p->m_ne3 > 0x7fffffff)) return MI355_E_SHAPE;
     if (p->k_nb1 < 0 || p->k_nb1 > 0x7fffffff || (with_dst && (p->v_nb1 < 0 || p->v_nb1 > 0x7fffffff))) return MI355_E_SHAPE;
     const int64_t f32s = (int64_t)(uintptr_t)p->q | p->q_nb1 | p->q_nb2 | p->q_nb3 |
                          (with_dst ? (int64_t)(uintptr_t)p->dst | p->d_nb1 | p->d_nb2 | p->d_nb3 : 0) | (int64_t)(uintptr_t)workspace;
@@ -849,7 +929,8 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     a.q = (const char *)p->q; a.q_nb1 = p->q_nb1; a.q_nb2 = p->q_nb2; a.q_nb3 = p->q_nb3;
     a.k = (const char *)p->k; a.k_nb1 = (uint32_t)p->k_nb1; a.k_nb2 = p->k_nb2; a.k_nb3 = p->k_nb3;
     a.v = (const char *)p->v; a.v_nb1 = (uint32_t)p->v_nb1; a.v_nb2 = p->v_nb2; a.v_nb3 = p->v_nb3;
-    a.mask = (const char *)p->mask; a.m_nb1 = p->m_nb1; a.m_nb2 = p->m_nb2; a.m_nb3 = p->m_nb3; a.m_ne2 = p->m_ne2; a.m_ne3 = p->m_ne3;
+    a.mask = (const char *)p->mask; a.m_nb1 = p->m_nb1; a.m_nb2 = p->m_nb2; a.m_nb3 = p->m_nb3; a.m_ne2 = (int)p->m_ne2; a.m_ne3 = (int)p->m_ne3;
+    a.ratio = (int)(p->n_head / p->n_head_kv); a.by_ratio = a.ratio > 1 ? (uint32_t)(((1ull << 32) + a.ratio - 1) / a.ratio) : 0;
     a.dst = with_dst ? (char *)p->dst : nullptr; a.d_nb1 = p->d_nb1; a.d_nb2 = p->d_nb2; a.d_nb3 = p->d_nb3;
     a.mass_in = w->decay != 0.0f ? (const char *)w->mass_in : nullptr; a.in_nb2 = w->in_nb2; a.in_nb3 = w->in_nb3;
     a.mass_out = (char *)w->mass_out; a.out_nb2 = w->out_nb2; a.out_nb3 = w->out_nb3;
