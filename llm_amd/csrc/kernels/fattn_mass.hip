@@ -204,7 +204,8 @@ mass_step_kernel(const MArgs a) {
     typedef _Float16 hk_t __attribute__((ext_vector_type(KS)));
     __shared__ __attribute__((aligned(16))) uint8_t lds[NW][VB];
     __shared__ v4i qs[RT][KS][P][64];
-    __shared__ __attribute__((aligned(16))) uint8_t raw[RAW ? NW : 1][RAW ? 32 * PR * PB + 16 : 16];
+    uint8_t (&raw)[NW][VB] = lds;                               // RAW: raw rows of K, then of V, then V's values, one after the other
+    static_assert(!RAW || VB >= 32 * PR * PB + 16, "raw rows fit");
     __shared__ __attribute__((aligned(16))) uint16_t kd[F::quant ? NW : 1][F::quant ? 32 * KS : 8], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 * KS : 8];
     __shared__ float wm[NW][16 * RT], wl[NW][16 * RT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -553,13 +554,15 @@ mass_step_kernel(const MArgs a) {
                     }
                 }
             }
+            v4i vt16[VN];
 #pragma unroll
             for (int i = 0; i < VN; i++) {
-                v4i x;
-                if constexpr (RAW) x = raw_chunk<TYPE>(raw[wave] + (VR * i + lane / (D / 8)) * PR * PB, vcc).operand(vcc);
-                else x = vc[i].operand(vcc);
-                *(v4i *)(lds[wave] + (VR * i + lane / (D / 8)) * VP + lane % (D / 8) * 16) = x;
+                if constexpr (RAW) vt16[i] = raw_chunk<TYPE>(raw[wave] + (VR * i + lane / (D / 8)) * PR * PB, vcc).operand(vcc);
+                else vt16[i] = vc[i].operand(vcc);
             }
+            if constexpr (RAW) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int i = 0; i < VN; i++) *(v4i *)(lds[wave] + (VR * i + lane / (D / 8)) * VP + lane % (D / 8) * 16) = vt16[i];
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (next) load_v(tn);
             // ---- O^T
