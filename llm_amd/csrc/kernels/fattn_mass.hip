@@ -9,6 +9,8 @@
 
 namespace {
 
+struct RowC { float qe, slope, m, inv; };      // per row: power of two of q, ALiBi slope (log2 domain), maximum, 1 / sum
+
 struct MArgs {
     const char * q; int64_t q_nb1, q_nb2, q_nb3;
     const char * k; uint32_t k_nb1; int64_t k_nb2, k_nb3;        // (rows at most 2 GiB apart: a row's address is one 32 x 32 + 64 bit multiply-add)
@@ -21,13 +23,13 @@ struct MArgs {
     float scale, max_bias, logit_softcap, m0, m1, decay;
     uint32_t n_head_log2;
     int ratio; uint32_t by_ratio;   // heads per KV head; ceil(2^32 / ratio), 0 for ratio 1 (r / ratio without a division)
-    int nsplit, lpitch;
+    int nsplit, nchunk, lpitch;
     float * logits;     // steps: [ne3][n_head_kv][rows][lpitch], log2 domain
-    float * stats;      // steps: [ne3][n_head_kv][nsplit][rows][2]: maximum (log2 domain) and sum; prompts: [ne3][n_head][n_q][2]: m, 1 / l
-    float * part;       // steps: [ne3][n_head_kv][nsplit][rows][D]
+    float * stats;      // [ne3][n_head_kv][nsplit][rows][2]: maximum (log2 domain) and sum of a slice
+    float * part;       // steps: [ne3][n_head_kv][nsplit][rows][D]; prompts: [ne3][n_head_kv][nchunk][n_kv]
+    RowC * rowc; // prompts: [ne3][n_head_kv][rows]
+    uint16_t * qparts;  // prompts: [ne3][n_head_kv][rows][2][D] f16
 };
-
-constexpr int MT = 256;
 
 template <int TYPE> static __device__ __forceinline__ float kv_value(const char * row, int e) {
     if (TYPE == MI355_TYPE_F16) return h2f(((const uint16_t *)row)[e]);
@@ -46,16 +48,6 @@ static __device__ __forceinline__ const char * m_mask(const MArgs & a, int iq, i
 static __device__ __forceinline__ float m_slope(const MArgs & a, uint32_t h) {
     if (!(a.max_bias > 0.0f)) return 1.0f;
     return h < a.n_head_log2 ? powf(a.m0, h + 1) : powf(a.m1, 2 * (h - a.n_head_log2) + 1);
-}
-
-// logit of slot j for a query row in LDS; -inf where the mask hides the slot
-template <int TYPE> static __device__ __forceinline__ float logit(const MArgs & a, const float * q, const char * krow, const char * mrow, float slope, int j) {
-    const float mv = mrow ? slope * h2f(((const uint16_t *)mrow)[j]) : 0.0f;
-    if (mv == -INFINITY) return -INFINITY;
-    float t = 0.0f;
-    for (int e = 0; e < a.d; e++) t = __builtin_fmaf(q[e], kv_value<TYPE>(krow, e), t);
-    t = a.logit_softcap != 0.0f ? a.logit_softcap * tanhf(t * (a.scale / a.logit_softcap)) : t * a.scale;
-    return t + mv;
 }
 
 // ---- decode steps (at most 8 queries): one pass over K and V on the matrix cores --------------------------------------------------------
@@ -817,79 +809,507 @@ static int64_t step_splits(const mi355_fattn_args * p) {
     return n < 1 ? 1 : n;
 }
 
-// ---- prompts ------------------------------------------------------------------------------------------------------------------------------
-// one workgroup per (query, head, sequence): statistics
-template <int TYPE>
-__global__ void __launch_bounds__(MT)
-mass_rows_kernel(const MArgs a) {
-    __shared__ float q[256], sh[MT / 64], shm[MT / 64];
-    const int tid = threadIdx.x, h = blockIdx.x, iq = blockIdx.y, i3 = blockIdx.z;
-    const int hk = h / (a.n_head / a.n_head_kv);
-    const float * qr = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
-    if (tid < a.d) q[tid] = qr[tid];
-    __syncthreads();
-    const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
-    const char * mrow = a.mask ? m_mask(a, iq, h, i3) : nullptr;
-    const float slope = m_slope(a, h);
-    const int64_t row = ((int64_t)i3 * a.n_head + h) * a.n_q + iq;
-    float m = -INFINITY, l = 0.0f;
-    for (int j = tid; j < a.n_kv; j += MT) {
-        const float s = logit<TYPE>(a, q, kb + (int64_t)j * a.k_nb1, mrow, slope, j);
-        if (s == -INFINITY) continue;
-        const float mn = fmaxf(m, s);
-        l = l * expf(m - mn) + expf(s - mn);
-        m = mn;
-    }
-    float M = m;
-    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    if ((tid & 63) == 0) shm[tid >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(shm[0], shm[1]), fmaxf(shm[2], shm[3]));
-    const float L = block_sum_n<MT / 64>(m == -INFINITY ? l : l * expf(m - M), sh);
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (tid == 0) { a.stats[row * 2] = M; a.stats[row * 2 + 1] = inv; }
+// ---- prompts: any number of queries, the weights alone ---------------------------------------------------------------------------------------
+//
+// Keeping the logits would move 8 bytes per (query, slot) pair; computing them twice costs 2 d products each on the matrix cores, which is less:
+//   prompt_q      q as two f16 parts (scale and log2(e) on it, rows brought to [2^14, 2^15) by a power of two), once
+//   prompt_stats  S^T = K Q^T, a running maximum and sum per row: a wave holds 32 rows of Q in registers, K passes through LDS
+//   prompt_mass   S^T again and sum over the rows of 2^(s - m) / l: a wave holds 32 or 64 slots of K, Q passes through LDS; the sums stay in
+//                 registers, one per (slot, lane), and meet across the lanes once at the end
+//   prompt_sum    the row chunks' sums and decay * mass_in, in a fixed order
+// v_mfma_f32_32x32x16_f16 throughout: K of f16 as it is; bf16 rows times a power of two that brings the row's largest value to [2^14, 2^15) (exact
+// down to 2^-29 of it, below that an error of 2^-40); blocks as d * q, likewise, in two parts.  Bound by the matrix cores and by v_exp_f32
+// (a quarter of the vector rate) in equal parts.  Tiles that the mask hides from a whole workgroup (half of a causal prompt) cost their mask.
+typedef float v16f __attribute__((ext_vector_type(16)));
+constexpr int PT = 256;                  // threads: 4 waves
+constexpr int PA_ROWS = 128, PA_SLOTS = 64, PB_ROWS = 32;
+
+static __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-// one thread per slot: its weight over the heads and queries of its KV head
-template <int TYPE>
-__global__ void __launch_bounds__(MT)
-mass_slots_kernel(const MArgs a) {
-    __shared__ float q[256];
-    const int tid = threadIdx.x, j = blockIdx.x * MT + tid, hk = blockIdx.y, i3 = blockIdx.z;
-    const int ratio = a.n_head / a.n_head_kv;
-    const char * krow = a.k + (int64_t)(j < a.n_kv ? j : 0) * a.k_nb1 + hk * a.k_nb2 + i3 * a.k_nb3;
-    float t = 0.0f;
-    for (int h = hk * ratio; h < hk * ratio + ratio; h++)
-        for (int iq = 0; iq < a.n_q; iq++) {
-            const int64_t row = ((int64_t)i3 * a.n_head + h) * a.n_q + iq;
-            float s = -INFINITY;
-            __syncthreads();
-            if (tid < a.d) q[tid] = ((const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3))[tid];
-            __syncthreads();
-            const char * mrow = a.mask ? m_mask(a, iq, h, i3) : nullptr;
-            if (j < a.n_kv) s = logit<TYPE>(a, q, krow, mrow, m_slope(a, h), j);
-            if (s != -INFINITY) t += expf(s - a.stats[row * 2]) * a.stats[row * 2 + 1];
+// q rows -> ws: [row][2][D] f16 (parts), RowC.  16 lanes a row
+template <int D>
+__global__ void __launch_bounds__(PT)
+prompt_q_kernel(const MArgs a) {
+    constexpr int NF = D / 128 > 0 ? D / 128 : 1;               // chunks of 8 features per lane
+    const int lane = threadIdx.x & 15, hk = blockIdx.y, i3 = blockIdx.z, R = a.ratio * a.n_q;
+    const int r = blockIdx.x * (PT / 16) + (threadIdx.x >> 4);
+    if (r >= R) return;
+    const int iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
+    const float * qp = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
+    const float sc = a.logit_softcap != 0.0f ? a.scale / a.logit_softcap : a.scale * LOG2E;
+    float y[NF][8], amax = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NF; n++) {
+        const int f = 8 * (lane + 16 * n);
+        v4f y0 = {0.0f, 0.0f, 0.0f, 0.0f}, y1 = y0;
+        if (f < a.d) { y0 = *(const v4f *)(qp + f) * sc; y1 = *(const v4f *)(qp + f + 4) * sc; }
+#pragma unroll
+        for (int i = 0; i < 4; i++) { y[n][i] = y0[i]; y[n][4 + i] = y1[i]; amax = fmaxf(amax, fmaxf(fabsf(y0[i]), fabsf(y1[i]))); }
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+    const int e = amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+    const int64_t row = ((int64_t)i3 * a.n_head_kv + hk) * R + r;
+#pragma unroll
+    for (int n = 0; n < NF; n++) {
+        if (lane + 16 * n >= D / 8) continue;
+        v4i w[2];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[n][i] = ldexpf(y[n][i], -e);
+        split8<false, 2>(y[n], w);
+        *(v4i *)(a.qparts + (row * 2) * D + 8 * (lane + 16 * n)) = w[0];
+        *(v4i *)(a.qparts + (row * 2 + 1) * D + 8 * (lane + 16 * n)) = w[1];
+    }
+    if (lane == 0) { a.rowc[row].qe = ldexpf(1.0f, e); a.rowc[row].slope = m_slope(a, h) * LOG2E; }
+}
+
+// a chunk of 8 features of K on its way to f16: what is loaded, and its values
+template <int TYPE> struct KChunk {
+    v4i raw;
+    __device__ __forceinline__ void load(const char * row, int c) { raw = *(const v4i *)(row + c * 16); }
+    __device__ __forceinline__ void values(int, float * v) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float((uint32_t)raw[i] << 16); v[2 * i + 1] = __uint_as_float((uint32_t)raw[i] & 0xffff0000u); }
+    }
+};
+template <int TYPE> struct KBlockChunk {
+    Chunk<TYPE> c; uint16_t d;
+    __device__ __forceinline__ void load(const char * row, int j) { c.load(row + Chunk<TYPE>::at(j)); d = *(const uint16_t *)(row + (j >> 2) * Fmt<TYPE>::block); }
+    __device__ __forceinline__ void values(int j, float * v) const {
+        const h8 q = __builtin_bit_cast(h8, c.operand(j));
+        const float dd = h2f(d);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)q[i] * dd;
+    }
+};
+template <> struct KChunk<MI355_TYPE_Q8_0> : KBlockChunk<MI355_TYPE_Q8_0> {};
+template <> struct KChunk<MI355_TYPE_Q4_0> : KBlockChunk<MI355_TYPE_Q4_0> {};
+template <int TYPE> struct KForm { static constexpr int parts = Fmt<TYPE>::quant ? 2 : 1; static constexpr bool scaled = TYPE != MI355_TYPE_F16; };
+
+static __device__ __forceinline__ float amax8(const float * v) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));      // (a NaN stays in the values)
+    return m;
+}
+static __device__ __forceinline__ int row_exp(float amax) { return amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0; }
+// 8 values times 2^-e -> one or two f16 parts
+template <int P> static __device__ __forceinline__ void to_parts(float * v, int e, v4i * out) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = ldexpf(v[i], -e);
+    if constexpr (P == 2) split8<false, 2>(v, out);
+    else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[0][i] = __builtin_bit_cast(int, h2{(_Float16)v[2 * i], (_Float16)v[2 * i + 1]});
+    }
+}
+
+// mask of a 32-slot tile for a row, as the accumulator lays it out: slot 8 q + 4 (lane / 32) + i
+static __device__ __forceinline__ void tile_mask(const MArgs & a, const char * mrow, bool m8, int j0, u2 (&w)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int j = j0 + 8 * q + 4 * ((threadIdx.x >> 5) & 1);
+        if (m8 && j + 4 <= a.n_kv) w[q] = *(const u2 *)(mrow + 2 * (int64_t)j);
+        else {
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = j + i >= a.n_kv ? 0xfc00u : a.mask ? ((const uint16_t *)mrow)[j + i] : 0u;
+            w[q] = u2{y[0] | y[1] << 16, y[2] | y[3] << 16};
         }
+    }
+}
+static __device__ __forceinline__ bool mask_sees(const u2 (&w)[4]) {
+    bool all = true;
+#pragma unroll
+    for (int q = 0; q < 4; q++) all &= w[q].x == 0xfc00fc00u && w[q].y == 0xfc00fc00u;
+    return !all;
+}
+static __device__ __forceinline__ bool mask_zero(const u2 (&w)[4]) {
+    uint32_t o = 0;
+#pragma unroll
+    for (int q = 0; q < 4; q++) o |= w[q].x | w[q].y;
+    return o == 0;
+}
+static __device__ __forceinline__ float mask_at(const u2 (&w)[4], int i) { return h2f((uint16_t)(w[i >> 2][(i & 3) >> 1] >> (16 * (i & 1)))); }
+
+// logits (log2 domain) of a 32 x 32 tile: c holds the products, ks the slots' scales (accumulator layout)
+template <bool SCALED> static __device__ __forceinline__ void tile_logits(const MArgs & a, const v16f & c, const float * ks, float qe, float slope, const u2 (&w)[4],
+                                                                          bool zero, float * s) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = SCALED ? c[i] * ks[i] * qe : c[i] * qe;
+    if (a.logit_softcap != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = a.logit_softcap * LOG2E * tanhf(s[i]);
+    }
+    if (!zero) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float mv = mask_at(w, i);
+            s[i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope, s[i]);
+        }
+    }
+}
+
+template <int TYPE, int D>
+__global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
+prompt_stats_kernel(const MArgs a) {
+    constexpr int KS = D / 16, KP = KForm<TYPE>::parts, RP = D * 2 + 16, CN = PA_SLOTS * (D / 8) / PT;
+    constexpr bool scaled = KForm<TYPE>::scaled;
+    __shared__ __attribute__((aligned(16))) uint8_t kt[2][KP][PA_SLOTS * RP];
+    __shared__ __attribute__((aligned(16))) float ksc[2][scaled ? PA_SLOTS : 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
+    const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;
+    const int rt = blockIdx.x / a.nsplit * PA_ROWS, r_ = rt + wave * 32 + lr, r = r_ < R ? r_ : R - 1;
+    const int iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
+    const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
+    const char * mrow = m_mask(a, iq, h, i3);
+    const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
+    const bool mine = rt + wave * 32 < R;
+    const int64_t row = ((int64_t)i3 * a.n_head_kv + hk) * R + r;
+    const int nt = (a.n_kv + PA_SLOTS - 1) / PA_SLOTS;
+
+    KChunk<TYPE> kr[CN];
+    auto issue = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < CN; i++) {
+            const int c = PT * i + tid, j = t * PA_SLOTS + c / (D / 8), cc = c % (D / 8);
+            kr[i].load(kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1, cc < a.d / 8 ? cc : a.d / 8 - 1);
+        }
+    };
+    auto commit = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < CN; i++) {
+            const int c = PT * i + tid, j = c / (D / 8), cc = c % (D / 8), at = j * RP + cc * 16;
+            if constexpr (!scaled) *(v4i *)(kt[b][0] + at) = kr[i].raw;
+            else {
+                float v[8];
+                kr[i].values(cc < a.d / 8 ? cc : a.d / 8 - 1, v);
+                float m = amax8(v);
+#pragma unroll
+                for (int o = 1; o < D / 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+                const int e = row_exp(m);
+                v4i p[KP];
+                to_parts<KP>(v, e, p);
+#pragma unroll
+                for (int q = 0; q < KP; q++) *(v4i *)(kt[b][q] + at) = p[q];
+                if (cc == 0) ksc[b][j] = ldexpf(1.0f, e);
+            }
+        }
+    };
+    u2 ma[2][4], mb[2][4];
+    auto masks = [&](int t, u2 (&w)[2][4]) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) tile_mask(a, mrow, m8, t * PA_SLOTS + 32 * u, w[u]);
+    };
+    int t = split, b = 0;
+    if (t < nt) { issue(t); masks(t, ma); }
+    if (t + a.nsplit < nt) masks(t + a.nsplit, mb);
+    v4i qf[KS][2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int p = 0; p < 2; p++) qf[ks][p] = *(const v4i *)(a.qparts + (row * 2 + p) * D + 16 * ks + 8 * lh);
+    const float qe = a.rowc[row].qe, slope = a.rowc[row].slope;
+    float m = -INFINITY, l = 0.0f;               // of this lane's row over this lane's slots (two lanes share a row)
+    bool any = t < nt && mine && (mask_sees(ma[0]) || mask_sees(ma[1]));
+    if (t < nt) commit(0);                       // the first tile is fetched without asking
+    bool live = __syncthreads_or(any);
+    while (t < nt) {
+        const int tn = t + a.nsplit;
+        const bool anyn = tn < nt && mine && (mask_sees(mb[0]) || mask_sees(mb[1]));
+        const bool liven = __syncthreads_or(anyn);           // (the tile in buffer b is complete, the other one has been read)
+        if (liven) issue(tn);
+        if (live && __any(any)) {
+            float s[2][16];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                v16f c;
+#pragma unroll
+                for (int i = 0; i < 16; i++) c[i] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const int at = (32 * u + lr) * RP + ks * 32 + lh * 16;
+                    const v4i k0 = *(const v4i *)(kt[b][0] + at);
+                    if constexpr (KP == 2) c = mfma32(*(const v4i *)(kt[b][KP - 1] + at), qf[ks][0], c);
+                    c = mfma32(k0, qf[ks][1], c);
+                    c = mfma32(k0, qf[ks][0], c);
+                }
+                float kv[16];
+                if constexpr (scaled) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) { const v4f x = *(const v4f *)&ksc[b][32 * u + 8 * q + 4 * lh]; for (int i = 0; i < 4; i++) kv[4 * q + i] = x[i]; }
+                }
+                tile_logits<scaled>(a, c, kv, qe, slope, ma[u], __all(mask_zero(ma[u])), s[u]);
+            }
+            float mx = m;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
+            const float ms = mx == -INFINITY ? 0.0f : mx;
+            l *= __builtin_amdgcn_exp2f(m - ms);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) l += __builtin_amdgcn_exp2f(s[u][i] - ms);
+            m = mx;
+        }
+        if (liven) commit(b ^ 1);
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) ma[u][q] = mb[u][q];
+        if (tn + a.nsplit < nt) masks(tn + a.nsplit, mb);
+        any = anyn; live = liven; t = tn; b ^= 1;
+    }
+    const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
+    const float M = fmaxf(m, mo), ms = M == -INFINITY ? 0.0f : M;
+    const float L = l * __builtin_amdgcn_exp2f(m - ms) + lo * __builtin_amdgcn_exp2f(mo - ms);
+    if (lh == 0 && r_ < R) *(v2f *)(a.stats + ((((int64_t)i3 * a.n_head_kv + hk) * a.nsplit + split) * R + r_) * 2) = v2f{M, L};
+}
+
+// the slices' statistics of a row -> maximum (0: sees nothing) and 1 / sum
+__global__ void __launch_bounds__(PT)
+prompt_rows_kernel(const MArgs a) {
+    const int R = a.ratio * a.n_q, r = blockIdx.x * PT + threadIdx.x, hk = blockIdx.y, i3 = blockIdx.z;
+    if (r >= R) return;
+    const int64_t hrow = (int64_t)i3 * a.n_head_kv + hk;
+    const v2f * st = (const v2f *)a.stats + hrow * a.nsplit * R + r;
+    float M = -INFINITY, L = 0.0f;
+    for (int s = 0; s < a.nsplit; s += 4) {
+        v2f x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = s + i < a.nsplit ? st[(int64_t)(s + i) * R] : v2f{-INFINITY, 0.0f};
+        const float mn = fmaxf(fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)), M), ms = mn == -INFINITY ? 0.0f : mn;
+        L *= __builtin_amdgcn_exp2f(M - ms);
+#pragma unroll
+        for (int i = 0; i < 4; i++) L = __builtin_fmaf(x[i].y, __builtin_amdgcn_exp2f(x[i].x - ms), L);
+        M = mn;
+    }
+    *(v2f *)&a.rowc[hrow * R + r].m = v2f{M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L};
+}
+
+// NS: 32-slot tiles of a wave
+template <int TYPE, int D, int NS>
+__global__ void __launch_bounds__(PT, D <= 128 && NS * KForm<TYPE>::parts <= 2 ? 2 : 1)
+prompt_mass_kernel(const MArgs a) {
+    constexpr int KS = D / 16, KP = KForm<TYPE>::parts, RP = D * 2 + 16, CN = PB_ROWS * 2 * (D / 8) / PT;
+    constexpr bool scaled = KForm<TYPE>::scaled;
+    __shared__ __attribute__((aligned(16))) uint8_t qt[2][2][PB_ROWS * RP];
+    __shared__ RowC rc[2][PB_ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
+    const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, chunk = blockIdx.x % a.nchunk;
+    const int j0 = (blockIdx.x / a.nchunk * 4 + wave) * 32 * NS;         // this wave's slots
+    const int64_t base = ((int64_t)i3 * a.n_head_kv + hk) * R;
+    const int nt = (R + PB_ROWS - 1) / PB_ROWS;
+    const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
+
+    v4i qr[CN];
+    RowC rr = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto issue = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < CN; i++) {
+            const int c = PT * i + tid, x = c / (D / 8), row = t * PB_ROWS + (x >> 1);      // x: (row, part)
+            qr[i] = *(const v4i *)(a.qparts + ((base + (row < R ? row : R - 1)) * 2 + (x & 1)) * D + c % (D / 8) * 8);
+        }
+        if (tid < PB_ROWS) {                                    // rows past the last one weigh nothing
+            const int row = t * PB_ROWS + tid;
+            rr = row < R ? a.rowc[base + row] : RowC{0.0f, 0.0f, INFINITY, 0.0f};
+        }
+    };
+    auto commit = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < CN; i++) {
+            const int c = PT * i + tid, x = c / (D / 8);
+            *(v4i *)(qt[b][x & 1] + (x >> 1) * RP + c % (D / 8) * 16) = qr[i];
+        }
+        if (tid < PB_ROWS) rc[b][tid] = rr;
+    };
+    u2 ma[NS][4], mb[NS][4];
+    auto masks = [&](int t, u2 (&w)[NS][4]) {
+        const int r = t * PB_ROWS + lr < R ? t * PB_ROWS + lr : R - 1, iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
+        const char * mrow = m_mask(a, iq, h, i3);
+#pragma unroll
+        for (int u = 0; u < NS; u++) tile_mask(a, mrow, m8, j0 + 32 * u, w[u]);
+    };
+    auto sees = [&](const u2 (&w)[NS][4]) { bool any = false; for (int u = 0; u < NS; u++) any |= mask_sees(w[u]); return any; };
+
+    // this wave's K rows, as the A operand holds them, the largest finite value brought to [2^14, 2^15)
+    v4i kf[NS][KS][KP];
+    float kscale = 1.0f;
+    {
+        const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
+#pragma unroll
+        for (int u = 0; u < NS; u++) {
+            const int j = j0 + 32 * u + lr;
+            const char * row = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
+            if constexpr (!scaled) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) { const int cc = 2 * ks + lh; kf[u][ks][0] = *(const v4i *)(row + (cc < a.d / 8 ? cc : a.d / 8 - 1) * 16); }
+            }
+        }
+        if constexpr (scaled) {
+            float m = 0.0f;
+            auto each = [&](auto f) {
+#pragma unroll
+                for (int u = 0; u < NS; u++) {
+                    const int j = j0 + 32 * u + lr;
+                    const char * row = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        const int cc = 2 * ks + lh < a.d / 8 ? 2 * ks + lh : a.d / 8 - 1;
+                        KChunk<TYPE> c;
+                        c.load(row, cc);
+                        float v[8];
+                        c.values(cc, v);
+                        f(u, ks, v);
+                    }
+                }
+            };
+            each([&](int, int, float * v) { const float x = amax8(v); if (x < INFINITY) m = fmaxf(m, x); });
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            const int e = row_exp(m);
+            kscale = ldexpf(1.0f, e);
+            each([&](int u, int ks, float * v) { to_parts<KP>(v, e, kf[u][ks]); });
+        }
+    }
+    float acc[NS][16];
+#pragma unroll
+    for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[u][i] = 0.0f;
+
+    int t = chunk, b = 0;
+    if (t < nt) { issue(t); masks(t, ma); commit(0); }
+    if (t + a.nchunk < nt) masks(t + a.nchunk, mb);
+    bool any = t < nt && sees(ma);
+    bool live = __syncthreads_or(any);
+    while (t < nt) {
+        const int tn = t + a.nchunk;
+        const bool anyn = tn < nt && sees(mb);
+        const bool liven = __syncthreads_or(anyn);
+        if (liven) issue(tn);
+        if (live && __any(any)) {
+            const RowC c4 = rc[b][lr];
+            v16f c[NS];
+#pragma unroll
+            for (int u = 0; u < NS; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const v4i q0 = *(const v4i *)(qt[b][0] + lr * RP + ks * 32 + lh * 16), q1 = *(const v4i *)(qt[b][1] + lr * RP + ks * 32 + lh * 16);
+#pragma unroll
+                for (int u = 0; u < NS; u++) {
+                    if constexpr (KP == 2) c[u] = mfma32(kf[u][ks][KP - 1], q0, c[u]);
+                    c[u] = mfma32(kf[u][ks][0], q1, c[u]);
+                    c[u] = mfma32(kf[u][ks][0], q0, c[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < NS; u++) {
+                float s[16];
+                tile_logits<false>(a, c[u], nullptr, c4.qe * kscale, c4.slope, ma[u], __all(mask_zero(ma[u])), s);
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[u][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[i] - c4.m), c4.inv, acc[u][i]);
+            }
+        }
+        if (liven) commit(b ^ 1);
+#pragma unroll
+        for (int u = 0; u < NS; u++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) ma[u][q] = mb[u][q];
+        if (tn + a.nchunk < nt) masks(tn + a.nchunk, mb);
+        any = anyn; live = liven; t = tn; b ^= 1;
+    }
+    // over the 32 lanes (rows) of each half: 16 sums per tile
+#pragma unroll
+    for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float x = acc[u][i];
+            x += dpp_f32<0xB1>(x); x += dpp_f32<0x4E>(x); x += dpp_f32<0x141>(x); x += dpp_f32<0x140>(x);
+            x += __shfl_xor(x, 16, 64);
+            const int j = j0 + 32 * u + 8 * (i >> 2) + 4 * lh + (i & 3);
+            if (lr == 0 && j < a.n_kv) a.part[(((int64_t)i3 * a.n_head_kv + hk) * a.nchunk + chunk) * a.n_kv + j] = x;
+        }
+}
+
+__global__ void __launch_bounds__(PT)
+prompt_sum_kernel(const MArgs a) {
+    const int j = blockIdx.x * PT + threadIdx.x, hk = blockIdx.y, i3 = blockIdx.z;
     if (j >= a.n_kv) return;
+    const float * p = a.part + ((int64_t)i3 * a.n_head_kv + hk) * a.nchunk * a.n_kv + j;
+    float t = 0.0f;
+#pragma unroll 8
+    for (int c = 0; c < a.nchunk; c++) t += p[(int64_t)c * a.n_kv];
     if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
     ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
 }
 
-template <int TYPE> static int mass_launch(const MArgs & a, int ne3, hipStream_t s) {
-    if (a.n_kv == 0) return MI355_OK;
-    MI355_LAUNCH("fattn_mass_rows", mass_rows_kernel<TYPE>, dim3((unsigned)a.n_head, (unsigned)a.n_q, (unsigned)ne3), dim3(MT), 0, s, a);
+// slots of a wave in the second pass: 64 where its K fits 128 registers
+template <int TYPE, int D> constexpr int prompt_ns() { return D * KForm<TYPE>::parts <= 128 ? 2 : 1; }
+static int prompt_slots(int type, int64_t d) {           // slots of a workgroup in the second pass
+    const int parts = type == MI355_TYPE_Q8_0 || type == MI355_TYPE_Q4_0 ? 2 : 1;
+    return step_d(d) * parts <= 128 ? 256 : 128;
+}
+// both passes get about 2048 workgroups (4 rounds of two per CU: causal prompts have long and short ones) where there is work for them
+static int64_t prompt_splits(const mi355_fattn_args * p) {
+    const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (p->n_kv + PA_SLOTS - 1) / PA_SLOTS, base = (R + PA_ROWS - 1) / PA_ROWS * p->n_head_kv * p->ne3;
+    int64_t n = 2048 / base, most = (tiles + 3) / 4;
+    if (n > most) n = most;
+    if (n > 64) n = 64;
+    return n < 1 ? 1 : n;
+}
+static int64_t prompt_chunks(const mi355_fattn_args * p) {
+    const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (R + PB_ROWS - 1) / PB_ROWS;
+    const int64_t ws = prompt_slots(p->type_k, p->d), base = (p->n_kv + ws - 1) / ws * p->n_head_kv * p->ne3;
+    int64_t n = base > 0 ? 2048 / base : 1, most = (tiles + 3) / 4;
+    if (n > most) n = most;
+    if (n > 64) n = 64;
+    return n < 1 ? 1 : n;
+}
+
+template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hipStream_t s) {
+    const int R = a.ratio * a.n_q, ws = 128 * prompt_ns<TYPE, D>();
+    const unsigned hk = (unsigned)a.n_head_kv, z = (unsigned)ne3;
+    MI355_LAUNCH("attn_mass_q", prompt_q_kernel<D>, dim3((unsigned)((R + 15) / 16), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
-    MI355_LAUNCH("fattn_mass", mass_slots_kernel<TYPE>, dim3((unsigned)((a.n_kv + MT - 1) / MT), (unsigned)a.n_head_kv, (unsigned)ne3), dim3(MT), 0, s, a);
+    MI355_LAUNCH("attn_mass_stats", (prompt_stats_kernel<TYPE, D>), dim3((unsigned)((R + PA_ROWS - 1) / PA_ROWS * a.nsplit), hk, z), dim3(PT), 0, s, a);
+    MI355_CHECK_LAUNCH();
+    MI355_LAUNCH("attn_mass_rows", prompt_rows_kernel, dim3((unsigned)((R + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
+    MI355_CHECK_LAUNCH();
+    MI355_LAUNCH("attn_mass", (prompt_mass_kernel<TYPE, D, prompt_ns<TYPE, D>()>), dim3((unsigned)((a.n_kv + ws - 1) / ws * a.nchunk), hk, z), dim3(PT), 0, s, a);
+    MI355_CHECK_LAUNCH();
+    MI355_LAUNCH("attn_mass_sum", prompt_sum_kernel, dim3((unsigned)((a.n_kv + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
     return MI355_OK;
 }
+template <int TYPE> static int prompt_dispatch(const MArgs & a, int ne3, hipStream_t s) {
+    if (a.n_kv == 0) return MI355_OK;
+    switch (step_d(a.d)) {
+        case 64:  return prompt_launch<TYPE, 64>(a, ne3, s);
+        case 128: return prompt_launch<TYPE, 128>(a, ne3, s);
+    }
+    return prompt_launch<TYPE, 256>(a, ne3, s);
+}
 
-// steps: [statistics][partial rows of dst][logits]; prompts: statistics
-struct WsParts { int64_t nsplit, lpitch, stats, part, logits; };
+// steps: [statistics][partial rows of dst][logits]; prompts: [statistics][sums of the row chunks][row constants][parts of q] (in floats)
+struct WsParts { int64_t nsplit, nchunk, lpitch, stats, part, logits, rowc, q; };
 static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     const int64_t rows = p->ne3 * p->n_head * p->n_q;
-    WsParts w = {1, 0, rows * 2, 0, 0};
-    if (p->n_q <= MI355_MASS_MAX_Q) {
+    WsParts w = {1, 1, 0, 0, 0, 0, 0, 0};
+    if (p->n_q > MI355_MASS_MAX_Q) {
+        w.nsplit = prompt_splits(p);
+        w.nchunk = prompt_chunks(p);
+        w.stats = (w.nsplit * rows * 2 + 3) / 4 * 4;
+        w.part = (p->ne3 * p->n_head_kv * w.nchunk * p->n_kv + 3) / 4 * 4;
+        w.rowc = rows * 4;
+        w.q = rows * step_d(p->d);                  // two f16 rows
+    } else {
         w.nsplit = step_splits(p);
         w.lpitch = (p->n_kv + 3) / 4 * 4;
         w.stats = (w.nsplit * rows * 2 + 3) / 4 * 4;
@@ -901,7 +1321,7 @@ static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
 static int64_t mass_workspace(const mi355_fattn_args * p, bool with_dst) {
     if (!p || p->n_q < 0 || p->n_kv < 0 || p->n_head < 1 || p->n_head_kv < 1 || p->n_head % p->n_head_kv || p->ne3 < 1 || p->d < 8 || p->d > 256) return -1;
     const WsParts w = mass_parts(p, with_dst);
-    return (w.stats + w.part + w.logits) * 4;
+    return (w.stats + w.part + w.logits + w.rowc + w.q) * 4;
 }
 
 static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, bool with_dst, void * workspace, int64_t workspace_bytes, void * stream) {
@@ -943,10 +1363,12 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     a.m0 = powf(2.0f, -(p->max_bias) / a.n_head_log2);
     a.m1 = powf(2.0f, -(p->max_bias / 2.0f) / a.n_head_log2);
     const WsParts parts = mass_parts(p, with_dst);
-    a.nsplit = (int)parts.nsplit; a.lpitch = (int)parts.lpitch;
+    a.nsplit = (int)parts.nsplit; a.nchunk = (int)parts.nchunk; a.lpitch = (int)parts.lpitch;
     a.stats = (float *)workspace;
     a.part = a.stats + parts.stats;
     a.logits = a.part + parts.part;
+    a.rowc = (RowC *)(a.logits + parts.logits);
+    a.qparts = (uint16_t *)(a.logits + parts.logits + parts.rowc);
     hipStream_t s = (hipStream_t)stream;
     if (p->n_q <= MI355_MASS_MAX_Q) switch (p->type_k) {
         case MI355_TYPE_F16:  return with_dst ? step_dispatch<MI355_TYPE_F16, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_F16, false>(a, (int)p->ne3, s);
@@ -955,11 +1377,11 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
         case MI355_TYPE_Q4_0: return with_dst ? step_dispatch<MI355_TYPE_Q4_0, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_Q4_0, false>(a, (int)p->ne3, s);
     }
     switch (p->type_k) {
-        case MI355_TYPE_F16:  return mass_launch<MI355_TYPE_F16>(a, (int)p->ne3, s);
-        case MI355_TYPE_BF16: return mass_launch<MI355_TYPE_BF16>(a, (int)p->ne3, s);
-        case MI355_TYPE_Q8_0: return mass_launch<MI355_TYPE_Q8_0>(a, (int)p->ne3, s);
+        case MI355_TYPE_F16:  return prompt_dispatch<MI355_TYPE_F16>(a, (int)p->ne3, s);
+        case MI355_TYPE_BF16: return prompt_dispatch<MI355_TYPE_BF16>(a, (int)p->ne3, s);
+        case MI355_TYPE_Q8_0: return prompt_dispatch<MI355_TYPE_Q8_0>(a, (int)p->ne3, s);
     }
-    return mass_launch<MI355_TYPE_Q4_0>(a, (int)p->ne3, s);
+    return prompt_dispatch<MI355_TYPE_Q4_0>(a, (int)p->ne3, s);
 }
 
 } // namespace
