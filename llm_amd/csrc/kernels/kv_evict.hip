@@ -1,10 +1,15 @@
 // kv_evict.hip -- which slots of a bounded KV cache to keep, by the attention weight they have drawn (mi355_kv_evict).
 //
 // Per (sequence, KV head): the n_keep slots with the largest key, ties to the lower slot; key = the slot's mass, or +inf where its position
-// is one of the first n_sink or the newest n_recent (NaN counts as -inf, -0 as +0).  A radix search over the 32-bit images of the keys
-// (order-preserving: sign flipped for positive floats, all bits for negative ones) finds the n_keep-th largest and how many of its equals
-// belong to the kept ones; one ordered pass then writes both index lists ascending.  All integer work: the result does not depend on
-// timing.  The rows are gathered by a second launch.
+// is one of the first n_sink or the newest n_recent (NaN counts as -inf, -0 as +0).  The keys' 32-bit images (order-preserving: sign flipped for
+// positive floats, all bits for negative ones) are searched for the n_keep-th largest; one ordered pass then writes both index lists
+// ascending.  All integer work: the result does not depend on timing.  The rows are gathered by a second launch.
+//
+// Bound by latency: one workgroup per head has to agree on every step of the search.  A step parts the range of keys that can still hold the
+// wanted one into 2048 buckets (an LDS histogram), so three steps settle 32 bits, and masses, which spread over the range as logarithms do,
+// seldom meet in a bucket; the +inf of sinks and recent slots is counted aside, and a wave whose lanes all fall into one bucket adds once.
+// Up to 32768 slots the keys stay in registers; beyond, every step reads them again.  2049 / 32768 slots, 128 / 8 heads: @STEP us.
+// (Digits of 8 bits from the top, keys re-read: 54 / 147 us, atomics queued on the few exponents; bisection with a vote per bit: 15.5 / 48 us.)
 #include "common.h"
 
 namespace {
@@ -19,8 +24,6 @@ struct KeArgs {
     int n_kv, n_keep, n_evict, n_sink, n_recent, n_head_kv;
 };
 
-constexpr int KE_THREADS = 1024, KE_WAVES = KE_THREADS / 64;
-
 static __device__ __forceinline__ uint32_t ke_key(float m, bool keep) {
     if (keep) return 0xff800000u;                     // the image of +inf
     if (m != m) m = -INFINITY;
@@ -29,75 +32,174 @@ static __device__ __forceinline__ uint32_t ke_key(float m, bool keep) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// exclusive prefix sum of a flag over the workgroup; `total` for every thread
-static __device__ __forceinline__ int ke_prefix(bool f, int * sh, int & total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t b = __ballot(f);
-    __syncthreads();
-    if (lane == 0) sh[wave] = __popcll(b);
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < KE_WAVES; w++) { before += w < wave ? sh[w] : 0; all += sh[w]; }
-    total = all;
-    return before + __popcll(b & ((1ull << lane) - 1));
+constexpr int KE_BINS = 2048;
+
+// reductions and prefix sums over a wave with DPP moves inside rows of 16 lanes and v_readlane between them (a ds_bpermute costs ~100 clocks)
+template <int CTRL> static __device__ __forceinline__ uint32_t ke_dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+template <class OP> static __device__ __forceinline__ uint32_t ke_reduce(uint32_t v, OP op) {
+    v = op(v, ke_dpp<0xB1>(v));      // quad_perm [1,0,3,2]
+    v = op(v, ke_dpp<0x4E>(v));      // quad_perm [2,3,0,1]
+    v = op(v, ke_dpp<0x141>(v));     // row_half_mirror
+    v = op(v, ke_dpp<0x140>(v));     // row_mirror
+    const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16), c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+    return op(op(a, b), op(c, d));
+}
+static __device__ __forceinline__ uint32_t ke_scan(uint32_t v) {      // inclusive prefix sum
+    v += ke_dpp<0x111>(v);           // row_shr:1 .. 8, zeros shifted in
+    v += ke_dpp<0x112>(v);
+    v += ke_dpp<0x114>(v);
+    v += ke_dpp<0x118>(v);
+    const uint32_t a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
 }
 
-__global__ void __launch_bounds__(KE_THREADS)
+// Wave w holds the slots from 64 C w on, lane by lane, C slots a lane: slot order is (wave, i, lane).  KPT > 0: C = KPT, keys in registers;
+// KPT == 0: C from the length, keys read at every use.
+template <int KPT, int NW>
+__global__ void __launch_bounds__(64 * NW)
 kv_select_kernel(const KeArgs a) {
-    __shared__ int hist[256], sh[KE_WAVES], pick[2];
-    const int tid = threadIdx.x, hk = blockIdx.x, i3 = blockIdx.y;
+    constexpr int NT = 64 * NW, PER = KE_BINS / NT;
+    __shared__ uint32_t hist[KE_BINS], lim[3][NW], part[NW], pick[3];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hk = blockIdx.x, i3 = blockIdx.y;
     const float * mass = (const float *)(a.mass + hk * a.mass_nb2 + i3 * a.mass_nb3);
     const int32_t * pos = (const int32_t *)(a.pos + hk * a.pos_nb2 + i3 * a.pos_nb3);
     int32_t * kept = (int32_t *)(a.kept + hk * a.kept_nb2 + i3 * a.kept_nb3);
     int32_t * evicted = a.evicted ? (int32_t *)(a.evicted + hk * a.ev_nb2 + i3 * a.ev_nb3) : nullptr;
+    const int C = KPT > 0 ? KPT : (a.n_kv + NT - 1) / NT, first = wave * 64 * C + lane;
+    float m[KPT > 0 ? KPT : 1]; int p[KPT > 0 ? KPT : 1];
+    if constexpr (KPT > 0) {
+#pragma unroll
+        for (int i = 0; i < KPT; i++) {
+            const int j = first + 64 * i;
+            m[i] = j < a.n_kv ? mass[j] : 0.0f;
+            p[i] = j < a.n_kv ? pos[j] : 0;
+        }
+    }
     int n = a.n_used ? ((const int32_t *)a.n_used)[i3] : a.n_kv;
     n = n < 0 ? 0 : n < a.n_kv ? n : a.n_kv;
     const int64_t recent = (int64_t)((const int32_t *)a.n_past)[i3] - a.n_recent;
-    auto key = [&](int j) { const int p = pos[j]; return ke_key(mass[j], p < a.n_sink || p >= recent); };
-
-    // the smallest kept key T and the number of kept slots that equal it
-    uint32_t T = 0;
-    int equal = 0x7fffffff;
-    if (n > a.n_keep) {
-        int want = a.n_keep;                          // rank of the wanted key, counted from the largest
-        uint32_t mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int j = tid; j < n; j += KE_THREADS) { const uint32_t k = key(j); if ((k & mask) == T) atomicAdd(&hist[k >> shift & 255], 1); }
-            __syncthreads();
-            if (tid == 0) {
-                int c = 0, b = 255;
-                while (b > 0 && c + hist[b] < want) { c += hist[b]; b--; }
-                pick[0] = b; pick[1] = want - c;
+    uint32_t key[KPT > 0 ? KPT : 1];                  // 0: not in use (below the image of -inf)
+    if constexpr (KPT > 0) {
+#pragma unroll
+        for (int i = 0; i < KPT; i++) key[i] = first + 64 * i < n ? ke_key(m[i], p[i] < a.n_sink || p[i] >= recent) : 0;
+    }
+    auto each = [&](auto f) {                         // f(slot, key), in slot order within the wave, by all lanes
+        if constexpr (KPT > 0) {
+#pragma unroll
+            for (int i = 0; i < KPT; i++) f(first + 64 * i, key[i]);
+        } else {
+            for (int i = 0; i < C; i++) {
+                const int j = first + 64 * i;
+                uint32_t k = 0;
+                if (j < n) { const int q = pos[j]; k = ke_key(mass[j], q < a.n_sink || q >= recent); }
+                f(j, k);
             }
-            __syncthreads();
-            T |= (uint32_t)pick[0] << shift;
-            want = pick[1];
-            mask |= 255u << shift;
-            __syncthreads();
         }
-        equal = want;
+    };
+
+    uint32_t T = 1;                                   // kept: key >= T, of which those equal to T only the first `equal`
+    uint32_t equal = 0xffffffffu;
+    if (n > a.n_keep) {
+        // the range of the keys, the +inf among them counted aside
+        constexpr uint32_t INF = 0xff800000u;
+        uint32_t lo = 0xffffffffu, hi = 0, inf = 0;
+        each([&](int, uint32_t k) {
+            if (k == INF) inf++;
+            else if (k) { lo = lo < k ? lo : k; hi = hi > k ? hi : k; }
+        });
+        lo = ke_reduce(lo, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+        hi = ke_reduce(hi, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+        inf = ke_reduce(inf, [](uint32_t x, uint32_t y) { return x + y; });
+        if (lane == 0) { lim[0][wave] = lo; lim[1][wave] = hi; lim[2][wave] = inf; }
+        for (int i = tid; i < KE_BINS; i += NT) hist[i] = 0;
+        __syncthreads();
+        inf = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w++) { lo = lo < lim[0][w] ? lo : lim[0][w]; hi = hi > lim[1][w] ? hi : lim[1][w]; inf += lim[2][w]; }
+        lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi); inf = __builtin_amdgcn_readfirstlane(inf);
+        if (inf >= (uint32_t)a.n_keep) { T = INF; equal = a.n_keep; }
+        else {
+            uint32_t want = a.n_keep - inf;           // rank of the wanted key among those in [lo, hi], from the largest
+            for (;;) {
+                const int bits = 32 - __builtin_clz((hi - lo) | 1), shift = bits > 11 ? bits - 11 : 0;
+                each([&](int, uint32_t k) {
+                    const bool in = k >= lo && k <= hi;
+                    const uint32_t bin = (k - lo) >> shift;
+                    const uint64_t who = __ballot(in);
+                    if (!who) return;
+                    const uint32_t one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(who));
+                    if (__ballot(in && bin == one) == who) { if (lane == 0) atomicAdd(&hist[one], (uint32_t)__popcll(who)); }
+                    else if (in) atomicAdd(&hist[bin], 1u);
+                });
+                __syncthreads();
+                // thread t owns the bins from the top down: PER (t + 1) - 1 .. PER t counted from the highest
+                uint32_t h[PER], sum = 0;
+#pragma unroll
+                for (int i = 0; i < PER; i++) { h[i] = hist[KE_BINS - 1 - (tid * PER + i)]; sum += h[i]; }
+                const uint32_t incl = ke_scan(sum);
+                if (lane == 63) part[wave] = incl;
+                __syncthreads();                      // (every bin has been read)
+                uint32_t above = incl - sum;
+#pragma unroll
+                for (int w = 0; w < NW; w++) above += w < wave ? part[w] : 0;
+                if (above < want && want <= above + sum) {
+#pragma unroll
+                    for (int i = 0; i < PER; i++) {
+                        if (above < want && want <= above + h[i]) { pick[0] = KE_BINS - 1 - (tid * PER + i); pick[1] = want - above; pick[2] = h[i]; }
+                        above += h[i];
+                    }
+                }
+                for (int i = tid; i < KE_BINS; i += NT) hist[i] = 0;
+                __syncthreads();
+                const uint32_t bin = pick[0], in_bin = pick[2];
+                want = pick[1];
+                lo += bin << shift;
+                if (shift == 0 || want == in_bin) { T = lo; if (want != in_bin) equal = want; break; }
+                const uint32_t top = lo + ((1u << shift) - 1);
+                hi = top < hi ? top : hi;
+            }
+        }
+        T = __builtin_amdgcn_readfirstlane(T); equal = __builtin_amdgcn_readfirstlane(equal);
     }
-    // one ordered pass: slot j stays if its key is above T, or equals T and fewer than `equal` equals lie before it
-    int kept_n = 0, eq_n = 0, ev_n = 0;
-    for (int j0 = 0; j0 < n; j0 += KE_THREADS) {
-        const int j = j0 + tid;
-        const uint32_t k = j < n ? key(j) : 0;
-        int t_eq, t_keep, t_ev;
-        const bool eq = j < n && k == T;
-        const int p_eq = ke_prefix(eq, sh, t_eq);
-        const bool keep = j < n && (k > T || (eq && eq_n + p_eq < equal));
-        const int p_keep = ke_prefix(keep, sh, t_keep);
-        const bool ev = j < n && !keep;
-        const int p_ev = ke_prefix(ev, sh, t_ev);
-        if (keep) kept[kept_n + p_keep] = j;
-        if (ev && evicted && ev_n + p_ev < a.n_evict) evicted[ev_n + p_ev] = j;
-        eq_n += t_eq; kept_n += t_keep; ev_n += t_ev;
+    // the wave's equals (where not all are kept) and kept ones before it, then each slot's own rank
+    uint32_t eq_before = 0;
+    const bool ties = equal != 0xffffffffu;
+    const uint64_t below = (1ull << lane) - 1;
+    if (ties) {
+        uint32_t eq = 0;
+        each([&](int, uint32_t k) { eq += __popcll(__ballot(k == T)); });
+        __syncthreads();                              // (part has been read)
+        if (lane == 0) part[wave] = eq;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; w++) eq_before += w < wave ? part[w] : 0;
     }
-    for (int j = kept_n + tid; j < a.n_keep; j += KE_THREADS) kept[j] = -1;
-    if (evicted) for (int j = ev_n + tid; j < a.n_evict; j += KE_THREADS) evicted[j] = -1;
+    uint32_t e = eq_before;
+    auto stays = [&](uint32_t k) {                    // the kept lanes at one i; called for i = 0, 1, ... in turn
+        if (!ties) return (uint64_t)__ballot(k >= T);
+        const uint64_t be = __ballot(k == T);
+        const uint64_t b = __ballot(k > T || (k == T && e + __popcll(be & below) < equal));
+        e += __popcll(be);
+        return b;
+    };
+    int mine = 0;
+    each([&](int, uint32_t k) { mine += __popcll(stays(k)); });
+    if (lane == 0) lim[0][wave] = mine;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) { before += w < wave ? lim[0][w] : 0; all += lim[0][w]; }
+    e = eq_before;
+    each([&](int j, uint32_t k) {
+        const uint64_t b = stays(k);
+        const int rank = before + __popcll(b & below);
+        if (b >> lane & 1) kept[rank] = j;
+        else if (j < n && evicted && j - rank < a.n_evict) evicted[j - rank] = j;      // (j - rank slots before j are not kept)
+        before += __popcll(b);
+    });
+    for (int j = all + tid; j < a.n_keep; j += NT) kept[j] = -1;
+    if (evicted) for (int j = n - all + tid; j < a.n_evict; j += NT) evicted[j] = -1;
 }
 
 struct KgArgs {
@@ -112,24 +214,63 @@ struct KgArgs {
     int64_t mo_nb2, mo_nb3, po_nb2, po_nb3;
 };
 
-// one wave per kept slot: the K and V rows in 2-byte pieces, the tables' entries
+// A group of W lanes (a power of two, the pieces of a row rounded up) copies a row; a workgroup takes 4 groups' worth of rows per thread, whose
+// loads are all requested before the first is stored.  Bound by the rows' bytes, once in and once out.
+template <class PIECE>
 __global__ void __launch_bounds__(256)
-kv_gather_kernel(const KgArgs a) {
-    const int lane = threadIdx.x & 63, hk = blockIdx.y, i3 = blockIdx.z;
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= a.n_keep) return;
-    const int j = ((const int32_t *)(a.kept + hk * a.kept_nb2 + i3 * a.kept_nb3))[i];
+kv_gather_kernel(const KgArgs a, int log2_w) {
+    const int hk = blockIdx.y, i3 = blockIdx.z, lane = threadIdx.x & ((1 << log2_w) - 1), rows = 256 >> log2_w;
+    const int32_t * kept = (const int32_t *)(a.kept + hk * a.kept_nb2 + i3 * a.kept_nb3);
+    const char * src[2] = {a.src[0] + hk * a.s_nb2[0] + i3 * a.s_nb3[0], a.src[1] + hk * a.s_nb2[1] + i3 * a.s_nb3[1]};
+    char * dst[2] = {a.dst[0] + hk * a.d_nb2[0] + i3 * a.d_nb3[0], a.dst[1] + hk * a.d_nb2[1] + i3 * a.d_nb3[1]};
+    int i[4], j[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        i[u] = blockIdx.x * 4 * rows + u * rows + ((int)threadIdx.x >> log2_w);
+        j[u] = i[u] < a.n_keep ? kept[i[u]] : -1;
+    }
     if (lane == 0) {
-        if (a.mass_out) ((float *)(a.mass_out + hk * a.mo_nb2 + i3 * a.mo_nb3))[i] = j < 0 ? 0.0f : ((const float *)(a.mass + hk * a.mass_nb2 + i3 * a.mass_nb3))[j];
-        if (a.pos_out) ((int32_t *)(a.pos_out + hk * a.po_nb2 + i3 * a.po_nb3))[i] = j < 0 ? -1 : ((const int32_t *)(a.pos + hk * a.pos_nb2 + i3 * a.pos_nb3))[j];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (i[u] >= a.n_keep) continue;
+            if (a.mass_out) ((float *)(a.mass_out + hk * a.mo_nb2 + i3 * a.mo_nb3))[i[u]] = j[u] < 0 ? 0.0f : ((const float *)(a.mass + hk * a.mass_nb2 + i3 * a.mass_nb3))[j[u]];
+            if (a.pos_out) ((int32_t *)(a.pos_out + hk * a.po_nb2 + i3 * a.po_nb3))[i[u]] = j[u] < 0 ? -1 : ((const int32_t *)(a.pos + hk * a.pos_nb2 + i3 * a.pos_nb3))[j[u]];
+        }
     }
-    if (j < 0) return;
-    for (int s = 0; s < 2; s++) {
-        if (!a.src[s]) continue;
-        const uint16_t * x = (const uint16_t *)(a.src[s] + j * a.s_nb1[s] + hk * a.s_nb2[s] + i3 * a.s_nb3[s]);
-        uint16_t * y = (uint16_t *)(a.dst[s] + i * a.d_nb1[s] + hk * a.d_nb2[s] + i3 * a.d_nb3[s]);
-        for (int e = lane; e < a.row_bytes[s] / 2; e += 64) y[e] = x[e];
+    for (int e = lane; e * (int)sizeof(PIECE) < (a.row_bytes[0] > a.row_bytes[1] ? a.row_bytes[0] : a.row_bytes[1]); e += 1 << log2_w) {
+        PIECE x[2][4];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) if (j[u] >= 0 && e * (int)sizeof(PIECE) < a.row_bytes[s]) x[s][u] = *(const PIECE *)(src[s] + j[u] * a.s_nb1[s] + e * (int)sizeof(PIECE));
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) if (j[u] >= 0 && e * (int)sizeof(PIECE) < a.row_bytes[s]) *(PIECE *)(dst[s] + i[u] * a.d_nb1[s] + e * (int)sizeof(PIECE)) = x[s][u];
     }
+}
+
+template <class PIECE> static int gather_launch(const KgArgs & g, int64_t n_keep, int64_t hk, int64_t ne3, hipStream_t s) {
+    const int bytes = g.row_bytes[0] > g.row_bytes[1] ? g.row_bytes[0] : g.row_bytes[1], pieces = bytes / (int)sizeof(PIECE);
+    int w = 0;
+    while (w < 6 && (1 << w) < pieces) w++;
+    const int64_t rows = 4 * (256 >> w);
+    MI355_LAUNCH("kv_gather", kv_gather_kernel<PIECE>, dim3((unsigned)((n_keep + rows - 1) / rows), (unsigned)hk, (unsigned)ne3), dim3(256), 0, s, g, w);
+    MI355_CHECK_LAUNCH();
+    return MI355_OK;
+}
+template <int KPT, int NW> static int select_launch(const KeArgs & a, int64_t ne3, hipStream_t s) {
+    MI355_LAUNCH("kv_select", (kv_select_kernel<KPT, NW>), dim3((unsigned)a.n_head_kv, (unsigned)ne3), dim3(64 * NW), 0, s, a);
+    MI355_CHECK_LAUNCH();
+    return MI355_OK;
+}
+static int select_dispatch(const KeArgs & a, int64_t ne3, hipStream_t s) {
+    if (a.n_kv <= 1024)  return select_launch<4, 4>(a, ne3, s);
+    if (a.n_kv <= 4096)  return select_launch<8, 8>(a, ne3, s);
+    if (a.n_kv <= 8192)  return select_launch<8, 16>(a, ne3, s);
+    if (a.n_kv <= 16384) return select_launch<16, 16>(a, ne3, s);
+    if (a.n_kv <= 32768) return select_launch<32, 16>(a, ne3, s);
+    return select_launch<0, 16>(a, ne3, s);
 }
 
 } // namespace
@@ -167,8 +308,8 @@ int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
     a.evicted = (char *)p->evicted; a.ev_nb2 = p->ev_nb2; a.ev_nb3 = p->ev_nb3;
     a.n_kv = (int)p->n_kv; a.n_keep = (int)p->n_keep; a.n_evict = (int)p->n_evict; a.n_sink = p->n_sink; a.n_recent = p->n_recent; a.n_head_kv = (int)p->n_head_kv;
     hipStream_t s = (hipStream_t)stream;
-    MI355_LAUNCH("kv_select", kv_select_kernel, dim3((unsigned)p->n_head_kv, (unsigned)p->ne3), dim3(KE_THREADS), 0, s, a);
-    MI355_CHECK_LAUNCH();
+    const int rc = select_dispatch(a, p->ne3, s);
+    if (rc != MI355_OK) return rc;
     if (!p->k && !p->v && !p->mass_out && !p->pos_out) return MI355_OK;
 
     KgArgs g;
@@ -182,9 +323,14 @@ int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
     g.mass = a.mass; g.mass_nb2 = a.mass_nb2; g.mass_nb3 = a.mass_nb3; g.pos = a.pos; g.pos_nb2 = a.pos_nb2; g.pos_nb3 = a.pos_nb3;
     g.mass_out = (char *)p->mass_out; g.mo_nb2 = p->mo_nb2; g.mo_nb3 = p->mo_nb3;
     g.pos_out = (char *)p->pos_out; g.po_nb2 = p->po_nb2; g.po_nb3 = p->po_nb3;
-    MI355_LAUNCH("kv_gather", kv_gather_kernel, dim3((unsigned)((a.n_keep + 3) / 4), (unsigned)p->n_head_kv, (unsigned)p->ne3), dim3(256), 0, s, g);
-    MI355_CHECK_LAUNCH();
-    return MI355_OK;
+    // the widest piece that rows, strides and row lengths allow
+    int64_t low = rows;
+    if (p->k) low |= g.row_bytes[0];
+    if (p->v) low |= g.row_bytes[1];
+    if ((low & 15) == 0) return gather_launch<v4i>(g, p->n_keep, p->n_head_kv, p->ne3, s);
+    if ((low & 7) == 0)  return gather_launch<v2i>(g, p->n_keep, p->n_head_kv, p->ne3, s);
+    if ((low & 3) == 0)  return gather_launch<uint32_t>(g, p->n_keep, p->n_head_kv, p->ne3, s);
+    return gather_launch<uint16_t>(g, p->n_keep, p->n_head_kv, p->ne3, s);
 }
 
 } // extern "C"

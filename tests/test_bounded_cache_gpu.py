@@ -304,6 +304,7 @@ EVICT = [
     (1, 1, 1, 1, 0, 0, None, "spread"), (1, 2, 2, 1, 0, 0, None, "spread"), (2, 3, 65, 64, 4, 16, None, "spread"), (1, 8, 2049, 2048, 4, 512, None, "spread"),
     (3, 2, 1000, 100, 4, 25, [1000, 100, 99], "ties"), (4, 1, 777, 300, 0, 0, [0, 1, 301, 5000], "equal"), (2, 2, 500, 123, 0, 0, [-7, 500], "odd"),
     (1, 2, 4097, 17, 17, 0, None, "ties"), (1, 2, 5000, 4999, 0, 4999, None, "odd"), (1, 1, 100, 200, 10, 10, None, "spread"),
+    (2, 2, 3000, 1500, 0, 0, [3000, 2999], "ties"), (1, 3, 8000, 7999, 4, 100, None, "equal"), (1, 2, 16000, 1, 0, 0, None, "spread"), (3, 1, 50000, 20000, 4, 1024, [50000, 100, 40000], "odd"),
     (2, 4, 32768, 4096, 4, 1024, [32768, 20001], "spread"), (1, 2, 70001, 9000, 4, 100, None, "ties"), (1, 1, 140000, 100000, 4, 100, None, "odd"),
 ]
 
