@@ -60,7 +60,8 @@ template <int KPT, int NW>
 __global__ void __launch_bounds__(64 * NW)
 kv_select_kernel(const KeArgs a) {
     constexpr int NT = 64 * NW, PER = KE_BINS / NT;
-    __shared__ uint32_t hist[KE_BINS], lim[3][NW], part[NW], pick[3];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[KE_BINS];
+    __shared__ uint32_t lim[3][NW], part[NW], pick[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hk = blockIdx.x, i3 = blockIdx.y;
     const float * mass = (const float *)(a.mass + hk * a.mass_nb2 + i3 * a.mass_nb3);
     const int32_t * pos = (const int32_t *)(a.pos + hk * a.pos_nb2 + i3 * a.pos_nb3);
@@ -111,6 +112,7 @@ kv_select_kernel(const KeArgs a) {
         lo = ke_reduce(lo, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
         hi = ke_reduce(hi, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
         inf = ke_reduce(inf, [](uint32_t x, uint32_t y) { return x + y; });
+        if (tid == 0) pick[3] = 0;
         if (lane == 0) { lim[0][wave] = lo; lim[1][wave] = hi; lim[2][wave] = inf; }
         for (int i = tid; i < KE_BINS; i += NT) hist[i] = 0;
         __syncthreads();
@@ -158,6 +160,24 @@ kv_select_kernel(const KeArgs a) {
                 if (shift == 0 || want == in_bin) { T = lo; if (want != in_bin) equal = want; break; }
                 const uint32_t top = lo + ((1u << shift) - 1);
                 hi = top < hi ? top : hi;
+                if (in_bin <= 128) {                  // few are left: a thread each ranks them against one another (a pass more costs 1.5 us)
+                    each([&](int, uint32_t k) { if (k >= lo && k <= hi) hist[atomicAdd(&pick[3], 1u)] = k; });
+                    __syncthreads();
+                    if (tid < (int)in_bin) {
+                        const uint32_t k = hist[tid];
+                        uint32_t over = 0, same = 0;
+                        for (uint32_t i = 0; i < in_bin; i += 4) {      // (cells past the last hold 0)
+                            const v4i x = *(const v4i *)&hist[i];
+#pragma unroll
+                            for (int q = 0; q < 4; q++) { over += (uint32_t)x[q] > k; same += (uint32_t)x[q] == k; }
+                        }
+                        if (over < want && want <= over + same) { pick[0] = k; pick[1] = want - over; pick[2] = same; }   // (every equal writes the same)
+                    }
+                    __syncthreads();
+                    T = pick[0];
+                    if (pick[1] != pick[2]) equal = pick[1];
+                    break;
+                }
             }
         }
         T = __builtin_amdgcn_readfirstlane(T); equal = __builtin_amdgcn_readfirstlane(equal);

@@ -295,6 +295,10 @@ def evict_case(S, HK, n, seed, kind="spread"):
     elif kind == "odd":                  # infinities, NaNs, negative and subnormal values, neighbours in the last bit
         pool = np.array([np.inf, -np.inf, np.nan, -np.nan, 0.0, -0.0, 1e-45, -1e-45, 1.0, np.nextafter(np.float32(1), np.float32(2)), -1.0, 3e38, -3e38], np.float32)
         mass = pool[r.integers(0, len(pool), (S, HK, n))]
+    elif kind == "border":               # a few hundred keys around the border, one step of the last bit apart, some of them equal
+        mass = (np.float32(1.0).view(np.uint32) + r.integers(0, 100, (S, HK, n)).astype(np.uint32)).view(np.float32)
+        mass[..., ::7] = 5.0
+        mass[..., 3::7] = -2.0
     pos = np.stack([r.permutation(2 * n + 3)[:n] for _ in range(S * HK)]).reshape(S, HK, n).astype(np.int32)
     return mass, pos
 
@@ -305,6 +309,7 @@ EVICT = [
     (3, 2, 1000, 100, 4, 25, [1000, 100, 99], "ties"), (4, 1, 777, 300, 0, 0, [0, 1, 301, 5000], "equal"), (2, 2, 500, 123, 0, 0, [-7, 500], "odd"),
     (1, 2, 4097, 17, 17, 0, None, "ties"), (1, 2, 5000, 4999, 0, 4999, None, "odd"), (1, 1, 100, 200, 10, 10, None, "spread"),
     (2, 2, 3000, 1500, 0, 0, [3000, 2999], "ties"), (1, 3, 8000, 7999, 4, 100, None, "equal"), (1, 2, 16000, 1, 0, 0, None, "spread"), (3, 1, 50000, 20000, 4, 1024, [50000, 100, 40000], "odd"),
+    (2, 2, 600, 300, 0, 0, None, "border"), (1, 2, 150, 60, 0, 0, None, "border"), (1, 1, 9000, 4000, 4, 10, None, "border"), (1, 2, 40000, 17000, 4, 10, None, "border"),
     (2, 4, 32768, 4096, 4, 1024, [32768, 20001], "spread"), (1, 2, 70001, 9000, 4, 100, None, "ties"), (1, 1, 140000, 100000, 4, 100, None, "odd"),
 ]
 
