@@ -38,68 +38,160 @@ static __device__ __forceinline__ double qn_freq(const QnArgs & a, int i) {
     return w * f;
 }
 
-template <int TYPE> static __device__ __forceinline__ void qn_store(char * row, int e, float v) {
-    if (TYPE == MI355_TYPE_F32)       ((float *)row)[e] = v;
-    else if (TYPE == MI355_TYPE_F16)  ((__half *)row)[e] = cvt<float, __half>(v);
-    else if (TYPE == MI355_TYPE_BF16) ((bf16_bits *)row)[e] = cvt<float, bf16_bits>(v);
+// 4 consecutive values of a row
+template <int TYPE> static __device__ __forceinline__ void qn_store4(char * row, int e, const float * v) {
+    if (TYPE == MI355_TYPE_F32) *(v4f *)((float *)row + e) = v4f{v[0], v[1], v[2], v[3]};
+    else {
+        uint16_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = TYPE == MI355_TYPE_F16 ? __half_as_ushort(cvt<float, __half>(v[i])) : cvt<float, bf16_bits>(v[i]).bits;
+        *(v2i *)((uint16_t *)row + e) = v2i{h[0] | h[1] << 16, h[2] | h[3] << 16};
+    }
 }
 
-// one wave per row (a head of q, k or v of one token)
-template <int TYPE>
-__global__ void __launch_bounds__(64)
-qk_norm_rope_kernel(const QnArgs a) {
-    __shared__ float x[256];
-    const int lane = threadIdx.x;
-    const int r = blockIdx.y, t = blockIdx.x % a.n, i3 = blockIdx.x / a.n;
-    const bool is_q = r < a.n_head, is_v = r >= a.n_head + a.n_head_kv;
-    const int hk = is_q ? 0 : is_v ? r - a.n_head - a.n_head_kv : r - a.n_head;
-    const int d = is_v ? a.dv : a.d;
-    const float * src = (const float *)(is_q ? a.q + t * a.q_nb1 + r * a.q_nb2 + i3 * a.q_nb3 : is_v ? a.v + t * a.v_nb1 + hk * a.v_nb2 + i3 * a.v_nb3
-                                                                                                    : a.k + t * a.k_nb1 + hk * a.k_nb2 + i3 * a.k_nb3);
-    const int pos = *(const int32_t *)(a.pos + t * a.pos_nb1 + i3 * a.pos_nb3);
-    float ss = 0.0f;
-    for (int e = lane; e < d; e += 64) { const float f = src[e]; x[e] = f; ss += f * f; }
-    if (!is_v) {
-        const float s = 1.0f / sqrtf(wave_sum(ss) / d + a.eps);
-        const float * w = is_q ? a.qw : a.kw;
-        for (int e = lane; e < d; e += 64) x[e] = x[e] * s * (w ? w[e] : 1.0f);
-        __syncthreads();
-        for (int i = lane; i < a.n_dims / 2; i += 64) {
-            const int ia = a.neox ? i : 2 * i, ib = a.neox ? i + a.n_dims / 2 : 2 * i + 1;
-            const double rev = (double)pos * qn_freq(a, i);
-            float c, sn;
-            sincospif(2.0f * (float)(rev - rint(rev)), &sn, &c);
-            c *= a.mscale; sn *= a.mscale;
-            const float xa = x[ia], xb = x[ib];
-            x[ia] = xa * c - xb * sn;
-            x[ib] = xa * sn + xb * c;
-        }
+// A group of L lanes takes a row (a head of q, k or v of one token), 8 values a lane: rotating rows as 4 and 4 values whose pairs the lane
+// holds itself -- NEOX: 4 i.. and n_dims / 2 + 4 i..; NORMAL and the features past n_dims: 8 i.. -- so nothing crosses lanes but the sum of
+// squares.  A workgroup first forms cos and sin of all pairs of its TT tokens in LDS (64-bit angles: ~100 clocks a pair, shared by every head),
+// then walks their rows two at a time, loads ahead.  Bound by the rows' bytes at prompts (@PROMPT), by one launch at steps (@STEP).
+constexpr int QN_THREADS = 256;
+
+template <int TYPE, int L>
+__global__ void __launch_bounds__(QN_THREADS)
+qk_norm_rope_kernel(const QnArgs a, int tt, int chunks) {
+    constexpr bool quant = TYPE == MI355_TYPE_Q8_0 || TYPE == MI355_TYPE_Q4_0;
+    constexpr int G = QN_THREADS / L;
+    extern __shared__ __attribute__((aligned(16))) float cs[];       // [tt][2][n_dims / 2], then rows to quantize [G][8 L]
+    const int tid = threadIdx.x, j = tid % L, g = tid / L, half = a.n_dims / 2;
+    const int t0 = blockIdx.x / chunks * tt, chunk = blockIdx.x % chunks, T = a.n * a.ne3, nt = T - t0 < tt ? T - t0 : tt;
+    const int H = a.n_head, HK = a.n_head_kv, R = H + (a.vo ? 2 : 1) * HK;
+
+    const bool rotates = 8 * j < a.n_dims, in = 8 * j < a.d, vin = 8 * j < a.dv;
+    const int ea = a.neox && rotates ? 4 * j : 8 * j, eb = a.neox && rotates ? half + 4 * j : 8 * j + 4;
+    // rows of this workgroup's chunk: (token, row) pairs n = chunk * G + g, + chunks * G, ...
+    struct Row { const float * src; int t, i3, r, kind; };            // kind: 0 q, 1 k, 2 v
+    auto locate = [&](int n) {
+        Row x;
+        const int tok = t0 + n / R;
+        x.r = n % R;
+        x.i3 = tok / a.n; x.t = tok - x.i3 * a.n;
+        x.kind = x.r < H ? 0 : x.r < H + HK ? 1 : 2;
+        if (x.kind) x.r -= x.kind == 1 ? H : H + HK;
+        x.src = (const float *)(x.kind == 0 ? a.q + x.t * a.q_nb1 + x.r * a.q_nb2 + x.i3 * a.q_nb3 : x.kind == 1 ? a.k + x.t * a.k_nb1 + x.r * a.k_nb2 + x.i3 * a.k_nb3
+                                                                                                                : a.v + x.t * a.v_nb1 + x.r * a.v_nb2 + x.i3 * a.v_nb3);
+        return x;
+    };
+    auto load = [&](const Row & x, v4f & A, v4f & B) {
+        A = B = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (x.kind == 2 ? vin : in) { A = *(const v4f *)(x.src + (x.kind == 2 ? 8 * j : ea)); B = *(const v4f *)(x.src + (x.kind == 2 ? 8 * j + 4 : eb)); }
+    };
+    const int rows = nt * R, step = chunks * G;
+    int n = chunk * G + g;
+    Row x0, x1;
+    v4f A0, B0, A1, B1;
+    if (n < rows) { x0 = locate(n); load(x0, A0, B0); }
+    if (n + step < rows) { x1 = locate(n + step); load(x1, A1, B1); }
+
+    for (int i = tid; i < nt * half; i += QN_THREADS) {
+        const int tok = i / half, p = i - tok * half, i3 = (t0 + tok) / a.n, t = t0 + tok - i3 * a.n;
+        const double rev = (double)*(const int32_t *)(a.pos + t * a.pos_nb1 + i3 * a.pos_nb3) * qn_freq(a, p);
+        float c, s;
+        sincospif(2.0f * (float)(rev - rint(rev)), &s, &c);
+        cs[tok * 2 * half + p] = c * a.mscale;
+        cs[tok * 2 * half + half + p] = s * a.mscale;
+    }
+    v4f wq[2], wk[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        wq[i] = wk[i] = v4f{1.0f, 1.0f, 1.0f, 1.0f};
+        if (in && a.qw) wq[i] = *(const v4f *)(a.qw + (i ? eb : ea));
+        if (in && a.kw) wk[i] = *(const v4f *)(a.kw + (i ? eb : ea));
     }
     __syncthreads();
-    if (is_q) {
-        float * o = (float *)(a.qo + t * a.qo_nb1 + r * a.qo_nb2 + i3 * a.qo_nb3);
-        for (int e = lane; e < d; e += 64) o[e] = x[e];
-        return;
-    }
-    const int64_t row = a.rows ? *(const int32_t *)(a.rows + t * a.rows_nb1 + hk * a.rows_nb2 + i3 * a.rows_nb3) : t;
-    if (row < 0 || row >= a.n_rows) return;           // as SET_ROWS: an index outside the cache stores nothing
-    char * o = is_v ? a.vo + row * a.vo_nb1 + hk * a.vo_nb2 + i3 * a.vo_nb3 : a.ko + row * a.ko_nb1 + hk * a.ko_nb2 + i3 * a.ko_nb3;
-    if constexpr (TYPE == MI355_TYPE_Q8_0 || TYPE == MI355_TYPE_Q4_0) {
-        if (lane < d / 32) quant_block<TYPE>(x + 32 * lane, (uint8_t *)o + QBlk<TYPE>::bytes * lane);
-    } else {
-        for (int e = lane; e < d; e += 64) qn_store<TYPE>(o, e, x[e]);
-    }
-    if (!is_v && lane == 0) {
-        if (a.slot_pos)  ((int32_t *)(a.slot_pos + hk * a.sp_nb2 + i3 * a.sp_nb3))[row] = pos;
-        if (a.slot_mass) ((float *)(a.slot_mass + hk * a.sm_nb2 + i3 * a.sm_nb3))[row] = 0.0f;
+
+    while (n < rows) {
+        const Row x = x0;
+        float A[4] = {A0[0], A0[1], A0[2], A0[3]}, B[4] = {B0[0], B0[1], B0[2], B0[3]};
+        const int tok = n / R;
+        x0 = x1; A0 = A1; B0 = B1;
+        if (n + 2 * step < rows) { x1 = locate(n + 2 * step); load(x1, A1, B1); }
+        n += step;
+        if (x.kind != 2) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) ss += A[i] * A[i];
+#pragma unroll
+            for (int i = 0; i < 4; i++) ss += B[i] * B[i];
+            ss += dpp_f32<0xB1>(ss);
+            ss += dpp_f32<0x4E>(ss);
+            ss += dpp_f32<0x141>(ss);
+            if (L >= 16) ss += dpp_f32<0x140>(ss);
+            if (L == 32) ss += __shfl_xor(ss, 16, 64);
+            const float s = 1.0f / sqrtf(ss / a.d + a.eps);
+            const v4f w0 = x.kind == 0 ? wq[0] : wk[0], w1 = x.kind == 0 ? wq[1] : wk[1];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { A[i] = A[i] * s * w0[i]; B[i] = B[i] * s * w1[i]; }
+            if (rotates) {
+                const v4f c = *(const v4f *)(cs + tok * 2 * half + 4 * j), sn = *(const v4f *)(cs + tok * 2 * half + half + 4 * j);
+                if (a.neox) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float u = A[i], v = B[i];
+                        A[i] = u * c[i] - v * sn[i];
+                        B[i] = u * sn[i] + v * c[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float u = A[2 * i], v = A[2 * i + 1], y = B[2 * i], z = B[2 * i + 1];
+                        A[2 * i] = u * c[i] - v * sn[i];         A[2 * i + 1] = u * sn[i] + v * c[i];
+                        B[2 * i] = y * c[2 + i] - z * sn[2 + i]; B[2 * i + 1] = y * sn[2 + i] + z * c[2 + i];
+                    }
+                }
+            }
+        }
+        if (x.kind == 0) {
+            float * o = (float *)(a.qo + x.t * a.qo_nb1 + x.r * a.qo_nb2 + x.i3 * a.qo_nb3);
+            if (in) { *(v4f *)(o + ea) = v4f{A[0], A[1], A[2], A[3]}; *(v4f *)(o + eb) = v4f{B[0], B[1], B[2], B[3]}; }
+            continue;
+        }
+        const int64_t row = a.rows ? *(const int32_t *)(a.rows + x.t * a.rows_nb1 + x.r * a.rows_nb2 + x.i3 * a.rows_nb3) : x.t;
+        const bool stored = row >= 0 && row < a.n_rows;                   // as SET_ROWS: an index outside the cache stores nothing
+        char * o = x.kind == 2 ? a.vo + row * a.vo_nb1 + x.r * a.vo_nb2 + x.i3 * a.vo_nb3 : a.ko + row * a.ko_nb1 + x.r * a.ko_nb2 + x.i3 * a.ko_nb3;
+        const bool mine = (x.kind == 2 ? vin : in) && stored;
+        const int pa = x.kind == 2 ? 8 * j : ea, pb = x.kind == 2 ? 8 * j + 4 : eb;
+        if constexpr (!quant) {
+            if (mine) { qn_store4<TYPE>(o, pa, A); qn_store4<TYPE>(o, pb, B); }
+        } else {
+            // a block is 32 consecutive values: through LDS, then a lane per block
+            float * xs = cs + tt * 2 * half + g * 8 * L;
+            *(v4f *)(xs + pa) = v4f{A[0], A[1], A[2], A[3]};
+            *(v4f *)(xs + pb) = v4f{B[0], B[1], B[2], B[3]};
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (stored && j < (x.kind == 2 ? a.dv : a.d) / 32) quant_block<TYPE>(xs + 32 * j, (uint8_t *)o + QBlk<TYPE>::bytes * j);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        if (x.kind == 1 && j == 0 && stored) {
+            if (a.slot_pos)  ((int32_t *)(a.slot_pos + x.r * a.sp_nb2 + x.i3 * a.sp_nb3))[row] = *(const int32_t *)(a.pos + x.t * a.pos_nb1 + x.i3 * a.pos_nb3);
+            if (a.slot_mass) ((float *)(a.slot_mass + x.r * a.sm_nb2 + x.i3 * a.sm_nb3))[row] = 0.0f;
+        }
     }
 }
 
-template <int TYPE> static int qn_launch(const QnArgs & a, hipStream_t s) {
-    const int rows = a.n_head + (a.vo ? 2 : 1) * a.n_head_kv;
-    MI355_LAUNCH("qk_norm_rope", qk_norm_rope_kernel<TYPE>, dim3((unsigned)(a.n * a.ne3), (unsigned)rows), dim3(64), 0, s, a);
+template <int TYPE, int L> static int qn_launch_l(const QnArgs & a, hipStream_t s) {
+    // 4 tokens a workgroup share its sines while that leaves 1024 workgroups; a few tokens are spread over as many workgroups as they have rows for
+    const int64_t T = (int64_t)a.n * a.ne3, R = a.n_head + (a.vo ? 2 : 1) * a.n_head_kv, G = QN_THREADS / L;
+    const int tt = T >= 4096 ? 4 : 1;
+    const int64_t most = (tt * R + G - 1) / G, groups = (T + tt - 1) / tt;
+    int64_t chunks = groups >= 1024 ? 1 : 1024 / groups;
+    if (chunks > most) chunks = most;
+    const size_t lds = ((size_t)tt * a.n_dims + (TYPE == MI355_TYPE_Q8_0 || TYPE == MI355_TYPE_Q4_0 ? QN_THREADS * 8 : 0)) * sizeof(float);
+    MI355_LAUNCH("qk_norm_rope", (qk_norm_rope_kernel<TYPE, L>), dim3((unsigned)(groups * chunks)), dim3(QN_THREADS), lds, s, a, tt, (int)chunks);
     MI355_CHECK_LAUNCH();
     return MI355_OK;
+}
+template <int TYPE> static int qn_launch(const QnArgs & a, hipStream_t s) {
+    const int d = a.vo && a.dv > a.d ? a.dv : a.d;
+    return d <= 64 ? qn_launch_l<TYPE, 8>(a, s) : d <= 128 ? qn_launch_l<TYPE, 16>(a, s) : qn_launch_l<TYPE, 32>(a, s);
 }
 
 } // namespace
