@@ -28,6 +28,7 @@ struct MArgs {
     float * stats;      // [ne3][n_head_kv][nsplit][rows][2]: maximum (log2 domain) and sum of a slice
     float * part;       // steps: [ne3][n_head_kv][nsplit][rows][D]; prompts: [ne3][n_head_kv][nchunk][n_kv]
     RowC * rowc; // prompts: [ne3][n_head_kv][rows]
+    uint8_t * cls; int cpitch;  // prompts: [m_ne3][m_ne2][n_q][cpitch] classes of the mask's 32-slot tiles
     uint16_t * qparts;  // prompts: [ne3][n_head_kv][rows][2][D] f16
 };
 
@@ -920,35 +921,65 @@ static __device__ __forceinline__ void tile_mask(const MArgs & a, const char * m
         }
     }
 }
-static __device__ __forceinline__ bool mask_sees(const u2 (&w)[4]) {
-    bool all = true;
+// What a 32-slot tile of the mask is to a query: nothing visible, all of it zero, or anything else (the tile past the last slot too).  Looked up
+// by both passes and by every head that shares the mask, so that they read the mask itself only where it is neither (the diagonal of a prompt).
+enum { MASK_HIDDEN = 0, MASK_ZERO = 1, MASK_MIXED = 2 };
+__global__ void __launch_bounds__(PT)
+prompt_class_kernel(const MArgs a) {
+    const int lane = threadIdx.x & 63, iq = blockIdx.y * 4 + (threadIdx.x >> 6), plane = blockIdx.z;
+    if (iq >= a.n_q) return;
+    const char * mrow = a.mask + iq * a.m_nb1 + plane % a.m_ne2 * a.m_nb2 + plane / a.m_ne2 * a.m_nb3;
+    uint8_t * out = a.cls + ((int64_t)plane * a.n_q + iq) * a.cpitch;
+    const int j0 = blockIdx.x * 1024;
+    uint16_t v[16];
 #pragma unroll
-    for (int q = 0; q < 4; q++) all &= w[q].x == 0xfc00fc00u && w[q].y == 0xfc00fc00u;
-    return !all;
+    for (int i = 0; i < 16; i++) { const int j = j0 + 64 * i + lane; v[i] = j < a.n_kv ? ((const uint16_t *)mrow)[j] : 0xfc00; }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        if (j0 + 64 * i >= a.n_kv) break;
+        const uint64_t hid = __ballot(v[i] == 0xfc00), zero = __ballot((v[i] & 0x7fff) == 0);
+        if (lane < 2) {
+            const uint32_t h = (uint32_t)(hid >> (32 * lane)), z = (uint32_t)(zero >> (32 * lane));
+            out[(j0 + 64 * i) / 32 + lane] = h == 0xffffffffu ? MASK_HIDDEN : z == 0xffffffffu ? MASK_ZERO : MASK_MIXED;
+        }
+    }
 }
-static __device__ __forceinline__ bool mask_zero(const u2 (&w)[4]) {
-    uint32_t o = 0;
+// classes of the N tiles from slot j0 on, a byte each (no mask: zero up to the last whole tile)
+template <int N> static __device__ __forceinline__ void tile_class(const MArgs & a, const uint8_t * crow, int j0, int (&c)[N]) {
 #pragma unroll
-    for (int q = 0; q < 4; q++) o |= w[q].x | w[q].y;
-    return o == 0;
+    for (int u = 0; u < N; u++) {
+        const int j = j0 + 32 * u;
+        c[u] = j >= a.n_kv ? MASK_HIDDEN : a.mask ? crow[j / 32] : j + 32 <= a.n_kv ? MASK_ZERO : MASK_MIXED;
+    }
+}
+static __device__ __forceinline__ const uint8_t * class_row(const MArgs & a, int iq, int h, int i3) {
+    const int plane = (a.m_ne3 > 1 ? i3 % a.m_ne3 : 0) * a.m_ne2 + (a.m_ne2 > 1 ? h % a.m_ne2 : 0);
+    return a.cls + ((int64_t)plane * a.n_q + iq) * a.cpitch;
 }
 static __device__ __forceinline__ float mask_at(const u2 (&w)[4], int i) { return h2f((uint16_t)(w[i >> 2][(i & 3) >> 1] >> (16 * (i & 1)))); }
 
-// logits (log2 domain) of a 32 x 32 tile: c holds the products, ks the slots' scales (accumulator layout)
-template <bool SCALED> static __device__ __forceinline__ void tile_logits(const MArgs & a, const v16f & c, const float * ks, float qe, float slope, const u2 (&w)[4],
-                                                                          bool zero, float * s) {
+// logits (log2 domain) of a 32 x 32 tile from slot j0 on: c holds the products, ks the slots' scales (accumulator layout), cl the tile's class
+// for this lane's query
+template <bool SCALED> static __device__ __forceinline__ void tile_logits(const MArgs & a, const v16f & c, const float * ks, float qe, float slope, int cl, const char * mrow,
+                                                                          bool m8, int j0, float * s) {
 #pragma unroll
     for (int i = 0; i < 16; i++) s[i] = SCALED ? c[i] * ks[i] * qe : c[i] * qe;
     if (a.logit_softcap != 0.0f) {
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = a.logit_softcap * LOG2E * tanhf(s[i]);
     }
-    if (!zero) {
+    if (__all(cl == MASK_ZERO)) return;
+    if (__any(cl == MASK_MIXED)) {
+        u2 w[4];
+        tile_mask(a, mrow, m8, j0, w);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const float mv = mask_at(w, i);
             s[i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope, s[i]);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = cl == MASK_HIDDEN ? -INFINITY : s[i];
     }
 }
 
@@ -998,14 +1029,11 @@ prompt_stats_kernel(const MArgs a) {
             }
         }
     };
-    u2 ma[2][4], mb[2][4];
-    auto masks = [&](int t, u2 (&w)[2][4]) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) tile_mask(a, mrow, m8, t * PA_SLOTS + 32 * u, w[u]);
-    };
+    const uint8_t * crow = class_row(a, iq, h, i3);
+    int ca[2] = {0, 0}, cb[2] = {0, 0};
     int t = split, b = 0;
-    if (t < nt) { issue(t); masks(t, ma); }
-    if (t + a.nsplit < nt) masks(t + a.nsplit, mb);
+    if (t < nt) { issue(t); tile_class(a, crow, t * PA_SLOTS, ca); }
+    if (t + a.nsplit < nt) tile_class(a, crow, (t + a.nsplit) * PA_SLOTS, cb);
     v4i qf[KS][2];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++)
@@ -1013,12 +1041,12 @@ prompt_stats_kernel(const MArgs a) {
         for (int p = 0; p < 2; p++) qf[ks][p] = *(const v4i *)(a.qparts + (row * 2 + p) * D + 16 * ks + 8 * lh);
     const float qe = a.rowc[row].qe, slope = a.rowc[row].slope;
     float m = -INFINITY, l = 0.0f;               // of this lane's row over this lane's slots (two lanes share a row)
-    bool any = t < nt && mine && (mask_sees(ma[0]) || mask_sees(ma[1]));
+    bool any = mine && (ca[0] | ca[1]) != MASK_HIDDEN;
     if (t < nt) commit(0);                       // the first tile is fetched without asking
     bool live = __syncthreads_or(any);
     while (t < nt) {
         const int tn = t + a.nsplit;
-        const bool anyn = tn < nt && mine && (mask_sees(mb[0]) || mask_sees(mb[1]));
+        const bool anyn = tn < nt && mine && (cb[0] | cb[1]) != MASK_HIDDEN;
         const bool liven = __syncthreads_or(anyn);           // (the tile in buffer b is complete, the other one has been read)
         if (liven) issue(tn);
         if (live && __any(any)) {
@@ -1041,7 +1069,7 @@ prompt_stats_kernel(const MArgs a) {
 #pragma unroll
                     for (int q = 0; q < 4; q++) { const v4f x = *(const v4f *)&ksc[b][32 * u + 8 * q + 4 * lh]; for (int i = 0; i < 4; i++) kv[4 * q + i] = x[i]; }
                 }
-                tile_logits<scaled>(a, c, kv, qe, slope, ma[u], __all(mask_zero(ma[u])), s[u]);
+                tile_logits<scaled>(a, c, kv, qe, slope, ca[u], mrow, m8, t * PA_SLOTS + 32 * u, s[u]);
             }
             float mx = m;
 #pragma unroll
@@ -1057,11 +1085,8 @@ prompt_stats_kernel(const MArgs a) {
             m = mx;
         }
         if (liven) commit(b ^ 1);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) ma[u][q] = mb[u][q];
-        if (tn + a.nsplit < nt) masks(tn + a.nsplit, mb);
+        ca[0] = cb[0]; ca[1] = cb[1];
+        if (tn + a.nsplit < nt) tile_class(a, crow, (tn + a.nsplit) * PA_SLOTS, cb);
         any = anyn; live = liven; t = tn; b ^= 1;
     }
     const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
@@ -1127,14 +1152,12 @@ prompt_mass_kernel(const MArgs a) {
         }
         if (tid < PB_ROWS) rc[b][tid] = rr;
     };
-    u2 ma[NS][4], mb[NS][4];
-    auto masks = [&](int t, u2 (&w)[NS][4]) {
+    int ca[NS], cb[NS];
+    auto classes = [&](int t, int (&c)[NS]) {
         const int r = t * PB_ROWS + lr < R ? t * PB_ROWS + lr : R - 1, iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
-        const char * mrow = m_mask(a, iq, h, i3);
-#pragma unroll
-        for (int u = 0; u < NS; u++) tile_mask(a, mrow, m8, j0 + 32 * u, w[u]);
+        tile_class(a, class_row(a, iq, h, i3), j0, c);
     };
-    auto sees = [&](const u2 (&w)[NS][4]) { bool any = false; for (int u = 0; u < NS; u++) any |= mask_sees(w[u]); return any; };
+    auto sees = [&](const int (&c)[NS]) { int any = 0; for (int u = 0; u < NS; u++) any |= c[u]; return any != MASK_HIDDEN; };
 
     // this wave's K rows, as the A operand holds them, the largest finite value brought to [2^14, 2^15)
     v4i kf[NS][KS][KP];
@@ -1183,17 +1206,20 @@ prompt_mass_kernel(const MArgs a) {
         for (int i = 0; i < 16; i++) acc[u][i] = 0.0f;
 
     int t = chunk, b = 0;
-    if (t < nt) { issue(t); masks(t, ma); commit(0); }
-    if (t + a.nchunk < nt) masks(t + a.nchunk, mb);
-    bool any = t < nt && sees(ma);
+    for (int u = 0; u < NS; u++) ca[u] = cb[u] = 0;
+    if (t < nt) { issue(t); classes(t, ca); commit(0); }
+    if (t + a.nchunk < nt) classes(t + a.nchunk, cb);
+    bool any = t < nt && sees(ca);
     bool live = __syncthreads_or(any);
     while (t < nt) {
         const int tn = t + a.nchunk;
-        const bool anyn = tn < nt && sees(mb);
+        const bool anyn = tn < nt && sees(cb);
         const bool liven = __syncthreads_or(anyn);
         if (liven) issue(tn);
         if (live && __any(any)) {
             const RowC c4 = rc[b][lr];
+            const int r = t * PB_ROWS + lr < R ? t * PB_ROWS + lr : R - 1, iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
+            const char * mrow = m_mask(a, iq, h, i3);
             v16f c[NS];
 #pragma unroll
             for (int u = 0; u < NS; u++)
@@ -1212,17 +1238,15 @@ prompt_mass_kernel(const MArgs a) {
 #pragma unroll
             for (int u = 0; u < NS; u++) {
                 float s[16];
-                tile_logits<false>(a, c[u], nullptr, c4.qe * kscale, c4.slope, ma[u], __all(mask_zero(ma[u])), s);
+                tile_logits<false>(a, c[u], nullptr, c4.qe * kscale, c4.slope, ca[u], mrow, m8, j0 + 32 * u, s);
 #pragma unroll
                 for (int i = 0; i < 16; i++) acc[u][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[i] - c4.m), c4.inv, acc[u][i]);
             }
         }
         if (liven) commit(b ^ 1);
 #pragma unroll
-        for (int u = 0; u < NS; u++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) ma[u][q] = mb[u][q];
-        if (tn + a.nchunk < nt) masks(tn + a.nchunk, mb);
+        for (int u = 0; u < NS; u++) ca[u] = cb[u];
+        if (tn + a.nchunk < nt) classes(tn + a.nchunk, cb);
         any = anyn; live = liven; t = tn; b ^= 1;
     }
     // over the 32 lanes (rows) of each half: 16 sums per tile
@@ -1276,6 +1300,10 @@ static int64_t prompt_chunks(const mi355_fattn_args * p) {
 template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hipStream_t s) {
     const int R = a.ratio * a.n_q, ws = 128 * prompt_ns<TYPE, D>();
     const unsigned hk = (unsigned)a.n_head_kv, z = (unsigned)ne3;
+    if (a.mask) {
+        MI355_LAUNCH("attn_mass_class", prompt_class_kernel, dim3((unsigned)((a.n_kv + 1023) / 1024), (unsigned)((a.n_q + 3) / 4), (unsigned)(a.m_ne2 * a.m_ne3)), dim3(PT), 0, s, a);
+        MI355_CHECK_LAUNCH();
+    }
     MI355_LAUNCH("attn_mass_q", prompt_q_kernel<D>, dim3((unsigned)((R + 15) / 16), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
     MI355_LAUNCH("attn_mass_stats", (prompt_stats_kernel<TYPE, D>), dim3((unsigned)((R + PA_ROWS - 1) / PA_ROWS * a.nsplit), hk, z), dim3(PT), 0, s, a);
@@ -1297,11 +1325,11 @@ template <int TYPE> static int prompt_dispatch(const MArgs & a, int ne3, hipStre
     return prompt_launch<TYPE, 256>(a, ne3, s);
 }
 
-// steps: [statistics][partial rows of dst][logits]; prompts: [statistics][sums of the row chunks][row constants][parts of q] (in floats)
-struct WsParts { int64_t nsplit, nchunk, lpitch, stats, part, logits, rowc, q; };
+// steps: [statistics][partial rows of dst][logits]; prompts: [statistics][sums of the row chunks][row constants][parts of q][classes of the mask] (in floats)
+struct WsParts { int64_t nsplit, nchunk, lpitch, stats, part, logits, rowc, q, cls; };
 static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     const int64_t rows = p->ne3 * p->n_head * p->n_q;
-    WsParts w = {1, 1, 0, 0, 0, 0, 0, 0};
+    WsParts w = {1, 1, 0, 0, 0, 0, 0, 0, 0};
     if (p->n_q > MI355_MASS_MAX_Q) {
         w.nsplit = prompt_splits(p);
         w.nchunk = prompt_chunks(p);
@@ -1309,6 +1337,7 @@ static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
         w.part = (p->ne3 * p->n_head_kv * w.nchunk * p->n_kv + 3) / 4 * 4;
         w.rowc = rows * 4;
         w.q = rows * step_d(p->d);                  // two f16 rows
+        if (p->mask) w.cls = (p->m_ne2 * p->m_ne3 * p->n_q * ((p->n_kv + 63) / 64 * 2) + 3) / 4;
     } else {
         w.nsplit = step_splits(p);
         w.lpitch = (p->n_kv + 3) / 4 * 4;
@@ -1319,9 +1348,9 @@ static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     return w;
 }
 static int64_t mass_workspace(const mi355_fattn_args * p, bool with_dst) {
-    if (!p || p->n_q < 0 || p->n_kv < 0 || p->n_head < 1 || p->n_head_kv < 1 || p->n_head % p->n_head_kv || p->ne3 < 1 || p->d < 8 || p->d > 256) return -1;
+    if (!p || p->n_q < 0 || p->n_kv < 0 || (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1)) || p->n_head < 1 || p->n_head_kv < 1 || p->n_head % p->n_head_kv || p->ne3 < 1 || p->d < 8 || p->d > 256) return -1;
     const WsParts w = mass_parts(p, with_dst);
-    return (w.stats + w.part + w.logits + w.rowc + w.q) * 4;
+    return (w.stats + w.part + w.logits + w.rowc + w.q + w.cls) * 4;
 }
 
 static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, bool with_dst, void * workspace, int64_t workspace_bytes, void * stream) {
@@ -1336,7 +1365,7 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     if (p->n_head < 1 || p->n_head > 65535 || p->n_head_kv < 1 || p->n_head % p->n_head_kv != 0 || p->n_q < 1 || p->n_q > 65535 || p->n_kv < 0 ||
         p->n_kv > (1 << 30) || p->ne3 < 1 || p->ne3 > 65535) return MI355_E_SHAPE;
     if (with_dst && p->n_q > MI355_MASS_MAX_Q) return MI355_E_UNSUPPORTED;
-    if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1 || p->m_ne2 > 0x7fffffff || p->m_ne3 > 0x7fffffff)) return MI355_E_SHAPE;
+    if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1 || p->m_ne2 * p->m_ne3 > 65535 || p->m_ne2 > 65535 || p->m_ne3 > 65535)) return MI355_E_SHAPE;
     if (p->k_nb1 < 0 || p->k_nb1 > 0x7fffffff || (with_dst && (p->v_nb1 < 0 || p->v_nb1 > 0x7fffffff))) return MI355_E_SHAPE;
     const int64_t f32s = (int64_t)(uintptr_t)p->q | p->q_nb1 | p->q_nb2 | p->q_nb3 |
                          (with_dst ? (int64_t)(uintptr_t)p->dst | p->d_nb1 | p->d_nb2 | p->d_nb3 : 0) | (int64_t)(uintptr_t)workspace;
@@ -1369,6 +1398,7 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     a.logits = a.part + parts.part;
     a.rowc = (RowC *)(a.logits + parts.logits);
     a.qparts = (uint16_t *)(a.logits + parts.logits + parts.rowc);
+    a.cls = (uint8_t *)(a.logits + parts.logits + parts.rowc + parts.q); a.cpitch = (int)((p->n_kv + 63) / 64 * 2);
     hipStream_t s = (hipStream_t)stream;
     if (p->n_q <= MI355_MASS_MAX_Q) switch (p->type_k) {
         case MI355_TYPE_F16:  return with_dst ? step_dispatch<MI355_TYPE_F16, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_F16, false>(a, (int)p->ne3, s);
