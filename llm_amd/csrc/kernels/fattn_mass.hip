@@ -27,9 +27,9 @@ struct MArgs {
     float * logits;     // steps: [ne3][n_head_kv][rows][lpitch], log2 domain
     float * stats;      // [ne3][n_head_kv][nsplit][rows][2]: maximum (log2 domain) and sum of a slice
     float * part;       // steps: [ne3][n_head_kv][nsplit][rows][D]; prompts: [ne3][n_head_kv][nchunk][n_kv]
-    RowC * rowc; // prompts: [ne3][n_head_kv][rows]
-    uint8_t * cls; int cpitch;  // prompts: [m_ne3][m_ne2][n_q][cpitch] classes of the mask's 32-slot tiles
-    uint16_t * qparts;  // prompts: [ne3][n_head_kv][rows][2][D] f16
+    RowC * rowc;        // prompts: [ne3][n_head_kv][rows]
+    uint8_t * cls; int cpitch;      // prompts: [m_ne3][m_ne2][n_q][cpitch] classes of the mask's 32-slot tiles
+    uint16_t * qparts;  // prompts: [ne3][n_head_kv][rows][parts][D]
 };
 
 template <int TYPE> static __device__ __forceinline__ float kv_value(const char * row, int e) {
@@ -41,11 +41,18 @@ template <int TYPE> static __device__ __forceinline__ float kv_value(const char 
     return h2f(*(const uint16_t *)b) * (float)(n - 8);
 }
 
-// row r of a KV head = (query, head of the group); r < 2^16
+// row r of a KV head = (query, head of the group); r * ratio < 2^32
 static __device__ __forceinline__ int m_query(const MArgs & a, int r) { return a.by_ratio ? (int)__umulhi((uint32_t)r, a.by_ratio) : r; }
 static __device__ __forceinline__ const char * m_mask(const MArgs & a, int iq, int h, int i3) {
     return a.mask + iq * a.m_nb1 + (a.m_ne2 > 1 ? h % a.m_ne2 : 0) * a.m_nb2 + (a.m_ne3 > 1 ? i3 % a.m_ne3 : 0) * a.m_nb3;
 }
+// mass_out of a slot whose weight is t
+static __device__ __forceinline__ void mass_store(const MArgs & a, int hk, int i3, int j, float t) {
+    if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
+    ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
+}
+// exponent that brings a row's largest value to [2^14, 2^15)
+static __device__ __forceinline__ int row_exp(float amax) { return amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0; }
 static __device__ __forceinline__ float m_slope(const MArgs & a, uint32_t h) {
     if (!(a.max_bias > 0.0f)) return 1.0f;
     return h < a.n_head_log2 ? powf(a.m0, h + 1) : powf(a.m1, 2 * (h - a.n_head_log2) + 1);
@@ -720,9 +727,7 @@ mass_finish_kernel(const MArgs a, int mass_wgs) {
                 for (int i = 0; i < 4; i++) if (i0 + i < n && s4[i] != -INFINITY) t = __builtin_fmaf(__builtin_amdgcn_exp2f(s4[i] - sm[i0 + i]), sl[i0 + i], t);
             }
         }
-        if (j >= a.n_kv) return;
-        if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
-        ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
+        if (j < a.n_kv) mass_store(a, hk, i3, j, t);
         return;
     }
     // a row of dst: D / 4 threads per slice of the sum over the splits
@@ -813,31 +818,90 @@ static int64_t step_splits(const mi355_fattn_args * p) {
 // ---- prompts: any number of queries, the weights alone ---------------------------------------------------------------------------------------
 //
 // Keeping the logits would move 8 bytes per (query, slot) pair; computing them twice costs 2 d products each on the matrix cores, which is less:
-//   prompt_q      q as two f16 parts (scale and log2(e) on it, rows brought to [2^14, 2^15) by a power of two), once
+//   prompt_prep   q as two f16 (bf16 caches: three bf16) parts, scale and log2(e) on it, f16 rows brought to [2^14, 2^15) by a power of two; what
+//                 each 32-slot tile of the mask is to each query
 //   prompt_stats  S^T = K Q^T, a running maximum and sum per row: a wave holds 32 rows of Q in registers, K passes through LDS
 //   prompt_mass   S^T again and sum over the rows of 2^(s - m) / l: a wave holds 32 or 64 slots of K, Q passes through LDS; the sums stay in
 //                 registers, one per (slot, lane), and meet across the lanes once at the end
 //   prompt_sum    the row chunks' sums and decay * mass_in, in a fixed order
-// v_mfma_f32_32x32x16_f16 throughout: K of f16 as it is; bf16 rows times a power of two that brings the row's largest value to [2^14, 2^15) (exact
-// down to 2^-29 of it, below that an error of 2^-40); blocks as d * q, likewise, in two parts.  Bound by the matrix cores and by v_exp_f32
-// (a quarter of the vector rate) in equal parts.  Tiles that the mask hides from a whole workgroup (half of a causal prompt) cost their mask.
+// v_mfma_f32_32x32x16 throughout: K of f16 and bf16 as it is; blocks as d * q in two f16 parts, the slot's largest value brought to [2^14, 2^15) by
+// a power of two of its own.  What passes through LDS comes by DMA, two tiles ahead of the products.  A tile that the mask hides from all rows of a
+// wave (half of a causal prompt) costs its loads.
+// 64 queries x 32 heads over 16384 f16 slots: 5 + 24 + 5 + 33 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
+// until the first tile of 512 workgroups is there; without its products the first pass takes 20, without its exponentials 23.  2047
+// causal queries, bf16: 16 + 82 + 5 + 97 + 5 us, 45 a pass at that rate; the workgroups of the first slots see twice the rows of the average.
 typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int PT = 256;                  // threads: 4 waves
 constexpr int PA_ROWS = 128, PA_SLOTS = 64, PB_ROWS = 32;
 
-static __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+template <bool BF> static __device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    else              return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
+// 64 lanes x 16 (4) bytes, each from its own address, to consecutive places in LDS.  Counted by vmcnt; the compiler does not know of them: it
+// waits for too many loads where it waits for its own, never for too few
+static __device__ __forceinline__ void dma16(const void * src, uint32_t dst) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
+}
+static __device__ __forceinline__ void dma4(const void * src, uint32_t dst) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
+}
+static __device__ __forceinline__ uint32_t lds_at(const void * p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
+}
+// all but this wave's N newest loads and all its LDS reads are done, then the workgroup meets
+template <int N> static __device__ __forceinline__ void wait_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+// a value that was loaded, waited for here: a wait of the compiler's own in a loop that DMA runs through would wait for the DMA as well
+static __device__ __forceinline__ void arrived(v4i & x) { asm volatile("" : "+v"(x)); }
+static __device__ __forceinline__ void arrived(float & x) { asm volatile("" : "+v"(x)); }
+// Rows of D 16-bit values in LDS, 16-byte chunks: chunk c of row r lies at c ^ (r & swz<D>()), so that a chunk's column is read without
+// bank conflicts and a DMA's places stay consecutive
+template <int D> constexpr int swz() { return D == 128 ? 15 : 7; }
+template <int D> static __device__ __forceinline__ int lds_chunk(int r, int c) { return r * D * 2 + ((c ^ (r & swz<D>())) * 16); }
 
-// q rows -> ws: [row][2][D] f16 (parts), RowC.  16 lanes a row
-template <int D>
+// What a 32-slot tile of the mask is to a query: nothing visible, all of it zero, or anything else (the tile past the last slot too).  Looked up
+// by both passes and by every head that shares the mask, so that they read the mask itself only where it is neither (the diagonal of a prompt).
+// No mask: one row of classes for all.  A row goes on to the end of the last workgroup's slots.
+enum { MASK_HIDDEN = 0, MASK_ZERO = 1, MASK_MIXED = 2 };
+
+// workgroups 0 .. class_wgs - 1: classes of 4 queries x 1024 slots.  The others: 16 rows of q -> parts, RowC; 16 lanes a row
+template <int D, bool BF>
 __global__ void __launch_bounds__(PT)
-prompt_q_kernel(const MArgs a) {
-    constexpr int NF = D / 128 > 0 ? D / 128 : 1;               // chunks of 8 features per lane
-    const int lane = threadIdx.x & 15, hk = blockIdx.y, i3 = blockIdx.z, R = a.ratio * a.n_q;
-    const int r = blockIdx.x * (PT / 16) + (threadIdx.x >> 4);
+prompt_prep_kernel(const MArgs a, uint32_t class_wgs, uint32_t slot_wgs, uint32_t query_wgs, uint32_t row_wgs) {
+    if (blockIdx.x < class_wgs) {
+        const uint32_t y = blockIdx.x / slot_wgs, x = blockIdx.x - y * slot_wgs, plane = y / query_wgs;
+        const int lane = threadIdx.x & 63, iq = (int)(y - plane * query_wgs) * 4 + (threadIdx.x >> 6);
+        const int n_q = a.mask ? a.n_q : 1;
+        if (iq >= n_q) return;
+        const char * mrow = a.mask + iq * a.m_nb1 + plane % a.m_ne2 * a.m_nb2 + plane / a.m_ne2 * a.m_nb3;
+        uint8_t * out = a.cls + ((int64_t)plane * n_q + iq) * a.cpitch;
+        const int j0 = x * 1024;
+        uint16_t v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) { const int j = j0 + 64 * i + lane; v[i] = j >= a.n_kv ? 0xfc00 : a.mask ? ((const uint16_t *)mrow)[j] : 0; }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int at = (j0 + 64 * i) / 32 + lane;
+            const uint64_t hid = __ballot(v[i] == 0xfc00), zero = __ballot((v[i] & 0x7fff) == 0);
+            if (lane < 2 && at < a.cpitch) {
+                const uint32_t h = (uint32_t)(hid >> (32 * lane)), z = (uint32_t)(zero >> (32 * lane));
+                out[at] = h == 0xffffffffu ? MASK_HIDDEN : z == 0xffffffffu ? MASK_ZERO : MASK_MIXED;
+            }
+        }
+        return;
+    }
+    constexpr int NF = D / 128 > 0 ? D / 128 : 1, P = BF ? 3 : 2;   // chunks of 8 features per lane, parts
+    const uint32_t w = blockIdx.x - class_wgs, y_ = w / row_wgs;
+    const int lane = threadIdx.x & 15, hk = y_ % a.n_head_kv, i3 = y_ / a.n_head_kv, R = a.ratio * a.n_q;
+    const int r = (int)(w - y_ * row_wgs) * (PT / 16) + (threadIdx.x >> 4);
     if (r >= R) return;
-    const int iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
+    const int iq = m_query(a, r), h = hk * a.ratio + r - iq * a.ratio;
     const float * qp = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
     const float sc = a.logit_softcap != 0.0f ? a.scale / a.logit_softcap : a.scale * LOG2E;
     float y[NF][8], amax = 0.0f;
@@ -851,243 +915,211 @@ prompt_q_kernel(const MArgs a) {
     }
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-    const int e = amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+    const int e = BF ? 0 : row_exp(amax);
     const int64_t row = ((int64_t)i3 * a.n_head_kv + hk) * R + r;
 #pragma unroll
     for (int n = 0; n < NF; n++) {
         if (lane + 16 * n >= D / 8) continue;
-        v4i w[2];
+        v4i part[P];
 #pragma unroll
         for (int i = 0; i < 8; i++) y[n][i] = ldexpf(y[n][i], -e);
-        split8<false, 2>(y[n], w);
-        *(v4i *)(a.qparts + (row * 2) * D + 8 * (lane + 16 * n)) = w[0];
-        *(v4i *)(a.qparts + (row * 2 + 1) * D + 8 * (lane + 16 * n)) = w[1];
+        split8<BF, P>(y[n], part);
+#pragma unroll
+        for (int p = 0; p < P; p++) *(v4i *)(a.qparts + (row * P + p) * D + 8 * (lane + 16 * n)) = part[p];
     }
     if (lane == 0) { a.rowc[row].qe = ldexpf(1.0f, e); a.rowc[row].slope = m_slope(a, h) * LOG2E; }
 }
 
-// a chunk of 8 features of K on its way to f16: what is loaded, and its values
+// 8 features of a block row on their way to two f16 parts: what is loaded, and its values
 template <int TYPE> struct KChunk {
-    v4i raw;
-    __device__ __forceinline__ void load(const char * row, int c) { raw = *(const v4i *)(row + c * 16); }
-    __device__ __forceinline__ void values(int, float * v) const {
-#pragma unroll
-        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float((uint32_t)raw[i] << 16); v[2 * i + 1] = __uint_as_float((uint32_t)raw[i] & 0xffff0000u); }
-    }
-};
-template <int TYPE> struct KBlockChunk {
     Chunk<TYPE> c; uint16_t d;
     __device__ __forceinline__ void load(const char * row, int j) { c.load(row + Chunk<TYPE>::at(j)); d = *(const uint16_t *)(row + (j >> 2) * Fmt<TYPE>::block); }
-    __device__ __forceinline__ void values(int j, float * v) const {
+    __device__ __forceinline__ float values(int j, float * v) const {      // returns the largest magnitude
         const h8 q = __builtin_bit_cast(h8, c.operand(j));
         const float dd = h2f(d);
+        float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float)q[i] * dd;
+        for (int i = 0; i < 8; i++) { v[i] = (float)q[i] * dd; m = fmaxf(m, fabsf(v[i])); }
+        return m;
     }
 };
-template <> struct KChunk<MI355_TYPE_Q8_0> : KBlockChunk<MI355_TYPE_Q8_0> {};
-template <> struct KChunk<MI355_TYPE_Q4_0> : KBlockChunk<MI355_TYPE_Q4_0> {};
-template <int TYPE> struct KForm { static constexpr int parts = Fmt<TYPE>::quant ? 2 : 1; static constexpr bool scaled = TYPE != MI355_TYPE_F16; };
-
-static __device__ __forceinline__ float amax8(const float * v) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));      // (a NaN stays in the values)
-    return m;
-}
-static __device__ __forceinline__ int row_exp(float amax) { return amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0; }
-// 8 values times 2^-e -> one or two f16 parts
-template <int P> static __device__ __forceinline__ void to_parts(float * v, int e, v4i * out) {
+static __device__ __forceinline__ void to_parts(float * v, int e, v4i * out) {
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = ldexpf(v[i], -e);
-    if constexpr (P == 2) split8<false, 2>(v, out);
-    else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) out[0][i] = __builtin_bit_cast(int, h2{(_Float16)v[2 * i], (_Float16)v[2 * i + 1]});
-    }
+    split8<false, 2>(v, out);
 }
 
-// mask of a 32-slot tile for a row, as the accumulator lays it out: slot 8 q + 4 (lane / 32) + i
-static __device__ __forceinline__ void tile_mask(const MArgs & a, const char * mrow, bool m8, int j0, u2 (&w)[4]) {
+// cap log2(e) tanh(x), c2 = cap log2(e): tanh x = 1 - 2 / (e^2x + 1).  Off by some 2^-23 of the cap like the logit itself, and short: tanhf's two
+// branches, 16 times over, took the loop out of the instruction cache
+static __device__ __forceinline__ float capped_logit(float x, float c2) {
+    return __builtin_fmaf(-2.0f * c2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * x) + 1.0f), c2);
+}
+// logits (log2 domain) of a 32 x 32 tile from slot j0 on, in place of its products: sc what they lack, cl the tile's class for this lane's query
+static __device__ __forceinline__ void tile_logits(const MArgs & a, v16f & c, float sc, float slope, int cl, const char * mrow, bool m8, int j0) {
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
+    for (int i = 0; i < 16; i++) c[i] *= sc;
+    if (a.logit_softcap != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) c[i] = capped_logit(c[i], a.logit_softcap * LOG2E);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {                               // slot 8 q + 4 (lane / 32) + i
         const int j = j0 + 8 * q + 4 * ((threadIdx.x >> 5) & 1);
-        if (m8 && j + 4 <= a.n_kv) w[q] = *(const u2 *)(mrow + 2 * (int64_t)j);
+        u2 w;
+        if (cl != MASK_MIXED) w = u2{0u, 0u};
+        else if (m8 && j + 4 <= a.n_kv) w = *(const u2 *)(mrow + 2 * (int64_t)j);
         else {
             uint32_t y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = j + i >= a.n_kv ? 0xfc00u : a.mask ? ((const uint16_t *)mrow)[j + i] : 0u;
-            w[q] = u2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+            w = u2{y[0] | y[1] << 16, y[2] | y[3] << 16};
         }
-    }
-}
-// What a 32-slot tile of the mask is to a query: nothing visible, all of it zero, or anything else (the tile past the last slot too).  Looked up
-// by both passes and by every head that shares the mask, so that they read the mask itself only where it is neither (the diagonal of a prompt).
-enum { MASK_HIDDEN = 0, MASK_ZERO = 1, MASK_MIXED = 2 };
-__global__ void __launch_bounds__(PT)
-prompt_class_kernel(const MArgs a) {
-    const int lane = threadIdx.x & 63, iq = blockIdx.y * 4 + (threadIdx.x >> 6), plane = blockIdx.z;
-    if (iq >= a.n_q) return;
-    const char * mrow = a.mask + iq * a.m_nb1 + plane % a.m_ne2 * a.m_nb2 + plane / a.m_ne2 * a.m_nb3;
-    uint8_t * out = a.cls + ((int64_t)plane * a.n_q + iq) * a.cpitch;
-    const int j0 = blockIdx.x * 1024;
-    uint16_t v[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) { const int j = j0 + 64 * i + lane; v[i] = j < a.n_kv ? ((const uint16_t *)mrow)[j] : 0xfc00; }
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        if (j0 + 64 * i >= a.n_kv) break;
-        const uint64_t hid = __ballot(v[i] == 0xfc00), zero = __ballot((v[i] & 0x7fff) == 0);
-        if (lane < 2) {
-            const uint32_t h = (uint32_t)(hid >> (32 * lane)), z = (uint32_t)(zero >> (32 * lane));
-            out[(j0 + 64 * i) / 32 + lane] = h == 0xffffffffu ? MASK_HIDDEN : z == 0xffffffffu ? MASK_ZERO : MASK_MIXED;
+        for (int i = 0; i < 4; i++) {
+            const float mv = cl == MASK_HIDDEN ? -INFINITY : h2f((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+            c[4 * q + i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope, c[4 * q + i]);
         }
-    }
-}
-// classes of the N tiles from slot j0 on, a byte each (no mask: zero up to the last whole tile)
-template <int N> static __device__ __forceinline__ void tile_class(const MArgs & a, const uint8_t * crow, int j0, int (&c)[N]) {
-#pragma unroll
-    for (int u = 0; u < N; u++) {
-        const int j = j0 + 32 * u;
-        c[u] = j >= a.n_kv ? MASK_HIDDEN : a.mask ? crow[j / 32] : j + 32 <= a.n_kv ? MASK_ZERO : MASK_MIXED;
     }
 }
 static __device__ __forceinline__ const uint8_t * class_row(const MArgs & a, int iq, int h, int i3) {
+    if (!a.mask) return a.cls;
     const int plane = (a.m_ne3 > 1 ? i3 % a.m_ne3 : 0) * a.m_ne2 + (a.m_ne2 > 1 ? h % a.m_ne2 : 0);
     return a.cls + ((int64_t)plane * a.n_q + iq) * a.cpitch;
-}
-static __device__ __forceinline__ float mask_at(const u2 (&w)[4], int i) { return h2f((uint16_t)(w[i >> 2][(i & 3) >> 1] >> (16 * (i & 1)))); }
-
-// logits (log2 domain) of a 32 x 32 tile from slot j0 on: c holds the products, ks the slots' scales (accumulator layout), cl the tile's class
-// for this lane's query
-template <bool SCALED> static __device__ __forceinline__ void tile_logits(const MArgs & a, const v16f & c, const float * ks, float qe, float slope, int cl, const char * mrow,
-                                                                          bool m8, int j0, float * s) {
-#pragma unroll
-    for (int i = 0; i < 16; i++) s[i] = SCALED ? c[i] * ks[i] * qe : c[i] * qe;
-    if (a.logit_softcap != 0.0f) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = a.logit_softcap * LOG2E * tanhf(s[i]);
-    }
-    if (__all(cl == MASK_ZERO)) return;
-    if (__any(cl == MASK_MIXED)) {
-        u2 w[4];
-        tile_mask(a, mrow, m8, j0, w);
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float mv = mask_at(w, i);
-            s[i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope, s[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = cl == MASK_HIDDEN ? -INFINITY : s[i];
-    }
 }
 
 template <int TYPE, int D>
 __global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
 prompt_stats_kernel(const MArgs a) {
-    constexpr int KS = D / 16, KP = KForm<TYPE>::parts, RP = D * 2 + 16, CN = PA_SLOTS * (D / 8) / PT;
-    constexpr bool scaled = KForm<TYPE>::scaled;
-    __shared__ __attribute__((aligned(16))) uint8_t kt[2][KP][PA_SLOTS * RP];
-    __shared__ __attribute__((aligned(16))) float ksc[2][scaled ? PA_SLOTS : 4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
-    const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;
-    const int rt = blockIdx.x / a.nsplit * PA_ROWS, r_ = rt + wave * 32 + lr, r = r_ < R ? r_ : R - 1;
-    const int iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
+    typedef Fmt<TYPE> F;
+    constexpr int KS = D / 16, QP = F::parts, KP = F::quant ? 2 : 1, S = F::quant ? 2 : 3;      // S: tiles in LDS
+    constexpr int RS = PT / (D / 8), CN = PA_SLOTS / RS;        // rows a pass of the workgroup's chunks covers, passes of a tile
+    __shared__ __attribute__((aligned(16))) uint8_t kt[S][KP][PA_SLOTS * D * 2];
+    __shared__ __attribute__((aligned(16))) float ksc[F::quant ? S : 1][PA_SLOTS];
+    __shared__ uint32_t cl[S][PT / 64][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
+    const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;      // the last rows first: a causal mask lets them see most
+    const int rt = (int)(gridDim.x - 1 - blockIdx.x) / a.nsplit * PA_ROWS, r_ = rt + wave * 32 + lr, r = r_ < R ? r_ : R - 1;
+    const int iq = m_query(a, r), h = hk * a.ratio + r - iq * a.ratio;
     const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
     const char * mrow = m_mask(a, iq, h, i3);
+    const uint8_t * crow = class_row(a, iq, h, i3);
     const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
     const bool mine = rt + wave * 32 < R;
     const int64_t row = ((int64_t)i3 * a.n_head_kv + hk) * R + r;
-    const int nt = (a.n_kv + PA_SLOTS - 1) / PA_SLOTS;
+    const int nt = (a.n_kv + PA_SLOTS - 1) / PA_SLOTS, ns = a.nsplit;
 
-    KChunk<TYPE> kr[CN];
-    auto issue = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < CN; i++) {
-            const int c = PT * i + tid, j = t * PA_SLOTS + c / (D / 8), cc = c % (D / 8);
-            kr[i].load(kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1, cc < a.d / 8 ? cc : a.d / 8 - 1);
-        }
-    };
-    auto commit = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < CN; i++) {
-            const int c = PT * i + tid, j = c / (D / 8), cc = c % (D / 8), at = j * RP + cc * 16;
-            if constexpr (!scaled) *(v4i *)(kt[b][0] + at) = kr[i].raw;
-            else {
-                float v[8];
-                kr[i].values(cc < a.d / 8 ? cc : a.d / 8 - 1, v);
-                float m = amax8(v);
-#pragma unroll
-                for (int o = 1; o < D / 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-                const int e = row_exp(m);
-                v4i p[KP];
-                to_parts<KP>(v, e, p);
-#pragma unroll
-                for (int q = 0; q < KP; q++) *(v4i *)(kt[b][q] + at) = p[q];
-                if (cc == 0) ksc[b][j] = ldexpf(1.0f, e);
-            }
-        }
-    };
-    const uint8_t * crow = class_row(a, iq, h, i3);
-    int ca[2] = {0, 0}, cb[2] = {0, 0};
-    int t = split, b = 0;
-    if (t < nt) { issue(t); tile_class(a, crow, t * PA_SLOTS, ca); }
-    if (t + a.nsplit < nt) tile_class(a, crow, (t + a.nsplit) * PA_SLOTS, cb);
-    v4i qf[KS][2];
+    v4i qf[KS][QP];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-        for (int p = 0; p < 2; p++) qf[ks][p] = *(const v4i *)(a.qparts + (row * 2 + p) * D + 16 * ks + 8 * lh);
-    const float qe = a.rowc[row].qe, slope = a.rowc[row].slope;
+        for (int p = 0; p < QP; p++) qf[ks][p] = *(const v4i *)(a.qparts + (row * QP + p) * D + 16 * ks + 8 * lh);
+    float qe = a.rowc[row].qe, slope = a.rowc[row].slope;
+
+    // this lane's chunk of a pass: chunks past the head size re-read the last one and meet zeros of q, slots past the end the last one and are hidden
+    const int pos = tid % (D / 8), j_ = tid / (D / 8), c_ = F::quant ? pos : pos ^ (j_ & swz<D>()), cc = c_ < a.d / 8 ? c_ : a.d / 8 - 1;
+    KChunk<F::quant ? TYPE : (int)MI355_TYPE_Q8_0> kr[F::quant ? CN : 1];
+    uint64_t off[CN];                                           // of this lane's chunks in a tile
+#pragma unroll
+    for (int i = 0; i < CN; i++) off[i] = (uint64_t)(uint32_t)(j_ + RS * i) * a.k_nb1 + (F::quant ? 0 : cc * 16);
+    const uint32_t klds = lds_at(kt) + wave * 1024, clds = lds_at(cl) + wave * 256;
+    auto fetch = [&](int t, int b) {
+        const char * tile = kb + (uint64_t)((uint32_t)t * PA_SLOTS) * a.k_nb1;
+        const char * src[CN];
+        const int last = a.n_kv - 1 - t * PA_SLOTS;
+#pragma unroll
+        for (int i = 0; i < CN; i++) src[i] = tile + off[i];
+        if (last < PA_SLOTS - 1) {
+#pragma unroll
+            for (int i = 0; i < CN; i++) if (j_ + RS * i > last) src[i] = tile + (uint64_t)(uint32_t)last * a.k_nb1 + (F::quant ? 0 : cc * 16);
+        }
+        if constexpr (F::quant) {
+#pragma unroll
+            for (int i = 0; i < CN; i++) kr[i].load(src[i], cc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CN; i++) dma16(src[i], klds + b * (PA_SLOTS * D * 2) + i * (PT * 16));
+        }
+        dma4(crow + (t * 2 & ~3), clds + b * (int)sizeof(cl[0]));
+    };
+    auto commit = [&](int b) {
+        if constexpr (F::quant) {
+#pragma unroll
+            for (int i = 0; i < CN; i++) {
+                const int j = j_ + RS * i;
+                float v[8], m = kr[i].values(cc, v);
+#pragma unroll
+                for (int o = 1; o < D / 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+                const int e = row_exp(m);
+                v4i p[2];
+                to_parts(v, e, p);
+#pragma unroll
+                for (int q = 0; q < KP; q++) *(v4i *)(kt[b][q] + lds_chunk<D>(j, pos)) = p[q];
+                if (pos == 0) ksc[b][j] = ldexpf(1.0f, e);
+            }
+        }
+    };
+    int t = split, b = 0;
+    if (t < nt) { fetch(t, 0); commit(0); }
+    if (S == 3 && t + ns < nt) fetch(t + ns, 1);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int p = 0; p < QP; p++) arrived(qf[ks][p]);
+    arrived(qe); arrived(slope);
     float m = -INFINITY, l = 0.0f;               // of this lane's row over this lane's slots (two lanes share a row)
-    bool any = mine && (ca[0] | ca[1]) != MASK_HIDDEN;
-    if (t < nt) commit(0);                       // the first tile is fetched without asking
-    bool live = __syncthreads_or(any);
-    while (t < nt) {
-        const int tn = t + a.nsplit;
-        const bool anyn = tn < nt && mine && (cb[0] | cb[1]) != MASK_HIDDEN;
-        const bool liven = __syncthreads_or(anyn);           // (the tile in buffer b is complete, the other one has been read)
-        if (liven) issue(tn);
-        if (live && __any(any)) {
-            float s[2][16];
+    for (; t < nt; t += ns) {
+        if (S == 2 || t + ns >= nt) wait_meet<0>();
+        else wait_meet<CN + 1>();
+        // tile t is there, and the place of the one before it is free
+        const int ahead = t + (S - 1) * ns, bf = b == 0 ? S - 1 : b - 1;
+        if (ahead < nt) fetch(ahead, bf);
+        const uint32_t bytes = cl[b][wave][lane] >> (16 * (t & 1));
+        const int c0 = bytes & 255, c1 = bytes >> 8 & 255;
+        if (mine && __any((c0 | c1) != MASK_HIDDEN)) {
+            v16f c[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                v16f c;
 #pragma unroll
-                for (int i = 0; i < 16; i++) c[i] = 0.0f;
+                for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
-                    const int at = (32 * u + lr) * RP + ks * 32 + lh * 16;
+                    const int at = lds_chunk<D>(32 * u + lr, 2 * ks + lh);
                     const v4i k0 = *(const v4i *)(kt[b][0] + at);
-                    if constexpr (KP == 2) c = mfma32(*(const v4i *)(kt[b][KP - 1] + at), qf[ks][0], c);
-                    c = mfma32(k0, qf[ks][1], c);
-                    c = mfma32(k0, qf[ks][0], c);
-                }
-                float kv[16];
-                if constexpr (scaled) {
+                    if constexpr (KP == 2) c[u] = mfma32<F::bf>(*(const v4i *)(kt[b][KP - 1] + at), qf[ks][0], c[u]);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) { const v4f x = *(const v4f *)&ksc[b][32 * u + 8 * q + 4 * lh]; for (int i = 0; i < 4; i++) kv[4 * q + i] = x[i]; }
+                    for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(k0, qf[ks][p], c[u]);
                 }
-                tile_logits<scaled>(a, c, kv, qe, slope, ca[u], mrow, m8, t * PA_SLOTS + 32 * u, s[u]);
+                if constexpr (F::quant) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const v4f x = *(const v4f *)&ksc[b][32 * u + 8 * q + 4 * lh];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) c[u][4 * q + i] *= x[i];
+                    }
+                }
             }
-            float mx = m;
+            float sc = qe;
+            if (a.logit_softcap != 0.0f || !__all(c0 == MASK_ZERO && c1 == MASK_ZERO)) {
+                tile_logits(a, c[0], qe, slope, c0, mrow, m8, t * PA_SLOTS);
+                tile_logits(a, c[1], qe, slope, c1, mrow, m8, t * PA_SLOTS + 32);
+                sc = 1.0f;
+            }
+            float mx = c[0][0];
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[u][i]);
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, c[u][i]);
+            mx = fmaxf(m, mx * sc);
             const float ms = mx == -INFINITY ? 0.0f : mx;
             l *= __builtin_amdgcn_exp2f(m - ms);
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) l += __builtin_amdgcn_exp2f(s[u][i] - ms);
+                for (int i = 0; i < 16; i++) l += __builtin_amdgcn_exp2f(__builtin_fmaf(c[u][i], sc, -ms));
             m = mx;
         }
-        if (liven) commit(b ^ 1);
-        ca[0] = cb[0]; ca[1] = cb[1];
-        if (tn + a.nsplit < nt) tile_class(a, crow, (tn + a.nsplit) * PA_SLOTS, cb);
-        any = anyn; live = liven; t = tn; b ^= 1;
+        if (S == 2 && ahead < nt) commit(bf);
+        b = b == S - 1 ? 0 : b + 1;
     }
     const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
     const float M = fmaxf(m, mo), ms = M == -INFINITY ? 0.0f : M;
@@ -1103,123 +1135,111 @@ prompt_rows_kernel(const MArgs a) {
     const int64_t hrow = (int64_t)i3 * a.n_head_kv + hk;
     const v2f * st = (const v2f *)a.stats + hrow * a.nsplit * R + r;
     float M = -INFINITY, L = 0.0f;
-    for (int s = 0; s < a.nsplit; s += 4) {
-        v2f x[4];
+    for (int s = 0; s < a.nsplit; s += 8) {
+        v2f x[8];
+        float mn = M;
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = s + i < a.nsplit ? st[(int64_t)(s + i) * R] : v2f{-INFINITY, 0.0f};
-        const float mn = fmaxf(fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)), M), ms = mn == -INFINITY ? 0.0f : mn;
+        for (int i = 0; i < 8; i++) { x[i] = s + i < a.nsplit ? st[(int64_t)(s + i) * R] : v2f{-INFINITY, 0.0f}; mn = fmaxf(mn, x[i].x); }
+        const float ms = mn == -INFINITY ? 0.0f : mn;
         L *= __builtin_amdgcn_exp2f(M - ms);
 #pragma unroll
-        for (int i = 0; i < 4; i++) L = __builtin_fmaf(x[i].y, __builtin_amdgcn_exp2f(x[i].x - ms), L);
+        for (int i = 0; i < 8; i++) L = __builtin_fmaf(x[i].y, __builtin_amdgcn_exp2f(x[i].x - ms), L);
         M = mn;
     }
     *(v2f *)&a.rowc[hrow * R + r].m = v2f{M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L};
 }
 
-// NS: 32-slot tiles of a wave
-template <int TYPE, int D, int NS>
-__global__ void __launch_bounds__(PT, D <= 128 && NS * KForm<TYPE>::parts <= 2 ? 2 : 1)
+// slots of a wave in the second pass: 64 where its K takes at most 64 registers so
+template <int TYPE, int D> constexpr int prompt_ns() { return D * (Fmt<TYPE>::quant ? 2 : 1) <= 128 ? 2 : 1; }
+
+template <int TYPE, int D>
+__global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
 prompt_mass_kernel(const MArgs a) {
-    constexpr int KS = D / 16, KP = KForm<TYPE>::parts, RP = D * 2 + 16, CN = PB_ROWS * 2 * (D / 8) / PT;
-    constexpr bool scaled = KForm<TYPE>::scaled;
-    __shared__ __attribute__((aligned(16))) uint8_t qt[2][2][PB_ROWS * RP];
-    __shared__ RowC rc[2][PB_ROWS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 31, lh = lane >> 5;
+    typedef Fmt<TYPE> F;
+    constexpr int NS = prompt_ns<TYPE, D>();
+    constexpr int KS = D / 16, QP = F::parts, KP = F::quant ? 2 : 1, S = D <= 128 ? 3 : 2;      // S: tiles in LDS
+    constexpr int RS = PT / (D / 8), CP = PB_ROWS / RS, CN = QP * CP;       // passes of a part, of a tile
+    __shared__ __attribute__((aligned(16))) uint8_t qt[S][QP][PB_ROWS * D * 2];
+    __shared__ __attribute__((aligned(16))) float rc[S][PT / 64][64];       // RowC of the rows, twice
+    __shared__ uint32_t cl[S][PT / 64][64];
+    __shared__ __attribute__((aligned(16))) float ksc[F::quant ? 128 * NS : 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
     const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, chunk = blockIdx.x % a.nchunk;
-    const int j0 = (blockIdx.x / a.nchunk * 4 + wave) * 32 * NS;         // this wave's slots
+    const int j0 = (blockIdx.x / a.nchunk * 4 + wave) * 32 * NS;            // this wave's slots
     const int64_t base = ((int64_t)i3 * a.n_head_kv + hk) * R;
-    const int nt = (R + PB_ROWS - 1) / PB_ROWS;
+    const int nt = (R + PB_ROWS - 1) / PB_ROWS, nc = a.nchunk;
     const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
+    const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
 
-    v4i qr[CN];
-    RowC rr = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto issue = [&](int t) {
+    const int pos = tid % (D / 8), x_ = tid / (D / 8), cc = pos ^ (x_ & swz<D>());
+    const uint32_t qoff = (uint32_t)(x_ * QP * D + cc * 8) * 2, qlds = lds_at(qt) + wave * 1024, rlds = lds_at(rc) + wave * 256, clds = lds_at(cl) + wave * 256;
+    auto fetch = [&](int t, int b) {                            // rows past the last one repeat it
+        const int last = R - 1 - t * PB_ROWS;
+        const char * tile = (const char *)a.qparts + (base + t * PB_ROWS) * (QP * D * 2), * rows = (const char *)(a.rowc + base + t * PB_ROWS);
+        uint32_t o[CP], ro = 4 * (tid & 127);
+        int r = t * PB_ROWS + lr;
 #pragma unroll
-        for (int i = 0; i < CN; i++) {
-            const int c = PT * i + tid, x = c / (D / 8), row = t * PB_ROWS + (x >> 1);      // x: (row, part)
-            qr[i] = *(const v4i *)(a.qparts + ((base + (row < R ? row : R - 1)) * 2 + (x & 1)) * D + c % (D / 8) * 8);
-        }
-        if (tid < PB_ROWS) {                                    // rows past the last one weigh nothing
-            const int row = t * PB_ROWS + tid;
-            rr = row < R ? a.rowc[base + row] : RowC{0.0f, 0.0f, INFINITY, 0.0f};
-        }
-    };
-    auto commit = [&](int b) {
+        for (int i = 0; i < CP; i++) o[i] = qoff + RS * i * QP * D * 2;
+        if (last < PB_ROWS - 1) {
 #pragma unroll
-        for (int i = 0; i < CN; i++) {
-            const int c = PT * i + tid, x = c / (D / 8);
-            *(v4i *)(qt[b][x & 1] + (x >> 1) * RP + c % (D / 8) * 16) = qr[i];
+            for (int i = 0; i < CP; i++) if (x_ + RS * i > last) o[i] = (uint32_t)(last * QP * D + cc * 8) * 2;
+            if ((tid & 127) / 4 > last) ro = 16 * last + 4 * (tid & 3);
+            if (lr > last) r = R - 1;
         }
-        if (tid < PB_ROWS) rc[b][tid] = rr;
+#pragma unroll
+        for (int i = 0; i < CN; i++) dma16(tile + o[i % CP] + i / CP * (D * 2), qlds + b * (int)sizeof(qt[0]) + i * (PT * 16));
+        dma4(rows + ro, rlds + b * (int)sizeof(rc[0]));
+        const int iq = m_query(a, r);
+        dma4(class_row(a, iq, hk * a.ratio + r - iq * a.ratio, i3) + (j0 / 32 & ~3), clds + b * (int)sizeof(cl[0]));
     };
-    int ca[NS], cb[NS];
-    auto classes = [&](int t, int (&c)[NS]) {
-        const int r = t * PB_ROWS + lr < R ? t * PB_ROWS + lr : R - 1, iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
-        tile_class(a, class_row(a, iq, h, i3), j0, c);
-    };
-    auto sees = [&](const int (&c)[NS]) { int any = 0; for (int u = 0; u < NS; u++) any |= c[u]; return any != MASK_HIDDEN; };
+    int t = chunk, b = 0;
+    if (t < nt) fetch(t, 0);
+    if (S == 3 && t + nc < nt) fetch(t + nc, 1);
 
-    // this wave's K rows, as the A operand holds them, the largest finite value brought to [2^14, 2^15)
+    // this wave's K rows, as the A operand holds them
     v4i kf[NS][KS][KP];
-    float kscale = 1.0f;
-    {
-        const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
 #pragma unroll
-        for (int u = 0; u < NS; u++) {
-            const int j = j0 + 32 * u + lr;
-            const char * row = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
-            if constexpr (!scaled) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) { const int cc = 2 * ks + lh; kf[u][ks][0] = *(const v4i *)(row + (cc < a.d / 8 ? cc : a.d / 8 - 1) * 16); }
-            }
-        }
-        if constexpr (scaled) {
+    for (int u = 0; u < NS; u++) {
+        const int j = j0 + 32 * u + lr;
+        const char * krow = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
+        auto chunk_at = [&](int ks) { return 2 * ks + lh < a.d / 8 ? 2 * ks + lh : a.d / 8 - 1; };
+        if constexpr (F::quant) {
             float m = 0.0f;
-            auto each = [&](auto f) {
 #pragma unroll
-                for (int u = 0; u < NS; u++) {
-                    const int j = j0 + 32 * u + lr;
-                    const char * row = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        const int cc = 2 * ks + lh < a.d / 8 ? 2 * ks + lh : a.d / 8 - 1;
-                        KChunk<TYPE> c;
-                        c.load(row, cc);
-                        float v[8];
-                        c.values(cc, v);
-                        f(u, ks, v);
-                    }
-                }
-            };
-            each([&](int, int, float * v) { const float x = amax8(v); if (x < INFINITY) m = fmaxf(m, x); });
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            for (int ks = 0; ks < KS; ks++) { KChunk<TYPE> c; float v[8]; c.load(krow, chunk_at(ks)); m = fmaxf(m, c.values(chunk_at(ks), v)); }
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
             const int e = row_exp(m);
-            kscale = ldexpf(1.0f, e);
-            each([&](int u, int ks, float * v) { to_parts<KP>(v, e, kf[u][ks]); });
+            ksc[(wave * NS + u) * 32 + lr] = ldexpf(1.0f, e);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) { KChunk<TYPE> c; float v[8]; c.load(krow, chunk_at(ks)); c.values(chunk_at(ks), v); to_parts(v, e, kf[u][ks]); }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) kf[u][ks][0] = *(const v4i *)(krow + chunk_at(ks) * 16);
         }
     }
+#pragma unroll
+    for (int u = 0; u < NS; u++)
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) arrived(kf[u][ks][0]);
     float acc[NS][16];
 #pragma unroll
     for (int u = 0; u < NS; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[u][i] = 0.0f;
 
-    int t = chunk, b = 0;
-    for (int u = 0; u < NS; u++) ca[u] = cb[u] = 0;
-    if (t < nt) { issue(t); classes(t, ca); commit(0); }
-    if (t + a.nchunk < nt) classes(t + a.nchunk, cb);
-    bool any = t < nt && sees(ca);
-    bool live = __syncthreads_or(any);
-    while (t < nt) {
-        const int tn = t + a.nchunk;
-        const bool anyn = tn < nt && sees(cb);
-        const bool liven = __syncthreads_or(anyn);
-        if (liven) issue(tn);
-        if (live && __any(any)) {
-            const RowC c4 = rc[b][lr];
-            const int r = t * PB_ROWS + lr < R ? t * PB_ROWS + lr : R - 1, iq = r / a.ratio, h = hk * a.ratio + r - iq * a.ratio;
-            const char * mrow = m_mask(a, iq, h, i3);
+    for (; t < nt; t += nc) {
+        if (S == 2 || t + nc >= nt) wait_meet<0>();
+        else wait_meet<CN + 2>();
+        const int ahead = t + (S - 1) * nc;
+        if (ahead < nt) fetch(ahead, b == 0 ? S - 1 : b - 1);
+        const uint32_t bytes = cl[b][wave][lane] >> (8 * (j0 / 32 & 3));
+        int cu[NS], seen = MASK_HIDDEN;
+        bool zero = a.logit_softcap == 0.0f;
+#pragma unroll
+        for (int u = 0; u < NS; u++) { cu[u] = bytes >> (8 * u) & 255; seen |= cu[u]; zero &= cu[u] == MASK_ZERO; }
+        if (__any(seen != MASK_HIDDEN)) {
+            RowC c4 = *(const RowC *)&rc[b][0][4 * lr];
+            if (t * PB_ROWS + lr >= R) { c4.m = INFINITY; c4.inv = 0.0f; }      // weighs nothing
             v16f c[NS];
 #pragma unroll
             for (int u = 0; u < NS; u++)
@@ -1227,29 +1247,43 @@ prompt_mass_kernel(const MArgs a) {
                 for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const v4i q0 = *(const v4i *)(qt[b][0] + lr * RP + ks * 32 + lh * 16), q1 = *(const v4i *)(qt[b][1] + lr * RP + ks * 32 + lh * 16);
+                v4i q[QP];
 #pragma unroll
-                for (int u = 0; u < NS; u++) {
-                    if constexpr (KP == 2) c[u] = mfma32(kf[u][ks][KP - 1], q0, c[u]);
-                    c[u] = mfma32(kf[u][ks][0], q1, c[u]);
-                    c[u] = mfma32(kf[u][ks][0], q0, c[u]);
-                }
+                for (int p = 0; p < QP; p++) q[p] = *(const v4i *)(qt[b][p] + lds_chunk<D>(lr, 2 * ks + lh));
+#pragma unroll
+                for (int p = QP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int u = 0; u < NS; u++) {
+                        if constexpr (KP == 2) if (p == 0) c[u] = mfma32<F::bf>(kf[u][ks][KP - 1], q[0], c[u]);
+                        c[u] = mfma32<F::bf>(kf[u][ks][0], q[p], c[u]);
+                    }
+            }
+            if constexpr (F::quant) {
+#pragma unroll
+                for (int u = 0; u < NS; u++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const v4f x = *(const v4f *)&ksc[(wave * NS + u) * 32 + 8 * q + 4 * lh];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) c[u][4 * q + i] *= x[i];
+                    }
+            }
+            float sc = c4.qe;
+            if (!__all(zero)) {
+                const int r = t * PB_ROWS + lr < R ? t * PB_ROWS + lr : R - 1, iq = m_query(a, r);
+                const char * mrow = m_mask(a, iq, hk * a.ratio + r - iq * a.ratio, i3);
+#pragma unroll
+                for (int u = 0; u < NS; u++) tile_logits(a, c[u], sc, c4.slope, cu[u], mrow, m8, j0 + 32 * u);
+                sc = 1.0f;
             }
 #pragma unroll
-            for (int u = 0; u < NS; u++) {
-                float s[16];
-                tile_logits<false>(a, c[u], nullptr, c4.qe * kscale, c4.slope, ca[u], mrow, m8, j0 + 32 * u, s);
+            for (int u = 0; u < NS; u++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) acc[u][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[i] - c4.m), c4.inv, acc[u][i]);
-            }
+                for (int i = 0; i < 16; i++) acc[u][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(c[u][i], sc, -c4.m)), c4.inv, acc[u][i]);
         }
-        if (liven) commit(b ^ 1);
-#pragma unroll
-        for (int u = 0; u < NS; u++) ca[u] = cb[u];
-        if (tn + a.nchunk < nt) classes(tn + a.nchunk, cb);
-        any = anyn; live = liven; t = tn; b ^= 1;
+        b = b == S - 1 ? 0 : b + 1;
     }
-    // over the 32 lanes (rows) of each half: 16 sums per tile
+    // over the 32 lanes (rows) of each half: 16 sums per tile.  One chunk: its sums are the weights
 #pragma unroll
     for (int u = 0; u < NS; u++)
 #pragma unroll
@@ -1258,7 +1292,9 @@ prompt_mass_kernel(const MArgs a) {
             x += dpp_f32<0xB1>(x); x += dpp_f32<0x4E>(x); x += dpp_f32<0x141>(x); x += dpp_f32<0x140>(x);
             x += __shfl_xor(x, 16, 64);
             const int j = j0 + 32 * u + 8 * (i >> 2) + 4 * lh + (i & 3);
-            if (lr == 0 && j < a.n_kv) a.part[(((int64_t)i3 * a.n_head_kv + hk) * a.nchunk + chunk) * a.n_kv + j] = x;
+            if (lr != 0 || j >= a.n_kv) continue;
+            if (nc > 1) a.part[(((int64_t)i3 * a.n_head_kv + hk) * nc + chunk) * a.n_kv + j] = x;
+            else mass_store(a, hk, i3, j, x);
         }
 }
 
@@ -1270,28 +1306,26 @@ prompt_sum_kernel(const MArgs a) {
     float t = 0.0f;
 #pragma unroll 8
     for (int c = 0; c < a.nchunk; c++) t += p[(int64_t)c * a.n_kv];
-    if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
-    ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
+    mass_store(a, hk, i3, j, t);
 }
 
-// slots of a wave in the second pass: 64 where its K fits 128 registers
-template <int TYPE, int D> constexpr int prompt_ns() { return D * KForm<TYPE>::parts <= 128 ? 2 : 1; }
 static int prompt_slots(int type, int64_t d) {           // slots of a workgroup in the second pass
-    const int parts = type == MI355_TYPE_Q8_0 || type == MI355_TYPE_Q4_0 ? 2 : 1;
-    return step_d(d) * parts <= 128 ? 256 : 128;
+    return step_d(d) * (type == MI355_TYPE_Q8_0 || type == MI355_TYPE_Q4_0 ? 2 : 1) <= 128 ? 256 : 128;
 }
-// both passes get about 2048 workgroups (4 rounds of two per CU: causal prompts have long and short ones) where there is work for them
+// Slices of the slots in the first pass: 1024 workgroups, two rounds of two a CU, so that the short and the long rows of a causal prompt even out
+// (2047 x 2047: 82 us, with 512 83, with 2048 86), four tiles a workgroup or more, and few slices to join (64: 8 us, 32: 5)
 static int64_t prompt_splits(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (p->n_kv + PA_SLOTS - 1) / PA_SLOTS, base = (R + PA_ROWS - 1) / PA_ROWS * p->n_head_kv * p->ne3;
-    int64_t n = 2048 / base, most = (tiles + 3) / 4;
+    int64_t n = 1024 / base, most = (tiles + 3) / 4;
     if (n > most) n = most;
-    if (n > 64) n = 64;
+    if (n > 32) n = 32;
     return n < 1 ? 1 : n;
 }
+// Slices of the rows in the second: 512 workgroups, one round (2047 x 2047: 97 us, with 1024 93, with 256 129; 64 x 16384: 33, with 1024 39)
 static int64_t prompt_chunks(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (R + PB_ROWS - 1) / PB_ROWS;
     const int64_t ws = prompt_slots(p->type_k, p->d), base = (p->n_kv + ws - 1) / ws * p->n_head_kv * p->ne3;
-    int64_t n = base > 0 ? 2048 / base : 1, most = (tiles + 3) / 4;
+    int64_t n = base > 0 ? 512 / base : 1, most = (tiles + 3) / 4;
     if (n > most) n = most;
     if (n > 64) n = 64;
     return n < 1 ? 1 : n;
@@ -1300,18 +1334,19 @@ static int64_t prompt_chunks(const mi355_fattn_args * p) {
 template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hipStream_t s) {
     const int R = a.ratio * a.n_q, ws = 128 * prompt_ns<TYPE, D>();
     const unsigned hk = (unsigned)a.n_head_kv, z = (unsigned)ne3;
-    if (a.mask) {
-        MI355_LAUNCH("attn_mass_class", prompt_class_kernel, dim3((unsigned)((a.n_kv + 1023) / 1024), (unsigned)((a.n_q + 3) / 4), (unsigned)(a.m_ne2 * a.m_ne3)), dim3(PT), 0, s, a);
-        MI355_CHECK_LAUNCH();
-    }
-    MI355_LAUNCH("attn_mass_q", prompt_q_kernel<D>, dim3((unsigned)((R + 15) / 16), hk, z), dim3(PT), 0, s, a);
+    const int64_t slot_wgs = (a.n_kv + 1023) / 1024, query_wgs = a.mask ? (a.n_q + 3) / 4 : 1, class_wgs = slot_wgs * query_wgs * a.m_ne2 * a.m_ne3;
+    const int64_t row_wgs = (R + 15) / 16, prep = class_wgs + row_wgs * hk * z;
+    if (prep > 0x7fffffff) return MI355_E_SHAPE;
+    MI355_LAUNCH("attn_mass_prep", (prompt_prep_kernel<D, Fmt<TYPE>::bf>), dim3((unsigned)prep), dim3(PT), 0, s, a, (uint32_t)class_wgs, (uint32_t)slot_wgs,
+                 (uint32_t)query_wgs, (uint32_t)row_wgs);
     MI355_CHECK_LAUNCH();
     MI355_LAUNCH("attn_mass_stats", (prompt_stats_kernel<TYPE, D>), dim3((unsigned)((R + PA_ROWS - 1) / PA_ROWS * a.nsplit), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
     MI355_LAUNCH("attn_mass_rows", prompt_rows_kernel, dim3((unsigned)((R + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
-    MI355_LAUNCH("attn_mass", (prompt_mass_kernel<TYPE, D, prompt_ns<TYPE, D>()>), dim3((unsigned)((a.n_kv + ws - 1) / ws * a.nchunk), hk, z), dim3(PT), 0, s, a);
+    MI355_LAUNCH("attn_mass", (prompt_mass_kernel<TYPE, D>), dim3((unsigned)((a.n_kv + ws - 1) / ws * a.nchunk), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
+    if (a.nchunk == 1) return MI355_OK;
     MI355_LAUNCH("attn_mass_sum", prompt_sum_kernel, dim3((unsigned)((a.n_kv + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
     return MI355_OK;
@@ -1327,6 +1362,7 @@ template <int TYPE> static int prompt_dispatch(const MArgs & a, int ne3, hipStre
 
 // steps: [statistics][partial rows of dst][logits]; prompts: [statistics][sums of the row chunks][row constants][parts of q][classes of the mask] (in floats)
 struct WsParts { int64_t nsplit, nchunk, lpitch, stats, part, logits, rowc, q, cls; };
+static int64_t class_pitch(int64_t n_kv) { return (n_kv + 511) / 512 * 16; }    // a byte per tile, whole workgroups of either pass
 static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     const int64_t rows = p->ne3 * p->n_head * p->n_q;
     WsParts w = {1, 1, 0, 0, 0, 0, 0, 0, 0};
@@ -1336,8 +1372,8 @@ static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
         w.stats = (w.nsplit * rows * 2 + 3) / 4 * 4;
         w.part = (p->ne3 * p->n_head_kv * w.nchunk * p->n_kv + 3) / 4 * 4;
         w.rowc = rows * 4;
-        w.q = rows * step_d(p->d);                  // two f16 rows
-        if (p->mask) w.cls = (p->m_ne2 * p->m_ne3 * p->n_q * ((p->n_kv + 63) / 64 * 2) + 3) / 4;
+        w.q = rows * step_d(p->d) / 2 * (p->type_k == MI355_TYPE_BF16 ? 3 : 2);
+        w.cls = (p->mask ? p->m_ne2 * p->m_ne3 * p->n_q : 1) * class_pitch(p->n_kv) / 4;
     } else {
         w.nsplit = step_splits(p);
         w.lpitch = (p->n_kv + 3) / 4 * 4;
@@ -1364,8 +1400,10 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     if (quant && (p->d % 32 != 0 || (with_dst && dv % 32 != 0))) return MI355_E_SHAPE;
     if (p->n_head < 1 || p->n_head > 65535 || p->n_head_kv < 1 || p->n_head % p->n_head_kv != 0 || p->n_q < 1 || p->n_q > 65535 || p->n_kv < 0 ||
         p->n_kv > (1 << 30) || p->ne3 < 1 || p->ne3 > 65535) return MI355_E_SHAPE;
+    const int64_t ratio = p->n_head / p->n_head_kv;
+    if (ratio * ratio * p->n_q > 0xffffffffll) return MI355_E_SHAPE;
     if (with_dst && p->n_q > MI355_MASS_MAX_Q) return MI355_E_UNSUPPORTED;
-    if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1 || p->m_ne2 * p->m_ne3 > 65535 || p->m_ne2 > 65535 || p->m_ne3 > 65535)) return MI355_E_SHAPE;
+    if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1 || p->m_ne2 > 65535 || p->m_ne3 > 65535 || p->m_ne2 * p->m_ne3 > 65535)) return MI355_E_SHAPE;
     if (p->k_nb1 < 0 || p->k_nb1 > 0x7fffffff || (with_dst && (p->v_nb1 < 0 || p->v_nb1 > 0x7fffffff))) return MI355_E_SHAPE;
     const int64_t f32s = (int64_t)(uintptr_t)p->q | p->q_nb1 | p->q_nb2 | p->q_nb3 |
                          (with_dst ? (int64_t)(uintptr_t)p->dst | p->d_nb1 | p->d_nb2 | p->d_nb3 : 0) | (int64_t)(uintptr_t)workspace;
@@ -1381,8 +1419,8 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     a.q = (const char *)p->q; a.q_nb1 = p->q_nb1; a.q_nb2 = p->q_nb2; a.q_nb3 = p->q_nb3;
     a.k = (const char *)p->k; a.k_nb1 = (uint32_t)p->k_nb1; a.k_nb2 = p->k_nb2; a.k_nb3 = p->k_nb3;
     a.v = (const char *)p->v; a.v_nb1 = (uint32_t)p->v_nb1; a.v_nb2 = p->v_nb2; a.v_nb3 = p->v_nb3;
-    a.mask = (const char *)p->mask; a.m_nb1 = p->m_nb1; a.m_nb2 = p->m_nb2; a.m_nb3 = p->m_nb3; a.m_ne2 = (int)p->m_ne2; a.m_ne3 = (int)p->m_ne3;
-    a.ratio = (int)(p->n_head / p->n_head_kv); a.by_ratio = a.ratio > 1 ? (uint32_t)(((1ull << 32) + a.ratio - 1) / a.ratio) : 0;
+    a.mask = (const char *)p->mask; a.m_nb1 = p->m_nb1; a.m_nb2 = p->m_nb2; a.m_nb3 = p->m_nb3; a.m_ne2 = p->mask ? (int)p->m_ne2 : 1; a.m_ne3 = p->mask ? (int)p->m_ne3 : 1;
+    a.ratio = (int)ratio; a.by_ratio = a.ratio > 1 ? (uint32_t)(((1ull << 32) + a.ratio - 1) / a.ratio) : 0;
     a.dst = with_dst ? (char *)p->dst : nullptr; a.d_nb1 = p->d_nb1; a.d_nb2 = p->d_nb2; a.d_nb3 = p->d_nb3;
     a.mass_in = w->decay != 0.0f ? (const char *)w->mass_in : nullptr; a.in_nb2 = w->in_nb2; a.in_nb3 = w->in_nb3;
     a.mass_out = (char *)w->mass_out; a.out_nb2 = w->out_nb2; a.out_nb3 = w->out_nb3;
@@ -1398,7 +1436,7 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     a.logits = a.part + parts.part;
     a.rowc = (RowC *)(a.logits + parts.logits);
     a.qparts = (uint16_t *)(a.logits + parts.logits + parts.rowc);
-    a.cls = (uint8_t *)(a.logits + parts.logits + parts.rowc + parts.q); a.cpitch = (int)((p->n_kv + 63) / 64 * 2);
+    a.cls = (uint8_t *)(a.logits + parts.logits + parts.rowc + parts.q); a.cpitch = (int)class_pitch(p->n_kv);
     hipStream_t s = (hipStream_t)stream;
     if (p->n_q <= MI355_MASS_MAX_Q) switch (p->type_k) {
         case MI355_TYPE_F16:  return with_dst ? step_dispatch<MI355_TYPE_F16, true>(a, (int)p->ne3, s) : step_dispatch<MI355_TYPE_F16, false>(a, (int)p->ne3, s);
