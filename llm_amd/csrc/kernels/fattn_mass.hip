@@ -9,6 +9,8 @@
 
 namespace {
 
+constexpr float LOG2E = 1.4426950408889634f;
+
 struct RowC { float qe, slope, m, inv; };      // per row: power of two of q, ALiBi slope (log2 domain), maximum, 1 / sum
 
 struct MArgs {
@@ -32,13 +34,10 @@ struct MArgs {
     uint16_t * qparts;  // prompts: [ne3][n_head_kv][rows][parts][D]
 };
 
+// value e of a row of f16 or bf16
 template <int TYPE> static __device__ __forceinline__ float kv_value(const char * row, int e) {
-    if (TYPE == MI355_TYPE_F16) return h2f(((const uint16_t *)row)[e]);
-    if (TYPE == MI355_TYPE_BF16) return __uint_as_float((uint32_t)((const uint16_t *)row)[e] << 16);
-    if (TYPE == MI355_TYPE_Q8_0) { const char * b = row + (e >> 5) * 34; return h2f(*(const uint16_t *)b) * (float)((const int8_t *)(b + 2))[e & 31]; }
-    const char * b = row + (e >> 5) * 18;
-    const int n = ((const uint8_t *)(b + 2))[e & 15] >> ((e & 16) ? 4 : 0) & 15;
-    return h2f(*(const uint16_t *)b) * (float)(n - 8);
+    const uint16_t y = ((const uint16_t *)row)[e];
+    return TYPE == MI355_TYPE_F16 ? h2f(y) : __uint_as_float((uint32_t)y << 16);
 }
 
 // row r of a KV head = (query, head of the group); r * ratio < 2^32
@@ -50,6 +49,11 @@ static __device__ __forceinline__ const char * m_mask(const MArgs & a, int iq, i
 static __device__ __forceinline__ void mass_store(const MArgs & a, int hk, int i3, int j, float t) {
     if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
     ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
+}
+// cap log2(e) tanh(x), c2 = cap log2(e): tanh x = 1 - 2 / (e^2x + 1).  Off by some 2^-23 of the cap like the logit itself, and short: tanhf's two
+// branches, 16 times over, took the loop out of the instruction cache
+static __device__ __forceinline__ float capped_logit(float x, float c2) {
+    return __builtin_fmaf(-2.0f * c2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * x) + 1.0f), c2);
 }
 // exponent that brings a row's largest value to [2^14, 2^15)
 static __device__ __forceinline__ int row_exp(float amax) { return amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0; }
@@ -72,8 +76,6 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
-
-constexpr float LOG2E = 1.4426950408889634f;
 
 template <int TYPE> struct Fmt {       // 16-bit format of the operands and the parts an f32 is split into
     static constexpr bool bf = TYPE == MI355_TYPE_BF16, quant = TYPE == MI355_TYPE_Q8_0 || TYPE == MI355_TYPE_Q4_0;
@@ -181,14 +183,14 @@ static __device__ __forceinline__ float sum_groups(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-// RT: 16-row tiles of a workgroup.  RP (blocks only): the 16 columns of a tile are RP rows times 16 / RP classes of 32-blocks -- at GQA 4 or 8
+// RP (blocks only): the 16 columns of a tile are RP rows times 16 / RP classes of 32-blocks -- at GQA 4 or 8
 // the columns that would repeat a row each scale P by the blocks of their class, so a lane forms D / 32 / (16 / RP) scaled copies of P and not
 // D / 32; a feature tile takes its result from the columns of its block's class.
 // RAW (blocks only, step_raw): rows come in as consecutive pieces of D / 16 bytes (17 or 9 a row) and are taken apart in LDS.  A lane that loads
 // the 8 bytes of its own chunk reads at every second byte address, which the address unit serves a lane per clock: the 20 loads of a
 // tile then cost a CU's 8 waves 4 us before the first product.
-template <int TYPE, int D, int NW, bool HASV, int RT, int RP, bool RAW>
-__global__ void __launch_bounds__(NW * 64, D <= 64 ? (RT == 1 ? 3 : 2) : D <= 128 ? 2 : 1)
+template <int TYPE, int D, int NW, bool HASV, int RP, bool RAW>
+__global__ void __launch_bounds__(NW * 64, D <= 64 ? 3 : D <= 128 ? 2 : 1)
 mass_step_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
     static_assert(!RAW || F::quant, "raw rows are block rows");
@@ -203,29 +205,22 @@ mass_step_kernel(const MArgs a) {
     typedef uint32_t piece_t __attribute__((ext_vector_type(PB / 4)));
     typedef _Float16 hk_t __attribute__((ext_vector_type(KS)));
     __shared__ __attribute__((aligned(16))) uint8_t lds[NW][VB];
-    __shared__ v4i qs[RT][KS][P][64];
+    __shared__ v4i qs[KS][P][64];
     uint8_t (&raw)[NW][VB] = lds;                               // RAW: raw rows of K, then of V, then V's values, one after the other
     static_assert(!RAW || VB >= 32 * PR * PB + 16, "raw rows fit");
     __shared__ __attribute__((aligned(16))) uint16_t kd[F::quant ? NW : 1][F::quant ? 32 * KS : 8], vd[F::quant && HASV ? NW : 1][F::quant && HASV ? 32 * KS : 8];
-    __shared__ float wm[NW][16 * RT], wl[NW][16 * RT];
+    __shared__ float wm[NW][16], wl[NW][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, g = lane >> 4;
     const int ratio = a.ratio, R = ratio * a.n_q;
-    const int hk = blockIdx.y, rb = blockIdx.x / a.nsplit * 16 * RT, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;
+    const int hk = blockIdx.y, rb = blockIdx.x / a.nsplit * 16, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;
     const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
     const char * vb = HASV ? a.v + hk * a.v_nb2 + i3 * a.v_nb3 : nullptr;
     const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
     const bool capped = a.logit_softcap != 0.0f;
-    // this lane's rows (columns past the last one repeat it)
-    int r[RT];
-    const char * mrow[RT];
-#pragma unroll
-    for (int x = 0; x < RT; x++) {
-        r[x] = rb + 16 * x + lr % RP;
-        if (r[x] >= R) r[x] = R - 1;
-        const int iq = m_query(a, r[x]), h = hk * ratio + r[x] - iq * ratio;
-        mrow[x] = m_mask(a, iq, h, i3);
-    }
+    // this lane's row (columns past the last one repeat it)
+    const int r = rb + lr % RP < R ? rb + lr % RP : R - 1, iq = m_query(a, r), h = hk * ratio + r - iq * ratio;
+    const char * mrow = m_mask(a, iq, h, i3);
 
     // chunks past the head size re-read the last one: they meet zeros of q, and features of V that are not stored.  Slots past the end re-read
     // the last one and are hidden
@@ -301,32 +296,25 @@ mass_step_kernel(const MArgs a) {
         }
     };
     // mask of slots 32 t + 16 u + 4 g + i as it lies, -inf past the last slot
-    auto load_mask = [&](int t, u2 (&w)[RT][2]) {
+    auto load_mask = [&](int t, u2 (&w)[2]) {
 #pragma unroll
-        for (int x = 0; x < RT; x++)
+        for (int u = 0; u < 2; u++) {
+            const int j = 32 * t + 16 * u + 4 * g;
+            if (m8 && j + 4 <= a.n_kv) w[u] = *(const u2 *)(mrow + 2 * (int64_t)j);
+            else {
+                uint32_t y[4];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int j = 32 * t + 16 * u + 4 * g;
-                if (m8 && j + 4 <= a.n_kv) w[x][u] = *(const u2 *)(mrow[x] + 2 * (int64_t)j);
-                else {
-                    uint32_t y[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) y[i] = j + i >= a.n_kv ? 0xfc00u : a.mask ? ((const uint16_t *)mrow[x])[j + i] : 0u;
-                    w[x][u] = u2{y[0] | y[1] << 16, y[2] | y[3] << 16};
-                }
+                for (int i = 0; i < 4; i++) y[i] = j + i >= a.n_kv ? 0xfc00u : a.mask ? ((const uint16_t *)mrow)[j + i] : 0u;
+                w[u] = u2{y[0] | y[1] << 16, y[2] | y[3] << 16};
             }
+        }
     };
-    auto sees = [&](const u2 (&w)[RT][2]) {
-        bool all = true;
-#pragma unroll
-        for (int x = 0; x < RT; x++) all &= w[x][0].x == 0xfc00fc00u && w[x][0].y == 0xfc00fc00u && w[x][1].x == 0xfc00fc00u && w[x][1].y == 0xfc00fc00u;
-        return __any(!all);
-    };
+    auto sees = [&](const u2 (&w)[2]) { return __any(!(w[0].x == 0xfc00fc00u && w[0].y == 0xfc00fc00u && w[1].x == 0xfc00fc00u && w[1].y == 0xfc00fc00u)); };
 
     // tiles are dealt to the waves of all slices in turn: sequences shorter than the range keep them all busy.  A tile hidden from every row
     // costs its mask, which runs one tile ahead of the rows; the first tile is fetched without asking: one round trip instead of two
     int t = split * NW + wave;
-    u2 mk[RT][2], mkn[RT][2];
+    u2 mk[2], mkn[2];
     if (t < ntiles) { load_k(t); load_v(t); load_mask(t, mk); }
     if (t + TW < ntiles) load_mask(t + TW, mkn);
 
@@ -334,82 +322,60 @@ mass_step_kernel(const MArgs a) {
     // the row's largest value is brought to [2^14, 2^15) by a power of two that the logits get back (its small values then stay clear of the
     // subnormal range)
     constexpr int QN = (KS + NW - 1) / NW;
-    float qe[RT], slope[RT], y[RT][QN][8];
+    float y[QN][8], amax = 0.0f;
+    const float slope = m_slope(a, h) * LOG2E, sc = capped ? a.scale / a.logit_softcap : a.scale * LOG2E;
+    const float * qp = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        const int iq = m_query(a, r[x]), h = hk * ratio + r[x] - iq * ratio;
-        slope[x] = m_slope(a, h) * LOG2E;
-        const float * qp = (const float *)(a.q + iq * a.q_nb1 + h * a.q_nb2 + i3 * a.q_nb3);
-        const float sc = capped ? a.scale / a.logit_softcap : a.scale * LOG2E;
-        float amax = 0.0f;
+    for (int n = 0; n < QN; n++) {
+        const int f = 32 * (wave + NW * n) + 8 * g;
+        v4f y0 = {0.0f, 0.0f, 0.0f, 0.0f}, y1 = y0;
+        if (f < a.d) { y0 = *(const v4f *)(qp + f) * sc; y1 = *(const v4f *)(qp + f + 4) * sc; }
 #pragma unroll
-        for (int n = 0; n < QN; n++) {
-            const int f = 32 * (wave + NW * n) + 8 * g;
-            v4f y0 = {0.0f, 0.0f, 0.0f, 0.0f}, y1 = y0;
-            if (f < a.d) { y0 = *(const v4f *)(qp + f) * sc; y1 = *(const v4f *)(qp + f + 4) * sc; }
-#pragma unroll
-            for (int i = 0; i < 4; i++) { y[x][n][i] = y0[i]; y[x][n][4 + i] = y1[i]; amax = fmaxf(amax, fmaxf(fabsf(y0[i]), fabsf(y1[i]))); }
-        }
-        if (!F::bf) {
-            amax = max_groups(amax);
-            if (g == 0) wm[wave][16 * x + lr] = amax;
-        }
+        for (int i = 0; i < 4; i++) { y[n][i] = y0[i]; y[n][4 + i] = y1[i]; amax = fmaxf(amax, fmaxf(fabsf(y0[i]), fabsf(y1[i]))); }
     }
-    if (!F::bf) __syncthreads();
+    int e = 0;
+    if constexpr (!F::bf) {
+        amax = max_groups(amax);
+        if (g == 0) wm[wave][lr] = amax;
+        __syncthreads();
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        int e = 0;
-        if (!F::bf) {
-            float amax = 0.0f;
+        for (int w = 0; w < NW; w++) amax = fmaxf(amax, wm[w][lr]);
+        e = row_exp(amax);
+    }
+    const float qe = ldexpf(1.0f, e);
 #pragma unroll
-            for (int w = 0; w < NW; w++) amax = fmaxf(amax, wm[w][16 * x + lr]);
-            e = amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
-        }
-        qe[x] = ldexpf(1.0f, e);
+    for (int n = 0; n < QN; n++) {
+        if (wave + NW * n >= KS) continue;
+        v4i w[P];
 #pragma unroll
-        for (int n = 0; n < QN; n++) {
-            if (wave + NW * n >= KS) continue;
-            v4i w[P];
+        for (int i = 0; i < 8; i++) y[n][i] = ldexpf(y[n][i], -e);
+        split8<F::bf, P>(y[n], w);
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[x][n][i] = ldexpf(y[x][n][i], -e);
-            split8<F::bf, P>(y[x][n], w);
-#pragma unroll
-            for (int p = 0; p < P; p++) qs[x][wave + NW * n][p][lane] = w[p];
-        }
+        for (int p = 0; p < P; p++) qs[wave + NW * n][p][lane] = w[p];
     }
     __syncthreads();
 
-    float m[RT], l[RT];                         // of this lane's rows; l over this lane's slots only
-    int E[RT];                                  // blocks: o holds 2^(14 - E) times its value, E the exponent of the largest scale of V met so far
-    v4f o[RT][HASV ? FT : 1];
-    float * lg[RT];
+    float m = -INFINITY, l = 0.0f;      // of this lane's row; l over this lane's slots only
+    int E = -64;                        // blocks: o holds 2^(14 - E) times its value, E the exponent of the largest scale of V met so far
+    v4f o[HASV ? FT : 1];
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        m[x] = -INFINITY; l[x] = 0.0f; E[x] = -64;
-#pragma unroll
-        for (int i = 0; i < (HASV ? FT : 1); i++) o[x][i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        lg[x] = a.logits + (((int64_t)i3 * a.n_head_kv + hk) * R + r[x]) * a.lpitch;
-    }
-    auto mine = [&](int x) { return lr < RP && rb + 16 * x + lr < R; };      // the lane that stores row r[x]
+    for (int i = 0; i < (HASV ? FT : 1); i++) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float * lg = a.logits + (((int64_t)i3 * a.n_head_kv + hk) * R + r) * a.lpitch;
+    const bool mine = lr < RP && rb + lr < R;           // the lane that stores row r
 
     while (t < ntiles) {
-        u2 mc[RT][2];
-#pragma unroll
-        for (int x = 0; x < RT; x++) { mc[x][0] = mk[x][0]; mc[x][1] = mk[x][1]; }
+        const u2 mc[2] = {mk[0], mk[1]};
         int tn = t + TW;                        // the next tile that a row sees
         while (tn < ntiles && !sees(mkn)) {
+            if (mine) {
 #pragma unroll
-            for (int x = 0; x < RT; x++)
-                if (mine(x)) {
-#pragma unroll
-                    for (int u = 0; u < 2; u++) if (32 * tn + 16 * u + 4 * g < a.lpitch) *(v4f *)(lg[x] + 32 * tn + 16 * u + 4 * g) = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                }
+                for (int u = 0; u < 2; u++) if (32 * tn + 16 * u + 4 * g < a.lpitch) *(v4f *)(lg + 32 * tn + 16 * u + 4 * g) = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            }
             tn += TW;
             if (tn < ntiles) load_mask(tn, mkn);
         }
         const bool next = tn < ntiles;
-#pragma unroll
-        for (int x = 0; x < RT; x++) { mk[x][0] = mkn[x][0]; mk[x][1] = mkn[x][1]; }
+        mk[0] = mkn[0]; mk[1] = mkn[1];
         if constexpr (RAW) { put_raw(kp); raw_scales(kd[wave]); __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
         else if constexpr (F::quant) {          // K's integers to rows, the scales of the 32 slots where every lane can read them
 #pragma unroll
@@ -422,7 +388,7 @@ mass_step_kernel(const MArgs a) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         // ---- S^T
-        v4f c[RT][2];
+        v4f c[2];
         {
             hk_t dk[2][4];
             if constexpr (F::quant) {
@@ -431,117 +397,101 @@ mass_step_kernel(const MArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) dk[u][i] = *(const hk_t *)&kd[wave][(16 * u + 4 * g + i) * KS];
             }
-#pragma unroll
-            for (int x = 0; x < RT; x++) c[x][0] = c[x][1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            c[0] = c[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                v4i qv[RT][P];
+                v4i qv[P];
 #pragma unroll
-                for (int x = 0; x < RT; x++)
-#pragma unroll
-                    for (int p = 0; p < P; p++) qv[x][p] = qs[x][ks][p][lane];
+                for (int p = 0; p < P; p++) qv[p] = qs[ks][p][lane];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     v4i kop;
                     if constexpr (RAW) kop = raw_chunk<TYPE>(raw[wave] + (16 * u + lr) * PR * PB, 4 * ks + g).operand(g);
                     else if constexpr (F::quant) kop = *(const v4i *)(lds[wave] + (16 * u + lr) * VP + (4 * ks + g) * 16);
                     else kop = kc[u][ks].operand(g);
+                    v4f b = F::quant ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : c[u];
 #pragma unroll
-                    for (int x = 0; x < RT; x++) {
-                        v4f b = F::quant ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : c[x][u];
+                    for (int p = P - 1; p >= 0; p--) b = mfma16<F::bf>(kop, qv[p], b);
+                    if constexpr (F::quant) {
 #pragma unroll
-                        for (int p = P - 1; p >= 0; p--) b = mfma16<F::bf>(kop, qv[x][p], b);
-                        if constexpr (F::quant) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++) c[x][u][i] = __builtin_fmaf(b[i], (float)dk[u][i][ks], c[x][u][i]);
-                        } else c[x][u] = b;
-                    }
+                        for (int i = 0; i < 4; i++) c[u][i] = __builtin_fmaf(b[i], (float)dk[u][i][ks], c[u][i]);
+                    } else c[u] = b;
                 }
             }
         }
         if (next) load_k(tn);                   // in flight during the rest of this tile
         if (tn + TW < ntiles) load_mask(tn + TW, mkn);
-        float s[RT][8], p[RT][8], corr[RT];     // slots 32 t + 16 (i >> 2) + 4 g + (i & 3)
+        float s[8], p[8];           // slots 32 t + 16 (i >> 2) + 4 g + (i & 3)
         bool some = false;                      // some row does not see some slot of the tile
+        float mx = m;
 #pragma unroll
-        for (int x = 0; x < RT; x++) {
-            float mx = m[x];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float mv = h2f((uint16_t)(mc[x][i >> 2][(i & 3) >> 1] >> (16 * (i & 1))));
-                float y = c[x][i >> 2][i & 3] * qe[x];
-                if (capped) y = a.logit_softcap * LOG2E * tanhf(y);
-                s[x][i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope[x], y);
-                mx = fmaxf(mx, s[x][i]);
-                some |= s[x][i] == -INFINITY;
-            }
-            if (mine(x)) {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const int j = 32 * t + 16 * u + 4 * g;
-                    if (j < a.lpitch) *(v4f *)(lg[x] + j) = v4f{s[x][4 * u], s[x][4 * u + 1], s[x][4 * u + 2], s[x][4 * u + 3]};
-                }
-            }
-            mx = max_groups(mx);
-            const float ms = mx == -INFINITY ? 0.0f : mx;
-            corr[x] = __builtin_amdgcn_exp2f(m[x] - ms);        // m = -inf: 0
-            l[x] *= corr[x];
-#pragma unroll
-            for (int i = 0; i < 8; i++) { p[x][i] = __builtin_amdgcn_exp2f(s[x][i] - ms); l[x] += p[x][i]; }
-            m[x] = mx;
+        for (int i = 0; i < 8; i++) {
+            const float mv = h2f((uint16_t)(mc[i >> 2][(i & 3) >> 1] >> (16 * (i & 1))));
+            float y = c[i >> 2][i & 3] * qe;
+            if (capped) y = capped_logit(y, a.logit_softcap * LOG2E);
+            s[i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope, y);
+            mx = fmaxf(mx, s[i]);
+            some |= s[i] == -INFINITY;
         }
+        if (mine) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int j = 32 * t + 16 * u + 4 * g;
+                if (j < a.lpitch) *(v4f *)(lg + j) = v4f{s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]};
+            }
+        }
+        mx = max_groups(mx);
+        const float ms = mx == -INFINITY ? 0.0f : mx;
+        float corr = __builtin_amdgcn_exp2f(m - ms);        // m = -inf: 0
+        l *= corr;
+#pragma unroll
+        for (int i = 0; i < 8; i++) { p[i] = __builtin_amdgcn_exp2f(s[i] - ms); l += p[i]; }
+        m = mx;
         if constexpr (HASV) {
             const bool hidden = __any(some);
-            _Float16 dd[RT][SETS][8];
+            _Float16 dd[SETS][8];
             if constexpr (RAW) { put_raw(vp); raw_scales(vd[wave]); __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
             if constexpr (F::quant) {
                 // the scales of V go on P, those of this lane's class of blocks.  A hidden slot's is taken as 0 (it may be NaN)
+                _Float16 dm = 0;
 #pragma unroll
-                for (int x = 0; x < RT; x++) {
-                    _Float16 dm = 0;
+                for (int q = 0; q < SETS; q++)
 #pragma unroll
-                    for (int q = 0; q < SETS; q++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const int b = q * NC + lr / RP;
-                            dd[x][q][i] = __builtin_bit_cast(_Float16, vd[wave][(16 * (i >> 2) + 4 * g + (i & 3)) * KS + (b < KS ? b : 0)]);
-                        }
-                    if (hidden) {
-#pragma unroll
-                        for (int q = 0; q < SETS; q++)
-#pragma unroll
-                            for (int i = 0; i < 8; i++) if (s[x][i] == -INFINITY) dd[x][q][i] = 0;
+                    for (int i = 0; i < 8; i++) {
+                        const int b = q * NC + lr / RP;
+                        dd[q][i] = __builtin_bit_cast(_Float16, vd[wave][(16 * (i >> 2) + 4 * g + (i & 3)) * KS + (b < KS ? b : 0)]);
                     }
+                if (hidden) {
 #pragma unroll
                     for (int q = 0; q < SETS; q++)
 #pragma unroll
-                        for (int i = 0; i < 8; i++) dm = __builtin_elementwise_max(dm, __builtin_elementwise_abs(dd[x][q][i]));
-                    const float dmx = max_groups((float)dm);
-                    const int e = dmx > 0.0f && dmx < INFINITY ? __builtin_amdgcn_frexp_expf(dmx) - 1 : -64;
-                    const int En = E[x] > e ? E[x] : e;
-                    corr[x] = ldexpf(corr[x], E[x] - En);
-                    E[x] = En;
+                        for (int i = 0; i < 8; i++) if (s[i] == -INFINITY) dd[q][i] = 0;
                 }
+#pragma unroll
+                for (int q = 0; q < SETS; q++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) dm = __builtin_elementwise_max(dm, __builtin_elementwise_abs(dd[q][i]));
+                const float dmx = max_groups((float)dm);
+                const int e = dmx > 0.0f && dmx < INFINITY ? __builtin_amdgcn_frexp_expf(dmx) - 1 : -64;
+                const int En = E > e ? E : e;
+                corr = ldexpf(corr, E - En);
+                E = En;
             }
+            if (__any(corr != 1.0f)) {
 #pragma unroll
-            for (int x = 0; x < RT; x++)
-                if (__any(corr[x] != 1.0f)) {
-#pragma unroll
-                    for (int i = 0; i < FT; i++) o[x][i] = o[x][i] * corr[x];
-                }
+                for (int i = 0; i < FT; i++) o[i] = o[i] * corr;
+            }
             // ---- V tile into LDS.  A slot that some row does not see must not reach that row through 0 * NaN: its non-finite values are
             // taken out here and added below to the rows that do see it
             uint32_t bad = 0;                                   // slots of the tile with values taken out
             if constexpr (!F::quant) if (hidden) {
                 uint32_t unseen = 0;                            // bit j: slot 32 t + j is hidden from some row
 #pragma unroll
-                for (int x = 0; x < RT; x++)
+                for (int i = 0; i < 8; i++) {
+                    const uint64_t b = __ballot(s[i] == -INFINITY);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const uint64_t b = __ballot(s[x][i] == -INFINITY);
-#pragma unroll
-                        for (int gg = 0; gg < 4; gg++) if ((b >> (16 * gg)) & 0xffff) unseen |= 1u << (16 * (i >> 2) + 4 * gg + (i & 3));
-                    }
+                    for (int gg = 0; gg < 4; gg++) if ((b >> (16 * gg)) & 0xffff) unseen |= 1u << (16 * (i >> 2) + 4 * gg + (i & 3));
+                }
 #pragma unroll
                 for (int i = 0; i < VN; i++) {
                     const int row = VR * i + lane / (D / 8);
@@ -567,27 +517,21 @@ mass_step_kernel(const MArgs a) {
             if (next) load_v(tn);
             // ---- O^T
             const uint8_t * vt = lds[wave] + (4 * g + (lr >> 2)) * VP + 8 * (lr & 3);
-            v4i pf[RT][P];
+            v4i pf[P];
+            if constexpr (!F::bf) {                             // f16 parts: clear of the subnormal range
+                const float up = F::quant ? ldexpf(1.0f, 14 - E) : 16384.0f;
 #pragma unroll
-            for (int x = 0; x < RT; x++) {
-                if constexpr (!F::bf) {                         // f16 parts: clear of the subnormal range
-                    const float up = F::quant ? ldexpf(1.0f, 14 - E[x]) : 16384.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) p[x][i] *= up;
-                }
-                if constexpr (!F::quant) split8<F::bf, P>(p[x], pf[x]);
+                for (int i = 0; i < 8; i++) p[i] *= up;
             }
+            if constexpr (!F::quant) split8<F::bf, P>(p, pf);
 #pragma unroll
             for (int f = 0; f < FT; f++) {
                 if constexpr (F::quant) {
                     if (f % (FT / SETS) == 0) {                 // the next scaled copy
+                        float y[8];
 #pragma unroll
-                        for (int x = 0; x < RT; x++) {
-                            float y[8];
-#pragma unroll
-                            for (int i = 0; i < 8; i++) y[i] = p[x][i] * (float)dd[x][f / (FT / SETS)][i];
-                            split8<false, 2>(y, pf[x]);
-                        }
+                        for (int i = 0; i < 8; i++) y[i] = p[i] * (float)dd[f / (FT / SETS)][i];
+                        split8<false, 2>(y, pf);
                     }
                 }
                 const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(vt + 32 * f));
@@ -596,80 +540,68 @@ mass_step_kernel(const MArgs a) {
                 __builtin_memcpy(&vop, &lo, 8);
                 __builtin_memcpy((char *)&vop + 8, &hi, 8);
 #pragma unroll
-                for (int x = 0; x < RT; x++)
-#pragma unroll
-                    for (int q = P - 1; q >= 0; q--) o[x][f] = mfma16<F::bf>(vop, pf[x][q], o[x][f]);
+                for (int q = P - 1; q >= 0; q--) o[f] = mfma16<F::bf>(vop, pf[q], o[f]);
             }
-            if (!F::quant && bad) {                             // non-finite values of slots that only some rows see
+            if constexpr (!F::quant) if (bad) {                 // non-finite values of slots that only some rows see
                 for (int row = 0; row < 32; row++) {
                     if (!(bad >> row & 1)) continue;
                     const int from = ((row & 15) >> 2) * 16 + lr, i = (row >> 4) * 4 + (row & 3), j = 32 * t + row;
                     if (j >= a.n_kv) continue;
                     const char * vr = vb + (uint64_t)(uint32_t)j * a.v_nb1;
+                    float pr = 0.0f, sr = -INFINITY;
 #pragma unroll
-                    for (int x = 0; x < RT; x++) {
-                        float pr = 0.0f, sr = -INFINITY;
-#pragma unroll
-                        for (int q = 0; q < 8; q++) {
-                            const float a0 = __shfl(p[x][q], from, 64), a1 = __shfl(s[x][q], from, 64);
-                            if (q == i) { pr = a0; sr = a1; }
-                        }
-#pragma unroll
-                        for (int f = 0; f < FT; f++)
-#pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const int e = 16 * f + 4 * g + q;
-                                if (e >= a.dv) continue;
-                                const float y = kv_value<TYPE>(vr, e);
-                                if (sr != -INFINITY && !(fabsf(y) < INFINITY)) o[x][f][q] += pr * y;
-                            }
+                    for (int q = 0; q < 8; q++) {
+                        const float a0 = __shfl(p[q], from, 64), a1 = __shfl(s[q], from, 64);
+                        if (q == i) { pr = a0; sr = a1; }
                     }
+#pragma unroll
+                    for (int f = 0; f < FT; f++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int e = 16 * f + 4 * g + q;
+                            if (e >= a.dv) continue;
+                            const float y = kv_value<TYPE>(vr, e);
+                            if (sr != -INFINITY && !(fabsf(y) < INFINITY)) o[f][q] += pr * y;
+                        }
                 }
             }
         }
         t = tn;
     }
     // ---- the waves' states meet in LDS
+    l = sum_groups(l);
+    if (g == 0 && lr < RP) { wm[wave][lr] = m; wl[wave][lr] = l; }
+    if constexpr (HASV) {
+        float * ob = (float *)lds[wave] + lr % RP * OP + 4 * g;
+        const float back = F::bf ? 1.0f : F::quant ? ldexpf(1.0f, E - 14) : 1.0f / 16384.0f;
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        l[x] = sum_groups(l[x]);
-        if (g == 0 && lr < RP) { wm[wave][16 * x + lr] = m[x]; wl[wave][16 * x + lr] = l[x]; }
+        for (int f = 0; f < FT; f++) if (NC == 1 || f / 2 % NC == lr / RP) *(v4f *)(ob + 16 * f) = o[f] * back;
     }
+    __syncthreads();
+    const int rows = R - rb < RP ? R - rb : RP;
     const int64_t base = (((int64_t)i3 * a.n_head_kv + hk) * a.nsplit + split) * R + rb;
+    if constexpr (HASV) {
+        for (int idx = tid; idx < rows * (D / 4); idx += NW * 64) {
+            const int rr = idx / (D / 4), f4 = idx % (D / 4);
+            if (4 * f4 >= a.dv) continue;
+            float M = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < RT; x++) {
-        const int rows = R - rb - 16 * x < RP ? R - rb - 16 * x : RP;
-        if constexpr (HASV) {
-            if (x > 0) __syncthreads();                         // the tile before this one has been read
-            float * ob = (float *)lds[wave] + lr % RP * OP + 4 * g;
-            const float back = F::bf ? 1.0f : F::quant ? ldexpf(1.0f, E[x] - 14) : 1.0f / 16384.0f;
-#pragma unroll
-            for (int f = 0; f < FT; f++) if (NC == 1 || f / 2 % NC == lr / RP) *(v4f *)(ob + 16 * f) = o[x][f] * back;
-        }
-        __syncthreads();
-        if constexpr (HASV) {
-            for (int idx = tid; idx < rows * (D / 4); idx += NW * 64) {
-                const int rr = idx / (D / 4), f4 = idx % (D / 4);
-                if (4 * f4 >= a.dv) continue;
-                float M = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][16 * x + rr]);
-                const float ms = M == -INFINITY ? 0.0f : M;
-                v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int w = 0; w < NW; w++) O = O + *(const v4f *)((const float *)lds[w] + rr * OP + 4 * f4) * __builtin_amdgcn_exp2f(wm[w][16 * x + rr] - ms);
-                *(v4f *)(a.part + (base + 16 * x + rr) * D + 4 * f4) = O;
-            }
-        }
-        if (tid < rows) {
-            float M = -INFINITY, L = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][16 * x + tid]);
+            for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][rr]);
             const float ms = M == -INFINITY ? 0.0f : M;
+            v4f O = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < NW; w++) L = __builtin_fmaf(wl[w][16 * x + tid], __builtin_amdgcn_exp2f(wm[w][16 * x + tid] - ms), L);
-            *(v2f *)(a.stats + (base + 16 * x + tid) * 2) = v2f{M, L};
+            for (int w = 0; w < NW; w++) O = O + *(const v4f *)((const float *)lds[w] + rr * OP + 4 * f4) * __builtin_amdgcn_exp2f(wm[w][rr] - ms);
+            *(v4f *)(a.part + (base + rr) * D + 4 * f4) = O;
         }
+    }
+    if (tid < rows) {
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) M = fmaxf(M, wm[w][tid]);
+        const float ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < NW; w++) L = __builtin_fmaf(wl[w][tid], __builtin_amdgcn_exp2f(wm[w][tid] - ms), L);
+        *(v2f *)(a.stats + (base + tid) * 2) = v2f{M, L};
     }
 }
 
@@ -768,7 +700,7 @@ constexpr int STEP_WAVES = 4;
 
 template <int TYPE, int D, bool HASV, int RP, bool RAW> static int step_launch(const MArgs & a, int ne3, hipStream_t s) {
     const int R = a.ratio * a.n_q;
-    MI355_LAUNCH("fattn_mass_step", (mass_step_kernel<TYPE, D, STEP_WAVES, HASV, 1, RP, RAW>),
+    MI355_LAUNCH("fattn_mass_step", (mass_step_kernel<TYPE, D, STEP_WAVES, HASV, RP, RAW>),
                  dim3((unsigned)(a.nsplit * ((R + 15) / 16)), (unsigned)a.n_head_kv, (unsigned)ne3), dim3(STEP_WAVES * 64), 0, s, a);
     MI355_CHECK_LAUNCH();
     const int mass_wgs = (a.n_kv + 255) / 256;
@@ -949,11 +881,6 @@ static __device__ __forceinline__ void to_parts(float * v, int e, v4i * out) {
     split8<false, 2>(v, out);
 }
 
-// cap log2(e) tanh(x), c2 = cap log2(e): tanh x = 1 - 2 / (e^2x + 1).  Off by some 2^-23 of the cap like the logit itself, and short: tanhf's two
-// branches, 16 times over, took the loop out of the instruction cache
-static __device__ __forceinline__ float capped_logit(float x, float c2) {
-    return __builtin_fmaf(-2.0f * c2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * x) + 1.0f), c2);
-}
 // logits (log2 domain) of a 32 x 32 tile from slot j0 on, in place of its products: sc what they lack, cl the tile's class for this lane's query
 static __device__ __forceinline__ void tile_logits(const MArgs & a, v16f & c, float sc, float slope, int cl, const char * mrow, bool m8, int j0) {
 #pragma unroll

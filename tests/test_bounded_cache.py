@@ -106,7 +106,8 @@ BOTH = [
     (E_TYPE, dict(type_k=B.F32, type_v=B.F32)), (E_TYPE, dict(type_k=B.Q4_K, type_v=B.Q4_K)),
     (E_SHAPE, dict(type_k=B.Q8_0, type_v=B.Q8_0, d=80)), (E_SHAPE, dict(n_head=0)), (E_SHAPE, dict(n_head_kv=3)), (E_SHAPE, dict(n_head_kv=0)),
     (E_SHAPE, dict(n_q=0)), (E_SHAPE, dict(n_q=65536)), (E_SHAPE, dict(n_kv=-1)), (E_SHAPE, dict(n_kv=1 << 31)), (E_SHAPE, dict(ne3=0)),
-    (E_SHAPE, dict(m_ne2=0)), (E_SHAPE, dict(m_ne3=0)), (E_SHAPE, dict(n_head=65536, n_head_kv=1)),
+    (E_SHAPE, dict(m_ne2=0)), (E_SHAPE, dict(m_ne3=0)), (E_SHAPE, dict(n_head=65536, n_head_kv=1)), (E_SHAPE, dict(n_head=65535, n_head_kv=1, n_q=2)),
+    (E_SHAPE, dict(k_nb1=-512)), (E_SHAPE, dict(k_nb1=1 << 31)), (E_SHAPE, dict(m_ne2=65536)), (E_SHAPE, dict(m_ne2=1000, m_ne3=1000)), (E_SHAPE, dict(m_ne3=1 << 62, m_ne2=4)),
     (E_ALIGN, dict(q=P + 4)), (E_ALIGN, dict(q_nb1=520)), (E_ALIGN, dict(k=P + 8)), (E_ALIGN, dict(k_nb1=264)), (E_ALIGN, dict(mask=P + 1)),
     (E_ALIGN, dict(m_nb1=511)), (E_ALIGN, dict(mass_in=P + 2)), (E_ALIGN, dict(out_nb3=1022)), (E_ALIGN, dict(type_k=B.Q4_0, type_v=B.Q4_0, k_nb2=4097)),
 ]
@@ -115,6 +116,7 @@ BOTH = [
 @pytest.mark.parametrize("code, kw", BOTH + [
     (E_NULL, dict(v=None)), (E_NULL, dict(dst=None)), (E_UNSUPPORTED, dict(dv=136)), (E_UNSUPPORTED, dict(dv=12)), (E_TYPE, dict(type_v=B.BF16)),
     (E_SHAPE, dict(type_k=B.Q8_0, type_v=B.Q8_0, dv=40)), (E_UNSUPPORTED, dict(n_q=9)), (E_ALIGN, dict(v_nb3=8)), (E_ALIGN, dict(dst=P + 4)),
+    (E_SHAPE, dict(v_nb1=1 << 31)), (E_SHAPE, dict(v_nb1=-512)),
 ])
 def test_flash_attn_ext_mass_refuses(code, kw):
     assert K.lib.mi355_flash_attn_ext_mass(*attn_args(**kw), P, 1 << 40, None) == code
@@ -136,3 +138,5 @@ def test_attention_mass_workspaces():
                 assert fn(a, w, P, need - 1, None) == E_WORKSPACE and fn(a, w, None, 0, None) == E_WORKSPACE
                 assert fn(a, w, P + 4, need, None) == E_ALIGN
     assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=-1)[0]) == -1
+    assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=100, m_ne2=0)[0]) == -1
+    assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=100, m_ne2=0, mask=None)[0]) > 0

@@ -666,3 +666,146 @@ def test_attention_mass_wrapper_refuses_what_does_not_fit():
         ops.flash_attn_ext_mass(q.expand(1, 4, 9, 64).contiguous(), k, v, None, B.F16, 0.1)
     with pytest.raises(K.Mi355Error):
         ops.flash_attn_ext_mass(q[:, :3], k, v, None, B.F16, 0.1)
+
+
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("n", [2, 40])
+def test_attention_mass_hidden_rows_may_be_huge(t, n):
+    """rows that no query sees, finite and near the end of the type's range, between rows that all see; visible rows of very different sizes"""
+    S, H, HK, slots, d = 1, 4, 2, 300, 128
+    q, k, v, mass = attn_case(S, H, HK, n, slots, d, d if n <= 8 else 0, t, 500 + n)
+    mask = torch.zeros((1, 1, n, slots)).half()
+    mask[..., 3::5] = float("-inf")
+    for x in ((k, v) if v is not None else (k,)):
+        if t in DTYPE:
+            x[:, :, 3::5] = torch.finfo(DTYPE[t]).max / 2 if t == B.F16 else 1e30
+            x[:, :, 4::5] *= 2.0 ** -9
+        else:
+            b = x.view(S, HK, slots, -1, B.TYPE_SIZE[t])
+            b[:, :, 3::5, :, :2] = torch.tensor([60000.0]).half().view(torch.uint8)
+            b[:, :, 4::5, :, 1] = 0                           # the scale's upper byte: a subnormal one
+    check_attn(q, k, v, t, mask, 1 / math.sqrt(d), mass, 0.5)
+
+
+@pytest.mark.parametrize("t", [B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("G,n,d", [(4, 1, 64), (8, 1, 64), (2, 8, 64), (3, 1, 128), (7, 1, 128), (4, 5, 128), (4, 1, 256), (5, 4, 256), (4, 3, 96), (9, 4, 128)])
+def test_attention_mass_of_blocks_at_every_alignment(t, G, n, d):
+    """rows that start 2, 4, 8 bytes past 16 and lie an odd number of 2-byte units apart: every way to load them gives the same"""
+    HK, slots, size = 2, 203, B.TYPE_SIZE[t] * d // 32
+    q, k, v, _ = attn_case(1, G * HK, HK, n, slots, d, d, t, d + G)
+    res = []
+    for off, pitch in ((0, (size + 15) // 16 * 16), (0, size), (2, size + 2), (4, size + 6), (8, (size + 15) // 16 * 16)):
+        def place(x):
+            raw = torch.full((HK * slots * pitch + 64,), 255, dtype=torch.uint8, device="cuda")
+            y = raw[off:].as_strided((1, HK, slots, size), (0, slots * pitch, pitch, 1), off)
+            y.copy_(x)
+            return y
+        kg, vg = place(k), place(v)
+        dst, mass = ops.flash_attn_ext_mass(q.cuda(), kg, vg, None, t, 0.1)
+        res.append((dst, mass, ops.attn_mass(q.cuda(), kg, None, t, 0.1)))
+    wd, ed, wm, em = attn_oracle(q, values(k, t), values(v, t), None, 0.1, None, 0.0)
+    for dst, mass, alone in res:
+        assert ((dst.cpu().double() - wd).abs() <= ed).all() and ((mass.cpu().double() - wm).abs() <= em).all() and ((alone.cpu().double() - wm).abs() <= em).all()
+        assert torch.equal(dst, res[0][0]) and torch.equal(mass, res[0][1])
+
+
+@pytest.mark.parametrize("t,d", [(B.Q4_0, 128), (B.F16, 64)])
+def test_attention_mass_of_a_long_cache(t, d):
+    """more slots than every slice takes in one go; and few queries of a prompt over them"""
+    q, k, v, mass = attn_case(1, 4, 2, 1, 140001, d, d, t, 9)
+    check_attn(q, k, v, t, None, 1 / math.sqrt(d), mass, 0.9)
+    q9 = torch.randn((1, 4, 9, d), generator=gen(1))
+    check_attn(q9, k, None, t, causal(1, 9, 140001), 1 / math.sqrt(d), mass, 0.9)
+
+
+# ---- the operators as they are used --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0])
+def test_prompt_then_decode_in_a_cache_that_stays_full(t):
+    """a prompt is stored, its last queries weigh it, its heaviest slots move to the bounded cache; then steps: a token goes to the slot that the
+    step before gave up, attention adds up the weights, the next slot is chosen.  The same steps eager and as replays of one graph"""
+    S, H, HK, d, n, W, budget, steps = 2, 8, 2, 64, 100, 16, 33, 24
+    g = gen(21)
+    total = n + steps
+    qx, kx, vx = torch.randn((S, total, H, d), generator=g), torch.randn((S, total, HK, d), generator=g), torch.randn((S, total, HK, d), generator=g)
+    qw, kw = 1 + 0.2 * torch.randn(d, generator=g), 1 + 0.2 * torch.randn(d, generator=g)
+    pos = torch.arange(total, dtype=torch.int32)[None].expand(S, total).contiguous()
+    qg, kg, vg, pg, qwg, kwg = (x.cuda() for x in (qx, kx, vx, pos, qw, kw))
+    scale, opt = 1 / math.sqrt(d), dict(freq_base=10000.0)
+    width = d if t in DTYPE else d // 32 * B.TYPE_SIZE[t]
+    fresh = lambda slots: torch.zeros((S, HK, slots, width), dtype=DTYPE.get(t, torch.uint8), device="cuda")  # noqa: E731
+
+    # what the cache holds of every token: the operators' own rows, checked once against the formula
+    all_k, all_v = fresh(total), fresh(total)
+    q_rot = ops.qk_norm_rope(qg, kg, vg, qwg, kwg, 1e-6, pg, all_k, all_v, t, **opt)
+    wq, eq = store_oracle(qx, qw, 1e-6, pos, d, 2)
+    assert ((q_rot.cpu().double() - wq).abs() <= eq).all()
+    if t in DTYPE:
+        check_rows(all_k.cpu(), fresh(total).cpu(), torch.arange(total, dtype=torch.int32)[None, None].expand(S, HK, total), *store_oracle(kx, kw, 1e-6, pos, d, 2), t)
+
+    def prompt():
+        ck, cv = fresh(n), fresh(n)
+        sp, sm = torch.zeros((S, HK, n), dtype=torch.int32, device="cuda"), torch.zeros((S, HK, n), device="cuda")
+        q = ops.qk_norm_rope(qg[:, :n], kg[:, :n], vg[:, :n], qwg, kwg, 1e-6, pg[:, :n], ck, cv, t, slot_pos=sp, slot_mass=sm, **opt)
+        assert torch.equal(ck, all_k[:, :, :n]) and torch.equal(cv, all_v[:, :, :n]) and torch.equal(sp, pg[:, None, :n].expand(S, HK, n))
+        assert torch.equal(q, q_rot[:, :, :n])
+        mask = causal(1, W, n)
+        weight = ops.attn_mass(q[:, :, n - W:], ck, mask.cuda(), t, scale)
+        _, _, wm, em = attn_oracle(q[:, :, n - W:].cpu(), values(ck.cpu(), t), None, mask, scale, None, 0.0)
+        assert ((weight.cpu().double() - wm).abs() <= em).all()
+        past = torch.full((S,), n, dtype=torch.int32, device="cuda")
+        bk, bv = fresh(budget), fresh(budget)
+        kept, _, mo, po = ops.kv_evict(weight, sp, past, budget - 1, 4, 8, k=ck, v=cv, type_kv=t, k_out=bk[:, :, : budget - 1], v_out=bv[:, :, : budget - 1])
+        want, _ = evict_oracle(weight.cpu().numpy(), sp.cpu().numpy(), [n] * S, [n] * S, budget - 1, 1, 4, 8)
+        assert np.array_equal(kept.cpu().numpy(), want)
+        mass, where = torch.zeros((S, HK, budget), device="cuda"), torch.zeros((S, HK, budget), dtype=torch.int32, device="cuda")
+        mass[..., : budget - 1], where[..., : budget - 1] = mo, po
+        return dict(k=bk, v=bv, mass=mass, pos=where, free=torch.full((S, HK, 1), budget - 1, dtype=torch.int32, device="cuda"),
+                    q=qg[:, :1].clone(), kk=kg[:, :1].clone(), vv=vg[:, :1].clone(), at=pg[:, :1].clone(), past=torch.zeros(S, dtype=torch.int32, device="cuda"))
+
+    def step(c):
+        q = ops.qk_norm_rope(c["q"], c["kk"], c["vv"], qwg, kwg, 1e-6, c["at"], c["k"], c["v"], t, rows=c["free"], slot_pos=c["pos"], slot_mass=c["mass"], **opt)
+        dst, _ = ops.flash_attn_ext_mass(q, c["k"], c["v"], None, t, scale, mass=c["mass"], decay=0.95, mass_out=c["mass"])
+        _, out = ops.kv_evict(c["mass"], c["pos"], c["past"], budget - 1, 4, 8)
+        c["free"].copy_(out)
+        return q, dst
+
+    def feed(c, i):
+        for name, x in (("q", qg), ("kk", kg), ("vv", vg), ("at", pg)):
+            c[name].copy_(x[:, n + i: n + i + 1])
+        c["past"].fill_(n + i + 1)
+
+    eager, replayed = prompt(), prompt()
+    results = []
+    for i in range(steps):
+        feed(eager, i)
+        old, free = eager["mass"].cpu(), eager["free"].cpu().long()
+        q, dst = step(eager)
+        old.scatter_(2, free, 0.0)
+        k, v, p = (eager[x].cpu() for x in ("k", "v", "pos"))
+        at = (torch.arange(S)[:, None, None], torch.arange(HK)[None, :, None], p.long())
+        assert torch.equal(k, all_k.cpu()[at]) and torch.equal(v, all_v.cpu()[at])            # every slot holds the token that slot_pos names
+        assert (torch.gather(p, 2, free) == n + i).all() and len({tuple(x) for x in p.reshape(-1, budget).tolist()}) >= 1
+        assert all(len(set(x)) == budget for x in p.reshape(-1, budget).tolist())             # each token once
+        wd, ed, wm, em = attn_oracle(q.cpu(), values(k, t), values(v, t), None, scale, old, 0.95)
+        assert ((dst.cpu().double() - wd).abs() <= ed).all() and ((eager["mass"].cpu().double() - wm).abs() <= em).all()
+        _, want = evict_oracle(eager["mass"].cpu().numpy(), p.numpy(), [n + i + 1] * S, [budget] * S, budget - 1, 1, 4, 8)
+        assert np.array_equal(eager["free"].cpu().numpy(), want)
+        assert not (torch.gather(p, 2, eager["free"].cpu().long()) < 4).any()                 # the sink stays
+        results.append(dst.clone())
+
+    feed(replayed, 0)
+    saved = {x: y.clone() for x, y in replayed.items()}
+    step(replayed)                                  # (a run before the capture, taken back)
+    for x, y in saved.items():
+        replayed[x].copy_(y)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, dst = step(replayed)
+    for i in range(steps):
+        feed(replayed, i)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dst, results[i])
+    assert all(torch.equal(replayed[x], eager[x]) for x in ("k", "v", "mass", "pos", "free"))
