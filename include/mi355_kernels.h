@@ -774,7 +774,8 @@ MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stre
 
 /* FLASH_ATTN_EXT of a decode step (at most MI355_MASS_MAX_Q queries per sequence) that also accumulates the attention weight every slot draws:
  *   mass_out[j] = decay * mass_in[j] + sum over the queries and the heads that share the KV head of softmax(...)[j]
- * args as for mi355_flash_attn_ext (K and V of one type).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be
+ * args as for mi355_flash_attn_ext (K and V of one type; rows of K and V at most 2^31 - 1 bytes apart, at most 65535 planes of mask, (heads per KV
+ * head)^2 x queries below 2^32, else MI355_E_SHAPE; block rows 2-byte aligned, faster where a row's address is a multiple of d / 16).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be
  * mass_out itself; NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate (the query is not rounded to the cache's type, the
  * weights are not rounded before they meet V).  A slot hidden by the mask takes no part whatever its row holds; a query that sees no slot gives
  * a row of zeros and no weight.  workspace: *_workspace_bytes, 16-byte aligned, no initial contents, not shared by calls that can overlap. */

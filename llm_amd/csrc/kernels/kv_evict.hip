@@ -8,7 +8,8 @@
 // Bound by latency: one workgroup per head has to agree on every step of the search.  A step parts the range of keys that can still hold the
 // wanted one into 2048 buckets (an LDS histogram), so three steps settle 32 bits, and masses, which spread over the range as logarithms do,
 // seldom meet in a bucket; the +inf of sinks and recent slots is counted aside, and a wave whose lanes all fall into one bucket adds once.
-// Up to 32768 slots the keys stay in registers; beyond, every step reads them again.  2049 / 32768 slots, 128 / 8 heads: @STEP us.
+// Up to 32768 slots the keys stay in registers; beyond, every step reads them again.  2049 slots x 128 heads 10.9 us, 32768 x 8
+// heads 31 us (8 of them loading 256 KB on each of 8 CUs, 7 writing the lists) and 10.6 us for the rows.
 // (Digits of 8 bits from the top, keys re-read: 54 / 147 us, atomics queued on the few exponents; bisection with a vote per bit: 15.5 / 48 us.)
 #include "common.h"
 
@@ -227,7 +228,7 @@ struct KgArgs {
     int64_t kept_nb2, kept_nb3;
     const char * src[2]; char * dst[2];
     int64_t s_nb1[2], s_nb2[2], s_nb3[2], d_nb1[2], d_nb2[2], d_nb3[2];
-    int row_bytes[2], n_keep, n_head_kv;
+    int row_bytes[2], n_keep;
     const char * mass, * pos;
     int64_t mass_nb2, mass_nb3, pos_nb2, pos_nb3;
     char * mass_out, * pos_out;
@@ -339,7 +340,7 @@ int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
     g.src[1] = (const char *)p->v; g.s_nb1[1] = p->v_nb1; g.s_nb2[1] = p->v_nb2; g.s_nb3[1] = p->v_nb3;
     g.dst[1] = (char *)p->v_out; g.d_nb1[1] = p->vo_nb1; g.d_nb2[1] = p->vo_nb2; g.d_nb3[1] = p->vo_nb3;
     g.row_bytes[0] = p->k ? (int)mi355_row_size(p->type_kv, p->d) : 0; g.row_bytes[1] = p->v ? (int)mi355_row_size(p->type_kv, dv) : 0;
-    g.n_keep = a.n_keep; g.n_head_kv = a.n_head_kv;
+    g.n_keep = a.n_keep;
     g.mass = a.mass; g.mass_nb2 = a.mass_nb2; g.mass_nb3 = a.mass_nb3; g.pos = a.pos; g.pos_nb2 = a.pos_nb2; g.pos_nb3 = a.pos_nb3;
     g.mass_out = (char *)p->mass_out; g.mo_nb2 = p->mo_nb2; g.mo_nb3 = p->mo_nb3;
     g.pos_out = (char *)p->pos_out; g.po_nb2 = p->po_nb2; g.po_nb3 = p->po_nb3;
