@@ -812,7 +812,7 @@ static int64_t step_splits(const mi355_fattn_args * p) {
 // wave (half of a causal prompt) costs its loads.
 // 64 queries x 32 heads over 16384 f16 slots: 5 + 24 + 5 + 33 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
 // until the first tile of 512 workgroups is there; without its products the first pass takes 20, without its exponentials 23.  2047
-// causal queries, bf16: 16 + 82 + 5 + 97 + 5 us, 45 a pass at that rate; the workgroups of the first slots see twice the rows of the average.
+// causal queries, bf16: 16 + 67 + 5 + 87 + 5 us, 45 a pass at that rate.
 typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int PT = 256;                  // threads: 4 waves
 constexpr int PA_ROWS = 128, PA_SLOTS = 64, PB_ROWS = 32;
@@ -965,6 +965,11 @@ static __device__ __forceinline__ const uint8_t * class_row(const MArgs & a, int
     return a.cls + ((int64_t)plane * a.n_q + iq) * a.cpitch;
 }
 
+// Workgroups come to the CUs in turn, so a CU holds those a multiple of 256 apart: under a causal mask the same place of another head, twice the
+// longest on one CU and twice the shortest on another.  Heads of every second 256 workgroups take their places from the other end
+// (2047 x 2047: 82 + 95 -> 67 + 87 us)
+static __device__ __forceinline__ bool turned() { return (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x / 256 & 1; }
+
 template <int TYPE, int D>
 __global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
 prompt_stats_kernel(const MArgs a) {
@@ -976,7 +981,7 @@ prompt_stats_kernel(const MArgs a) {
     __shared__ uint32_t cl[S][PT / 64][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
     const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;      // the last rows first: a causal mask lets them see most
-    const int rt = (int)(gridDim.x - 1 - blockIdx.x) / a.nsplit * PA_ROWS, r_ = rt + wave * 32 + lr, r = r_ < R ? r_ : R - 1;
+    const int rt = (int)(turned() ? blockIdx.x : gridDim.x - 1 - blockIdx.x) / a.nsplit * PA_ROWS, r_ = rt + wave * 32 + lr, r = r_ < R ? r_ : R - 1;
     const int iq = m_query(a, r), h = hk * a.ratio + r - iq * a.ratio;
     const char * kb = a.k + hk * a.k_nb2 + i3 * a.k_nb3;
     const char * mrow = m_mask(a, iq, h, i3);
@@ -1143,7 +1148,7 @@ prompt_mass_kernel(const MArgs a) {
     __shared__ __attribute__((aligned(16))) float ksc[F::quant ? 128 * NS : 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
     const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, chunk = blockIdx.x % a.nchunk;
-    const int j0 = (blockIdx.x / a.nchunk * 4 + wave) * 32 * NS;            // this wave's slots
+    const int j0 = ((int)(turned() ? gridDim.x - 1 - blockIdx.x : blockIdx.x) / a.nchunk * 4 + wave) * 32 * NS;     // this wave's slots
     const int64_t base = ((int64_t)i3 * a.n_head_kv + hk) * R;
     const int nt = (R + PB_ROWS - 1) / PB_ROWS, nc = a.nchunk;
     const bool m8 = a.mask && (((uintptr_t)a.mask | (uintptr_t)a.m_nb1 | (uintptr_t)a.m_nb2 | (uintptr_t)a.m_nb3) & 7) == 0;
@@ -1290,16 +1295,16 @@ prompt_sum_kernel(const MArgs a) {
 static int prompt_slots(int type, int64_t d) {           // slots of a workgroup in the second pass
     return step_d(d) * (type == MI355_TYPE_Q8_0 || type == MI355_TYPE_Q4_0 ? 2 : 1) <= 128 ? 256 : 128;
 }
-// Slices of the slots in the first pass: 1024 workgroups, two rounds of two a CU, so that the short and the long rows of a causal prompt even out
-// (2047 x 2047: 82 us, with 512 83, with 2048 86), four tiles a workgroup or more, and few slices to join (64: 8 us, 32: 5)
+// Slices of the slots in the first pass: 512 workgroups, one round of two a CU (2047 x 2047: 67 us, with 1024 80, with 2048 87), four tiles a
+// workgroup or more, and few slices to join (64: 8 us, 32: 5)
 static int64_t prompt_splits(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (p->n_kv + PA_SLOTS - 1) / PA_SLOTS, base = (R + PA_ROWS - 1) / PA_ROWS * p->n_head_kv * p->ne3;
-    int64_t n = 1024 / base, most = (tiles + 3) / 4;
+    int64_t n = 512 / base, most = (tiles + 3) / 4;
     if (n > most) n = most;
     if (n > 32) n = 32;
     return n < 1 ? 1 : n;
 }
-// Slices of the rows in the second: 512 workgroups, one round (2047 x 2047: 97 us, with 1024 93, with 256 129; 64 x 16384: 33, with 1024 39)
+// Slices of the rows in the second: likewise (2047 x 2047: 87 us, with 1024 93, with 768 104; 64 x 16384: 34, with 1024 38)
 static int64_t prompt_chunks(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (R + PB_ROWS - 1) / PB_ROWS;
     const int64_t ws = prompt_slots(p->type_k, p->d), base = (p->n_kv + ws - 1) / ws * p->n_head_kv * p->ne3;
