@@ -965,6 +965,8 @@ static __device__ __forceinline__ const uint8_t * class_row(const MArgs & a, int
     return a.cls + ((int64_t)plane * a.n_q + iq) * a.cpitch;
 }
 
+// statistics of a row -> maximum (0: sees nothing) and 1 / sum
+static __device__ __forceinline__ v2f row_result(float M, float L) { return v2f{M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L}; }
 // Workgroups come to the CUs in turn, so a CU holds those a multiple of 256 apart: under a causal mask the same place of another head, twice the
 // longest on one CU and twice the shortest on another.  Heads of every second 256 workgroups take their places from the other end
 // (2047 x 2047: 82 + 95 -> 67 + 87 us)
@@ -1107,10 +1109,12 @@ prompt_stats_kernel(const MArgs a) {
     const float mo = __shfl_xor(m, 32, 64), lo = __shfl_xor(l, 32, 64);
     const float M = fmaxf(m, mo), ms = M == -INFINITY ? 0.0f : M;
     const float L = l * __builtin_amdgcn_exp2f(m - ms) + lo * __builtin_amdgcn_exp2f(mo - ms);
-    if (lh == 0 && r_ < R) *(v2f *)(a.stats + ((((int64_t)i3 * a.n_head_kv + hk) * a.nsplit + split) * R + r_) * 2) = v2f{M, L};
+    if (lh != 0 || r_ >= R) return;
+    if (ns == 1) *(v2f *)&a.rowc[row].m = row_result(M, L);      // one slice: its statistics are the row's
+    else *(v2f *)(a.stats + ((((int64_t)i3 * a.n_head_kv + hk) * ns + split) * R + r_) * 2) = v2f{M, L};
 }
 
-// the slices' statistics of a row -> maximum (0: sees nothing) and 1 / sum
+// several slices: their statistics of a row meet
 __global__ void __launch_bounds__(PT)
 prompt_rows_kernel(const MArgs a) {
     const int R = a.ratio * a.n_q, r = blockIdx.x * PT + threadIdx.x, hk = blockIdx.y, i3 = blockIdx.z;
@@ -1129,7 +1133,7 @@ prompt_rows_kernel(const MArgs a) {
         for (int i = 0; i < 8; i++) L = __builtin_fmaf(x[i].y, __builtin_amdgcn_exp2f(x[i].x - ms), L);
         M = mn;
     }
-    *(v2f *)&a.rowc[hrow * R + r].m = v2f{M == -INFINITY ? 0.0f : M, L == 0.0f ? 0.0f : 1.0f / L};
+    *(v2f *)&a.rowc[hrow * R + r].m = row_result(M, L);
 }
 
 // slots of a wave in the second pass: 64 where its K takes at most 64 registers so
@@ -1295,11 +1299,13 @@ prompt_sum_kernel(const MArgs a) {
 static int prompt_slots(int type, int64_t d) {           // slots of a workgroup in the second pass
     return step_d(d) * (type == MI355_TYPE_Q8_0 || type == MI355_TYPE_Q4_0 ? 2 : 1) <= 128 ? 256 : 128;
 }
-// Slices of the slots in the first pass: 512 workgroups, one round of two a CU (2047 x 2047: 67 us, with 1024 80, with 2048 87), four tiles a
-// workgroup or more, and few slices to join (64: 8 us, 32: 5)
+// Slices of the slots in the first pass: 512 workgroups, one round of two a CU (2047 x 2047: 67 us, with 1024 80, with 2048 87) and few
+// slices to join (64: 8 us, 32: 5).  Small problems: a tile takes a workgroup that has the CU to itself 1.3 us, the launch that joins slices 4 -- up to 4
+// tiles one slice, else down to one tile each (64 x 1024 x 32 heads, f16, the whole call: 26 us, with four tiles each 35,
+// with two 29; 64 x 64: 21, 27, 23)
 static int64_t prompt_splits(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (p->n_kv + PA_SLOTS - 1) / PA_SLOTS, base = (R + PA_ROWS - 1) / PA_ROWS * p->n_head_kv * p->ne3;
-    int64_t n = 512 / base, most = (tiles + 3) / 4;
+    int64_t n = 512 / base, most = tiles <= 4 ? 1 : tiles;
     if (n > most) n = most;
     if (n > 32) n = 32;
     return n < 1 ? 1 : n;
@@ -1308,9 +1314,9 @@ static int64_t prompt_splits(const mi355_fattn_args * p) {
 static int64_t prompt_chunks(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (R + PB_ROWS - 1) / PB_ROWS;
     const int64_t ws = prompt_slots(p->type_k, p->d), base = (p->n_kv + ws - 1) / ws * p->n_head_kv * p->ne3;
-    int64_t n = base > 0 ? 512 / base : 1, most = (tiles + 3) / 4;
+    int64_t n = base > 0 ? 512 / base : 1, most = tiles <= 4 ? 1 : tiles;
     if (n > most) n = most;
-    if (n > 64) n = 64;
+    if (n > 32) n = 32;
     return n < 1 ? 1 : n;
 }
 
@@ -1325,8 +1331,10 @@ template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hi
     MI355_CHECK_LAUNCH();
     MI355_LAUNCH("attn_mass_stats", (prompt_stats_kernel<TYPE, D>), dim3((unsigned)((R + PA_ROWS - 1) / PA_ROWS * a.nsplit), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
-    MI355_LAUNCH("attn_mass_rows", prompt_rows_kernel, dim3((unsigned)((R + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
-    MI355_CHECK_LAUNCH();
+    if (a.nsplit > 1) {
+        MI355_LAUNCH("attn_mass_rows", prompt_rows_kernel, dim3((unsigned)((R + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
+        MI355_CHECK_LAUNCH();
+    }
     MI355_LAUNCH("attn_mass", (prompt_mass_kernel<TYPE, D>), dim3((unsigned)((a.n_kv + ws - 1) / ws * a.nchunk), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
     if (a.nchunk == 1) return MI355_OK;
@@ -1352,8 +1360,8 @@ static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     if (p->n_q > MI355_MASS_MAX_Q) {
         w.nsplit = prompt_splits(p);
         w.nchunk = prompt_chunks(p);
-        w.stats = (w.nsplit * rows * 2 + 3) / 4 * 4;
-        w.part = (p->ne3 * p->n_head_kv * w.nchunk * p->n_kv + 3) / 4 * 4;
+        w.stats = w.nsplit > 1 ? (w.nsplit * rows * 2 + 3) / 4 * 4 : 0;
+        w.part = w.nchunk > 1 ? (p->ne3 * p->n_head_kv * w.nchunk * p->n_kv + 3) / 4 * 4 : 0;
         w.rowc = rows * 4;
         w.q = rows * step_d(p->d) / 2 * (p->type_k == MI355_TYPE_BF16 ? 3 : 2);
         w.cls = (p->mask ? p->m_ne2 * p->m_ne3 * p->n_q : 1) * class_pitch(p->n_kv) / 4;
