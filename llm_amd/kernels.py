@@ -13,6 +13,10 @@ LIB_PATH = os.path.join(_HERE, "lib", "libmi355_kernels.so")
 if not os.path.exists(LIB_PATH):
     raise ImportError(f"{LIB_PATH} is not built: run `make -C llm_amd/csrc` (or __graft_entry__.build()); "
                       "there is no CPU fallback for the MI355X kernels")
+try:                     # torch's HIP runtime first, where there is one: the library then binds to it and not to a second one of its own
+    import torch  # noqa: F401
+except ImportError:
+    pass
 lib = C.CDLL(LIB_PATH)
 
 _vp, _i64, _i32 = C.c_void_p, C.c_int64, C.c_int32

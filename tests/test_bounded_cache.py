@@ -140,3 +140,14 @@ def test_attention_mass_workspaces():
     assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=-1)[0]) == -1
     assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=100, m_ne2=0)[0]) == -1
     assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=100, m_ne2=0, mask=None)[0]) > 0
+
+
+def test_library_and_torch_share_one_hip_runtime():
+    """whichever is imported first: two runtimes in a process refuse each other's device"""
+    import os
+    import subprocess
+    import sys
+    code = ("import llm_amd.kernels, torch\n"
+            "libs = {l.split()[-1] for l in open('/proc/self/maps') if 'libamdhip64' in l}\n"
+            "assert len(libs) == 1, libs")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
