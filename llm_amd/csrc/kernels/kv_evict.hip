@@ -301,7 +301,8 @@ extern "C" {
 int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
     if (!p || (p->n_kv > 0 && (!p->mass || !p->slot_pos)) || !p->n_past || !p->kept) return MI355_E_NULL;
     if (!p->k != !p->k_out || !p->v != !p->v_out) return MI355_E_NULL;
-    if (p->n_kv < 0 || p->n_kv > 0x7fffffff || p->n_keep < 1 || p->n_keep > 0x7fffffff || p->n_evict < 0 || p->n_evict > 0x7fffffff) return MI355_E_SHAPE;
+    constexpr int64_t most = 1 << 30;                 // (32-bit slot numbers, a workgroup's stride past the last)
+    if (p->n_kv < 0 || p->n_kv > most || p->n_keep < 1 || p->n_keep > most || p->n_evict < 0 || p->n_evict > most) return MI355_E_SHAPE;
     if (p->n_sink < 0 || p->n_recent < 0 || (int64_t)p->n_sink + p->n_recent > p->n_keep) return MI355_E_SHAPE;
     if (p->n_head_kv < 1 || p->n_head_kv > 65535 || p->ne3 < 0 || p->ne3 > 65535) return MI355_E_SHAPE;
     const int64_t dv = p->dv ? p->dv : p->d;

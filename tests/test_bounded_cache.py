@@ -66,7 +66,7 @@ def evict_args(**kw):
 @pytest.mark.parametrize("code, kw", [
     (E_NULL, dict(mass=None)), (E_NULL, dict(slot_pos=None)), (E_NULL, dict(n_past=None)), (E_NULL, dict(kept=None)), (E_NULL, dict(k=None)),
     (E_NULL, dict(v_out=None)),
-    (E_SHAPE, dict(n_kv=-1)), (E_SHAPE, dict(n_kv=1 << 32)), (E_SHAPE, dict(n_keep=0)), (E_SHAPE, dict(n_evict=-1)), (E_SHAPE, dict(n_sink=-1)),
+    (E_SHAPE, dict(n_kv=-1)), (E_SHAPE, dict(n_kv=1 << 32)), (E_SHAPE, dict(n_kv=(1 << 30) + 1)), (E_SHAPE, dict(n_keep=(1 << 30) + 1)), (E_SHAPE, dict(n_evict=(1 << 30) + 1)), (E_SHAPE, dict(n_keep=0)), (E_SHAPE, dict(n_evict=-1)), (E_SHAPE, dict(n_sink=-1)),
     (E_SHAPE, dict(n_sink=26, n_recent=25)), (E_SHAPE, dict(n_recent=51)), (E_SHAPE, dict(n_sink=2 ** 31 - 1, n_recent=2 ** 31 - 1)),
     (E_SHAPE, dict(n_head_kv=0)), (E_SHAPE, dict(ne3=-1)), (E_SHAPE, dict(ne3=65536)), (E_SHAPE, dict(d=0)), (E_SHAPE, dict(type_kv=B.Q8_0, d=40)),
     (E_SHAPE, dict(type_kv=B.Q4_0, dv=8)), (E_TYPE, dict(type_kv=B.Q4_K)), (E_TYPE, dict(type_kv=99)),

@@ -496,6 +496,7 @@ def test_attention_mass_of_a_step(S, H, HK, n, slots, d, dv, t):
     (1, 8, 2, 17, 33, 64, B.F16), (1, 32, 8, 64, 1000, 128, B.F16), (2, 4, 1, 33, 300, 128, B.Q8_0), (1, 6, 2, 100, 100, 96, B.BF16), (1, 4, 4, 257, 257, 64, B.Q4_0),
     (1, 5, 1, 70, 515, 256, B.F16), (1, 2, 2, 9, 2049, 80, B.F16), (3, 8, 8, 12, 140, 128, B.BF16), (1, 64, 8, 10, 130, 128, B.Q4_0), (1, 4, 2, 300, 900, 128, B.F16),
     (1, 8, 1, 520, 520, 128, B.BF16), (1, 1, 1, 1, 5000, 128, B.Q8_0), (1, 3, 1, 130, 65, 8, B.F16),
+    (1, 4, 2, 20, 1, 128, B.F16), (1, 4, 1, 9, 31, 64, B.Q8_0), (2, 2, 1, 64, 64, 128, B.BF16), (1, 8, 8, 33, 257, 128, B.Q4_0), (1, 7, 1, 37, 511, 192, B.BF16),
 ])
 def test_attention_mass_of_a_prompt(S, H, HK, n, slots, d, t):
     q, k, _, mass = attn_case(S, H, HK, n, slots, d, 0, t, slots + n)
@@ -707,6 +708,16 @@ def test_attention_mass_of_blocks_at_every_alignment(t, G, n, d):
     for dst, mass, alone in res:
         assert ((dst.cpu().double() - wd).abs() <= ed).all() and ((mass.cpu().double() - wm).abs() <= em).all() and ((alone.cpu().double() - wm).abs() <= em).all()
         assert torch.equal(dst, res[0][0]) and torch.equal(mass, res[0][1])
+
+
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_mass_around_one_tile_a_wave(t, d):
+    """up to where one launch does it all and one slot beyond, with a full row tile and one row more"""
+    for slots in (31, 32, 33, 127, 128, 129, 255, 256, 257):
+        for H, HK, n in ((4, 4, 1), (16, 2, 2), (17, 1, 1)):
+            q, k, v, mass = attn_case(1, H, HK, n, slots, d, d, t, slots + H)
+            check_attn(q, k, v, t, causal(1, n, slots), 1 / math.sqrt(d), mass, 0.9)
 
 
 @pytest.mark.parametrize("t,d", [(B.Q4_0, 128), (B.F16, 64)])
