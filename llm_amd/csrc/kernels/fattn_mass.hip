@@ -810,9 +810,9 @@ static int64_t step_splits(const mi355_fattn_args * p) {
 // v_mfma_f32_32x32x16 throughout: K of f16 and bf16 as it is; blocks as d * q in two f16 parts, the slot's largest value brought to [2^14, 2^15) by
 // a power of two of its own.  What passes through LDS comes by DMA, two tiles ahead of the products.  A tile that the mask hides from all rows of a
 // wave (half of a causal prompt) costs its loads.
-// 64 queries x 32 heads over 16384 f16 slots: 5 + 24 + 5 + 33 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
+// 64 queries x 32 heads over 16384 f16 slots: 5 + 25 + 5 + 32 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
 // until the first tile of 512 workgroups is there; without its products the first pass takes 20, without its exponentials 23.  2047
-// causal queries, bf16: 16 + 67 + 5 + 87 + 5 us, 45 a pass at that rate.
+// causal queries, bf16: 16 + 68 + 83 + 5 us, 45 a pass at that rate.
 typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int PT = 256;                  // threads: 4 waves
 constexpr int PA_ROWS = 128, PA_SLOTS = 64, PB_ROWS = 32;
@@ -1259,8 +1259,10 @@ prompt_mass_kernel(const MArgs a) {
             if (!__all(zero)) {
                 const int r = t * PB_ROWS + lr < R ? t * PB_ROWS + lr : R - 1, iq = m_query(a, r);
                 const char * mrow = m_mask(a, iq, hk * a.ratio + r - iq * a.ratio, i3);
+                int jm = j0;
+                asm volatile("" : "+v"(jm));                    // (the comparisons of its slots with the last one would be kept through the loop)
 #pragma unroll
-                for (int u = 0; u < NS; u++) tile_logits(a, c[u], sc, c4.slope, cu[u], mrow, m8, j0 + 32 * u);
+                for (int u = 0; u < NS; u++) tile_logits(a, c[u], sc, c4.slope, cu[u], mrow, m8, jm + 32 * u);
                 sc = 1.0f;
             }
 #pragma unroll
@@ -1310,7 +1312,7 @@ static int64_t prompt_splits(const mi355_fattn_args * p) {
     if (n > 32) n = 32;
     return n < 1 ? 1 : n;
 }
-// Slices of the rows in the second: likewise (2047 x 2047: 87 us, with 1024 93, with 768 104; 64 x 16384: 34, with 1024 38)
+// Slices of the rows in the second: likewise (2047 x 2047: 87 us, with 1024 93, with 768 104; 64 x 16384: 34, with 1024 38; both since 83, 32)
 static int64_t prompt_chunks(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (R + PB_ROWS - 1) / PB_ROWS;
     const int64_t ws = prompt_slots(p->type_k, p->d), base = (p->n_kv + ws - 1) / ws * p->n_head_kv * p->ne3;
