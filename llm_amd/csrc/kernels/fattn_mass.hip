@@ -807,8 +807,7 @@ static int64_t step_splits(const mi355_fattn_args * p) {
 //   prompt_mass   S^T again and sum over the rows of 2^(s - m) / l: a wave holds 32 or 64 slots of K, Q passes through LDS; the sums stay in
 //                 registers, one per (slot, lane), and meet across the lanes once at the end
 //   prompt_sum    the row chunks' sums and decay * mass_in, in a fixed order
-// v_mfma_f32_32x32x16 throughout: K of f16 and bf16 as it is; blocks as d * q in two f16 parts, the slot's largest value brought to [2^14, 2^15) by
-// a power of two of its own.  What passes through LDS comes by DMA, two tiles ahead of the products.  A tile that the mask hides from all rows of a
+// v_mfma_f32_32x32x16 throughout: K of f16 and bf16 as it is; blocks as their integers, whose products a block's scale is put on in f32.  What passes through LDS comes by DMA, two tiles ahead of the products.  A tile that the mask hides from all rows of a
 // wave (half of a causal prompt) costs its loads.
 // 64 queries x 32 heads over 16384 f16 slots: 5 + 25 + 5 + 32 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
 // until the first tile of 512 workgroups is there; without its products the first pass takes 20, without its exponentials 23.  2047
@@ -913,23 +912,16 @@ prompt_prep_kernel(const MArgs a, uint32_t class_wgs, uint32_t slot_wgs, uint32_
     if (lane == 0) { a.rowc[row].qe = ldexpf(1.0f, e); a.rowc[row].slope = m_slope(a, h) * LOG2E; }
 }
 
-// 8 features of a block row on their way to two f16 parts: what is loaded, and its values
-template <int TYPE> struct KChunk {
-    Chunk<TYPE> c; uint16_t d;
-    __device__ __forceinline__ void load(const char * row, int j) { c.load(row + Chunk<TYPE>::at(j)); d = *(const uint16_t *)(row + (j >> 2) * Fmt<TYPE>::block); }
-    __device__ __forceinline__ float values(int j, float * v) const {      // returns the largest magnitude
-        const h8 q = __builtin_bit_cast(h8, c.operand(j));
-        const float dd = h2f(d);
-        float m = 0.0f;
+// blocks: the products of a 32-block's integers take their slots' scales (of the 16 slots that this lane's accumulator holds) and join the sums
+static __device__ __forceinline__ void fold_block(const uint16_t * scales, int lh, const v16f & part, v16f & c) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-        for (int i = 0; i < 8; i++) { v[i] = (float)q[i] * dd; m = fmaxf(m, fabsf(v[i])); }
-        return m;
+    for (int q = 0; q < 4; q++) {
+        const h4 d = *(const h4 *)(scales + 8 * q + 4 * lh);
+#pragma unroll
+        for (int i = 0; i < 4; i++) c[4 * q + i] = __builtin_fmaf(part[4 * q + i], (float)d[i], c[4 * q + i]);
     }
-};
-static __device__ __forceinline__ void to_parts(float * v, int e, v4i * out) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = ldexpf(v[i], -e);
-    split8<false, 2>(v, out);
+    asm volatile("" : "+v"(c));                                 // (put off, the sums of all blocks would have to be held: they do not fit)
 }
 
 // logits (log2 domain) of a 32 x 32 tile from slot j0 on, in place of its products: sc what they lack, cl the tile's class for this lane's query
@@ -976,10 +968,10 @@ template <int TYPE, int D>
 __global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
 prompt_stats_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
-    constexpr int KS = D / 16, QP = F::parts, KP = F::quant ? 2 : 1, S = F::quant ? 2 : 3;      // S: tiles in LDS
+    constexpr int KS = D / 16, QP = F::parts, S = F::quant ? 2 : 3;      // S: tiles in LDS
     constexpr int RS = PT / (D / 8), CN = PA_SLOTS / RS;        // rows a pass of the workgroup's chunks covers, passes of a tile
-    __shared__ __attribute__((aligned(16))) uint8_t kt[S][KP][PA_SLOTS * D * 2];
-    __shared__ __attribute__((aligned(16))) float ksc[F::quant ? S : 1][PA_SLOTS];
+    __shared__ __attribute__((aligned(16))) uint8_t kt[S][PA_SLOTS * D * 2];
+    __shared__ __attribute__((aligned(16))) uint16_t kd[F::quant ? S : 1][F::quant ? D / 32 : 1][PA_SLOTS];
     __shared__ uint32_t cl[S][PT / 64][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
     const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, split = blockIdx.x % a.nsplit;      // the last rows first: a causal mask lets them see most
@@ -1002,7 +994,8 @@ prompt_stats_kernel(const MArgs a) {
 
     // this lane's chunk of a pass: chunks past the head size re-read the last one and meet zeros of q, slots past the end the last one and are hidden
     const int pos = tid % (D / 8), j_ = tid / (D / 8), c_ = F::quant ? pos : pos ^ (j_ & swz<D>()), cc = c_ < a.d / 8 ? c_ : a.d / 8 - 1;
-    KChunk<F::quant ? TYPE : (int)MI355_TYPE_Q8_0> kr[F::quant ? CN : 1];
+    Chunk<F::quant ? TYPE : (int)MI355_TYPE_Q8_0> kr[F::quant ? CN : 1];
+    uint16_t kdr[F::quant ? CN : 1];
     uint64_t off[CN];                                           // of this lane's chunks in a tile
 #pragma unroll
     for (int i = 0; i < CN; i++) off[i] = (uint64_t)(uint32_t)(j_ + RS * i) * a.k_nb1 + (F::quant ? 0 : cc * 16);
@@ -1019,7 +1012,7 @@ prompt_stats_kernel(const MArgs a) {
         }
         if constexpr (F::quant) {
 #pragma unroll
-            for (int i = 0; i < CN; i++) kr[i].load(src[i], cc);
+            for (int i = 0; i < CN; i++) { kr[i].load(src[i] + Chunk<TYPE>::at(cc)); kdr[i] = *(const uint16_t *)(src[i] + (cc >> 2) * F::block); }
         } else {
 #pragma unroll
             for (int i = 0; i < CN; i++) dma16(src[i], klds + b * (PA_SLOTS * D * 2) + i * (PT * 16));
@@ -1030,16 +1023,8 @@ prompt_stats_kernel(const MArgs a) {
         if constexpr (F::quant) {
 #pragma unroll
             for (int i = 0; i < CN; i++) {
-                const int j = j_ + RS * i;
-                float v[8], m = kr[i].values(cc, v);
-#pragma unroll
-                for (int o = 1; o < D / 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-                const int e = row_exp(m);
-                v4i p[2];
-                to_parts(v, e, p);
-#pragma unroll
-                for (int q = 0; q < KP; q++) *(v4i *)(kt[b][q] + lds_chunk<D>(j, pos)) = p[q];
-                if (pos == 0) ksc[b][j] = ldexpf(1.0f, e);
+                *(v4i *)(kt[b] + lds_chunk<D>(j_ + RS * i, pos)) = kr[i].operand(cc);
+                if ((pos & 3) == 0) kd[b][pos >> 2][j_ + RS * i] = kdr[i];
             }
         }
     };
@@ -1061,25 +1046,25 @@ prompt_stats_kernel(const MArgs a) {
         const uint32_t bytes = cl[b][wave][lane] >> (16 * (t & 1));
         const int c0 = bytes & 255, c1 = bytes >> 8 & 255;
         if (mine && __any((c0 | c1) != MASK_HIDDEN)) {
-            v16f c[2];
+            v16f c[2], part;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
-                    const int at = lds_chunk<D>(32 * u + lr, 2 * ks + lh);
-                    const v4i k0 = *(const v4i *)(kt[b][0] + at);
-                    if constexpr (KP == 2) c[u] = mfma32<F::bf>(*(const v4i *)(kt[b][KP - 1] + at), qf[ks][0], c[u]);
+                    const v4i k0 = *(const v4i *)(kt[b] + lds_chunk<D>(32 * u + lr, 2 * ks + lh));
+                    if constexpr (F::quant) {
+                        if (ks % 2 == 0) {
 #pragma unroll
-                    for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(k0, qf[ks][p], c[u]);
-                }
-                if constexpr (F::quant) {
+                            for (int i = 0; i < 16; i++) part[i] = 0.0f;
+                        }
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const v4f x = *(const v4f *)&ksc[b][32 * u + 8 * q + 4 * lh];
+                        for (int p = QP - 1; p >= 0; p--) part = mfma32<F::bf>(k0, qf[ks][p], part);
+                        if (ks % 2 == 1) fold_block(&kd[b][ks / 2][32 * u], lh, part, c[u]);
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) c[u][4 * q + i] *= x[i];
+                        for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(k0, qf[ks][p], c[u]);
                     }
                 }
             }
@@ -1137,19 +1122,19 @@ prompt_rows_kernel(const MArgs a) {
 }
 
 // slots of a wave in the second pass: 64 where its K takes at most 64 registers so
-template <int TYPE, int D> constexpr int prompt_ns() { return D * (Fmt<TYPE>::quant ? 2 : 1) <= 128 ? 2 : 1; }
+template <int D> constexpr int prompt_ns() { return D <= 128 ? 2 : 1; }
 
 template <int TYPE, int D>
 __global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
 prompt_mass_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
-    constexpr int NS = prompt_ns<TYPE, D>();
-    constexpr int KS = D / 16, QP = F::parts, KP = F::quant ? 2 : 1, S = D <= 128 ? 3 : 2;      // S: tiles in LDS
+    constexpr int NS = prompt_ns<D>();
+    constexpr int KS = D / 16, QP = F::parts, S = D <= 128 ? 3 : 2;      // S: tiles in LDS
     constexpr int RS = PT / (D / 8), CP = PB_ROWS / RS, CN = QP * CP;       // passes of a part, of a tile
     __shared__ __attribute__((aligned(16))) uint8_t qt[S][QP][PB_ROWS * D * 2];
     __shared__ __attribute__((aligned(16))) float rc[S][PT / 64][64];       // RowC of the rows, twice
     __shared__ uint32_t cl[S][PT / 64][64];
-    __shared__ __attribute__((aligned(16))) float ksc[F::quant ? 128 * NS : 4];
+    __shared__ __attribute__((aligned(16))) uint16_t kd[F::quant ? PT / 64 : 1][F::quant ? D / 32 : 1][32 * NS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
     const int R = a.ratio * a.n_q, hk = blockIdx.y, i3 = blockIdx.z, chunk = blockIdx.x % a.nchunk;
     const int j0 = ((int)(turned() ? gridDim.x - 1 - blockIdx.x : blockIdx.x) / a.nchunk * 4 + wave) * 32 * NS;     // this wave's slots
@@ -1184,30 +1169,24 @@ prompt_mass_kernel(const MArgs a) {
     if (S == 3 && t + nc < nt) fetch(t + nc, 1);
 
     // this wave's K rows, as the A operand holds them
-    v4i kf[NS][KS][KP];
+    v4i kf[NS][KS];
 #pragma unroll
     for (int u = 0; u < NS; u++) {
         const int j = j0 + 32 * u + lr;
         const char * krow = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
-        auto chunk_at = [&](int ks) { return 2 * ks + lh < a.d / 8 ? 2 * ks + lh : a.d / 8 - 1; };
-        if constexpr (F::quant) {
-            float m = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) { KChunk<TYPE> c; float v[8]; c.load(krow, chunk_at(ks)); m = fmaxf(m, c.values(chunk_at(ks), v)); }
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            const int e = row_exp(m);
-            ksc[(wave * NS + u) * 32 + lr] = ldexpf(1.0f, e);
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) { KChunk<TYPE> c; float v[8]; c.load(krow, chunk_at(ks)); c.values(chunk_at(ks), v); to_parts(v, e, kf[u][ks]); }
-        } else {
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) kf[u][ks][0] = *(const v4i *)(krow + chunk_at(ks) * 16);
+        for (int ks = 0; ks < KS; ks++) {
+            const int cc = 2 * ks + lh < a.d / 8 ? 2 * ks + lh : a.d / 8 - 1;
+            Chunk<TYPE> c;
+            c.load(krow + Chunk<TYPE>::at(cc));
+            kf[u][ks] = c.operand(cc);
+            if constexpr (F::quant) if (ks % 2 == 0 && lh == 0) kd[wave][ks / 2][32 * u + lr] = *(const uint16_t *)(krow + (cc >> 2) * F::block);
         }
     }
 #pragma unroll
     for (int u = 0; u < NS; u++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) arrived(kf[u][ks][0]);
+        for (int ks = 0; ks < KS; ks++) arrived(kf[u][ks]);
     float acc[NS][16];
 #pragma unroll
     for (int u = 0; u < NS; u++)
@@ -1227,7 +1206,7 @@ prompt_mass_kernel(const MArgs a) {
         if (__any(seen != MASK_HIDDEN)) {
             RowC c4 = *(const RowC *)&rc[b][0][4 * lr];
             if (t * PB_ROWS + lr >= R) { c4.m = INFINITY; c4.inv = 0.0f; }      // weighs nothing
-            v16f c[NS];
+            v16f c[NS], part[NS];
 #pragma unroll
             for (int u = 0; u < NS; u++)
 #pragma unroll
@@ -1235,25 +1214,25 @@ prompt_mass_kernel(const MArgs a) {
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 v4i q[QP];
+                if constexpr (F::quant) if (ks % 2 == 0) {
+#pragma unroll
+                    for (int u = 0; u < NS; u++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) part[u][i] = 0.0f;
+                }
 #pragma unroll
                 for (int p = 0; p < QP; p++) q[p] = *(const v4i *)(qt[b][p] + lds_chunk<D>(lr, 2 * ks + lh));
 #pragma unroll
                 for (int p = QP - 1; p >= 0; p--)
 #pragma unroll
                     for (int u = 0; u < NS; u++) {
-                        if constexpr (KP == 2) if (p == 0) c[u] = mfma32<F::bf>(kf[u][ks][KP - 1], q[0], c[u]);
-                        c[u] = mfma32<F::bf>(kf[u][ks][0], q[p], c[u]);
+                        if constexpr (F::quant) part[u] = mfma32<F::bf>(kf[u][ks], q[p], part[u]);
+                        else c[u] = mfma32<F::bf>(kf[u][ks], q[p], c[u]);
                     }
-            }
-            if constexpr (F::quant) {
+                if constexpr (F::quant) if (ks % 2 == 1) {
 #pragma unroll
-                for (int u = 0; u < NS; u++)
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const v4f x = *(const v4f *)&ksc[(wave * NS + u) * 32 + 8 * q + 4 * lh];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) c[u][4 * q + i] *= x[i];
-                    }
+                    for (int u = 0; u < NS; u++) fold_block(&kd[wave][ks / 2][32 * u], lh, part[u], c[u]);
+                }
             }
             float sc = c4.qe;
             if (!__all(zero)) {
@@ -1298,8 +1277,8 @@ prompt_sum_kernel(const MArgs a) {
     mass_store(a, hk, i3, j, t);
 }
 
-static int prompt_slots(int type, int64_t d) {           // slots of a workgroup in the second pass
-    return step_d(d) * (type == MI355_TYPE_Q8_0 || type == MI355_TYPE_Q4_0 ? 2 : 1) <= 128 ? 256 : 128;
+static int prompt_slots(int64_t d) {                     // slots of a workgroup in the second pass
+    return step_d(d) <= 128 ? 256 : 128;
 }
 // Slices of the slots in the first pass: 512 workgroups, one round of two a CU (2047 x 2047: 67 us, with 1024 80, with 2048 87) and few
 // slices to join (64: 8 us, 32: 5).  Small problems: a tile takes a workgroup that has the CU to itself 1.3 us, the launch that joins slices 4 -- up to 4
@@ -1315,7 +1294,7 @@ static int64_t prompt_splits(const mi355_fattn_args * p) {
 // Slices of the rows in the second: likewise (2047 x 2047: 87 us, with 1024 93, with 768 104; 64 x 16384: 34, with 1024 38; both since 83, 32)
 static int64_t prompt_chunks(const mi355_fattn_args * p) {
     const int64_t R = p->n_head / p->n_head_kv * p->n_q, tiles = (R + PB_ROWS - 1) / PB_ROWS;
-    const int64_t ws = prompt_slots(p->type_k, p->d), base = (p->n_kv + ws - 1) / ws * p->n_head_kv * p->ne3;
+    const int64_t ws = prompt_slots(p->d), base = (p->n_kv + ws - 1) / ws * p->n_head_kv * p->ne3;
     int64_t n = base > 0 ? 512 / base : 1, most = tiles <= 4 ? 1 : tiles;
     if (n > most) n = most;
     if (n > 32) n = 32;
@@ -1323,7 +1302,7 @@ static int64_t prompt_chunks(const mi355_fattn_args * p) {
 }
 
 template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hipStream_t s) {
-    const int R = a.ratio * a.n_q, ws = 128 * prompt_ns<TYPE, D>();
+    const int R = a.ratio * a.n_q, ws = 128 * prompt_ns<D>();
     const unsigned hk = (unsigned)a.n_head_kv, z = (unsigned)ne3;
     const int64_t slot_wgs = (a.n_kv + 1023) / 1024, query_wgs = a.mask ? (a.n_q + 3) / 4 : 1, class_wgs = slot_wgs * query_wgs * a.m_ne2 * a.m_ne3;
     const int64_t row_wgs = (R + 15) / 16, prep = class_wgs + row_wgs * hk * z;
