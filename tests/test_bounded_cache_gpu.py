@@ -496,12 +496,21 @@ def test_attention_mass_of_a_step(S, H, HK, n, slots, d, dv, t):
     (1, 8, 2, 17, 33, 64, B.F16), (1, 32, 8, 64, 1000, 128, B.F16), (2, 4, 1, 33, 300, 128, B.Q8_0), (1, 6, 2, 100, 100, 96, B.BF16), (1, 4, 4, 257, 257, 64, B.Q4_0),
     (1, 5, 1, 70, 515, 256, B.F16), (1, 2, 2, 9, 2049, 80, B.F16), (3, 8, 8, 12, 140, 128, B.BF16), (1, 64, 8, 10, 130, 128, B.Q4_0), (1, 4, 2, 300, 900, 128, B.F16),
     (1, 8, 1, 520, 520, 128, B.BF16), (1, 1, 1, 1, 5000, 128, B.Q8_0), (1, 3, 1, 130, 65, 8, B.F16),
-    (1, 4, 2, 20, 1, 128, B.F16), (1, 4, 1, 9, 31, 64, B.Q8_0), (2, 2, 1, 64, 64, 128, B.BF16), (1, 8, 8, 33, 257, 128, B.Q4_0), (1, 7, 1, 37, 511, 192, B.BF16),
+    (8, 64, 64, 9, 300, 64, B.F16), (1, 4, 2, 20, 1, 128, B.F16), (1, 4, 1, 9, 31, 64, B.Q8_0), (2, 2, 1, 64, 64, 128, B.BF16), (1, 8, 8, 33, 257, 128, B.Q4_0), (1, 7, 1, 37, 511, 192, B.BF16),
 ])
 def test_attention_mass_of_a_prompt(S, H, HK, n, slots, d, t):
     q, k, _, mass = attn_case(S, H, HK, n, slots, d, 0, t, slots + n)
     check_attn(q, k, None, t, causal(S, n, slots), 1 / math.sqrt(d), mass, 1.0)
     check_attn(q, k, None, t, None, 1 / math.sqrt(d), None, 1.0)
+
+
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_mass_of_prompts_that_fill_the_card(t, d):
+    """so many heads that a workgroup has many tiles of slots and of rows: they go round the places in LDS several times"""
+    S, H, HK, n, slots = 2, 32, 16, 200, 1000
+    q, k, _, mass = attn_case(S, H, HK, n, slots, d, 0, t, d)
+    check_attn(q, k, None, t, causal(S, n, slots, [slots, 700]), 1 / math.sqrt(d), mass, 1.0)
 
 
 @pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
@@ -708,6 +717,25 @@ def test_attention_mass_of_blocks_at_every_alignment(t, G, n, d):
     for dst, mass, alone in res:
         assert ((dst.cpu().double() - wd).abs() <= ed).all() and ((mass.cpu().double() - wm).abs() <= em).all() and ((alone.cpu().double() - wm).abs() <= em).all()
         assert torch.equal(dst, res[0][0]) and torch.equal(mass, res[0][1])
+
+
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
+def test_attention_mass_of_a_prompt_over_strided_caches(t, d):
+    """slot-major caches whose rows lie an odd number of the smallest allowed units apart, q as [token, head, d], a mask of odd pitch per sequence"""
+    S, H, HK, n, slots = 2, 6, 2, 21, 201
+    k, q = cache((S, HK, slots, d), t, gen(d)), torch.randn((S, n, H, d), generator=gen(d + 1))
+    width, unit = (k.shape[-1], 8) if t in DTYPE else (k.shape[-1], 2)          # values of 16 bits in 16-byte steps, bytes in 2-byte steps
+    off, pitch = 3 * unit, (HK * width + unit + 2 * unit - 1) // (2 * unit) * 2 * unit + unit
+    raw = torch.full((S * slots * pitch + off + 64,), 255, dtype=torch.uint8, device="cuda") if t not in DTYPE else torch.full((S * slots * pitch + off + 64,), float("nan"), dtype=k.dtype, device="cuda")
+    kg = raw.as_strided((S, HK, slots, width), (slots * pitch, width, pitch, 1), off)
+    kg.copy_(k)
+    mask = causal(S, n, slots, [slots, 100])
+    wide = torch.full((S, 1, n, slots + 6), float("-inf")).half().cuda()
+    wide[..., :slots] = mask.cuda()
+    _, _, wm, em = attn_oracle(q.transpose(1, 2), values(k, t), None, mask, 0.1, None, 0.0)
+    got = ops.attn_mass(q.cuda().transpose(1, 2), kg, wide[..., :slots], t, 0.1)
+    assert ((got.cpu().double() - wm).abs() <= em).all()
 
 
 @pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
