@@ -778,7 +778,9 @@ MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stre
  * head)^2 x queries below 2^32, else MI355_E_SHAPE; block rows 2-byte aligned, faster where a row's address is a multiple of d / 16).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be
  * mass_out itself; NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate (the query is not rounded to the cache's type, the
  * weights are not rounded before they meet V).  A slot hidden by the mask takes no part whatever its row holds; a query that sees no slot gives
- * a row of zeros and no weight.  workspace: *_workspace_bytes, 16-byte aligned, no initial contents, not shared by calls that can overlap. */
+ * a row of zeros and no weight.  At least one query and one sequence, at most 65535 of each, else MI355_E_SHAPE (ops.* answer a call of none themselves).
+ * workspace: *_workspace_bytes (-1 for sizes and types that the call itself refuses), 16-byte aligned, no initial contents, not shared by calls
+ * that can overlap. */
 #define MI355_MASS_MAX_Q 8
 typedef struct mi355_attn_mass_args {
     const float *mass_in; int64_t in_nb2, in_nb3;
@@ -788,7 +790,8 @@ typedef struct mi355_attn_mass_args {
 MI355_API int64_t mi355_flash_attn_ext_mass_workspace_bytes(const mi355_fattn_args *args);
 MI355_API int     mi355_flash_attn_ext_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace,
                                             int64_t workspace_bytes, void *stream);
-/* The weights alone, for any number of queries (a prompt, or the last ones of it): v, dst and dv of args are not used. */
+/* The weights alone, for up to 65535 queries (a prompt, or the last ones of it; a longer prompt in pieces, with a decay of 1 and mass_in = mass_out):
+ * v, dst and dv of args are not used. */
 MI355_API int64_t mi355_attn_mass_workspace_bytes(const mi355_fattn_args *args);
 MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace, int64_t workspace_bytes,
                                   void *stream);

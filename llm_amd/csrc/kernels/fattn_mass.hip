@@ -1358,14 +1358,8 @@ static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     }
     return w;
 }
-static int64_t mass_workspace(const mi355_fattn_args * p, bool with_dst) {
-    if (!p || p->n_q < 0 || p->n_kv < 0 || (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1)) || p->n_head < 1 || p->n_head_kv < 1 || p->n_head % p->n_head_kv || p->ne3 < 1 || p->d < 8 || p->d > 256) return -1;
-    const WsParts w = mass_parts(p, with_dst);
-    return (w.stats + w.part + w.logits + w.rowc + w.q + w.cls) * 4;
-}
-
-static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, bool with_dst, void * workspace, int64_t workspace_bytes, void * stream) {
-    if (!p || !w || !p->q || (p->n_kv > 0 && (!p->k || !w->mass_out)) || (with_dst && (!p->dst || (p->n_kv > 0 && !p->v)))) return MI355_E_NULL;
+// the shapes and types that both entry points take; what the workspace's size is formed from is bounded here, so its products stay within 64 bits
+static int mass_shape(const mi355_fattn_args * p, bool with_dst) {
     const int64_t dv = p->dv ? p->dv : p->d;
     if (p->d < 8 || p->d > 256 || p->d % 8 != 0) return MI355_E_UNSUPPORTED;
     if (with_dst && (dv < 8 || dv > p->d || dv % 8 != 0)) return MI355_E_UNSUPPORTED;
@@ -1379,6 +1373,22 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     if (ratio * ratio * p->n_q > 0xffffffffll) return MI355_E_SHAPE;
     if (with_dst && p->n_q > MI355_MASS_MAX_Q) return MI355_E_UNSUPPORTED;
     if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1 || p->m_ne2 > 65535 || p->m_ne3 > 65535 || p->m_ne2 * p->m_ne3 > 65535)) return MI355_E_SHAPE;
+    // steps keep a logit per (row, slot): more than 2^56 of them are no memory's size
+    if (p->n_q <= MI355_MASS_MAX_Q && p->ne3 * p->n_head * p->n_q > (1ll << 56) / (p->n_kv + 4)) return MI355_E_SHAPE;
+    return MI355_OK;
+}
+static int64_t mass_workspace(const mi355_fattn_args * p, bool with_dst) {
+    if (!p || mass_shape(p, with_dst) != MI355_OK) return -1;
+    const WsParts w = mass_parts(p, with_dst);
+    return (w.stats + w.part + w.logits + w.rowc + w.q + w.cls) * 4;
+}
+
+static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, bool with_dst, void * workspace, int64_t workspace_bytes, void * stream) {
+    if (!p || !w || !p->q || (p->n_kv > 0 && (!p->k || !w->mass_out)) || (with_dst && (!p->dst || (p->n_kv > 0 && !p->v)))) return MI355_E_NULL;
+    const int shape = mass_shape(p, with_dst);
+    if (shape != MI355_OK) return shape;
+    const int64_t dv = p->dv ? p->dv : p->d, ratio = p->n_head / p->n_head_kv;
+    const bool quant = p->type_k == MI355_TYPE_Q8_0 || p->type_k == MI355_TYPE_Q4_0;
     if (p->k_nb1 < 0 || p->k_nb1 > 0x7fffffff || (with_dst && (p->v_nb1 < 0 || p->v_nb1 > 0x7fffffff))) return MI355_E_SHAPE;
     const int64_t f32s = (int64_t)(uintptr_t)p->q | p->q_nb1 | p->q_nb2 | p->q_nb3 |
                          (with_dst ? (int64_t)(uintptr_t)p->dst | p->d_nb1 | p->d_nb2 | p->d_nb3 : 0) | (int64_t)(uintptr_t)workspace;

@@ -712,12 +712,19 @@ def _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bi
     return a, K.AttnMassArgs(ip, ns[1] * 4, ns[0] * 4, mass_out.data_ptr(), os[1] * 4, os[0] * 4, decay), dst, mass_out
 
 
+def _no_queries(mass, decay, mass_out):
+    """mass_out of a call without queries: what the earlier ones left"""
+    return mass_out.zero_() if mass is None or decay == 0.0 else torch.mul(mass, decay, out=mass_out)
+
+
 def flash_attn_ext_mass(q, k, v, mask, type_kv, scale, mass=None, decay=1.0, mass_out=None, max_bias=0.0, logit_softcap=0.0):
     """A decode step's attention and the weight every slot draws (mi355_flash_attn_ext_mass).  q f32 [seqs, heads, tokens <= 8, d], k, v
     [seqs, kv heads, slots, row] of type_kv, mask f16 [seqs | 1, heads | 1, >= tokens, slots] (or [seqs | 1, tokens, slots], [tokens, slots],
     None); mass f32 [seqs, kv heads, slots] or None; mass_out may be mass -> (f32 [seqs, tokens, heads, dv], mass_out = decay mass + weights)."""
     dev = torch.cuda.current_device()
     a, w, dst, mass_out = _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
+    if a.n_q == 0 or a.ne3 == 0:
+        return dst, _no_queries(mass, decay, mass_out)
     need = K.lib.mi355_flash_attn_ext_mass_workspace_bytes(a)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
     rc = K.lib.mi355_flash_attn_ext_mass(a, w, ws.data_ptr(), need, _raw_stream(dev))
@@ -727,9 +734,11 @@ def flash_attn_ext_mass(q, k, v, mask, type_kv, scale, mass=None, decay=1.0, mas
 
 
 def attn_mass(q, k, mask, type_kv, scale, mass=None, decay=1.0, mass_out=None, max_bias=0.0, logit_softcap=0.0):
-    """The weight every slot draws from any number of queries (mi355_attn_mass); arguments as flash_attn_ext_mass, without V -> mass_out."""
+    """The weight every slot draws from up to 65535 queries (mi355_attn_mass); arguments as flash_attn_ext_mass, without V -> mass_out."""
     dev = torch.cuda.current_device()
     a, w, _, mass_out = _mass_args(dev, q, k, None, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
+    if a.n_q == 0 or a.ne3 == 0:
+        return _no_queries(mass, decay, mass_out)
     need = K.lib.mi355_attn_mass_workspace_bytes(a)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
     rc = K.lib.mi355_attn_mass(a, w, ws.data_ptr(), need, _raw_stream(dev))

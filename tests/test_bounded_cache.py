@@ -142,6 +142,24 @@ def test_attention_mass_workspaces():
     assert K.lib.mi355_attn_mass_workspace_bytes(attn_args(n_q=100, m_ne2=0, mask=None)[0]) > 0
 
 
+@pytest.mark.parametrize("n_kv", [0, 200, 512, 100000])
+@pytest.mark.parametrize("kw", [dict(n_q=0), dict(n_q=0, d=256), dict(ne3=0), dict(n_q=0, mask=None)])
+def test_attention_mass_workspaces_of_no_queries(n_kv, kw):
+    """answered, not divided by: the size is asked for before the call itself can refuse"""
+    a, w = attn_args(n_kv=n_kv, **kw)
+    for size, run in ((K.lib.mi355_flash_attn_ext_mass_workspace_bytes, K.lib.mi355_flash_attn_ext_mass), (K.lib.mi355_attn_mass_workspace_bytes, K.lib.mi355_attn_mass)):
+        assert size(a) == -1 and run(a, w, P, 1 << 40, None) == E_SHAPE
+
+
+@pytest.mark.parametrize("kw", [dict(n_head=65535, n_head_kv=65535, n_q=8, ne3=65535, n_kv=1 << 30), dict(n_head=60000, n_head_kv=60000, ne3=60000, n_kv=1 << 30),
+                                dict(n_q=1 << 40), dict(n_kv=1 << 40), dict(ne3=1 << 40), dict(n_q=100, m_ne2=1 << 20, m_ne3=1 << 20)])
+def test_attention_mass_workspaces_past_64_bits(kw):
+    """a size whose product would wrap is refused by the size and by the call"""
+    a, w = attn_args(**kw)
+    for size, run in ((K.lib.mi355_flash_attn_ext_mass_workspace_bytes, K.lib.mi355_flash_attn_ext_mass), (K.lib.mi355_attn_mass_workspace_bytes, K.lib.mi355_attn_mass)):
+        assert size(a) == -1 and run(a, w, P, 1 << 62, None) in (E_SHAPE, E_UNSUPPORTED)
+
+
 def test_library_and_torch_share_one_hip_runtime():
     """whichever is imported first: two runtimes in a process refuse each other's device"""
     import os

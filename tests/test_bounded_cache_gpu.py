@@ -678,6 +678,21 @@ def test_attention_mass_wrapper_refuses_what_does_not_fit():
         ops.flash_attn_ext_mass(q[:, :3], k, v, None, B.F16, 0.1)
 
 
+@pytest.mark.parametrize("S,n,slots", [(1, 0, 5), (2, 0, 512), (1, 0, 100000), (0, 1, 512), (0, 40, 300), (1, 0, 0)])
+def test_attention_mass_of_no_queries(S, n, slots):
+    """an empty batch: an empty dst, and what earlier calls left, decayed"""
+    q = torch.zeros((S, 8, n, 64), device="cuda")
+    k = torch.zeros((S, 2, slots, 64), dtype=torch.float16, device="cuda")
+    mass = torch.rand((S, 2, slots), device="cuda")
+    for m, decay, want in ((mass, 0.5, mass * 0.5), (None, 1.0, mass * 0), (mass * float("nan"), 0.0, mass * 0)):
+        assert torch.equal(ops.attn_mass(q, k, None, B.F16, 0.1, mass=m, decay=decay), want)
+        if n <= 8:
+            dst, out = ops.flash_attn_ext_mass(q, k, k, None, B.F16, 0.1, mass=m, decay=decay)
+            assert dst.shape == (S, n, 8, 64) and torch.equal(out, want)
+    got = mass.clone()
+    assert ops.attn_mass(q, k, None, B.F16, 0.1, mass=got, decay=0.25, mass_out=got) is got and torch.equal(got, mass * 0.25)
+
+
 @pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
 @pytest.mark.parametrize("n", [2, 40])
 def test_attention_mass_hidden_rows_may_be_huge(t, n):
