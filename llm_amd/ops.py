@@ -519,6 +519,7 @@ def set_rows(src, ids, dst, type_dst):
 _KV_DTYPE = {B.F32: torch.float32, B.F16: torch.float16, B.BF16: torch.bfloat16, B.Q8_0: torch.uint8, B.Q4_0: torch.uint8}
 _KV_BYTES = {B.F32: 4, B.F16: 2, B.BF16: 2, B.Q8_0: 1, B.Q4_0: 1}          # of a cache tensor's element
 _BLOCK = {B.Q8_0: 34, B.Q4_0: 18}
+_MASK_DTYPE = (torch.float16, torch.int16, torch.uint16)
 
 
 # The entry points of the bounded KV cache are called once per layer and step: their wrappers read every tensor's shape and strides once.
@@ -687,8 +688,8 @@ def _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bi
         if len(sh) < 4:                       # the two first dimensions may be left out, or the heads'
             sh, st = ((1, 1) + sh, (0, 0) + st) if len(sh) == 2 else ((sh[0], 1) + sh[1:], (st[0], 0) + st[1:])
         e3, e2, m_n, m_s = sh
-        if mask.element_size() != 2 or m_n < n or m_s != slots or (slots > 1 and st[3] != 1):
-            raise ValueError("mask: f16 (or its bits) [seqs | 1, heads | 1, >= tokens, slots], the two first may be left out")
+        if mask.dtype not in _MASK_DTYPE or m_n < n or m_s != slots or (slots > 1 and st[3] != 1):
+            raise ValueError("mask: f16 (or its bits as int16 / uint16) [seqs | 1, heads | 1, >= tokens, slots], the two first may be left out")
         mp, m1, m2, m3 = mask.data_ptr(), st[2] * 2, st[1] * 2, st[0] * 2
     dst, vp, v1, v2, v3, dp, dv = None, None, 0, 0, 0, None, 0
     if v is not None:

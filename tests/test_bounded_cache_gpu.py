@@ -678,6 +678,21 @@ def test_attention_mass_wrapper_refuses_what_does_not_fit():
         ops.flash_attn_ext_mass(q[:, :3], k, v, None, B.F16, 0.1)
 
 
+def test_attention_mass_takes_a_mask_of_f16_or_its_bits_only():
+    """another 16-bit type's bits would be read as f16: bf16's -inf is a NaN there"""
+    q, k, v, _ = (x.cuda() for x in attn_case(1, 4, 2, 1, 40, 64, 64, B.F16, 1))
+    mask = causal(1, 1, 40, [30]).cuda()
+    want = ops.flash_attn_ext_mass(q, k, v, mask, B.F16, 0.1)
+    for same in (mask.view(torch.int16), mask.view(torch.uint16)):
+        got = ops.flash_attn_ext_mass(q, k, v, same, B.F16, 0.1)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(ops.attn_mass(q, k, same, B.F16, 0.1), ops.attn_mass(q, k, mask, B.F16, 0.1))
+    for bad in (mask.bfloat16(), mask.float(), mask == 0, mask.double()):
+        with pytest.raises(ValueError):
+            ops.flash_attn_ext_mass(q, k, v, bad, B.F16, 0.1)
+        with pytest.raises(ValueError):
+            ops.attn_mass(q, k, bad, B.F16, 0.1)
+
+
 @pytest.mark.parametrize("S,n,slots", [(1, 0, 5), (2, 0, 512), (1, 0, 100000), (0, 1, 512), (0, 40, 300), (1, 0, 0)])
 def test_attention_mass_of_no_queries(S, n, slots):
     """an empty batch: an empty dst, and what earlier calls left, decayed"""
