@@ -688,7 +688,7 @@ def _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bi
         if len(sh) < 4:                       # the two first dimensions may be left out, or the heads'
             sh, st = ((1, 1) + sh, (0, 0) + st) if len(sh) == 2 else ((sh[0], 1) + sh[1:], (st[0], 0) + st[1:])
         e3, e2, m_n, m_s = sh
-        if mask.dtype not in _MASK_DTYPE or m_n < n or m_s != slots or (slots > 1 and st[3] != 1):
+        if mask.dtype not in _MASK_DTYPE or e2 < 1 or e3 < 1 or H % e2 or S % e3 or m_n < n or m_s != slots or (slots > 1 and st[3] != 1):
             raise ValueError("mask: f16 (or its bits as int16 / uint16) [seqs | 1, heads | 1, >= tokens, slots], the two first may be left out")
         mp, m1, m2, m3 = mask.data_ptr(), st[2] * 2, st[1] * 2, st[0] * 2
     dst, vp, v1, v2, v3, dp, dv = None, None, 0, 0, 0, None, 0

@@ -693,6 +693,16 @@ def test_attention_mass_takes_a_mask_of_f16_or_its_bits_only():
             ops.attn_mass(q, k, bad, B.F16, 0.1)
 
 
+def test_attention_mass_refuses_a_mask_of_other_sequences_or_heads():
+    """planes that neither are one nor go into the sequences or heads evenly would be dealt out in turn"""
+    q, k, v, _ = (x.cuda() for x in attn_case(2, 6, 2, 1, 40, 64, 64, B.F16, 1))
+    for shape in ((3, 1, 1, 40), (1, 4, 1, 40), (2, 12, 1, 40), (4, 1, 1, 40), (3, 1, 40), (0, 1, 1, 40), (1, 0, 1, 40)):
+        with pytest.raises(ValueError):
+            ops.flash_attn_ext_mass(q, k, v, torch.zeros(shape, device="cuda").half(), B.F16, 0.1)
+        with pytest.raises(ValueError):
+            ops.attn_mass(q, k, torch.zeros(shape, device="cuda").half(), B.F16, 0.1)
+
+
 @pytest.mark.parametrize("S,n,slots", [(1, 0, 5), (2, 0, 512), (1, 0, 100000), (0, 1, 512), (0, 40, 300), (1, 0, 0)])
 def test_attention_mass_of_no_queries(S, n, slots):
     """an empty batch: an empty dst, and what earlier calls left, decayed"""
