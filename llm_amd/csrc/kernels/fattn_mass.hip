@@ -50,10 +50,32 @@ static __device__ __forceinline__ void mass_store(const MArgs & a, int hk, int i
     if (a.mass_in) t += a.decay * ((const float *)(a.mass_in + hk * a.in_nb2 + i3 * a.in_nb3))[j];
     ((float *)(a.mass_out + hk * a.out_nb2 + i3 * a.out_nb3))[j] = t;
 }
-// cap log2(e) tanh(x), c2 = cap log2(e): tanh x = 1 - 2 / (e^2x + 1).  Off by some 2^-23 of the cap like the logit itself, and short: tanhf's two
-// branches, 16 times over, took the loop out of the instruction cache
-static __device__ __forceinline__ float capped_logit(float x, float c2) {
-    return __builtin_fmaf(-2.0f * c2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * x) + 1.0f), c2);
+// x[i] -> cap log2(e) tanh(x[i]), c2 = cap log2(e), off by a few 2^-24 of the result itself.  Below 5/8 it is x + x^3 P(x^2), P the least-maximum fit
+// of (tanh x - x) / x^3 with 5 terms (relative error 2^-27.8); from there on 1 - 2 / (e^2|x| + 1), which would cancel nearer to 0 (2^-23 of the cap,
+// however small the logit).  Logits seldom reach 5/8 of the cap, and a wave that has none there leaves the second form out: 2047 x 2047 bf16
+// with a cap of 30 takes 221 us, with both forms at every logit 261 (or a cap of 3: 286), without a cap 157
+template <int N> static __device__ __forceinline__ void cap_logits(float (&x)[N], float c2) {
+    auto near = [](float x) {
+        const float z = x * x;
+        float p = __builtin_fmaf(z, -0.005717036779969931f, 0.020650578662753105f);
+        p = __builtin_fmaf(z, p, -0.05374349653720856f);
+        p = __builtin_fmaf(z, p, 0.13331490755081177f);
+        p = __builtin_fmaf(z, p, -0.3333328366279602f);
+        return __builtin_fmaf(x * z, p, x);
+    };
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) top = fmaxf(top, fabsf(x[i]));
+    if (__any(top >= 0.625f)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * fabsf(x[i])) + 1.0f), 1.0f);
+            x[i] = c2 * (fabsf(x[i]) < 0.625f ? near(x[i]) : copysignf(far, x[i]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = c2 * near(x[i]);
+    }
 }
 // exponent that brings a row's largest value to [2^14, 2^15)
 static __device__ __forceinline__ int row_exp(float amax) { return amax > 0.0f && amax < INFINITY ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0; }
@@ -426,11 +448,12 @@ mass_step_kernel(const MArgs a) {
         bool some = false;                      // some row does not see some slot of the tile
         float mx = m;
 #pragma unroll
+        for (int i = 0; i < 8; i++) s[i] = c[i >> 2][i & 3] * qe;
+        if (capped) cap_logits(s, a.logit_softcap * LOG2E);
+#pragma unroll
         for (int i = 0; i < 8; i++) {
             const float mv = h2f((uint16_t)(mc[i >> 2][(i & 3) >> 1] >> (16 * (i & 1))));
-            float y = c[i >> 2][i & 3] * qe;
-            if (capped) y = capped_logit(y, a.logit_softcap * LOG2E);
-            s[i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope, y);
+            s[i] = mv == -INFINITY ? -INFINITY : __builtin_fmaf(mv, slope, s[i]);
             mx = fmaxf(mx, s[i]);
             some |= s[i] == -INFINITY;
         }
@@ -925,12 +948,16 @@ static __device__ __forceinline__ void fold_block(const uint16_t * scales, int l
 }
 
 // logits (log2 domain) of a 32 x 32 tile from slot j0 on, in place of its products: sc what they lack, cl the tile's class for this lane's query
-static __device__ __forceinline__ void tile_logits(const MArgs & a, v16f & c, float sc, float slope, int cl, const char * mrow, bool m8, int j0) {
+template <bool CAP> static __device__ __forceinline__ void tile_logits(const MArgs & a, v16f & c, float sc, float slope, int cl, const char * mrow, bool m8, int j0) {
 #pragma unroll
     for (int i = 0; i < 16; i++) c[i] *= sc;
-    if (a.logit_softcap != 0.0f) {
+    if constexpr (CAP) {
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) c[i] = capped_logit(c[i], a.logit_softcap * LOG2E);
+        for (int i = 0; i < 16; i++) x[i] = c[i];
+        cap_logits(x, a.logit_softcap * LOG2E);
+#pragma unroll
+        for (int i = 0; i < 16; i++) c[i] = x[i];
     }
 #pragma unroll
     for (int q = 0; q < 4; q++) {                               // slot 8 q + 4 (lane / 32) + i
@@ -964,7 +991,7 @@ static __device__ __forceinline__ v2f row_result(float M, float L) { return v2f{
 // (2047 x 2047: 82 + 95 -> 67 + 87 us)
 static __device__ __forceinline__ bool turned() { return (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x / 256 & 1; }
 
-template <int TYPE, int D>
+template <int TYPE, int D, bool CAP>
 __global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
 prompt_stats_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
@@ -1069,9 +1096,9 @@ prompt_stats_kernel(const MArgs a) {
                 }
             }
             float sc = qe;
-            if (a.logit_softcap != 0.0f || !__all(c0 == MASK_ZERO && c1 == MASK_ZERO)) {
-                tile_logits(a, c[0], qe, slope, c0, mrow, m8, t * PA_SLOTS);
-                tile_logits(a, c[1], qe, slope, c1, mrow, m8, t * PA_SLOTS + 32);
+            if (CAP || !__all(c0 == MASK_ZERO && c1 == MASK_ZERO)) {
+                tile_logits<CAP>(a, c[0], qe, slope, c0, mrow, m8, t * PA_SLOTS);
+                tile_logits<CAP>(a, c[1], qe, slope, c1, mrow, m8, t * PA_SLOTS + 32);
                 sc = 1.0f;
             }
             float mx = c[0][0];
@@ -1124,7 +1151,7 @@ prompt_rows_kernel(const MArgs a) {
 // slots of a wave in the second pass: 64 where its K takes at most 64 registers so
 template <int D> constexpr int prompt_ns() { return D <= 128 ? 2 : 1; }
 
-template <int TYPE, int D>
+template <int TYPE, int D, bool CAP>
 __global__ void __launch_bounds__(PT, D <= 128 ? 2 : 1)
 prompt_mass_kernel(const MArgs a) {
     typedef Fmt<TYPE> F;
@@ -1200,7 +1227,7 @@ prompt_mass_kernel(const MArgs a) {
         if (ahead < nt) fetch(ahead, b == 0 ? S - 1 : b - 1);
         const uint32_t bytes = cl[b][wave][lane] >> (8 * (j0 / 32 & 3));
         int cu[NS], seen = MASK_HIDDEN;
-        bool zero = a.logit_softcap == 0.0f;
+        bool zero = !CAP;
 #pragma unroll
         for (int u = 0; u < NS; u++) { cu[u] = bytes >> (8 * u) & 255; seen |= cu[u]; zero &= cu[u] == MASK_ZERO; }
         if (__any(seen != MASK_HIDDEN)) {
@@ -1241,7 +1268,7 @@ prompt_mass_kernel(const MArgs a) {
                 int jm = j0;
                 asm volatile("" : "+v"(jm));                    // (the comparisons of its slots with the last one would be kept through the loop)
 #pragma unroll
-                for (int u = 0; u < NS; u++) tile_logits(a, c[u], sc, c4.slope, cu[u], mrow, m8, jm + 32 * u);
+                for (int u = 0; u < NS; u++) tile_logits<CAP>(a, c[u], sc, c4.slope, cu[u], mrow, m8, jm + 32 * u);
                 sc = 1.0f;
             }
 #pragma unroll
@@ -1301,7 +1328,8 @@ static int64_t prompt_chunks(const mi355_fattn_args * p) {
     return n < 1 ? 1 : n;
 }
 
-template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hipStream_t s) {
+// CAP (logit_softcap != 0) is a kernel of its own: the cap's code beside the other takes registers and 2 % of the time from q8_0 prompts without one
+template <int TYPE, int D, bool CAP> static int prompt_launch(const MArgs & a, int ne3, hipStream_t s) {
     const int R = a.ratio * a.n_q, ws = 128 * prompt_ns<D>();
     const unsigned hk = (unsigned)a.n_head_kv, z = (unsigned)ne3;
     const int64_t slot_wgs = (a.n_kv + 1023) / 1024, query_wgs = a.mask ? (a.n_q + 3) / 4 : 1, class_wgs = slot_wgs * query_wgs * a.m_ne2 * a.m_ne3;
@@ -1310,13 +1338,13 @@ template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hi
     MI355_LAUNCH("attn_mass_prep", (prompt_prep_kernel<D, Fmt<TYPE>::bf>), dim3((unsigned)prep), dim3(PT), 0, s, a, (uint32_t)class_wgs, (uint32_t)slot_wgs,
                  (uint32_t)query_wgs, (uint32_t)row_wgs);
     MI355_CHECK_LAUNCH();
-    MI355_LAUNCH("attn_mass_stats", (prompt_stats_kernel<TYPE, D>), dim3((unsigned)((R + PA_ROWS - 1) / PA_ROWS * a.nsplit), hk, z), dim3(PT), 0, s, a);
+    MI355_LAUNCH("attn_mass_stats", (prompt_stats_kernel<TYPE, D, CAP>), dim3((unsigned)((R + PA_ROWS - 1) / PA_ROWS * a.nsplit), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
     if (a.nsplit > 1) {
         MI355_LAUNCH("attn_mass_rows", prompt_rows_kernel, dim3((unsigned)((R + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
         MI355_CHECK_LAUNCH();
     }
-    MI355_LAUNCH("attn_mass", (prompt_mass_kernel<TYPE, D>), dim3((unsigned)((a.n_kv + ws - 1) / ws * a.nchunk), hk, z), dim3(PT), 0, s, a);
+    MI355_LAUNCH("attn_mass", (prompt_mass_kernel<TYPE, D, CAP>), dim3((unsigned)((a.n_kv + ws - 1) / ws * a.nchunk), hk, z), dim3(PT), 0, s, a);
     MI355_CHECK_LAUNCH();
     if (a.nchunk == 1) return MI355_OK;
     MI355_LAUNCH("attn_mass_sum", prompt_sum_kernel, dim3((unsigned)((a.n_kv + PT - 1) / PT), hk, z), dim3(PT), 0, s, a);
@@ -1325,11 +1353,12 @@ template <int TYPE, int D> static int prompt_launch(const MArgs & a, int ne3, hi
 }
 template <int TYPE> static int prompt_dispatch(const MArgs & a, int ne3, hipStream_t s) {
     if (a.n_kv == 0) return MI355_OK;
+    const bool cap = a.logit_softcap != 0.0f;
     switch (step_d(a.d)) {
-        case 64:  return prompt_launch<TYPE, 64>(a, ne3, s);
-        case 128: return prompt_launch<TYPE, 128>(a, ne3, s);
+        case 64:  return cap ? prompt_launch<TYPE, 64, true>(a, ne3, s) : prompt_launch<TYPE, 64, false>(a, ne3, s);
+        case 128: return cap ? prompt_launch<TYPE, 128, true>(a, ne3, s) : prompt_launch<TYPE, 128, false>(a, ne3, s);
     }
-    return prompt_launch<TYPE, 256>(a, ne3, s);
+    return cap ? prompt_launch<TYPE, 256, true>(a, ne3, s) : prompt_launch<TYPE, 256, false>(a, ne3, s);
 }
 
 // steps: [statistics][partial rows of dst][logits]; prompts: [statistics][sums of the row chunks][row constants][parts of q][classes of the mask] (in floats)

@@ -703,6 +703,53 @@ def test_attention_mass_refuses_a_mask_of_other_sequences_or_heads():
             ops.attn_mass(q, k, torch.zeros(shape, device="cuda").half(), B.F16, 0.1)
 
 
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("n", [1, 8, 40])
+@pytest.mark.parametrize("cap", [30.0, 50.0, 1000.0])
+def test_attention_mass_softcap_is_exact_relative_to_the_logit(t, n, cap):
+    """one feature of q is not zero, so a logit is one product and what is left of its error is the cap's: a few steps of the logit itself,
+    whatever the cap"""
+    H, HK, slots, d, scale = 8, 2, 40, 128, 0.125
+    g = gen(int(cap) + n)
+    q = torch.zeros((1, H, n, d))
+    q[..., 32] = torch.randn((1, H, n), generator=g) * 16
+    k = cache((1, HK, slots, d), t, g)
+    dot = q.double() @ values(k, t).repeat_interleave(H // HK, 1).transpose(2, 3)
+    s = cap * torch.tanh(dot * scale / cap)
+    # q in parts (4 steps of 2^-24), the parts' products and the block's scale (3), scale / cap, its product, the row's power of two (3), tanh (8), cap (2);
+    # the weight: its logit and those of the sum, exp and its argument, the sum over the slots
+    es = (20 * U32 * s.abs()).amax(-1, keepdim=True)
+    span = (s - s.amax(-1, keepdim=True)).abs().amax(-1, keepdim=True)
+    p = torch.softmax(s, -1)
+    rel = 2 * es + (10 + slots + 4 * span) * U32
+    fold = lambda x: x.reshape(1, HK, -1, slots).sum(2)  # noqa: E731
+    want, err = fold(p), fold(p * rel) + (H // HK * n + 4) * U32 * fold(p)
+    assert ((ops.attn_mass(q.cuda(), k.cuda(), None, t, scale, logit_softcap=cap).cpu().double() - want).abs() <= err).all()
+    if n <= 8:
+        v = cache((1, HK, slots, d), t, g)
+        dst, mass = ops.flash_attn_ext_mass(q.cuda(), k.cuda(), v.cuda(), None, t, scale, logit_softcap=cap)
+        assert ((mass.cpu().double() - want).abs() <= err).all()
+        vv = values(v, t).repeat_interleave(H // HK, 1)
+        bound = (p * rel) @ vv.abs() + (slots + 4) * U32 * (p @ vv.abs())
+        assert ((dst.cpu().double() - (p @ vv).transpose(1, 2)).abs() <= bound.transpose(1, 2) + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("t", [B.F16, B.BF16, B.Q8_0, B.Q4_0])
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("cap", [30.0, 50.0, 1000.0])
+def test_attention_mass_softcap_is_as_exact_as_f32(t, n, cap):
+    """no further from 64 bits than the same formula in f32 torch"""
+    H, HK, slots, d = 16, 4, 700, 128
+    q, k, _, _ = attn_case(1, H, HK, n, slots, d, 0, t, 7 + n)
+    kk = values(k, t).repeat_interleave(H // HK, 1).transpose(2, 3)
+    fold = lambda s: torch.softmax(s, -1).reshape(1, HK, -1, slots).sum(2)  # noqa: E731
+    want = fold(cap * torch.tanh(q.double() @ kk * 0.09 / cap))
+    f32 = fold(cap * torch.tanh((q @ kk.float()) * 0.09 / cap))
+    got = ops.attn_mass(q.cuda(), k.cuda(), None, t, 0.09, logit_softcap=cap)
+    far = lambda x: float((x.cpu().double() - want).norm() / want.norm())  # noqa: E731
+    assert far(got) <= 1.5 * far(f32) + 3e-7
+
+
 @pytest.mark.parametrize("S,n,slots", [(1, 0, 5), (2, 0, 512), (1, 0, 100000), (0, 1, 512), (0, 40, 300), (1, 0, 0)])
 def test_attention_mass_of_no_queries(S, n, slots):
     """an empty batch: an empty dst, and what earlier calls left, decayed"""
