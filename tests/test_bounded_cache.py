@@ -77,6 +77,23 @@ def test_kv_evict_refuses(code, kw):
     assert K.lib.mi355_kv_evict(evict_args(**kw), None) == code
 
 
+# caches of 100 slots x 256 bytes: slot-major (pitch 512: K and V of a slot side by side, heads 100 slots apart) and head-major ones
+SIDE = dict(k_nb1=512, v_nb1=512, v=6 * P + 256, k_nb2=51200, v_nb2=51200, ko_nb2=51200, vo_nb2=51200)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(k_out=6 * P + 256), dict(k_out=6 * P + 25600 - 256, k_nb2=25600), dict(k_out=6 * P - 49 * 256), dict(k_out=7 * P + 2, v_nb1=258), dict(v_out=6 * P + 4096),
+    dict(k_out=6 * P + (1 << 16), ne3=2), dict(k_out=8 * P, v_out=8 * P + 128), dict(k_out=8 * P, v_out=8 * P), dict(mass_out=P + 196), dict(mass_out=P - 100),
+    dict(pos_out=2 * P + 4096 + 200), dict(pos_out=P + 4), dict(kept=P + 8), dict(evicted=2 * P + 4), dict(kept=3 * P), dict(n_used=5 * P, evicted=5 * P),
+    dict(mass_out=10 * P, pos_out=10 * P + 100), dict(evicted=4 * P + 100), dict(kept=6 * P + 4), dict(mass_out=9 * P + 1000),
+    dict(SIDE, k_out=6 * P + 256, ko_nb1=512), dict(SIDE, k_out=6 * P + 128, ko_nb1=512), dict(SIDE, k_out=6 * P, ko_nb1=512), dict(SIDE, k_out=6 * P + 4, ko_nb1=516),
+    dict(k_nb1=-256, k_out=6 * P - 99 * 256), dict(k_nb2=-25600, k_out=6 * P - 25600),
+])
+def test_kv_evict_refuses_outputs_that_meet_what_it_reads(kw):
+    """a gathered row read after its place has been written: any byte in common, wherever the views begin"""
+    assert K.lib.mi355_kv_evict(evict_args(**kw), None) == E_UNSUPPORTED
+
+
 def test_kv_evict_of_no_sequences_launches_nothing():
     assert K.lib.mi355_kv_evict(None, None) == E_NULL
     assert K.lib.mi355_kv_evict(evict_args(ne3=0), None) == 0

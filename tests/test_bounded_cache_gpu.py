@@ -396,6 +396,38 @@ def test_evict_new_outputs_captured_and_refusals():
     assert (kept == -1).all() and evicted.shape == (S, HK, 0)
 
 
+@pytest.mark.parametrize("layout", ["behind", "turns", "side", "halves", "slots"])
+def test_evict_gathers_into_the_caches_own_buffer(layout):
+    """outputs in the same allocation as the caches, no byte in common: taken, and the caches stay as they were"""
+    S, HK, n, n_keep, d = 2, 3, 100, 40, 64
+    mass, pos = evict_case(S, HK, n, 5)
+    past = torch.full((S,), 2 * n + 3, dtype=torch.int32, device="cuda")
+    if layout == "behind":                       # one after the other
+        raw = torch.randn((2 * S * HK * (n + n_keep) * d,), generator=gen(1)).half().cuda()
+        sizes = [S * HK * m * d for m in (n, n, n_keep, n_keep)]
+        k, v, ko, vo = (x.view(S, HK, -1, d) for x in raw.split(sizes))
+    elif layout == "turns":                      # every head's slots, then the room for its copy
+        raw = torch.randn((2, S, HK, n + n_keep, d), generator=gen(1)).half().cuda()
+        (k, v), (ko, vo) = raw[:, :, :, :n], raw[:, :, :, n:]
+    elif layout == "side":                       # K and V of a slot side by side, so are their copies
+        raw = torch.randn((S, HK, n + n_keep, 2, d), generator=gen(1)).half().cuda()
+        k, v, ko, vo = raw[:, :, :n, 0], raw[:, :, :n, 1], raw[:, :, n:, 0], raw[:, :, n:, 1]
+    elif layout == "halves":                     # each slot's K, V and two rows of a copy
+        raw = torch.randn((S, HK, n, 4, d), generator=gen(1)).half().cuda()
+        k, v, ko, vo = raw[:, :, :, 0], raw[:, :, :, 1], raw[:, :, :n_keep, 2], raw[:, :, :n_keep, 3]
+    else:                                        # slot-major: all heads of a slot side by side
+        raw = torch.randn((S, n + n_keep, 2, HK, d), generator=gen(1)).half().cuda()
+        k, v, ko, vo = (x.transpose(1, 2) for x in (raw[:, :n, 0], raw[:, :n, 1], raw[:, n:, 0], raw[:, n:, 1]))
+    before = k.clone(), v.clone()
+    kept, _, mo, po = ops.kv_evict(torch.from_numpy(mass).cuda(), torch.from_numpy(pos).cuda(), past, n_keep, 4, 10, k=k, v=v, k_out=ko, v_out=vo)
+    wk, _ = evict_oracle(mass, pos, past.cpu().numpy(), [n] * S, n_keep, 0, 4, 10)
+    assert np.array_equal(kept.cpu().numpy(), wk) and torch.equal(k, before[0]) and torch.equal(v, before[1])
+    at = (torch.arange(S)[:, None, None], torch.arange(HK)[None, :, None], torch.from_numpy(wk).long())
+    assert torch.equal(ko.cpu(), before[0].cpu()[at]) and torch.equal(vo.cpu(), before[1].cpu()[at])
+    with pytest.raises(K.Mi355Error):            # a shifted view of the cache itself
+        ops.kv_evict(torch.from_numpy(mass).cuda(), torch.from_numpy(pos).cuda(), past, n_keep, 4, 10, k=k, v=v, k_out=k[:, :, 1:1 + n_keep], v_out=vo)
+
+
 # ---- attention with the weight every slot draws ----------------------------------------------------------------------------------------
 
 def attn_oracle(q, k, v, mask, scale, mass, decay, max_bias=0.0, softcap=0.0):
