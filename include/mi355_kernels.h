@@ -743,7 +743,8 @@ MI355_API int     mi355_flash_attn_ext_noalloc(const mi355_fattn_args *args, voi
  * rope(rms_norm(k) * k_norm), V cache row = v.  Replaces the node run RMS_NORM MUL ROPE (q and k) and the stores of K and V (SET_ROWS / CPY):
  * eight launches of ggml-cuda (norm.cu, binbcast.cu, rope.cu, set-rows.cu).
  *   q f32 [head_dim, n_head, n, ne3], k f32 [head_dim, n_head_kv, n, ne3], v f32 [dv, n_head_kv, n, ne3] (v and v_out may be NULL: no V):
- *   byte strides nb1 (token), nb2 (head), nb3 (sequence), 16-byte aligned; q_out likewise (it may be q itself)
+ *   byte strides nb1 (token), nb2 (head), nb3 (sequence), 16-byte aligned; q_out likewise (it may be q itself, row for row; else it
+ *   shares no memory with q, k and v: MI355_E_UNSUPPORTED)
  *   k_out, v_out: caches of type_kv f32 | f16 | bf16 (16-byte aligned) | q8_0 | q4_0 (2-byte aligned, whole 32-blocks, else MI355_E_SHAPE),
  *   byte strides nb1 (row), nb2 (head), nb3 (sequence), n_rows rows per head
  *   rows: int32 cache row of each (token, head, sequence), strides nb1 / nb2 / nb3 (0: shared); NULL: token i goes to row i.  A row outside
@@ -776,7 +777,7 @@ MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stre
  *   mass_out[j] = decay * mass_in[j] + sum over the queries and the heads that share the KV head of softmax(...)[j]
  * args as for mi355_flash_attn_ext (K and V of one type; rows of K and V at most 2^31 - 1 bytes apart, at most 65535 planes of mask, (heads per KV
  * head)^2 x queries below 2^32, else MI355_E_SHAPE; block rows 2-byte aligned, faster where a row's address is a multiple of d / 16).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be
- * mass_out itself; NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate (the query is not rounded to the cache's type, the
+ * mass_out itself, row for row, else they are apart (MI355_E_UNSUPPORTED); NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate (the query is not rounded to the cache's type, the
  * weights are not rounded before they meet V).  A slot hidden by the mask takes no part whatever its row holds; a query that sees no slot gives
  * a row of zeros and no weight.  At least one query and one sequence, at most 65535 of each, else MI355_E_SHAPE (ops.* answer a call of none themselves).
  * workspace: *_workspace_bytes (-1 for sizes and types that the call itself refuses), 16-byte aligned, no initial contents, not shared by calls

@@ -6,6 +6,7 @@
 // A slot that a query does not see (mask -inf) takes no part whatever its row holds, NaN included; a query that sees nothing gives a zero row and
 // no weight.  Everything between the cache's own values and the f32 results is f32.
 #include "common.h"
+#include "spans.h"
 
 namespace {
 
@@ -1426,6 +1427,10 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     const int64_t words = (int64_t)(uintptr_t)w->mass_in | w->in_nb2 | w->in_nb3 | (int64_t)(uintptr_t)w->mass_out | w->out_nb2 | w->out_nb3;
     const int64_t halves = p->mask ? (int64_t)(uintptr_t)p->mask | p->m_nb1 | p->m_nb2 | p->m_nb3 : 0;
     if ((f32s & 15) || (cache & (quant ? 1 : 15)) || (words & 3) || (halves & 1)) return MI355_E_ALIGN;
+    if (w->mass_in && w->decay != 0.0f) {             // in place or apart: a shifted table would be read after other slots of it have been written
+        const Span mi(w->mass_in, p->n_kv * 4, 1, 0, p->n_head_kv, w->in_nb2, p->ne3, w->in_nb3), mo(w->mass_out, p->n_kv * 4, 1, 0, p->n_head_kv, w->out_nb2, p->ne3, w->out_nb3);
+        if (!mi.same(mo) && spans_meet(mi, mo)) return MI355_E_UNSUPPORTED;
+    }
     const int64_t need = mass_workspace(p, with_dst);
     if (need > 0 && (!workspace || workspace_bytes < need)) return MI355_E_WORKSPACE;
 

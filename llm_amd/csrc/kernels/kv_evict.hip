@@ -12,6 +12,7 @@
 // heads 31 us (8 of them loading 256 KB on each of 8 CUs, 7 writing the lists) and 10.6 us for the rows.
 // (Digits of 8 bits from the top, keys re-read: 54 / 147 us, atomics queued on the few exponents; bisection with a vote per bit: 15.5 / 48 us.)
 #include "common.h"
+#include "spans.h"
 
 namespace {
 
@@ -271,46 +272,6 @@ kv_gather_kernel(const KgArgs a, int log2_w) {
     }
 }
 
-// What a call reads or writes: n3 x n2 planes of n1 rows of `row` bytes, and the first and last byte of all that
-struct Span {
-    int64_t row, n1, nb1, plane, nb[2], n[2];         // plane: bytes from a plane's first to its last; the planes' strides, the larger one first
-    uintptr_t low, end;
-    Span(const void * at, int64_t row_bytes, int64_t n1_, int64_t nb1_, int64_t n2, int64_t nb2, int64_t n3, int64_t nb3) : row(at ? row_bytes : 0), n1(n1_), nb1(nb1_) {
-        low = (uintptr_t)at + (nb1 < 0 ? (n1 - 1) * nb1 : 0) + (nb2 < 0 ? (n2 - 1) * nb2 : 0) + (nb3 < 0 ? (n3 - 1) * nb3 : 0);
-        if (nb2 < 0) nb2 = -nb2;
-        if (nb3 < 0) nb3 = -nb3;
-        plane = (n1 - 1) * (nb1 < 0 ? -nb1 : nb1) + row;
-        const int big = n2 < 2 || (n3 > 1 && nb3 >= nb2) ? 0 : 1;
-        n[big] = n3; nb[big] = nb3; n[!big] = n2; nb[!big] = nb2;
-        end = row > 0 && n1 > 0 ? low + (n2 - 1) * nb2 + (n3 - 1) * nb3 + plane : low;
-    }
-    bool apart(const Span & o) const { return end <= o.low || o.end <= low || end == low || o.end == o.low; }
-};
-// Can a byte belong to both, if not apart as wholes?  Never a wrong no.  Apart plane by plane (a cache and its copy take turns in memory), or as
-// rows of one pitch that lie in each other's gaps (K and V side by side); anything less regular counts as a yes
-static bool planes_meet(const Span & a, const Span & b) {
-    const bool pitch = a.nb1 == b.nb1 && a.nb1 >= a.row && a.nb1 >= b.row;
-    int left = 1 << 16;                               // comparisons
-    for (int64_t i = 0; i < a.n[0]; i++)
-        for (int64_t j = 0; j < a.n[1]; j++) {
-            const uintptr_t lo = a.low + i * a.nb[0] + j * a.nb[1];
-            for (int64_t k = 0; k < b.n[0]; k++) {
-                const uintptr_t some = b.low + k * b.nb[0];                    // the planes of one stride together, then each
-                if (--left < 0) return true;
-                if (some + (b.n[1] - 1) * b.nb[1] + b.plane <= lo || lo + a.plane <= some) continue;
-                for (int64_t l = 0; l < b.n[1]; l++) {
-                    const uintptr_t at = some + l * b.nb[1];
-                    if (--left < 0) return true;
-                    if (at + b.plane <= lo || lo + a.plane <= at) continue;
-                    if (!pitch) return true;
-                    const int64_t d = (int64_t)(at - lo) % a.nb1, r = d < 0 ? d + a.nb1 : d;
-                    if (r < a.row || a.nb1 - r < b.row) return true;
-                }
-            }
-        }
-    return false;
-}
-
 template <class PIECE> static int gather_launch(const KgArgs & g, int64_t n_keep, int64_t hk, int64_t ne3, hipStream_t s) {
     const int bytes = g.row_bytes[0] > g.row_bytes[1] ? g.row_bytes[0] : g.row_bytes[1], pieces = bytes / (int)sizeof(PIECE);
     int w = 0;
@@ -368,8 +329,8 @@ int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
                         {p->k_out, bk, placed, p->ko_nb1, hk, p->ko_nb2, ne3, p->ko_nb3}, {p->v_out, bv, placed, p->vo_nb1, hk, p->vo_nb2, ne3, p->vo_nb3},
                         {p->mass_out, p->n_keep * 4, 1, 0, hk, p->mo_nb2, ne3, p->mo_nb3}, {p->pos_out, p->n_keep * 4, 1, 0, hk, p->po_nb2, ne3, p->po_nb3}};
     if (ne3 > 0) for (const Span & o : out) {
-        for (const Span & x : in) if (!o.apart(x) && planes_meet(o, x)) return MI355_E_UNSUPPORTED;
-        for (const Span * x = out; x != &o; x++) if (!o.apart(*x) && planes_meet(o, *x)) return MI355_E_UNSUPPORTED;
+        for (const Span & x : in) if (spans_meet(o, x)) return MI355_E_UNSUPPORTED;
+        for (const Span * x = out; x != &o; x++) if (spans_meet(o, *x)) return MI355_E_UNSUPPORTED;
     }
     if (p->ne3 == 0) return MI355_OK;
 

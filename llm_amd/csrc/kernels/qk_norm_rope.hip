@@ -6,6 +6,7 @@
 // Angles are formed and reduced to one turn in 64 bits: in 32 bits the product alone is off by 0.01 rad at position 10^5.
 #include "row_formats.h"
 #include "rope.h"
+#include "spans.h"
 
 namespace {
 
@@ -220,6 +221,10 @@ int mi355_qk_norm_rope(const mi355_qk_norm_rope_args * p, void * stream) {
                           (int64_t)(uintptr_t)p->slot_mass | p->sm_nb2 | p->sm_nb3;
     if ((f32s & 15) || (cache & (quant ? 1 : 15)) || (words & 3)) return MI355_E_ALIGN;
     if (p->n == 0 || p->ne3 == 0) return MI355_OK;
+    // q_out is q itself, row for row, or shares no memory with what is read: another order of q's rows would be written before they are read
+    const Span qo(p->q_out, p->head_dim * 4, p->n, p->qo_nb1, p->n_head, p->qo_nb2, p->ne3, p->qo_nb3), q(p->q, p->head_dim * 4, p->n, p->q_nb1, p->n_head, p->q_nb2, p->ne3, p->q_nb3);
+    if (!qo.same(q) && (spans_meet(qo, q) || spans_meet(qo, Span(p->k, p->head_dim * 4, p->n, p->k_nb1, p->n_head_kv, p->k_nb2, p->ne3, p->k_nb3)) ||
+                        spans_meet(qo, Span(p->v, dv * 4, p->n, p->v_nb1, p->n_head_kv, p->v_nb2, p->ne3, p->v_nb3)))) return MI355_E_UNSUPPORTED;
 
     QnArgs a;
     a.q = (const char *)p->q; a.q_nb1 = p->q_nb1; a.q_nb2 = p->q_nb2; a.q_nb3 = p->q_nb3;

@@ -42,6 +42,15 @@ def test_qk_norm_rope_refuses(code, kw):
     assert K.lib.mi355_qk_norm_rope(store_args(**kw), None) == code
 
 
+@pytest.mark.parametrize("kw", [
+    dict(q_out=P + 512), dict(q_out=P - 512), dict(q_out=P, qo_nb2=1024), dict(q_out=P, n=4, qo_nb1=512, qo_nb2=2048), dict(q_out=P, ne3=2, qo_nb3=1 << 15),
+    dict(q_out=9 * P), dict(q_out=10 * P + 512), dict(q_out=9 * P - 3584), dict(q_out=P + 32, n=3), dict(q_out=P, n_head=2, ne3=2, q_nb3=1024, qo_nb2=1024, qo_nb3=512),
+])
+def test_qk_norm_rope_refuses_q_out_over_its_inputs(kw):
+    """in place means row for row; any other order would overwrite rows that are still to be read"""
+    assert K.lib.mi355_qk_norm_rope(store_args(**{**dict(k=9 * P, v=10 * P), **kw}), None) == E_UNSUPPORTED
+
+
 def test_qk_norm_rope_of_nothing_launches_nothing():
     assert K.lib.mi355_qk_norm_rope(None, None) == E_NULL
     assert K.lib.mi355_qk_norm_rope(store_args(n=0), None) == 0
@@ -142,6 +151,12 @@ def test_flash_attn_ext_mass_refuses(code, kw):
 @pytest.mark.parametrize("code, kw", BOTH)
 def test_attn_mass_refuses(code, kw):
     assert K.lib.mi355_attn_mass(*attn_args(**{k: v for k, v in kw.items()}), P, 1 << 40, None) == code
+
+
+@pytest.mark.parametrize("kw", [dict(mass_in=P + 4), dict(mass_in=P - 252), dict(mass_in=P, in_nb2=512), dict(mass_in=P + 256), dict(mass_in=P + 1024, ne3=2)])
+@pytest.mark.parametrize("fn", [K.lib.mi355_flash_attn_ext_mass, K.lib.mi355_attn_mass])
+def test_attention_mass_refuses_a_shifted_table(fn, kw):
+    assert fn(*attn_args(**kw), P, 1 << 40, None) == E_UNSUPPORTED
 
 
 def test_attention_mass_workspaces():
