@@ -798,7 +798,7 @@ MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn
                                   void *stream);
 
 /* The slots of a bounded cache that stay, per (sequence, KV head): of the first n_used[i3] slots the n_keep with the largest mass, where a slot
- * whose position is below n_sink or at least n_past[i3] - n_recent counts as +inf; ties go to the lower slot, NaN counts as -inf.
+ * whose position is below n_sink or at least n_past[i3] - n_recent comes before any mass, +inf included; ties go to the lower slot, NaN counts as -inf.
  *   mass f32, slot_pos int32 [n_kv, n_head_kv, ne3] (strides nb2 / nb3); n_used int32 [ne3] (NULL: n_kv; clamped to [0, n_kv]); n_past int32
  *   [ne3]: tokens the sequence has seen.  All read on the device: a captured call follows them.
  *   kept int32 [n_keep, n_head_kv, ne3]: the kept slots, ascending, -1 behind the last where n_used < n_keep

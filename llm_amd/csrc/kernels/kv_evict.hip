@@ -1,13 +1,13 @@
 // kv_evict.hip -- which slots of a bounded KV cache to keep, by the attention weight they have drawn (mi355_kv_evict).
 //
-// Per (sequence, KV head): the n_keep slots with the largest key, ties to the lower slot; key = the slot's mass, or +inf where its position
-// is one of the first n_sink or the newest n_recent (NaN counts as -inf, -0 as +0).  The keys' 32-bit images (order-preserving: sign flipped for
+// Per (sequence, KV head): the n_keep slots with the largest key, ties to the lower slot; key = the slot's mass, or more than any mass where its
+// position is one of the first n_sink or the newest n_recent, pinned (NaN counts as -inf, -0 as +0).  The keys' 32-bit images (order-preserving: sign flipped for
 // positive floats, all bits for negative ones) are searched for the n_keep-th largest; one ordered pass then writes both index lists
 // ascending.  All integer work: the result does not depend on timing.  The rows are gathered by a second launch.
 //
 // Bound by latency: one workgroup per head has to agree on every step of the search.  A step parts the range of keys that can still hold the
 // wanted one into 2048 buckets (an LDS histogram), so three steps settle 32 bits, and masses, which spread over the range as logarithms do,
-// seldom meet in a bucket; the +inf of sinks and recent slots is counted aside, and a wave whose lanes all fall into one bucket adds once.
+// seldom meet in a bucket; the pinned slots are counted aside, and a wave whose lanes all fall into one bucket adds once.
 // Up to 32768 slots the keys stay in registers; beyond, every step reads them again.  2049 slots x 128 heads 10.9 us, 32768 x 8
 // heads 31 us (8 of them loading 256 KB on each of 8 CUs, 7 writing the lists) and 10.6 us for the rows.
 // (Digits of 8 bits from the top, keys re-read: 54 / 147 us, atomics queued on the few exponents; bisection with a vote per bit: 15.5 / 48 us.)
@@ -26,8 +26,9 @@ struct KeArgs {
     int n_kv, n_keep, n_evict, n_sink, n_recent, n_head_kv;
 };
 
+constexpr uint32_t KE_PINNED = 0xff800001u;           // just above the image of +inf
 static __device__ __forceinline__ uint32_t ke_key(float m, bool keep) {
-    if (keep) return 0xff800000u;                     // the image of +inf
+    if (keep) return KE_PINNED;
     if (m != m) m = -INFINITY;
     if (m == 0.0f) m = 0.0f;                          // -0 and +0 are equal
     const uint32_t u = __float_as_uint(m);
@@ -104,27 +105,26 @@ kv_select_kernel(const KeArgs a) {
     uint32_t T = 1;                                   // kept: key >= T, of which those equal to T only the first `equal`
     uint32_t equal = 0xffffffffu;
     if (n > a.n_keep) {
-        // the range of the keys, the +inf among them counted aside
-        constexpr uint32_t INF = 0xff800000u;
-        uint32_t lo = 0xffffffffu, hi = 0, inf = 0;
+        // the range of the keys, the pinned ones counted aside
+        uint32_t lo = 0xffffffffu, hi = 0, pinned = 0;
         each([&](int, uint32_t k) {
-            if (k == INF) inf++;
+            if (k == KE_PINNED) pinned++;
             else if (k) { lo = lo < k ? lo : k; hi = hi > k ? hi : k; }
         });
         lo = ke_reduce(lo, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
         hi = ke_reduce(hi, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-        inf = ke_reduce(inf, [](uint32_t x, uint32_t y) { return x + y; });
+        pinned = ke_reduce(pinned, [](uint32_t x, uint32_t y) { return x + y; });
         if (tid == 0) pick[3] = 0;
-        if (lane == 0) { lim[0][wave] = lo; lim[1][wave] = hi; lim[2][wave] = inf; }
+        if (lane == 0) { lim[0][wave] = lo; lim[1][wave] = hi; lim[2][wave] = pinned; }
         for (int i = tid; i < KE_BINS; i += NT) hist[i] = 0;
         __syncthreads();
-        inf = 0;
+        pinned = 0;
 #pragma unroll
-        for (int w = 0; w < NW; w++) { lo = lo < lim[0][w] ? lo : lim[0][w]; hi = hi > lim[1][w] ? hi : lim[1][w]; inf += lim[2][w]; }
-        lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi); inf = __builtin_amdgcn_readfirstlane(inf);
-        if (inf >= (uint32_t)a.n_keep) { T = INF; equal = a.n_keep; }
+        for (int w = 0; w < NW; w++) { lo = lo < lim[0][w] ? lo : lim[0][w]; hi = hi > lim[1][w] ? hi : lim[1][w]; pinned += lim[2][w]; }
+        lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi); pinned = __builtin_amdgcn_readfirstlane(pinned);
+        if (pinned >= (uint32_t)a.n_keep) { T = KE_PINNED; equal = a.n_keep; }
         else {
-            uint32_t want = a.n_keep - inf;           // rank of the wanted key among those in [lo, hi], from the largest
+            uint32_t want = a.n_keep - pinned;          // rank of the wanted key among those in [lo, hi], from the largest
             for (;;) {
                 const int bits = 32 - __builtin_clz((hi - lo) | 1), shift = bits > 11 ? bits - 11 : 0;
                 each([&](int, uint32_t k) {

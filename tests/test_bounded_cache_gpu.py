@@ -396,6 +396,24 @@ def test_evict_new_outputs_captured_and_refusals():
     assert (kept == -1).all() and evicted.shape == (S, HK, 0)
 
 
+@pytest.mark.parametrize("n", [9, 1500, 5000, 20000, 40000])
+def test_evict_keeps_sinks_and_recent_slots_before_any_mass(n):
+    """a mass of +inf (a sum that overflowed) is the largest mass and no more: it does not take the place of a sink or of a recent position"""
+    r = np.random.default_rng(n)
+    mass = r.random((1, 2, n)).astype(np.float32)
+    mass[:, :, : n - 4] = np.inf
+    pos = np.stack([np.arange(n), n - 1 - np.arange(n)])[None].astype(np.int32)          # sinks at the lowest slots, and at the highest
+    past = torch.full((1,), n, dtype=torch.int32, device="cuda")
+    for n_keep, sink, recent in ((4, 2, 2), (5, 1, 3), (n - 2, 2, 2), (2, 0, 2), (3, 3, 0)):
+        kept, evicted = ops.kv_evict(torch.from_numpy(mass).cuda(), torch.from_numpy(pos).cuda(), past, n_keep, sink, recent)
+        for h in range(2):
+            pinned = np.nonzero((pos[0, h] < sink) | (pos[0, h] >= n - recent))[0]
+            others = [j for j in np.lexsort((np.arange(n), -mass[0, h].astype(np.float64))) if j not in set(pinned)]
+            want = np.sort(np.concatenate([pinned, np.array(others[: n_keep - len(pinned)], dtype=np.int64)]))
+            assert np.array_equal(kept[0, h].cpu().numpy(), want)
+            assert np.array_equal(evicted[0, h].cpu().numpy(), np.setdiff1d(np.arange(n), want))
+
+
 @pytest.mark.parametrize("layout", ["behind", "turns", "side", "halves", "slots"])
 def test_evict_gathers_into_the_caches_own_buffer(layout):
     """outputs in the same allocation as the caches, no byte in common: taken, and the caches stay as they were"""
