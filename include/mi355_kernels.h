@@ -792,7 +792,7 @@ MI355_API int64_t mi355_flash_attn_ext_mass_workspace_bytes(const mi355_fattn_ar
 MI355_API int     mi355_flash_attn_ext_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace,
                                             int64_t workspace_bytes, void *stream);
 /* The weights alone, for up to 65535 queries (a prompt, or the last ones of it; a longer prompt in pieces, with a decay of 1 and mass_in = mass_out):
- * v, dst and dv of args are not used. */
+ * v, dst and dv of args are not used.  At most 2^28 rows of q (sequences x heads x queries) and 2^36 places of mask in all, together, else MI355_E_SHAPE. */
 MI355_API int64_t mi355_attn_mass_workspace_bytes(const mi355_fattn_args *args);
 MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace, int64_t workspace_bytes,
                                   void *stream);
@@ -809,7 +809,7 @@ MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn
  *   tables of the gathered rows, 0 and -1 behind the last.
  * What is written must not share memory with what is read nor with another output, else MI355_E_UNSUPPORTED: a cache is not compacted in place.
  * (Rows of K_out between rows of V_out at one pitch, or in the part of a buffer behind the cache, are apart.)
- * n_sink + n_recent <= n_keep, n_keep >= 1, n_kv, n_keep and n_evict at most 2^30, else MI355_E_SHAPE. */
+ * n_sink + n_recent <= n_keep, n_keep >= 1, n_kv, n_keep and n_evict at most 2^30 (n_keep below 2^28 with rows to gather), else MI355_E_SHAPE. */
 typedef struct mi355_kv_evict_args {
     const float *mass; int64_t mass_nb2, mass_nb3;
     const int32_t *slot_pos; int64_t pos_nb2, pos_nb3;

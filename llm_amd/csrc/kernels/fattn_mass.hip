@@ -1335,7 +1335,6 @@ template <int TYPE, int D, bool CAP> static int prompt_launch(const MArgs & a, i
     const unsigned hk = (unsigned)a.n_head_kv, z = (unsigned)ne3;
     const int64_t slot_wgs = (a.n_kv + 1023) / 1024, query_wgs = a.mask ? (a.n_q + 3) / 4 : 1, class_wgs = slot_wgs * query_wgs * a.m_ne2 * a.m_ne3;
     const int64_t row_wgs = (R + 15) / 16, prep = class_wgs + row_wgs * hk * z;
-    if (prep > 0x7fffffff) return MI355_E_SHAPE;
     MI355_LAUNCH("attn_mass_prep", (prompt_prep_kernel<D, Fmt<TYPE>::bf>), dim3((unsigned)prep), dim3(PT), 0, s, a, (uint32_t)class_wgs, (uint32_t)slot_wgs,
                  (uint32_t)query_wgs, (uint32_t)row_wgs);
     MI355_CHECK_LAUNCH();
@@ -1388,6 +1387,10 @@ static WsParts mass_parts(const mi355_fattn_args * p, bool with_dst) {
     }
     return w;
 }
+static int64_t prep_workgroups(const mi355_fattn_args * p) {
+    const int64_t classes = (p->n_kv + 1023) / 1024 * (p->mask ? (p->n_q + 3) / 4 * p->m_ne2 * p->m_ne3 : 1);
+    return classes + (p->n_head / p->n_head_kv * p->n_q + 15) / 16 * p->n_head_kv * p->ne3;
+}
 // the shapes and types that both entry points take; what the workspace's size is formed from is bounded here, so its products stay within 64 bits
 static int mass_shape(const mi355_fattn_args * p, bool with_dst) {
     const int64_t dv = p->dv ? p->dv : p->d;
@@ -1403,6 +1406,8 @@ static int mass_shape(const mi355_fattn_args * p, bool with_dst) {
     if (ratio * ratio * p->n_q > 0xffffffffll) return MI355_E_SHAPE;
     if (with_dst && p->n_q > MI355_MASS_MAX_Q) return MI355_E_UNSUPPORTED;
     if (p->mask && (p->m_ne2 < 1 || p->m_ne3 < 1 || p->m_ne2 > 65535 || p->m_ne3 > 65535 || p->m_ne2 * p->m_ne3 > 65535)) return MI355_E_SHAPE;
+    // prompt_prep's grid: less than 2^32 threads, a workgroup of 256 for 16 rows of q or 4 x 1024 places of a mask
+    if (p->n_q > MI355_MASS_MAX_Q && prep_workgroups(p) * PT > 0xffffffffll) return MI355_E_SHAPE;
     // steps keep a logit per (row, slot): more than 2^56 of them are no memory's size
     if (p->n_q <= MI355_MASS_MAX_Q && p->ne3 * p->n_head * p->n_q > (1ll << 56) / (p->n_kv + 4)) return MI355_E_SHAPE;
     return MI355_OK;

@@ -332,6 +332,8 @@ int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
         for (const Span & x : in) if (spans_meet(o, x)) return MI355_E_UNSUPPORTED;
         for (const Span * x = out; x != &o; x++) if (spans_meet(o, *x)) return MI355_E_UNSUPPORTED;
     }
+    // a row of 64 pieces and more takes a wave, 16 of them a workgroup: a grid dimension's 2^32 threads hold 2^28 such rows
+    if ((p->k || p->v) && p->n_keep >= 1 << 28) return MI355_E_SHAPE;
     if (p->ne3 == 0) return MI355_OK;
 
     KeArgs a;
@@ -352,7 +354,7 @@ int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
     g.dst[0] = (char *)p->k_out; g.d_nb1[0] = p->ko_nb1; g.d_nb2[0] = p->ko_nb2; g.d_nb3[0] = p->ko_nb3;
     g.src[1] = (const char *)p->v; g.s_nb1[1] = p->v_nb1; g.s_nb2[1] = p->v_nb2; g.s_nb3[1] = p->v_nb3;
     g.dst[1] = (char *)p->v_out; g.d_nb1[1] = p->vo_nb1; g.d_nb2[1] = p->vo_nb2; g.d_nb3[1] = p->vo_nb3;
-    g.row_bytes[0] = p->k ? (int)mi355_row_size(p->type_kv, p->d) : 0; g.row_bytes[1] = p->v ? (int)mi355_row_size(p->type_kv, dv) : 0;
+    g.row_bytes[0] = (int)bk; g.row_bytes[1] = (int)bv;
     g.n_keep = a.n_keep;
     g.mass = a.mass; g.mass_nb2 = a.mass_nb2; g.mass_nb3 = a.mass_nb3; g.pos = a.pos; g.pos_nb2 = a.pos_nb2; g.pos_nb3 = a.pos_nb3;
     g.mass_out = (char *)p->mass_out; g.mo_nb2 = p->mo_nb2; g.mo_nb3 = p->mo_nb3;

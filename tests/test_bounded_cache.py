@@ -103,6 +103,13 @@ def test_kv_evict_refuses_outputs_that_meet_what_it_reads(kw):
     assert K.lib.mi355_kv_evict(evict_args(**kw), None) == E_UNSUPPORTED
 
 
+@pytest.mark.parametrize("kw", [dict(n_keep=1 << 30), dict(n_keep=1 << 28), dict(n_keep=1 << 29, k_nb1=258), dict(n_keep=1 << 28, ne3=0)])
+def test_kv_evict_refuses_more_rows_than_a_grid_holds(kw):
+    """before the first of its launches, not by the second's failure"""
+    far = {f: 1 << (50 + i) for i, f in enumerate(("k", "v", "k_out", "v_out", "mass_out", "pos_out", "kept", "evicted"))}
+    assert K.lib.mi355_kv_evict(evict_args(**far, **kw), None) == E_SHAPE
+
+
 def test_kv_evict_of_no_sequences_launches_nothing():
     assert K.lib.mi355_kv_evict(None, None) == E_NULL
     assert K.lib.mi355_kv_evict(evict_args(ne3=0), None) == 0
@@ -181,6 +188,12 @@ def test_attention_mass_workspaces_of_no_queries(n_kv, kw):
     a, w = attn_args(n_kv=n_kv, **kw)
     for size, run in ((K.lib.mi355_flash_attn_ext_mass_workspace_bytes, K.lib.mi355_flash_attn_ext_mass), (K.lib.mi355_attn_mass_workspace_bytes, K.lib.mi355_attn_mass)):
         assert size(a) == -1 and run(a, w, P, 1 << 40, None) == E_SHAPE
+
+
+@pytest.mark.parametrize("kw", [dict(n_q=65535, n_head=64, n_head_kv=8, ne3=65), dict(n_q=65535, n_kv=1 << 20, m_ne2=2), dict(n_q=60000, n_head=16, n_kv=1 << 20, m_ne3=10, ne3=10)])
+def test_attn_mass_refuses_more_than_a_grid_holds(kw):
+    a, w = attn_args(**kw)
+    assert K.lib.mi355_attn_mass_workspace_bytes(a) == -1 and K.lib.mi355_attn_mass(a, w, P, 1 << 62, None) == E_SHAPE
 
 
 @pytest.mark.parametrize("kw", [dict(n_head=65535, n_head_kv=65535, n_q=8, ne3=65535, n_kv=1 << 30), dict(n_head=60000, n_head_kv=60000, ne3=60000, n_kv=1 << 30),
