@@ -806,7 +806,7 @@ MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn
  *   mi355_qk_norm_rope takes as rows.
  *   k, v / k_out, v_out (optional): the kept rows, gathered into other memory in kept's order (type_kv, rows of d and dv values, strides nb1
  *   (slot) / nb2 / nb3; 2-byte aligned, faster at 16); rows behind the last kept one stay as they were.  mass_out, pos_out [n_keep, ..] (optional): the
- *   tables of the gathered rows, 0 and -1 behind the last.
+ *   tables of the gathered rows, 0 and -1 behind the last.  Tensors of no slots or no sequences may be NULL.
  * What is written must not share memory with what is read nor with another output, else MI355_E_UNSUPPORTED: a cache is not compacted in place.
  * (Rows of K_out between rows of V_out at one pitch, or in the part of a buffer behind the cache, are apart.)
  * n_sink + n_recent <= n_keep, n_keep >= 1, n_kv, n_keep and n_evict at most 2^30 (n_keep below 2^28 with rows to gather), else MI355_E_SHAPE. */

@@ -300,8 +300,9 @@ static int select_dispatch(const KeArgs & a, int64_t ne3, hipStream_t s) {
 extern "C" {
 
 int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
-    if (!p || (p->n_kv > 0 && (!p->mass || !p->slot_pos)) || !p->n_past || !p->kept) return MI355_E_NULL;
-    if (!p->k != !p->k_out || !p->v != !p->v_out) return MI355_E_NULL;
+    // (tensors of no sequences or no slots have no address)
+    if (!p || (p->ne3 != 0 && ((p->n_kv > 0 && (!p->mass || !p->slot_pos)) || !p->n_past || !p->kept))) return MI355_E_NULL;
+    if (p->ne3 != 0 && p->n_kv > 0 && (!p->k != !p->k_out || !p->v != !p->v_out)) return MI355_E_NULL;
     constexpr int64_t most = 1 << 30;                 // (32-bit slot numbers, a workgroup's stride past the last)
     if (p->n_kv < 0 || p->n_kv > most || p->n_keep < 1 || p->n_keep > most || p->n_evict < 0 || p->n_evict > most) return MI355_E_SHAPE;
     if (p->n_sink < 0 || p->n_recent < 0 || (int64_t)p->n_sink + p->n_recent > p->n_keep) return MI355_E_SHAPE;

@@ -113,6 +113,9 @@ def test_kv_evict_refuses_more_rows_than_a_grid_holds(kw):
 def test_kv_evict_of_no_sequences_launches_nothing():
     assert K.lib.mi355_kv_evict(None, None) == E_NULL
     assert K.lib.mi355_kv_evict(evict_args(ne3=0), None) == 0
+    assert K.lib.mi355_kv_evict(evict_args(ne3=0, mass=None, slot_pos=None, n_past=None, kept=None, evicted=None, k=None, v=None, k_out=None, v_out=None,
+                                           mass_out=None, pos_out=None), None) == 0
+    assert K.lib.mi355_kv_evict(evict_args(ne3=0, n_keep=0), None) == E_SHAPE
 
 
 def attn_args(**kw):

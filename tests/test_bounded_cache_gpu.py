@@ -414,6 +414,19 @@ def test_evict_keeps_sinks_and_recent_slots_before_any_mass(n):
             assert np.array_equal(evicted[0, h].cpu().numpy(), np.setdiff1d(np.arange(n), want))
 
 
+@pytest.mark.parametrize("t", [B.F16, B.Q8_0])
+@pytest.mark.parametrize("S,n", [(0, 10), (2, 0), (0, 0)])
+def test_evict_of_no_sequences_or_slots(S, n, t):
+    """with and without caches: empty results, -1 and 0 where nothing is kept"""
+    HK, n_keep, row = 2, 3, 64 if t in DTYPE else 2 * B.TYPE_SIZE[t]
+    mass, pos, past = torch.zeros((S, HK, n), device="cuda"), torch.zeros((S, HK, n), dtype=torch.int32, device="cuda"), torch.zeros(S, dtype=torch.int32, device="cuda")
+    kept, evicted = ops.kv_evict(mass, pos, past, n_keep)
+    assert kept.shape == (S, HK, n_keep) and (kept == -1).all() and evicted.shape == (S, HK, max(0, n - n_keep))
+    k, v = (torch.zeros((S, HK, n, row), dtype=DTYPE.get(t, torch.uint8), device="cuda") for _ in range(2))
+    kept, _, mo, po, ko, vo = ops.kv_evict(mass, pos, past, n_keep, 1, 1, n_used=past, k=k, v=v, type_kv=t)
+    assert (kept == -1).all() and (mo == 0).all() and (po == -1).all() and ko.shape == vo.shape == (S, HK, n_keep, row) and (ko == 0).all() and (vo == 0).all()
+
+
 @pytest.mark.parametrize("layout", ["behind", "turns", "side", "halves", "slots"])
 def test_evict_gathers_into_the_caches_own_buffer(layout):
     """outputs in the same allocation as the caches, no byte in common: taken, and the caches stay as they were"""
