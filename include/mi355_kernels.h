@@ -746,7 +746,7 @@ MI355_API int     mi355_flash_attn_ext_noalloc(const mi355_fattn_args *args, voi
  *   byte strides nb1 (token), nb2 (head), nb3 (sequence), 16-byte aligned; q_out likewise (it may be q itself, row for row; else it
  *   shares no memory with q, k and v: MI355_E_UNSUPPORTED)
  *   k_out, v_out: caches of type_kv f32 | f16 | bf16 (16-byte aligned) | q8_0 | q4_0 (2-byte aligned, whole 32-blocks, else MI355_E_SHAPE),
- *   byte strides nb1 (row), nb2 (head), nb3 (sequence), n_rows rows per head
+ *   byte strides nb1 (row), nb2 (head), nb3 (sequence), n_rows rows per head (0: may be NULL, nothing is stored)
  *   rows: int32 cache row of each (token, head, sequence), strides nb1 / nb2 / nb3 (0: shared); NULL: token i goes to row i.  A row outside
  *   [0, n_rows) is not stored (q_out is written all the same).  Rows of one call must be distinct per head and sequence.
  *   q_norm, k_norm f32 [head_dim]; NULL: no weight.  pos int32 [n, ne3], freq_factors f32 [n_dims / 2] or NULL, rope parameters as in

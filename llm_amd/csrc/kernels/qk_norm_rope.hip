@@ -201,7 +201,11 @@ template <int TYPE> static int qn_launch(const QnArgs & a, hipStream_t s) {
 extern "C" {
 
 int mi355_qk_norm_rope(const mi355_qk_norm_rope_args * p, void * stream) {
-    if (!p || !p->q || !p->k || !p->q_out || !p->k_out || !p->pos || !p->v != !p->v_out) return MI355_E_NULL;
+    if (!p) return MI355_E_NULL;
+    if (p->n != 0 && p->ne3 != 0) {                   // (tensors of no tokens or sequences, and caches of no rows, have no address)
+        if (!p->q || !p->k || !p->q_out || !p->pos) return MI355_E_NULL;
+        if (p->n_rows != 0 && (!p->k_out || !p->v != !p->v_out)) return MI355_E_NULL;
+    }
     const int64_t dv = p->dv ? p->dv : p->head_dim;
     if (p->head_dim < 8 || p->head_dim > 256 || p->head_dim % 8 || dv < 8 || dv > 256 || dv % 8) return MI355_E_UNSUPPORTED;
     if (p->n_dims < 0 || p->n_dims > p->head_dim) return MI355_E_SHAPE;
@@ -233,7 +237,7 @@ int mi355_qk_norm_rope(const mi355_qk_norm_rope_args * p, void * stream) {
     a.qw = p->q_norm; a.kw = p->k_norm; a.ff = p->freq_factors;
     a.qo = (char *)p->q_out; a.qo_nb1 = p->qo_nb1; a.qo_nb2 = p->qo_nb2; a.qo_nb3 = p->qo_nb3;
     a.ko = (char *)p->k_out; a.ko_nb1 = p->ko_nb1; a.ko_nb2 = p->ko_nb2; a.ko_nb3 = p->ko_nb3;
-    a.vo = (char *)p->v_out; a.vo_nb1 = p->vo_nb1; a.vo_nb2 = p->vo_nb2; a.vo_nb3 = p->vo_nb3;
+    a.vo = p->v ? (char *)p->v_out : nullptr; a.vo_nb1 = p->vo_nb1; a.vo_nb2 = p->vo_nb2; a.vo_nb3 = p->vo_nb3;
     a.pos = (const char *)p->pos; a.pos_nb1 = p->pos_nb1; a.pos_nb3 = p->pos_nb3;
     a.rows = (const char *)p->rows; a.rows_nb1 = p->rows_nb1; a.rows_nb2 = p->rows_nb2; a.rows_nb3 = p->rows_nb3;
     a.slot_pos = (char *)p->slot_pos; a.sp_nb2 = p->sp_nb2; a.sp_nb3 = p->sp_nb3;

@@ -55,6 +55,9 @@ def test_qk_norm_rope_of_nothing_launches_nothing():
     assert K.lib.mi355_qk_norm_rope(None, None) == E_NULL
     assert K.lib.mi355_qk_norm_rope(store_args(n=0), None) == 0
     assert K.lib.mi355_qk_norm_rope(store_args(ne3=0), None) == 0
+    none = dict(q=None, k=None, v=None, q_out=None, k_out=None, v_out=None, pos=None, rows=None)
+    assert K.lib.mi355_qk_norm_rope(store_args(ne3=0, **none), None) == 0 and K.lib.mi355_qk_norm_rope(store_args(n=0, **none), None) == 0
+    assert K.lib.mi355_qk_norm_rope(store_args(n_rows=0, q=None), None) == E_NULL
 
 
 def evict_args(**kw):

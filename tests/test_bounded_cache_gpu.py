@@ -220,6 +220,17 @@ def test_store_without_v_without_rows_of_nothing_and_of_zeros():
     assert out.shape == (1, 2, 0, 64)
 
 
+@pytest.mark.parametrize("t", [B.F16, B.Q4_0])
+def test_store_into_a_cache_of_no_rows(t):
+    """nothing to store into: q is normalised and rotated all the same"""
+    q, k, v, dev, qw, kw, _, _, _, pos = store_case(2, 3, 4, 2, 64, 64, 4, B.F16, 15)
+    none = torch.zeros((2, 2, 0, 64 if t in DTYPE else 2 * B.TYPE_SIZE[t]), dtype=DTYPE.get(t, torch.uint8), device="cuda")
+    want, err = store_oracle(q, qw, 1e-6, pos, 64, 2)
+    for vv, vc in ((dev["v"], none), (None, None)):
+        qo = ops.qk_norm_rope(dev["q"], dev["k"], vv, qw.cuda(), kw.cuda(), 1e-6, pos.cuda(), none, vc, t)
+        assert ((qo.cpu().double() - want).abs() <= err).all()
+
+
 def test_store_on_another_stream_and_captured():
     """launched on the current stream whatever it is; a captured launch reads new rows and positions at every replay"""
     S, n, H, HK, d, slots = 2, 1, 8, 2, 128, 16
