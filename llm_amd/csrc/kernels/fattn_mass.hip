@@ -209,9 +209,8 @@ static __device__ __forceinline__ float sum_groups(float v) {
 // RP (blocks only): the 16 columns of a tile are RP rows times 16 / RP classes of 32-blocks -- at GQA 4 or 8
 // the columns that would repeat a row each scale P by the blocks of their class, so a lane forms D / 32 / (16 / RP) scaled copies of P and not
 // D / 32; a feature tile takes its result from the columns of its block's class.
-// RAW (blocks only, step_raw): rows come in as consecutive pieces of D / 16 bytes (17 or 9 a row) and are taken apart in LDS.  A lane that loads
-// the 8 bytes of its own chunk reads at every second byte address, which the address unit serves a lane per clock: the 20 loads of a
-// tile then cost a CU's 8 waves 4 us before the first product.
+// RAW (blocks only, step_raw): rows come in as consecutive pieces of D / 16 bytes (17 or 9 a row) and are taken apart in LDS, where otherwise a lane
+// loads the 8 bytes of its own chunk at every second byte address.  Taken where it pays, raw_pays below.
 // ONE: a workgroup has all slots of its KV head and finishes by itself, without the second launch (step_one).
 template <int TYPE, int D, int NW, bool HASV, int RP, bool RAW, bool ONE>
 __global__ void __launch_bounds__(NW * 64, D <= 64 && !ONE ? 3 : D <= 128 ? 2 : 1)
@@ -771,9 +770,15 @@ template <int TYPE, int D, bool HASV, int RP, bool RAW> static int step_launch(c
 }
 static int step_d(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-// rows of blocks that are whole pieces (see the kernel): full width, pieces aligned, a tile within 32-bit offsets
-template <bool HASV> static bool step_raw(const MArgs & a) {
-    const int D = step_d(a.d);
+// Are rows of blocks taken in as pieces (see the kernel)?  Whole call, 8 KV heads, own chunks against pieces, us.  Pieces hold more registers, at D 64
+// and for q8_0 with V more than there are beside two or three waves:
+//   q8_0 with V  D 64: 6 x 32768, 4 / 20 rows  80 / 156 against 108 / 259;  D 128: the same 112 / 201 against 112 / 252, 8 x 4099, 4 / 12 rows
+//                30.6 / 35.0 against 32.1 / 39.7;  D 256: 4 x 32768, 4 rows  162 against 165, 8 x 4099, 4 / 20 rows  68 / 113 against 67 / 111
+//   q4_0 with V  D 64: 6 x 32768, 4 / 20 rows  70 / 152 against 72 / 156;  D 128: 102 / 198 against 99 / 198;  D 256: 4 x 32768  159 against 150
+//   without V    6 x 32768, 32 rows  D 64 q8_0 148 against 147, q4_0 146 against 144;  D 128 q8_0 181 against 169, q4_0 180 against 159
+template <int TYPE, int D, bool HASV> constexpr bool raw_pays() { return Fmt<TYPE>::quant && D > 64 && !(TYPE == MI355_TYPE_Q8_0 && D == 128 && HASV); }
+// and can they be: full width, pieces aligned, a tile within 32-bit offsets
+template <int D, bool HASV> static bool step_raw(const MArgs & a) {
     uint64_t low = (uint64_t)(uintptr_t)a.k | a.k_nb1 | (uint64_t)a.k_nb2 | (uint64_t)a.k_nb3;
     if (HASV) low |= (uint64_t)(uintptr_t)a.v | a.v_nb1 | (uint64_t)a.v_nb2 | (uint64_t)a.v_nb3;
     return a.d == D && (!HASV || a.dv == D) && (low & (uint64_t)(D / 16 - 1)) == 0 && a.k_nb1 < (1u << 26) && (!HASV || a.v_nb1 < (1u << 26));
@@ -791,21 +796,17 @@ template <int TYPE, int D, bool HASV> static int one_launch(const MArgs & a, int
     MI355_CHECK_LAUNCH();
     return MI355_OK;
 }
-template <int TYPE, bool HASV, bool RAW> static int step_size(const MArgs & a, int ne3, hipStream_t s) {
-    switch (step_d(a.d)) {
-        case 64:  return step_rows<TYPE, 64, HASV, RAW>(a, ne3, s);
-        case 128: return step_rows<TYPE, 128, HASV, RAW>(a, ne3, s);
-    }
-    return step_rows<TYPE, 256, HASV, RAW>(a, ne3, s);
+template <int TYPE, int D, bool HASV> static int step_size(const MArgs & a, int ne3, hipStream_t s) {
+    if (a.one) return one_launch<TYPE, D, HASV>(a, ne3, s);
+    if constexpr (raw_pays<TYPE, D, HASV>()) if (step_raw<D, HASV>(a)) return step_rows<TYPE, D, HASV, true>(a, ne3, s);
+    return step_rows<TYPE, D, HASV, false>(a, ne3, s);
 }
 template <int TYPE, bool HASV> static int step_dispatch(const MArgs & a, int ne3, hipStream_t s) {
-    if (a.one) switch (step_d(a.d)) {
-        case 64:  return one_launch<TYPE, 64, HASV>(a, ne3, s);
-        case 128: return one_launch<TYPE, 128, HASV>(a, ne3, s);
-        default:  return one_launch<TYPE, 256, HASV>(a, ne3, s);
+    switch (step_d(a.d)) {
+        case 64:  return step_size<TYPE, 64, HASV>(a, ne3, s);
+        case 128: return step_size<TYPE, 128, HASV>(a, ne3, s);
     }
-    if constexpr (Fmt<TYPE>::quant) if (step_raw<HASV>(a)) return step_size<TYPE, HASV, true>(a, ne3, s);
-    return step_size<TYPE, HASV, false>(a, ne3, s);
+    return step_size<TYPE, 256, HASV>(a, ne3, s);
 }
 
 // One launch: a row tile of queries, and no more slots than one tile a wave.  8 heads of 128, f16, GPU time: 1 / 128 / 256 slots 8.4 / 7.8 / 9.5 us against
