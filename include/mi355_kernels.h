@@ -779,7 +779,8 @@ MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stre
  * head)^2 x queries below 2^32, else MI355_E_SHAPE; block rows 2-byte aligned, faster where a row's address is a multiple of d / 16).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be
  * mass_out itself, row for row, else they are apart (MI355_E_UNSUPPORTED); NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate (the query is not rounded to the cache's type, the
  * weights are not rounded before they meet V).  A slot hidden by the mask takes no part whatever its row holds; a query that sees no slot gives
- * a row of zeros and no weight.  At least one query and one sequence, at most 65535 of each, else MI355_E_SHAPE (ops.* answer a call of none themselves).
+ * a row of zeros and no weight.  Infinities in a K row that a query sees count as in the formula (a logit of -inf weighs 0); a block of K with a scale that is not
+ * finite, and values of V that are not, leave the results of the queries that see them not finite, NaN or infinite.  At least one query and one sequence, at most 65535 of each, else MI355_E_SHAPE (ops.* answer a call of none themselves).
  * workspace: *_workspace_bytes (-1 for sizes and types that the call itself refuses), 16-byte aligned, no initial contents, not shared by calls
  * that can overlap. */
 #define MI355_MASS_MAX_Q 8

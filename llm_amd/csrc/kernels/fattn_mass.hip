@@ -197,6 +197,16 @@ template <bool BF> static __device__ __forceinline__ bool sanitize(v4i & x) {
     return bad;
 }
 
+// q and K in parts, sum over the parts p of q_p K: an infinity of K meets the parts' different signs and gives a NaN where the product is an infinity.
+// Only the largest part, which has q's sign, meets it: the others take K without its non-finite values.  (Where q's large part is 0 so is q, next to
+// its row's largest value.)  For tiles that have a NaN among their products
+template <bool BF> static __device__ __forceinline__ v4i finite(v4i x) {
+    asm volatile("" : "+v"(x));                                 // (formed where it is used: kept through a loop it takes the operands' registers again)
+    sanitize<BF>(x);
+    return x;
+}
+static __device__ __forceinline__ void read_again() { asm volatile("" ::: "memory"); }     // (so that what was read from LDS is not kept for a second use)
+
 static __device__ __forceinline__ float max_groups(float v) {       // over the four 16-lane groups, lanes of equal place
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
@@ -439,6 +449,23 @@ mass_step_kernel(const MArgs a) {
 #pragma unroll
                         for (int i = 0; i < 4; i++) c[u][i] = __builtin_fmaf(b[i], (float)dk[u][i][ks], c[u][i]);
                     } else c[u] = b;
+                }
+            }
+            if constexpr (!F::quant) {                          // an infinity in a row of K (see finite)
+                bool nan = false;
+#pragma unroll
+                for (int i = 0; i < 8; i++) nan |= c[i >> 2][i & 3] != c[i >> 2][i & 3];
+                if (__any(nan)) {
+                    read_again();
+                    c[0] = c[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const v4i f = finite<F::bf>(kc[u][ks].raw);
+#pragma unroll
+                            for (int p = P - 1; p >= 0; p--) c[u] = mfma16<F::bf>(p == 0 ? kc[u][ks].raw : f, qs[ks][p][lane], c[u]);
+                        }
                 }
             }
         }
@@ -1075,47 +1102,53 @@ prompt_stats_kernel(const MArgs a) {
         const uint32_t bytes = cl[b][wave][lane] >> (16 * (t & 1));
         const int c0 = bytes & 255, c1 = bytes >> 8 & 255;
         if (mine && __any((c0 | c1) != MASK_HIDDEN)) {
-            v16f c[2], part;
+            auto tile = [&](bool again) {                       // -> maximum and sum with this tile
+                v16f c[2], part;
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+                for (int u = 0; u < 2; u++) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
+                    for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const v4i k0 = *(const v4i *)(kt[b] + lds_chunk<D>(32 * u + lr, 2 * ks + lh));
-                    if constexpr (F::quant) {
-                        if (ks % 2 == 0) {
+                    for (int ks = 0; ks < KS; ks++) {
+                        const v4i k0 = *(const v4i *)(kt[b] + lds_chunk<D>(32 * u + lr, 2 * ks + lh));
+                        if constexpr (F::quant) {
+                            if (ks % 2 == 0) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) part[i] = 0.0f;
+                                for (int i = 0; i < 16; i++) part[i] = 0.0f;
+                            }
+#pragma unroll
+                            for (int p = QP - 1; p >= 0; p--) part = mfma32<F::bf>(k0, qf[ks][p], part);
+                            if (ks % 2 == 1) fold_block(&kd[b][ks / 2][32 * u], lh, part, c[u]);
+                        } else {
+                            const v4i f = again ? finite<F::bf>(k0) : k0;
+#pragma unroll
+                            for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(p == 0 ? k0 : f, qf[ks][p], c[u]);
                         }
-#pragma unroll
-                        for (int p = QP - 1; p >= 0; p--) part = mfma32<F::bf>(k0, qf[ks][p], part);
-                        if (ks % 2 == 1) fold_block(&kd[b][ks / 2][32 * u], lh, part, c[u]);
-                    } else {
-#pragma unroll
-                        for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(k0, qf[ks][p], c[u]);
                     }
                 }
-            }
-            float sc = qe;
-            if (CAP || !__all(c0 == MASK_ZERO && c1 == MASK_ZERO)) {
-                tile_logits<CAP>(a, c[0], qe, slope, c0, mrow, m8, t * PA_SLOTS);
-                tile_logits<CAP>(a, c[1], qe, slope, c1, mrow, m8, t * PA_SLOTS + 32);
-                sc = 1.0f;
-            }
-            float mx = c[0][0];
+                float sc = qe;
+                if (CAP || !__all(c0 == MASK_ZERO && c1 == MASK_ZERO)) {
+                    tile_logits<CAP>(a, c[0], qe, slope, c0, mrow, m8, t * PA_SLOTS);
+                    tile_logits<CAP>(a, c[1], qe, slope, c1, mrow, m8, t * PA_SLOTS + 32);
+                    sc = 1.0f;
+                }
+                float mx = c[0][0];
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, c[u][i]);
-            mx = fmaxf(m, mx * sc);
-            const float ms = mx == -INFINITY ? 0.0f : mx;
-            l *= __builtin_amdgcn_exp2f(m - ms);
+                    for (int i = 0; i < 16; i++) mx = fmaxf(mx, c[u][i]);
+                mx = fmaxf(m, mx * sc);
+                const float ms = mx == -INFINITY ? 0.0f : mx;
+                float ln = l * __builtin_amdgcn_exp2f(m - ms);
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) l += __builtin_amdgcn_exp2f(__builtin_fmaf(c[u][i], sc, -ms));
-            m = mx;
+                    for (int i = 0; i < 16; i++) ln += __builtin_amdgcn_exp2f(__builtin_fmaf(c[u][i], sc, -ms));
+                return v2f{mx, ln};
+            };
+            v2f x = tile(false);
+            if constexpr (!F::quant) if (__any(x.y != x.y && l == l)) { read_again(); x = tile(true); }     // an infinity in a row of K (see finite)
+            m = x.x; l = x.y;
         }
         if (S == 2 && ahead < nt) commit(bf);
         b = b == S - 1 ? 0 : b + 1;
@@ -1216,6 +1249,14 @@ prompt_mass_kernel(const MArgs a) {
     for (int u = 0; u < NS; u++)
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) arrived(kf[u][ks]);
+    bool odd = false;                                           // an infinity in a row of K (see finite)
+    if constexpr (!F::quant) {
+#pragma unroll
+        for (int u = 0; u < NS; u++)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) { v4i x = kf[u][ks]; odd |= sanitize<F::bf>(x); }
+        odd = __any(odd);
+    }
     float acc[NS][16];
 #pragma unroll
     for (int u = 0; u < NS; u++)
@@ -1261,6 +1302,20 @@ prompt_mass_kernel(const MArgs a) {
                 if constexpr (F::quant) if (ks % 2 == 1) {
 #pragma unroll
                     for (int u = 0; u < NS; u++) fold_block(&kd[wave][ks / 2][32 * u], lh, part[u], c[u]);
+                }
+            }
+            if constexpr (!F::quant) if (odd) {
+                read_again();
+#pragma unroll
+                for (int u = 0; u < NS; u++) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        const v4i f = finite<F::bf>(kf[u][ks]);
+#pragma unroll
+                        for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(p == 0 ? kf[u][ks] : f, *(const v4i *)(qt[b][p] + lds_chunk<D>(lr, 2 * ks + lh)), c[u]);
+                    }
                 }
             }
             float sc = c4.qe;

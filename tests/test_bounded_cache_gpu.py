@@ -824,6 +824,37 @@ def test_attention_mass_softcap_is_as_exact_as_f32(t, n, cap):
     assert far(got) <= 1.5 * far(f32) + 3e-7
 
 
+@pytest.mark.parametrize("t", [B.F16, B.BF16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_attention_mass_of_keys_with_infinities(t, d, n):
+    """a logit of -inf is a weight of 0, as if the slot were hidden; one of +inf makes its own query's results NaN and no other's"""
+    H, HK, slots, scale = 8, 2, 300, 0.08
+    q, k, v, _ = attn_case(1, H, HK, n, slots, d, d, t, d + n)
+    q[..., 7], q[..., 40] = -q[..., 7].abs() - 0.1, q[..., 40].abs() * 1e-3 + 1e-4
+    out = [3, 31, 32, 100, 201, 299]
+    k[:, :, out[::2], 7], k[:, :, out[1::2], 40] = float("inf"), float("-inf")
+    mask = causal(1, n, slots)
+    hidden, clean = mask.clone(), k.clone()
+    hidden[..., out] = float("-inf")
+    clean[:, :, out] = 0.0
+    wd, ed, wm, em = attn_oracle(q, values(clean, t), values(v, t), hidden, scale, None, 0.0)
+    args = (k.cuda(), mask.cuda(), t, scale)
+    assert ((ops.attn_mass(q.cuda(), *args).cpu().double() - wm).abs() <= em).all()
+    if n <= 8:
+        dst, mass = ops.flash_attn_ext_mass(q.cuda(), k.cuda(), v.cuda(), mask.cuda(), t, scale)
+        assert ((dst.cpu().double() - wd).abs() <= ed).all() and ((mass.cpu().double() - wm).abs() <= em).all()
+    q[0, 5, n - 1, 7] = 1.0                                   # the other sign: +inf among the logits of head 5's last query
+    mass = ops.attn_mass(q.cuda(), *args).cpu()
+    _, _, wm, em = attn_oracle(q[:, :4], values(clean, t)[:, :1], None, hidden, scale, None, 0.0)
+    assert torch.isnan(mass[0, 1, out[0]]) and ((mass[:, :1].double() - wm).abs() <= em).all()
+    if n <= 8:
+        dst, _ = ops.flash_attn_ext_mass(q.cuda(), k.cuda(), v.cuda(), args[1], t, scale)
+        other = torch.ones((n, H), dtype=torch.bool)
+        other[n - 1, 5] = False
+        assert torch.isnan(dst[0, n - 1, 5]).all() and ((dst.cpu().double() - wd).abs() <= ed)[0][other].all()
+
+
 @pytest.mark.parametrize("S,n,slots", [(1, 0, 5), (2, 0, 512), (1, 0, 100000), (0, 1, 512), (0, 40, 300), (1, 0, 0)])
 def test_attention_mass_of_no_queries(S, n, slots):
     """an empty batch: an empty dst, and what earlier calls left, decayed"""
