@@ -740,8 +740,9 @@ MI355_API int     mi355_flash_attn_ext_noalloc(const mi355_fattn_args *args, voi
  * position a slot holds (int32) and its accumulated weight, its "mass" (f32).  Keys are stored rotated, so a slot's place says nothing.
  *
  * Attention input of models that normalise queries and keys per head, in one launch: q_out = rope(rms_norm(q) * q_norm), K cache row =
- * rope(rms_norm(k) * k_norm), V cache row = v.  Replaces the node run RMS_NORM MUL ROPE (q and k) and the stores of K and V (SET_ROWS / CPY):
- * eight launches of ggml-cuda (norm.cu, binbcast.cu, rope.cu, set-rows.cu).
+ * rope(rms_norm(k) * k_norm), V cache row = v.  Computes the node run RMS_NORM MUL ROPE (q and k) and the stores of K and V (SET_ROWS / CPY),
+ * eight launches of ggml-cuda (norm.cu, binbcast.cu, rope.cu, set-rows.cu), for a binder that calls it; the plugin does not look for that run and
+ * launches its nodes one by one.
  *   q f32 [head_dim, n_head, n, ne3], k f32 [head_dim, n_head_kv, n, ne3], v f32 [dv, n_head_kv, n, ne3] (v and v_out may be NULL: no V):
  *   byte strides nb1 (token), nb2 (head), nb3 (sequence), 16-byte aligned; q_out likewise (it may be q itself, row for row; else it
  *   shares no memory with q, k and v: MI355_E_UNSUPPORTED)
@@ -798,8 +799,9 @@ MI355_API int64_t mi355_attn_mass_workspace_bytes(const mi355_fattn_args *args);
 MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace, int64_t workspace_bytes,
                                   void *stream);
 
-/* The slots of a bounded cache that stay, per (sequence, KV head): of the first n_used[i3] slots the n_keep with the largest mass, where a slot
- * whose position is below n_sink or at least n_past[i3] - n_recent comes before any mass, +inf included; ties go to the lower slot, NaN counts as -inf.
+/* The slots of a bounded cache that stay, per (sequence, KV head): of the first n_used[i3] slots the n_keep with the largest mass, ties to the lower
+ * slot, NaN counts as -inf.  A slot whose position is below n_sink (a negative one too: n_used leaves empty slots out) or at least
+ * n_past[i3] - n_recent comes before any mass, +inf included.
  *   mass f32, slot_pos int32 [n_kv, n_head_kv, ne3] (strides nb2 / nb3); n_used int32 [ne3] (NULL: n_kv; clamped to [0, n_kv]); n_past int32
  *   [ne3]: tokens the sequence has seen.  All read on the device: a captured call follows them.
  *   kept int32 [n_keep, n_head_kv, ne3]: the kept slots, ascending, -1 behind the last where n_used < n_keep

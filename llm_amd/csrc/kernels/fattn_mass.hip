@@ -1,10 +1,11 @@
 // fattn_mass.hip -- attention weight per cached slot: mi355_flash_attn_ext_mass (a decode step's attention together with it) and
-// mi355_attn_mass (the weight alone, for any number of queries).
+// mi355_attn_mass (the weight alone, for a prompt's queries).
 //
 //   s_ij = scale q_i . k_j [softcap] + slope mask_ij      p_ij = exp(s_ij - m_i) / l_i     (m_i, l_i: maximum and sum over the slots i sees)
 //   dst_i = sum_j p_ij v_j      mass_out[hk][j] = decay mass_in[hk][j] + sum over the heads of hk and all queries i of p_ij
 // A slot that a query does not see (mask -inf) takes no part whatever its row holds, NaN included; a query that sees nothing gives a zero row and
-// no weight.  Everything between the cache's own values and the f32 results is f32.
+// no weight.  Sums, maxima and logits are f32; what meets the matrix cores is 22 bits of q and p (two f16 parts), 24 over bf16 caches (three bf16
+// parts), and the cache's own values, exact.
 #include "common.h"
 #include "spans.h"
 
@@ -859,11 +860,14 @@ static int64_t step_splits(const mi355_fattn_args * p) {
 //   prompt_mass   S^T again and sum over the rows of 2^(s - m) / l: a wave holds 32 or 64 slots of K, Q passes through LDS; the sums stay in
 //                 registers, one per (slot, lane), and meet across the lanes once at the end
 //   prompt_sum    the row chunks' sums and decay * mass_in, in a fixed order
-// v_mfma_f32_32x32x16 throughout: K of f16 and bf16 as it is; blocks as their integers, whose products a block's scale is put on in f32.  What passes through LDS comes by DMA, two tiles ahead of the products.  A tile that the mask hides from all rows of a
-// wave (half of a causal prompt) costs its loads.
+// v_mfma_f32_32x32x16 throughout: K of f16 and bf16 as it is; blocks as their integers, whose products a block's scale is put on in f32.  On its way
+// through LDS: K of f16 and bf16 in the first pass by DMA, two tiles ahead of the products, blocks through registers, one ahead; Q in the second pass
+// by DMA, two tiles ahead, one with heads above 128 (LDS).  A tile that the mask hides from all rows of a wave (half of a causal prompt) costs its
+// loads and its meeting.
 // 64 queries x 32 heads over 16384 f16 slots: 5 + 25 + 5 + 32 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
 // until the first tile of 512 workgroups is there; without its products the first pass takes 20, without its exponentials 23.  2047
-// causal queries, bf16: 16 + 68 + 83 + 5 us, 45 a pass at that rate.
+// causal queries, bf16: 16 + 68 + 82 + 5 us, 45 a pass at that rate.  Matrix cores and vector units are each busy a third of either pass (30-40 %), a
+// wave waits for its turn or its operands most of the rest: 1.7 waves a SIMD do not cover one another's chains.
 typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int PT = 256;                  // threads: 4 waves
 constexpr int PA_ROWS = 128, PA_SLOTS = 64, PB_ROWS = 32;

@@ -1,9 +1,9 @@
 // kv_evict.hip -- which slots of a bounded KV cache to keep, by the attention weight they have drawn (mi355_kv_evict).
 //
 // Per (sequence, KV head): the n_keep slots with the largest key, ties to the lower slot; key = the slot's mass, or more than any mass where its
-// position is one of the first n_sink or the newest n_recent, pinned (NaN counts as -inf, -0 as +0).  The keys' 32-bit images (order-preserving: sign flipped for
-// positive floats, all bits for negative ones) are searched for the n_keep-th largest; one ordered pass then writes both index lists
-// ascending.  All integer work: the result does not depend on timing.  The rows are gathered by a second launch.
+// position is one of the first n_sink or the newest n_recent, pinned (NaN counts as -inf, -0 as +0).  The keys' 32-bit images (order-preserving: sign
+// flipped for positive floats, all bits for negative ones) are searched for the n_keep-th largest; one ordered pass then writes both index
+// lists ascending.  All integer work: the result does not depend on timing.  The rows are gathered by a second launch.
 //
 // Bound by latency: one workgroup per head has to agree on every step of the search.  A step parts the range of keys that can still hold the
 // wanted one into 2048 buckets (an LDS histogram), so three steps settle 32 bits, and masses, which spread over the range as logarithms do,
@@ -21,8 +21,6 @@ struct KeArgs {
     int64_t mass_nb2, mass_nb3, pos_nb2, pos_nb3;
     char * kept, * evicted;
     int64_t kept_nb2, kept_nb3, ev_nb2, ev_nb3;
-    char * mass_out, * pos_out;
-    int64_t mo_nb2, mo_nb3, po_nb2, po_nb3;
     int n_kv, n_keep, n_evict, n_sink, n_recent, n_head_kv;
 };
 

@@ -54,7 +54,8 @@ template <int TYPE> static __device__ __forceinline__ void qn_store4(char * row,
 // holds itself -- NEOX: 4 i.. and n_dims / 2 + 4 i..; NORMAL and the features past n_dims: 8 i.. -- so nothing crosses lanes but the sum of
 // squares.  A workgroup first forms cos and sin of all pairs of its TT tokens in LDS (64-bit angles: ~100 clocks a pair, shared by every head),
 // then walks their rows two at a time, loads ahead.  Bound by the rows' bytes at prompts (8192 tokens x 64 / 8 heads of 128 in f16:
-// 637 MB in 140 us, 4.5 TB/s; 1111 tokens x 32 / 8 in bf16: 10.6 us), by one launch at steps (4.1 us).
+// 638 MB in 138-149 us, 4.3-4.6 TB/s, into q8_0 or q4_0 caches 147 for the whole call; 1111 tokens x 24 / 4 heads of 96 in bf16: 10.6 us), by one launch
+// at steps (4.3 us, 6.0 with blocks to quantize: 16 sequences x 64 / 8 heads, a quarter of a row's lanes take 32 values each).
 constexpr int QN_THREADS = 256;
 
 template <int TYPE, int L>
