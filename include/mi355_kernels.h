@@ -777,11 +777,13 @@ MI355_API int mi355_qk_norm_rope(const mi355_qk_norm_rope_args *args, void *stre
 /* FLASH_ATTN_EXT of a decode step (at most MI355_MASS_MAX_Q queries per sequence) that also accumulates the attention weight every slot draws:
  *   mass_out[j] = decay * mass_in[j] + sum over the queries and the heads that share the KV head of softmax(...)[j]
  * args as for mi355_flash_attn_ext (K and V of one type; rows of K and V at most 2^31 - 1 bytes apart, at most 65535 planes of mask, (heads per KV
- * head)^2 x queries below 2^32, else MI355_E_SHAPE; block rows 2-byte aligned, faster where a row's address is a multiple of d / 16).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be
- * mass_out itself, row for row, else they are apart (MI355_E_UNSUPPORTED); NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate (the query is not rounded to the cache's type, the
- * weights are not rounded before they meet V).  A slot hidden by the mask takes no part whatever its row holds; a query that sees no slot gives
- * a row of zeros and no weight.  Infinities in a K row that a query sees count as in the formula (a logit of -inf weighs 0); a block of K with a scale that is not
- * finite, and values of V that are not, leave the results of the queries that see them not finite, NaN or infinite.  At least one query and one sequence, at most 65535 of each, else MI355_E_SHAPE (ops.* answer a call of none themselves).
+ * head)^2 x queries below 2^32, at least one query and one sequence, at most 65535 of each, else MI355_E_SHAPE -- ops.* answer a call of none
+ * themselves; block rows 2-byte aligned).  mass_in, mass_out f32 [n_kv, n_head_kv, ne3], strides nb2 / nb3; mass_in may be mass_out itself, row for row,
+ * else they are apart (MI355_E_UNSUPPORTED); NULL, or a decay of 0: nothing earlier is read.  Results are f32-accurate: the query and the weights
+ * are not rounded to the cache's type, they keep 22 bits each (24 over bf16 caches), or 2^-39 of their row's largest where that is more.
+ * A slot hidden by the mask takes no part whatever its row holds; a query that sees no slot gives a row of zeros and no weight.  Infinities in
+ * a K row that a query sees count as in the formula (a logit of -inf weighs 0); a block of K with a scale that is not finite, and values of V
+ * that are not, leave the results of the queries that see them not finite, NaN or infinite.
  * workspace: *_workspace_bytes (-1 for sizes and types that the call itself refuses), 16-byte aligned, no initial contents, not shared by calls
  * that can overlap. */
 #define MI355_MASS_MAX_Q 8
@@ -794,7 +796,7 @@ MI355_API int64_t mi355_flash_attn_ext_mass_workspace_bytes(const mi355_fattn_ar
 MI355_API int     mi355_flash_attn_ext_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace,
                                             int64_t workspace_bytes, void *stream);
 /* The weights alone, for up to 65535 queries (a prompt, or the last ones of it; a longer prompt in pieces, with a decay of 1 and mass_in = mass_out):
- * v, dst and dv of args are not used.  At most 2^28 rows of q (sequences x heads x queries) and 2^36 places of mask in all, together, else MI355_E_SHAPE. */
+ * v, dst and dv of args are not used.  At most 2^28 rows of q (sequences x heads x queries), less 1 for every 256 places of mask, else MI355_E_SHAPE. */
 MI355_API int64_t mi355_attn_mass_workspace_bytes(const mi355_fattn_args *args);
 MI355_API int     mi355_attn_mass(const mi355_fattn_args *args, const mi355_attn_mass_args *mass, void *workspace, int64_t workspace_bytes,
                                   void *stream);
