@@ -738,6 +738,7 @@ MI355_API int     mi355_flash_attn_ext_noalloc(const mi355_fattn_args *args, voi
  * steps) and mi355_attn_mass (prompts) accumulate the attention weight each slot draws, mi355_kv_evict picks the slots to keep and, for a
  * prompt, gathers them.  Per-slot tables beside K and V, [ne3][n_head_kv][slots] with byte strides nb2 (head) and nb3 (sequence): the
  * position a slot holds (int32) and its accumulated weight, its "mass" (f32).  Keys are stored rotated, so a slot's place says nothing.
+ * Rows and planes of what these entry points write lie apart from one another (no expanded outputs), else MI355_E_UNSUPPORTED.
  *
  * Attention input of models that normalise queries and keys per head, in one launch: q_out = rope(rms_norm(q) * q_norm), K cache row =
  * rope(rms_norm(k) * k_norm), V cache row = v.  Computes the node run RMS_NORM MUL ROPE (q and k) and the stores of K and V (SET_ROWS / CPY),

@@ -1498,6 +1498,8 @@ static int mass_run(const mi355_fattn_args * p, const mi355_attn_mass_args * w, 
     }
     const int64_t need = mass_workspace(p, with_dst);
     if (need > 0 && (!workspace || workspace_bytes < need)) return MI355_E_WORKSPACE;
+    if (Span(w->mass_out, p->n_kv * 4, 1, 0, p->n_head_kv, w->out_nb2, p->ne3, w->out_nb3).folds() ||       // no place is written twice
+        (with_dst && Span(p->dst, dv * 4, p->n_head, p->d_nb1, p->n_q, p->d_nb2, p->ne3, p->d_nb3).folds())) return MI355_E_UNSUPPORTED;
 
     MArgs a;
     a.q = (const char *)p->q; a.q_nb1 = p->q_nb1; a.q_nb2 = p->q_nb2; a.q_nb3 = p->q_nb3;

@@ -333,6 +333,7 @@ int mi355_kv_evict(const mi355_kv_evict_args * p, void * stream) {
     }
     // a row of 64 pieces and more takes a wave, 16 of them a workgroup: a grid dimension's 2^32 threads hold 2^28 such rows
     if ((p->k || p->v) && p->n_keep >= 1 << 28) return MI355_E_SHAPE;
+    if (ne3 > 0) for (const Span & o : out) if (o.folds()) return MI355_E_UNSUPPORTED;
     if (p->ne3 == 0) return MI355_OK;
 
     KeArgs a;

@@ -51,6 +51,13 @@ def test_qk_norm_rope_refuses_q_out_over_its_inputs(kw):
     assert K.lib.mi355_qk_norm_rope(store_args(**{**dict(k=9 * P, v=10 * P), **kw}), None) == E_UNSUPPORTED
 
 
+@pytest.mark.parametrize("kw", [dict(qo_nb2=0), dict(qo_nb2=256), dict(n=2, qo_nb1=0), dict(n=2, qo_nb1=2048), dict(ne3=2, qo_nb3=0), dict(ko_nb2=0), dict(ko_nb1=128), dict(ko_nb1=0),
+                                dict(ne3=2, ko_nb3=0), dict(vo_nb2=240), dict(ne3=2, vo_nb3=4096), dict(type_kv=B.Q8_0, vo_nb1=134, vo_nb2=4096)])
+def test_qk_norm_rope_refuses_outputs_that_share_memory_with_themselves(kw):
+    """an expanded tensor: several rows in one place"""
+    assert K.lib.mi355_qk_norm_rope(store_args(**{**dict(q_out=9 * P, k_out=10 * P, v_out=12 * P), **kw}), None) == E_UNSUPPORTED
+
+
 def test_qk_norm_rope_of_nothing_launches_nothing():
     assert K.lib.mi355_qk_norm_rope(None, None) == E_NULL
     assert K.lib.mi355_qk_norm_rope(store_args(n=0), None) == 0
@@ -104,6 +111,15 @@ SIDE = dict(k_nb1=512, v_nb1=512, v=6 * P + 256, k_nb2=51200, v_nb2=51200, ko_nb
 def test_kv_evict_refuses_outputs_that_meet_what_it_reads(kw):
     """a gathered row read after its place has been written: any byte in common, wherever the views begin"""
     assert K.lib.mi355_kv_evict(evict_args(**kw), None) == E_UNSUPPORTED
+
+
+NEST = dict(k_nb1=256, k_nb2=25600, k_nb3=51200, v_nb2=25600, v_nb3=51200, ko_nb2=12800, ko_nb3=25600, vo_nb2=12800, vo_nb3=25600)
+
+
+@pytest.mark.parametrize("kw", [dict(ko_nb2=0), dict(ko_nb1=0), dict(ko_nb1=128), dict(ko_nb2=12544), dict(ne3=2, ko_nb3=0), dict(vo_nb1=254), dict(ne3=2, vo_nb3=12800), dict(kept_nb2=0),
+                                dict(kept_nb2=196), dict(ev_nb2=100), dict(mo_nb2=0), dict(po_nb2=4), dict(ne3=2, mo_nb3=4000)])
+def test_kv_evict_refuses_outputs_that_share_memory_with_themselves(kw):
+    assert K.lib.mi355_kv_evict(evict_args(**{**NEST, **kw}), None) == E_UNSUPPORTED
 
 
 @pytest.mark.parametrize("kw", [dict(n_keep=1 << 30), dict(n_keep=1 << 28), dict(n_keep=1 << 29, k_nb1=258), dict(n_keep=1 << 28, ne3=0)])
@@ -170,6 +186,20 @@ def test_attn_mass_refuses(code, kw):
 @pytest.mark.parametrize("fn", [K.lib.mi355_flash_attn_ext_mass, K.lib.mi355_attn_mass])
 def test_attention_mass_refuses_a_shifted_table(fn, kw):
     assert fn(*attn_args(**kw), P, 1 << 40, None) == E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [dict(out_nb2=0), dict(out_nb2=252), dict(ne3=2, out_nb3=0), dict(ne3=2, out_nb3=256)])
+@pytest.mark.parametrize("fn", [K.lib.mi355_flash_attn_ext_mass, K.lib.mi355_attn_mass])
+def test_attention_mass_refuses_an_expanded_table(fn, kw):
+    a, w = attn_args(**{k: v for k, v in kw.items() if k != "out_nb2"}, mass_in=None)
+    w.out_nb2 = kw.get("out_nb2", 256)
+    assert fn(a, w, 9 * P, 1 << 40, None) == E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [dict(d_nb1=0), dict(d_nb1=256), dict(n_q=2, d_nb2=0), dict(ne3=2, d_nb3=0)])
+def test_flash_attn_ext_mass_refuses_an_expanded_dst(kw):
+    a, w = attn_args(**kw, mass_in=None)
+    assert K.lib.mi355_flash_attn_ext_mass(a, w, 9 * P, 1 << 40, None) == E_UNSUPPORTED
 
 
 def test_attention_mass_workspaces():

@@ -231,6 +231,22 @@ def test_store_into_a_cache_of_no_rows(t):
         assert ((qo.cpu().double() - want).abs() <= err).all()
 
 
+def test_store_with_rows_and_tables_that_all_heads_share():
+    """one slot for every head of a token: rows with a stride of 0 over the heads, slot_pos and slot_mass expanded over them"""
+    S, n, H, HK, d, slots = 2, 3, 4, 2, 64, 9
+    q, k, v, dev, qw, kw, _, kc, vc, pos = store_case(S, n, H, HK, d, d, slots, B.F16, 16)
+    rows = torch.stack([torch.randperm(slots, generator=gen(s))[:n] for s in range(S)]).to(torch.int32)[:, None]
+    kg, vg = kc.cuda(), vc.cuda()
+    sp, sm = torch.full((S, 1, slots), 7, dtype=torch.int32, device="cuda"), torch.full((S, 1, slots), 3.0, device="cuda")
+    ops.qk_norm_rope(dev["q"], dev["k"], dev["v"], qw.cuda(), kw.cuda(), 1e-6, pos.cuda(), kg, vg, B.F16, rows=rows.cuda().expand(S, HK, n),
+                     slot_pos=sp.expand(S, HK, slots), slot_mass=sm.expand(S, HK, slots))
+    check_rows(kg.cpu(), kc, rows.expand(S, HK, n), *store_oracle(k, kw, 1e-6, pos, d, 2), B.F16)
+    want = torch.full((S, slots), 7, dtype=torch.int32).scatter(1, rows[:, 0].long(), pos)
+    assert torch.equal(sp[:, 0].cpu(), want) and torch.equal(sm[:, 0].cpu(), torch.where(want == 7, 3.0, 0.0))
+    with pytest.raises(K.Mi355Error):             # a cache that the heads share is another matter
+        ops.qk_norm_rope(dev["q"], dev["k"], None, None, None, 1e-6, pos.cuda(), kg[:, :1].expand(S, HK, slots, d), None, B.F16)
+
+
 def test_store_on_another_stream_and_captured():
     """launched on the current stream whatever it is; a captured launch reads new rows and positions at every replay"""
     S, n, H, HK, d, slots = 2, 1, 8, 2, 128, 16
