@@ -62,6 +62,9 @@ def test_qk_norm_rope_of_nothing_launches_nothing():
     assert K.lib.mi355_qk_norm_rope(None, None) == E_NULL
     assert K.lib.mi355_qk_norm_rope(store_args(n=0), None) == 0
     assert K.lib.mi355_qk_norm_rope(store_args(ne3=0), None) == 0
+
+
+def test_qk_norm_rope_of_tensors_without_an_address():
     none = dict(q=None, k=None, v=None, q_out=None, k_out=None, v_out=None, pos=None, rows=None)
     assert K.lib.mi355_qk_norm_rope(store_args(ne3=0, **none), None) == 0 and K.lib.mi355_qk_norm_rope(store_args(n=0, **none), None) == 0
     assert K.lib.mi355_qk_norm_rope(store_args(n_rows=0, q=None), None) == E_NULL
@@ -132,6 +135,9 @@ def test_kv_evict_refuses_more_rows_than_a_grid_holds(kw):
 def test_kv_evict_of_no_sequences_launches_nothing():
     assert K.lib.mi355_kv_evict(None, None) == E_NULL
     assert K.lib.mi355_kv_evict(evict_args(ne3=0), None) == 0
+
+
+def test_kv_evict_of_tensors_without_an_address():
     assert K.lib.mi355_kv_evict(evict_args(ne3=0, mass=None, slot_pos=None, n_past=None, kept=None, evicted=None, k=None, v=None, k_out=None, v_out=None,
                                            mass_out=None, pos_out=None), None) == 0
     assert K.lib.mi355_kv_evict(evict_args(ne3=0, n_keep=0), None) == E_SHAPE
