@@ -200,13 +200,10 @@ template <bool BF> static __device__ __forceinline__ bool sanitize(v4i & x) {
 
 // q and K in parts, sum over the parts p of q_p K: an infinity of K meets the parts' different signs and gives a NaN where the product is an infinity.
 // Only the largest part, which has q's sign, meets it: the others take K without its non-finite values.  (Where q's large part is 0 so is q, next to
-// its row's largest value.)  For tiles that have a NaN among their products
-template <bool BF> static __device__ __forceinline__ v4i finite(v4i x) {
-    asm volatile("" : "+v"(x));                                 // (formed where it is used: kept through a loop it takes the operands' registers again)
-    sanitize<BF>(x);
-    return x;
-}
-static __device__ __forceinline__ void read_again() { asm volatile("" ::: "memory"); }     // (so that what was read from LDS is not kept for a second use)
+// its row's largest value.)  Nor does what is read in place of the features past the head size, which meets zeros of q.  For tiles that have a
+// NaN among their products
+template <bool BF> static __device__ __forceinline__ v4i finite(v4i x) { sanitize<BF>(x); return x; }
+static __device__ __forceinline__ float max_or_nan(float x, float y) { return __builtin_elementwise_maximum(x, y); }
 
 static __device__ __forceinline__ float max_groups(float v) {       // over the four 16-lane groups, lanes of equal place
     v = fmaxf(v, __shfl_xor(v, 16, 64));
@@ -456,16 +453,17 @@ mass_step_kernel(const MArgs a) {
                 bool nan = false;
 #pragma unroll
                 for (int i = 0; i < 8; i++) nan |= c[i >> 2][i & 3] != c[i >> 2][i & 3];
-                if (__any(nan)) {
-                    read_again();
+                if (__builtin_expect(__any(nan), 0)) {
+                    int again = lane;
+                    asm("" : "+v"(again));                      // (q read again: what the products above read is not kept for this)
                     c[0] = c[1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            const v4i f = finite<F::bf>(kc[u][ks].raw);
+                            const v4i f = finite<F::bf>(kc[u][ks].raw), k0 = 4 * ks + g < a.d / 8 ? kc[u][ks].raw : f;
 #pragma unroll
-                            for (int p = P - 1; p >= 0; p--) c[u] = mfma16<F::bf>(p == 0 ? kc[u][ks].raw : f, qs[ks][p][lane], c[u]);
+                            for (int p = P - 1; p >= 0; p--) c[u] = mfma16<F::bf>(p == 0 ? k0 : f, qs[ks][p][again], c[u]);
                         }
                 }
             }
@@ -1106,53 +1104,67 @@ prompt_stats_kernel(const MArgs a) {
         const uint32_t bytes = cl[b][wave][lane] >> (16 * (t & 1));
         const int c0 = bytes & 255, c1 = bytes >> 8 & 255;
         if (mine && __any((c0 | c1) != MASK_HIDDEN)) {
-            auto tile = [&](bool again) {                       // -> maximum and sum with this tile
-                v16f c[2], part;
+            v16f c[2], part;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const v4i k0 = *(const v4i *)(kt[b] + lds_chunk<D>(32 * u + lr, 2 * ks + lh));
+                    if constexpr (F::quant) {
+                        if (ks % 2 == 0) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) part[i] = 0.0f;
+                        }
+#pragma unroll
+                        for (int p = QP - 1; p >= 0; p--) part = mfma32<F::bf>(k0, qf[ks][p], part);
+                        if (ks % 2 == 1) fold_block(&kd[b][ks / 2][32 * u], lh, part, c[u]);
+                    } else {
+#pragma unroll
+                        for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(k0, qf[ks][p], c[u]);
+                    }
+                }
+            }
+            auto largest = [&]() {
+                float x = c[0][0];
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x = max_or_nan(x, c[u][i]);
+                return x;
+            };
+            float mx = F::quant ? 0.0f : largest();
+            if constexpr (!F::quant) if (__builtin_expect(__any(mx != mx), 0)) {     // an infinity in a row of K (see finite); q comes from memory, in a short loop
+                const uint16_t * qr = a.qparts + row * QP * D + 8 * lh;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
-#pragma unroll
+#pragma unroll 1
                     for (int ks = 0; ks < KS; ks++) {
-                        const v4i k0 = *(const v4i *)(kt[b] + lds_chunk<D>(32 * u + lr, 2 * ks + lh));
-                        if constexpr (F::quant) {
-                            if (ks % 2 == 0) {
+                        const v4i k0 = *(const v4i *)(kt[b] + lds_chunk<D>(32 * u + lr, 2 * ks + lh)), f = finite<F::bf>(k0);
 #pragma unroll
-                                for (int i = 0; i < 16; i++) part[i] = 0.0f;
-                            }
-#pragma unroll
-                            for (int p = QP - 1; p >= 0; p--) part = mfma32<F::bf>(k0, qf[ks][p], part);
-                            if (ks % 2 == 1) fold_block(&kd[b][ks / 2][32 * u], lh, part, c[u]);
-                        } else {
-                            const v4i f = again ? finite<F::bf>(k0) : k0;
-#pragma unroll
-                            for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(p == 0 ? k0 : f, qf[ks][p], c[u]);
-                        }
+                        for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(p == 0 && 2 * ks + lh < a.d / 8 ? k0 : f, *(const v4i *)(qr + p * D + 16 * ks), c[u]);
                     }
                 }
-                float sc = qe;
-                if (CAP || !__all(c0 == MASK_ZERO && c1 == MASK_ZERO)) {
-                    tile_logits<CAP>(a, c[0], qe, slope, c0, mrow, m8, t * PA_SLOTS);
-                    tile_logits<CAP>(a, c[1], qe, slope, c1, mrow, m8, t * PA_SLOTS + 32);
-                    sc = 1.0f;
-                }
-                float mx = c[0][0];
+                mx = largest();
+            }
+            float sc = qe;
+            if (CAP || !__all(c0 == MASK_ZERO && c1 == MASK_ZERO)) {
+                tile_logits<CAP>(a, c[0], qe, slope, c0, mrow, m8, t * PA_SLOTS);
+                tile_logits<CAP>(a, c[1], qe, slope, c1, mrow, m8, t * PA_SLOTS + 32);
+                sc = 1.0f;
+                mx = largest();
+            } else if (F::quant) mx = largest();
+            mx = max_or_nan(m, mx * sc);
+            const float ms = mx == -INFINITY ? 0.0f : mx;
+            l *= __builtin_amdgcn_exp2f(m - ms);
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) mx = fmaxf(mx, c[u][i]);
-                mx = fmaxf(m, mx * sc);
-                const float ms = mx == -INFINITY ? 0.0f : mx;
-                float ln = l * __builtin_amdgcn_exp2f(m - ms);
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) ln += __builtin_amdgcn_exp2f(__builtin_fmaf(c[u][i], sc, -ms));
-                return v2f{mx, ln};
-            };
-            v2f x = tile(false);
-            if constexpr (!F::quant) if (__any(x.y != x.y && l == l)) { read_again(); x = tile(true); }     // an infinity in a row of K (see finite)
-            m = x.x; l = x.y;
+                for (int i = 0; i < 16; i++) l += __builtin_amdgcn_exp2f(__builtin_fmaf(c[u][i], sc, -ms));
+            m = mx;
         }
         if (S == 2 && ahead < nt) commit(bf);
         b = b == S - 1 ? 0 : b + 1;
@@ -1281,45 +1293,56 @@ prompt_mass_kernel(const MArgs a) {
             RowC c4 = *(const RowC *)&rc[b][0][4 * lr];
             if (t * PB_ROWS + lr >= R) { c4.m = INFINITY; c4.inv = 0.0f; }      // weighs nothing
             v16f c[NS], part[NS];
-#pragma unroll
-            for (int u = 0; u < NS; u++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                v4i q[QP];
-                if constexpr (F::quant) if (ks % 2 == 0) {
-#pragma unroll
-                    for (int u = 0; u < NS; u++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) part[u][i] = 0.0f;
-                }
-#pragma unroll
-                for (int p = 0; p < QP; p++) q[p] = *(const v4i *)(qt[b][p] + lds_chunk<D>(lr, 2 * ks + lh));
-#pragma unroll
-                for (int p = QP - 1; p >= 0; p--)
-#pragma unroll
-                    for (int u = 0; u < NS; u++) {
-                        if constexpr (F::quant) part[u] = mfma32<F::bf>(kf[u][ks], q[p], part[u]);
-                        else c[u] = mfma32<F::bf>(kf[u][ks], q[p], c[u]);
-                    }
-                if constexpr (F::quant) if (ks % 2 == 1) {
-#pragma unroll
-                    for (int u = 0; u < NS; u++) fold_block(&kd[wave][ks / 2][32 * u], lh, part[u], c[u]);
-                }
-            }
-            if constexpr (!F::quant) if (odd) {
-                read_again();
+            if (!F::quant && __builtin_expect(odd, 0)) {        // (K comes from memory again, in a short loop)
 #pragma unroll
                 for (int u = 0; u < NS; u++) {
+                    const int j = j0 + 32 * u + lr;
+                    const char * krow = kb + (uint64_t)(uint32_t)(j < a.n_kv ? j : a.n_kv - 1) * a.k_nb1;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
+#pragma unroll 1
+                    for (int ks = 0; ks < KS; ks++) {
+                        const bool in = 2 * ks + lh < a.d / 8;
+                        const v4i k0 = *(const v4i *)(krow + 16 * (in ? 2 * ks + lh : 0)), f = finite<F::bf>(k0);
+#pragma unroll
+                        for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(p == 0 && in ? k0 : f, *(const v4i *)(qt[b][p] + lds_chunk<D>(lr, 2 * ks + lh)), c[u]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < NS; u++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) c[u][i] = 0.0f;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        const v4i f = finite<F::bf>(kf[u][ks]);
+                for (int ks = 0; ks < KS; ks++) {
+                    v4i q[QP];
+                    if constexpr (F::quant) if (ks % 2 == 0) {
 #pragma unroll
-                        for (int p = QP - 1; p >= 0; p--) c[u] = mfma32<F::bf>(p == 0 ? kf[u][ks] : f, *(const v4i *)(qt[b][p] + lds_chunk<D>(lr, 2 * ks + lh)), c[u]);
+                        for (int u = 0; u < NS; u++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) part[u][i] = 0.0f;
                     }
+#pragma unroll
+                    for (int p = 0; p < QP; p++) q[p] = *(const v4i *)(qt[b][p] + lds_chunk<D>(lr, 2 * ks + lh));
+#pragma unroll
+                    for (int p = QP - 1; p >= 0; p--)
+#pragma unroll
+                        for (int u = 0; u < NS; u++) {
+                            if constexpr (F::quant) part[u] = mfma32<F::bf>(kf[u][ks], q[p], part[u]);
+                            else c[u] = mfma32<F::bf>(kf[u][ks], q[p], c[u]);
+                        }
+                    if constexpr (F::quant) if (ks % 2 == 1) {
+#pragma unroll
+                        for (int u = 0; u < NS; u++) fold_block(&kd[wave][ks / 2][32 * u], lh, part[u], c[u]);
+                    }
+                }
+                // q is read two steps ahead of its products: beside the other branch the compiler reads it just before them (1024 x 1024, bf16, heads
+                // of 256: 73 us for this pass, 64 so)
+                if constexpr (!F::quant) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2 * QP, 0);
+#pragma unroll
+                    for (int ks = 0; ks < KS - 2; ks++) { __builtin_amdgcn_sched_group_barrier(0x8, QP * NS, 0); __builtin_amdgcn_sched_group_barrier(0x100, QP, 0); }
+                    __builtin_amdgcn_sched_group_barrier(0x8, 2 * QP * NS, 0);
                 }
             }
             float sc = c4.qe;

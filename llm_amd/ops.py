@@ -519,7 +519,7 @@ def set_rows(src, ids, dst, type_dst):
 _KV_DTYPE = {B.F32: torch.float32, B.F16: torch.float16, B.BF16: torch.bfloat16, B.Q8_0: torch.uint8, B.Q4_0: torch.uint8}
 _KV_BYTES = {B.F32: 4, B.F16: 2, B.BF16: 2, B.Q8_0: 1, B.Q4_0: 1}          # of a cache tensor's element
 _BLOCK = {B.Q8_0: 34, B.Q4_0: 18}
-_MASK_DTYPE = (torch.float16, torch.int16, torch.uint16)
+_MASK_DTYPE = (torch.float16, torch.int16, torch.uint16)                    # f16 or its bits
 
 
 # The entry points of the bounded KV cache are called once per layer and step: their wrappers read every tensor's shape and strides once.
@@ -688,7 +688,7 @@ def _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bi
         if len(sh) < 4:                       # the two first dimensions may be left out, or the heads'
             sh, st = ((1, 1) + sh, (0, 0) + st) if len(sh) == 2 else ((sh[0], 1) + sh[1:], (st[0], 0) + st[1:])
         e3, e2, m_n, m_s = sh
-        if mask.dtype not in _MASK_DTYPE or e2 < 1 or e3 < 1 or H % e2 or S % e3 or m_n < n or m_s != slots or (slots > 1 and st[3] != 1):
+        if (mask.dtype is not torch.float16 and mask.dtype not in _MASK_DTYPE) or e2 < 1 or e3 < 1 or H % e2 or S % e3 or m_n < n or m_s != slots or (slots > 1 and st[3] != 1):
             raise ValueError("mask: f16 (or its bits as int16 / uint16) [seqs | 1, heads | 1, >= tokens, slots], the two first may be left out")
         mp, m1, m2, m3 = mask.data_ptr(), st[2] * 2, st[1] * 2, st[0] * 2
     dst, vp, v1, v2, v3, dp, dv = None, None, 0, 0, 0, None, 0
@@ -708,6 +708,8 @@ def _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bi
         ip, ns = mass.data_ptr(), mass.stride()
         if mass.dtype is not f32 or mass.shape != (S, hk, slots) or (slots > 1 and ns[2] != 1):
             raise ValueError("mass: f32 [seqs, kv heads, slots], slots contiguous")
+    if n == 0 or S == 0:
+        return None, None, dst, mass_out
     a = K.FattnArgs(q.data_ptr(), qs[2] * 4, qs[1] * 4, qs[0] * 4, k.data_ptr(), type_kv, ks[2] * b, ks[1] * b, ks[0] * b, vp, type_kv, v1, v2, v3,
                     mp, m1, m2, m3, e2, e3, dp, dv * 4, H * dv * 4, n * H * dv * 4, d, n, slots, H, hk, S, scale, max_bias, logit_softcap, dv)
     return a, K.AttnMassArgs(ip, ns[1] * 4, ns[0] * 4, mass_out.data_ptr(), os[1] * 4, os[0] * 4, decay), dst, mass_out
@@ -724,7 +726,7 @@ def flash_attn_ext_mass(q, k, v, mask, type_kv, scale, mass=None, decay=1.0, mas
     None); mass f32 [seqs, kv heads, slots] or None; mass_out may be mass -> (f32 [seqs, tokens, heads, dv], mass_out = decay mass + weights)."""
     dev = torch.cuda.current_device()
     a, w, dst, mass_out = _mass_args(dev, q, k, v, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
-    if a.n_q == 0 or a.ne3 == 0:
+    if a is None:
         return dst, _no_queries(mass, decay, mass_out)
     need = K.lib.mi355_flash_attn_ext_mass_workspace_bytes(a)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
@@ -738,7 +740,7 @@ def attn_mass(q, k, mask, type_kv, scale, mass=None, decay=1.0, mass_out=None, m
     """The weight every slot draws from up to 65535 queries (mi355_attn_mass); arguments as flash_attn_ext_mass, without V -> mass_out."""
     dev = torch.cuda.current_device()
     a, w, _, mass_out = _mass_args(dev, q, k, None, mask, type_kv, scale, mass, decay, mass_out, max_bias, logit_softcap)
-    if a.n_q == 0 or a.ne3 == 0:
+    if a is None:
         return _no_queries(mass, decay, mass_out)
     need = K.lib.mi355_attn_mass_workspace_bytes(a)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)

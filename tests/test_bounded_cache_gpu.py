@@ -871,6 +871,25 @@ def test_attention_mass_of_keys_with_infinities(t, d, n):
         assert torch.isnan(dst[0, n - 1, 5]).all() and ((dst.cpu().double() - wd).abs() <= ed)[0][other].all()
 
 
+@pytest.mark.parametrize("t", [B.F16, B.BF16])
+@pytest.mark.parametrize("d", [8, 72, 80, 96, 112, 160, 192, 248])
+@pytest.mark.parametrize("n", [1, 3, 20])
+def test_attention_mass_of_infinities_at_the_end_of_a_key(t, d, n):
+    """heads that a larger size's kernel serves: what it reads in place of the features past the head size does not count"""
+    H, HK, slots, scale = 4, 2, 90, 0.1
+    q, k, v, _ = attn_case(1, H, HK, n, slots, d, d, t, d + n)
+    q[..., d - 1] = -q[..., d - 1].abs() - 0.1
+    out = [0, 5, 40, 64, 89]
+    k[:, :, out, d - 1] = float("inf")
+    hidden, clean = torch.zeros((1, 1, n, slots)).half(), k.clone()
+    hidden[..., out], clean[:, :, out] = float("-inf"), 0.0
+    wd, ed, wm, em = attn_oracle(q, values(clean, t), values(v, t), hidden, scale, None, 0.0)
+    assert ((ops.attn_mass(q.cuda(), k.cuda(), None, t, scale).cpu().double() - wm).abs() <= em).all()
+    if n <= 8:
+        dst, mass = ops.flash_attn_ext_mass(q.cuda(), k.cuda(), v.cuda(), None, t, scale)
+        assert ((dst.cpu().double() - wd).abs() <= ed).all() and ((mass.cpu().double() - wm).abs() <= em).all()
+
+
 @pytest.mark.parametrize("S,n,slots", [(1, 0, 5), (2, 0, 512), (1, 0, 100000), (0, 1, 512), (0, 40, 300), (1, 0, 0)])
 def test_attention_mass_of_no_queries(S, n, slots):
     """an empty batch: an empty dst, and what earlier calls left, decayed"""
