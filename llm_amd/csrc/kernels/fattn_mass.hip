@@ -862,9 +862,9 @@ static int64_t step_splits(const mi355_fattn_args * p) {
 // through LDS: K of f16 and bf16 in the first pass by DMA, two tiles ahead of the products, blocks through registers, one ahead; Q in the second pass
 // by DMA, two tiles ahead, one with heads above 128 (LDS).  A tile that the mask hides from all rows of a wave (half of a causal prompt) costs its
 // loads and its meeting.
-// 64 queries x 32 heads over 16384 f16 slots: 5 + 25 + 5 + 32 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
+// 64 queries x 32 heads over 16384 f16 slots: 6 + 24 + 5 + 32 us.  A pass is 17 GFLOP, 15 us at the rate a large product reaches here, behind 5 us
 // until the first tile of 512 workgroups is there; without its products the first pass takes 20, without its exponentials 23.  2047
-// causal queries, bf16: 16 + 68 + 82 + 5 us, 45 a pass at that rate.  Matrix cores and vector units are each busy a third of either pass (30-40 %), a
+// causal queries, bf16: 16 + 69 + 79 + 5 us, 45 a pass at that rate.  Matrix cores and vector units are each busy a third of either pass (30-40 %), a
 // wave waits for its turn or its operands most of the rest: 1.7 waves a SIMD do not cover one another's chains.
 typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int PT = 256;                  // threads: 4 waves
@@ -1337,7 +1337,7 @@ prompt_mass_kernel(const MArgs a) {
                     }
                 }
                 // q is read two steps ahead of its products: beside the other branch the compiler reads it just before them (1024 x 1024, bf16, heads
-                // of 256: 73 us for this pass, 64 so)
+                // of 256: 73 us for this pass, 61 so)
                 if constexpr (!F::quant) {
                     __builtin_amdgcn_sched_group_barrier(0x100, 2 * QP, 0);
 #pragma unroll
