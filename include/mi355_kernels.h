@@ -738,7 +738,8 @@ MI355_API int     mi355_flash_attn_ext_noalloc(const mi355_fattn_args *args, voi
  * steps) and mi355_attn_mass (prompts) accumulate the attention weight each slot draws, mi355_kv_evict picks the slots to keep and, for a
  * prompt, gathers them.  Per-slot tables beside K and V, [ne3][n_head_kv][slots] with byte strides nb2 (head) and nb3 (sequence): the
  * position a slot holds (int32) and its accumulated weight, its "mass" (f32).  Keys are stored rotated, so a slot's place says nothing.
- * Rows and planes of what these entry points write lie apart from one another (no expanded outputs), else MI355_E_UNSUPPORTED.
+ * Rows and planes of what these entry points write lie apart from one another (no expanded outputs), else MI355_E_UNSUPPORTED; a cache that is stored
+ * into by given rows may be a pool that sequences or heads share.
  *
  * Attention input of models that normalise queries and keys per head, in one launch: q_out = rope(rms_norm(q) * q_norm), K cache row =
  * rope(rms_norm(k) * k_norm), V cache row = v.  Computes the node run RMS_NORM MUL ROPE (q and k) and the stores of K and V (SET_ROWS / CPY),
@@ -750,7 +751,7 @@ MI355_API int     mi355_flash_attn_ext_noalloc(const mi355_fattn_args *args, voi
  *   k_out, v_out: caches of type_kv f32 | f16 | bf16 (16-byte aligned) | q8_0 | q4_0 (2-byte aligned, whole 32-blocks, else MI355_E_SHAPE),
  *   byte strides nb1 (row), nb2 (head), nb3 (sequence), n_rows rows per head (0: may be NULL, nothing is stored)
  *   rows: int32 cache row of each (token, head, sequence), strides nb1 / nb2 / nb3 (0: shared); NULL: token i goes to row i.  A row outside
- *   [0, n_rows) is not stored (q_out is written all the same).  Rows of one call must be distinct per head and sequence.
+ *   [0, n_rows) is not stored (q_out is written all the same).  Rows of one call must be distinct per head and sequence (over all that share a pool).
  *   q_norm, k_norm f32 [head_dim]; NULL: no weight.  pos int32 [n, ne3], freq_factors f32 [n_dims / 2] or NULL, rope parameters as in
  *   mi355_rope_f32, modes NORMAL and NEOX; n_dims 0: no rotation.  Angles are computed in 64 bits: at far positions they are nearer to the
  *   formula than mi355_rope_f32's, which follows the reference's 32-bit products.

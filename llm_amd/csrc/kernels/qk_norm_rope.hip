@@ -230,11 +230,11 @@ int mi355_qk_norm_rope(const mi355_qk_norm_rope_args * p, void * stream) {
     const Span qo(p->q_out, p->head_dim * 4, p->n, p->qo_nb1, p->n_head, p->qo_nb2, p->ne3, p->qo_nb3), q(p->q, p->head_dim * 4, p->n, p->q_nb1, p->n_head, p->q_nb2, p->ne3, p->q_nb3);
     if (!qo.same(q) && (spans_meet(qo, q) || spans_meet(qo, Span(p->k, p->head_dim * 4, p->n, p->k_nb1, p->n_head_kv, p->k_nb2, p->ne3, p->k_nb3)) ||
                         spans_meet(qo, Span(p->v, dv * 4, p->n, p->v_nb1, p->n_head_kv, p->v_nb2, p->ne3, p->v_nb3)))) return MI355_E_UNSUPPORTED;
-    // and no place is written twice: heads, rows and sequences of what is written lie apart (but for the slots' tables, which heads that share their
-    // rows may share: they write the same)
-    const int64_t rk = mi355_row_size(p->type_kv, p->head_dim), rv = mi355_row_size(p->type_kv, dv);
-    if (qo.folds() || Span(p->k_out, rk, p->n_rows, p->ko_nb1, p->n_head_kv, p->ko_nb2, p->ne3, p->ko_nb3).folds() ||
-        (p->v && Span(p->v_out, rv, p->n_rows, p->vo_nb1, p->n_head_kv, p->vo_nb2, p->ne3, p->vo_nb3).folds())) return MI355_E_UNSUPPORTED;
+    // and no place is written twice: heads, tokens and sequences of q_out lie apart, so do those of a cache whose rows are the tokens' own.  (Rows that
+    // are given may share a pool: heads or sequences at one address, in rows of their own)
+    const int64_t rk = mi355_row_size(p->type_kv, p->head_dim), rv = mi355_row_size(p->type_kv, dv), n1 = p->n < p->n_rows ? p->n : p->n_rows;
+    if (qo.folds() || (!p->rows && Span(p->k_out, rk, n1, p->ko_nb1, p->n_head_kv, p->ko_nb2, p->ne3, p->ko_nb3).folds()) ||
+        (!p->rows && p->v && Span(p->v_out, rv, n1, p->vo_nb1, p->n_head_kv, p->vo_nb2, p->ne3, p->vo_nb3).folds())) return MI355_E_UNSUPPORTED;
 
     QnArgs a;
     a.q = (const char *)p->q; a.q_nb1 = p->q_nb1; a.q_nb2 = p->q_nb2; a.q_nb3 = p->q_nb3;

@@ -55,7 +55,7 @@ def test_qk_norm_rope_refuses_q_out_over_its_inputs(kw):
                                 dict(ne3=2, ko_nb3=0), dict(vo_nb2=240), dict(ne3=2, vo_nb3=4096), dict(type_kv=B.Q8_0, vo_nb1=134, vo_nb2=4096)])
 def test_qk_norm_rope_refuses_outputs_that_share_memory_with_themselves(kw):
     """an expanded tensor: several rows in one place"""
-    assert K.lib.mi355_qk_norm_rope(store_args(**{**dict(q_out=9 * P, k_out=10 * P, v_out=12 * P), **kw}), None) == E_UNSUPPORTED
+    assert K.lib.mi355_qk_norm_rope(store_args(**{**dict(q_out=9 * P, k_out=10 * P, v_out=12 * P, rows=None, n=2), **kw}), None) == E_UNSUPPORTED
 
 
 def test_qk_norm_rope_of_nothing_launches_nothing():

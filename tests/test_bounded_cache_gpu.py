@@ -247,6 +247,22 @@ def test_store_with_rows_and_tables_that_all_heads_share():
         ops.qk_norm_rope(dev["q"], dev["k"], None, None, None, 1e-6, pos.cuda(), kg[:, :1].expand(S, HK, slots, d), None, B.F16)
 
 
+@pytest.mark.parametrize("t", [B.F16, B.BF16])
+def test_store_into_a_pool_that_sequences_share(t):
+    """one cache for all sequences (a stride of 0 over them), each token in a row of its own"""
+    S, n, H, HK, d, slots = 3, 4, 4, 2, 64, 20
+    q, k, v, dev, qw, kw, _, _, _, pos = store_case(S, n, H, HK, d, d, slots, t, 18)
+    g = gen(19)
+    rows = torch.stack([torch.randperm(slots, generator=g)[: S * n] for _ in range(HK)]).reshape(HK, S, n).transpose(0, 1).contiguous().to(torch.int32)
+    kc, vc = cache((1, HK, slots, d), t, g), cache((1, HK, slots, d), t, g)
+    kg, vg = kc.cuda(), vc.cuda()
+    ops.qk_norm_rope(dev["q"], dev["k"], dev["v"], qw.cuda(), kw.cuda(), 1e-6, pos.cuda(), kg.expand(S, HK, slots, d), vg.expand(S, HK, slots, d), t, rows=rows.cuda())
+    flat = lambda x: x.transpose(0, 1).reshape(1, HK, S * n, *x.shape[3:])  # noqa: E731
+    want, err = store_oracle(k, kw, 1e-6, pos, d, 2)
+    check_rows(kg.cpu(), kc, flat(rows), flat(want), flat(err), t)
+    check_rows(vg.cpu(), vc, flat(rows), flat(v.double().transpose(1, 2)), torch.zeros(()), t)
+
+
 def test_store_on_another_stream_and_captured():
     """launched on the current stream whatever it is; a captured launch reads new rows and positions at every replay"""
     S, n, H, HK, d, slots = 2, 1, 8, 2, 128, 16
